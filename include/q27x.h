@@ -240,6 +240,81 @@ int q27x_attn_rows_noalloc(const uint16_t* qh, const uint16_t* qkv_gate, int qkv
                            int kv_group, int nq, int nkv, int hd, int gate, int pos0, int nr,
                            uint16_t* out, int8_t* xq, float* xs, q27x_stream_t s);
 
+/* ---- one paged key/value cache for many sequences ----
+ * No counterpart in the reference, whose cache holds one sequence at consecutive positions
+ * (src/q27_attn.hip:258-463 reads it by position): serving a batch from one pool, images among the
+ * text, and a cache that stays within a bound.
+ *
+ * A pool of n_pages pages of `page` positions (a power of two); position i of page p is row
+ * p * page_stride + i of k, v (page_stride 0: page). A row is nkv*hd int8 codes with fp32 scales per
+ * kv_group (16, 32, 64) in ks, vs, as the cache of q27x_attn_rows (which is a pool: any page, a table
+ * that counts up), or nkv*hd bf16 values (kv_group 0; ks, vs unused). Key i of sequence b lies on
+ * page table[b][i / page]; keys on pages outside 0 .. n_pages-1 or behind the table are neither
+ * read nor written. lens[b]: keys that sequence b holds, the call's rows included. Sequence b's rows
+ * are row_start[b] .. row_start[b+1]-1 (not decreasing; NULL: row b), its last lens[b] - n .. lens[b]-1
+ * keys. Rows behind the last sequence are left as they were. k, v 16-byte aligned; hd 128 or 256;
+ * no two sequences that a call writes share a page. table, lens and row_start are device arrays:
+ * a captured graph follows them. */
+typedef struct q27x_paged_kv {
+    void* k; void* v;
+    float* ks; float* vs;
+    int kv_group, nkv, hd;
+    int n_pages, page, page_stride;
+    const int32_t* table;          /* [n_seq][table_stride] */
+    int table_stride;
+    const int32_t* lens;           /* [n_seq] */
+    const int32_t* row_start;      /* [n_seq + 1] or NULL */
+    int n_seq;
+} q27x_paged_kv_t;
+
+/* q27x_attn_prep_rows for rows of many sequences, any number of each, with rotary positions of up to
+ * four axes (time, height, width of image and video tokens; one axis: plain rotary): per head
+ * RMSNorm(1+w), then pair i of the first rot dims (dims i and i + rot/2; rot even, at most hd) turned
+ * by the angle of position pos[pair_axis[i]][row], row pos of the tables rope_cos, rope_sin
+ * [n_pos][rot/2] (positions outside are taken as the nearest end); q -> bf16 qh [nrows][nq*hd]; K
+ * (normed, turned) and V (raw) -> the row's position in its pages. pos: device [n_axes][pos_stride];
+ * pair_axis: host [rot/2], read before the call returns (NULL with one axis). qkv rows as in
+ * q27x_attn_prep_rows (q, with gate beside each head's gate, then k, then v). */
+int q27x_paged_prep_rows(const uint16_t* qkv, int qkv_stride, const uint16_t* q_norm_w,
+                         const uint16_t* k_norm_w, const float* rope_cos, const float* rope_sin,
+                         int rot, int n_pos, const int32_t* pos, int pos_stride, int n_axes,
+                         const uint8_t* pair_axis, const q27x_paged_kv_t* kv, uint16_t* qh, int nq,
+                         int gate, float eps, int nrows, q27x_stream_t s);
+
+/* q27x_attn_rows for many sequences over their pages: row i of a sequence's n rows (1 .. max_rows,
+ * at most 8; further ones are left as they were) sees keys 0 .. lens - n + i, of which those below
+ * max_len are read; out = bf16(softmax(q.k/sqrt(hd)) v * sigmoid(gate)) [nrows][nq*hd]; xq/xs its per-16
+ * quantization (nullable). A row that sees no key gets zeros. w (nullable): the weight that each
+ * key got from the row, summed over its query heads, w[row][0 .. min(lens, max_len)-1] (0 where
+ * the row does not see it; nothing behind is written), rows w_stride >= max_len apart: what q27x_paged_evict takes.
+ * A row's bits depend on its own keys only, not on the batch or the rows beside it. work: scratch of
+ * q27x_paged_attn_work_bytes bytes (weights: with w), 16-byte aligned, not shared by calls that may
+ * overlap; 0 for counts that the call refuses. */
+size_t q27x_paged_attn_work_bytes(int nq, int hd, int max_len, int nrows, int weights);
+int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_stride,
+                         const q27x_paged_kv_t* kv, int nq, int gate, int max_len, int max_rows,
+                         int nrows, void* work, uint16_t* out, int8_t* xq, float* xs, float* w,
+                         int w_stride, q27x_stream_t s);
+
+/* Eviction by accumulated attention weight, one layer's cache. For every sequence b and its keys
+ * i < len = min(lens[b], max_len): acc[b][i] = ((decay*acc[b][i]) + w[r0][i]) + w[r1][i] ... over its
+ * first n_acc[b] rows (NULL: all; w NULL: none; the rows that speculation rejected left out), in
+ * fp32; keys that came since the last call start from 0. Where len > high, the `recent` newest keys
+ * and the heaviest others stay, `budget` in all (recent <= budget <= high; ties to the lowest index,
+ * a sum that is not a number below all others), and new_lens[b] = budget, else len. Keys behind budget
+ * that stay move, with cache rows, acc and ord, into the places before it that fall free, both in
+ * ascending order: the cache's order is not kept, what lies behind new_lens is left as it was.
+ * ord [n_seq][acc_stride]: how many keys came before each; state [n_seq][2]: keys that acc and ord
+ * know, keys that ever came; zero state to begin a sequence, acc and ord need no start value. After a
+ * rollback pass the shorter lens. new_lens may be kv->lens. A later q27x_paged_attn_rows needs no
+ * positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
+ * aligned. */
+size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
+int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc,
+                     int nrows, float decay, float* acc, int32_t* ord, int acc_stride, int32_t* state,
+                     int high, int budget, int recent, int max_len, void* work, int32_t* new_lens,
+                     q27x_stream_t s);
+
 /* R18 argmax of nr rows of n logits: non-finite filtered, ties -> lowest index, all non-finite
  * -> index 0 / value -inf (replaces q27_argmax_val, include/q27.h:348; src/q27_elem.hip:216-322). */
 int q27x_argmax_rows(const float* logits, int n, int ld, int nr, int32_t* idx, float* val,

@@ -56,6 +56,15 @@ class I8G(ctypes.Structure):
                 ("rows", ctypes.c_int), ("K", ctypes.c_int)]
 
 
+class PagedKV(ctypes.Structure):
+    """q27x_paged_kv_t: a pool of pages and the sequences that lie on them (device pointers)."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p),
+                ("kv_group", ctypes.c_int), ("nkv", ctypes.c_int), ("hd", ctypes.c_int),
+                ("n_pages", ctypes.c_int), ("page", ctypes.c_int), ("page_stride", ctypes.c_int),
+                ("table", ctypes.c_void_p), ("table_stride", ctypes.c_int),
+                ("lens", ctypes.c_void_p), ("row_start", ctypes.c_void_p), ("n_seq", ctypes.c_int)]
+
+
 _lib = None
 VP, I, F, SZ, U64 = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_uint64
 
@@ -90,6 +99,11 @@ _SIGS = {
     "q27x_attn_work_bytes": ([I, I, I, I], SZ),
     "q27x_attn_rows": ([VP, VP, I, VP, VP, VP, VP, I, I, I, I, I, I, I, VP, VP, VP, VP, VP], I),
     "q27x_attn_rows_noalloc": ([VP, VP, I, VP, VP, VP, VP, I, I, I, I, I, I, I, VP, VP, VP, VP], I),
+    "q27x_paged_prep_rows": ([VP, I, VP, VP, VP, VP, I, I, VP, I, I, VP, VP, VP, I, I, F, I, VP], I),
+    "q27x_paged_attn_work_bytes": ([I, I, I, I, I], SZ),
+    "q27x_paged_attn_rows": ([VP, VP, I, VP, I, I, I, I, I, VP, VP, VP, VP, VP, I, VP], I),
+    "q27x_paged_evict_work_bytes": ([I, I], SZ),
+    "q27x_paged_evict": ([VP, VP, I, VP, I, F, VP, VP, I, VP, I, I, I, I, VP, VP, VP], I),
     "q27x_argmax_rows": ([VP, I, I, I, VP, VP, VP], I),
     "q27x_accept": ([VP, VP, I, VP, VP, VP], I),
     "q27x_math_test": ([VP, VP, I, I, VP], I),
