@@ -2,6 +2,8 @@
 // several axes, append) and attention of those rows over the pages.
 #include <math.h>
 
+#include <type_traits>
+
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -224,6 +226,7 @@ static int launch_prep(const PrepArgs& a, hipStream_t s) {
 // of two of the group's largest (undone in fp32), weights (at most 1) are rounded to fp16: 2^-11 each, below the bf16
 // output's 2^-8. bf16 pages: values exact, weights as two bf16 terms (2^-16).
 constexpr int kPSplit = 256;
+constexpr int kCUs = 256;             // compute units of an MI355X
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -299,8 +302,46 @@ __device__ __forceinline__ SeqOf seq_of(const PAttnArgs& a, int b) {
     return q;
 }
 
+__device__ __forceinline__ int splits_of(const SeqOf& q) {
+    return q.nr <= 0 ? 0 : q.len <= kPSplit ? 1 : (q.len + kPSplit - 1) / kPSplit;
+}
+// The call's (sequence, split) pairs in order, without those that are empty, 64 sequences at a time: lane l holds the running
+// count up to sequence base + l. A wave walks them forwards only.
+struct Items {
+    int base, before, upto;                          // sequences and pairs before these 64; upto: this lane's running count
+    __device__ __forceinline__ void load(const PAttnArgs& a, int b0, int n0) {
+        base = b0;
+        before = n0;
+        const int b = b0 + (int)(threadIdx.x & 63);
+        int x = b < a.kv.n_seq ? splits_of(seq_of(a, b)) : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int y = __shfl_up(x, o, 64);
+            x += (int)(threadIdx.x & 63) >= o ? y : 0;
+        }
+        upto = n0 + x;
+    }
+    // pair `item` (not smaller than the last one asked for): false behind the last
+    __device__ __forceinline__ bool find(const PAttnArgs& a, int item, int& b, int& sp) {
+        int last = __builtin_amdgcn_readlane(upto, 63);
+        while (item >= last) {
+            if (base + 64 >= a.kv.n_seq) return false;
+            load(a, base + 64, last);
+            last = __builtin_amdgcn_readlane(upto, 63);
+        }
+        const int k = __popcll(__ballot(upto <= item));
+        b = base + k;
+        sp = item - (k ? __builtin_amdgcn_readlane(upto, k - 1) : before);
+        return true;
+    }
+};
+
+// blocks of a compute unit, and the registers that leaves a lane (512 / it)
 template <int HD, int G, int RT>
-__global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
+struct AttnOcc { static constexpr int n = HD == 128 ? (RT == 1 && G ? 4 : 2) : RT == 1 ? 2 : 1; };
+
+template <int HD, int G, int RT>
+__global__ __launch_bounds__(256, (AttnOcc<HD, G, RT>::n)) void k_paged_attn(PAttnArgs a) {
     constexpr int E = HD / 16;                       // dims of V a lane holds
     constexpr int NM = HD / 32;                      // products of a score tile
     constexpr int NG = G ? HD / G : 1;               // scale groups of a head
@@ -308,29 +349,36 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
     constexpr int VW = G ? E / 4 : E / 2;            // registers of a key's V dims
     constexpr int CG = 8;                            // columns joined at a time
     constexpr float kNone = -__builtin_huge_valf();
-    const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
-    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const PagedArgs& kv = a.kv;
     const int grp = a.nq / kv.nkv;
-    // blocks b and b + 8 run on the same XCD: the kv heads of a split, which share its scales' lines, take one XCD
-    const int ncb = (a.max_rows * grp + 16 * RT - 1) / (16 * RT);
-    const unsigned id = blockIdx.x, per = (unsigned)(kv.nkv * ncb), sub = (id >> 3) % per, item = (id >> 3) / per * 8 + (id & 7);
-    const int b = (int)(item / (unsigned)a.ns), sp = (int)(item % (unsigned)a.ns);
-    const int kvh = (int)(sub % (unsigned)kv.nkv), cb = (int)(sub / (unsigned)kv.nkv);
-    if (b >= kv.n_seq) return;
-    const SeqOf q = seq_of(a, b);
-    const int ncol = min(q.nr * grp - cb * 16 * RT, 16 * RT);    // this block's columns
-    if (ncol <= 0 || (sp > 0 && sp * kPSplit >= q.len)) return;
-    const int k0 = sp * kPSplit + 64 * wv;
-
-    __shared__ int s_slot[4][64];
+    // Blocks j and j + 8 run on the same XCD: XCD x takes the pairs x, x + 8, .. with all their kv heads, which share the
+    // lines of the scales; its blocks take its (pair, head, columns) units in turn.
+    const int ncb = (a.max_rows * grp + 16 * RT - 1) / (16 * RT), per = kv.nkv * ncb;
+    __shared__ uint64_t s_off[4][64];
     __shared__ float s_m[4][16 * RT], s_l[4][16 * RT];
     __shared__ float s_o[4][CG][HD + 4];
+    Items items;
+    items.load(a, 0, 0);
+    const uint64_t width = (uint64_t)kv.nkv * HD;    // elements of a position
+    for (unsigned unit = blockIdx.x >> 3;; unit += gridDim.x >> 3) {
+    const int sub = (int)(unit % (unsigned)per);
+    int b, sp;
+    if (!items.find(a, (int)(unit / (unsigned)per * 8u + (blockIdx.x & 7u)), b, sp)) return;
+    const int kvh = sub % kv.nkv, cb = sub / kv.nkv;
+    const SeqOf q = seq_of(a, b);
+    const int ncol = min(q.nr * grp - cb * 16 * RT, 16 * RT);    // this unit's columns
+    if (ncol <= 0) continue;
+    const int k0 = sp * kPSplit + 64 * wv;
+    int t = threadIdx.x;                              // (opaque: what follows from it is not kept over the loop, which spills)
+    asm volatile("" : "+v"(t));
+    const int l = t & 63, c = l & 15, g = l >> 4;
+    __syncthreads();                                  // the unit before is read out of LDS
 
     // this wave's keys: lane l looks key k0 + l up
     const int my = k0 + l < q.len ? paged_slot(kv, b, k0 + l) : -1;
     const uint64_t valid = __ballot(my >= 0);
-    s_slot[wv][l] = my < 0 ? 0 : my;                  // (a key that is not there reads position 0 of the pool)
+    s_off[wv][l] = my < 0 ? 0 : (uint64_t)(unsigned)my * width;     // (a key that is not there reads position 0 of the pool)
     __builtin_amdgcn_wave_barrier();
 
     float m[RT], lsum[RT];
@@ -343,13 +391,13 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
         for (int e = 0; e < E; ++e) o[rt][e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if (valid) {
-        const size_t width = (size_t)kv.nkv * HD, hoff = (size_t)kvh * HD;
+        const uint64_t hoff = (uint64_t)kvh * HD;
         u32x4 kx[4][NM];                              // K: dims 32 i + 8 g .. of key 16 ti + c (int8: the low two words)
         uint32_t vx[4][4][VW];                        // V: dims E c .. of key 16 ti + 4 g + j
         float ksc[4][NS], vsc[4][NS];                 // scales of key 16 ti + 4 g + c % 4
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti) {
-            const size_t at = (size_t)s_slot[wv][16 * ti + c] * width + hoff;
+            const uint64_t at = s_off[wv][16 * ti + c] + hoff;
 #pragma unroll
             for (int i = 0; i < NM; ++i) {
                 if constexpr (G == 0) {
@@ -360,7 +408,7 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                 }
             }
             if constexpr (G != 0) {
-                const size_t srow = (size_t)s_slot[wv][16 * ti + 4 * g + (c & 3)] * (width / G) + hoff / G;
+                const uint64_t srow = (s_off[wv][16 * ti + 4 * g + (c & 3)] + hoff) / G;
 #pragma unroll
                 for (int u = 0; u < NS; ++u) {
                     ksc[ti][u] = kv.ks[srow + (NG >= 4 ? (c >> 2) + 4 * u : (c >> 2) % NG)];     // groups c / 4 + 4 u
@@ -368,17 +416,24 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                 }
             }
         }
+        typedef uint32_t vvec __attribute__((ext_vector_type(VW)));
+        auto v_at = [&](int k) __attribute__((always_inline)) {
+            const uint64_t at = s_off[wv][k] + hoff + E * c;
+            return *(const vvec*)(G == 0 ? (const char*)kv.v + 2 * at : (const char*)kv.v + at);
+        };
+        auto load_v = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int ti = 0; ti < 4; ++ti)
+            for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const size_t at = (size_t)s_slot[wv][16 * ti + 4 * g + j] * width + hoff + E * c;
-                const char* p = G == 0 ? (const char*)kv.v + 2 * at : (const char*)kv.v + at;
-                typedef uint32_t vvec __attribute__((ext_vector_type(VW)));
-                const vvec x = *(const vvec*)p;
+                for (int j = 0; j < 4; ++j) {
+                    const vvec x = v_at(16 * ti + 4 * g + j);
 #pragma unroll
-                for (int u = 0; u < VW; ++u) vx[ti][j][u] = x[u];
-            }
+                    for (int u = 0; u < VW; ++u) vx[ti][j][u] = x[u];
+                }
+        };
+        // (256-wide bf16 rows: K and V together are all of a lane's registers)
+        constexpr bool kLateV = G == 0 && HD == 256;
+        if constexpr (!kLateV) load_v();
         // the columns' queries: dims 32 i + 8 g .. + 7 of column c
         u32x4 qx[RT][NM];
         int last[RT];                                 // the last key that the column sees
@@ -403,6 +458,9 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
         float s[RT][4][4];
 #pragma unroll
         for (int ti = 0; ti < 4; ++ti) {
+            __builtin_amdgcn_sched_barrier(0);        // (tiles widened ahead of their products spill)
+            uint32_t low = g < 2 ? ~0u : 0u;           // (opaque: masked queries are not worth registers of their own)
+            if constexpr (G == 16) asm volatile("" : "+v"(low));
             f32x4 acc[RT];
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
@@ -428,9 +486,10 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                 constexpr int NH = G == 16 ? 2 : 1;
 #pragma unroll
                 for (int h = 0; h < NH; ++h) {
+                    if constexpr (NH == 2) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int rt = 0; rt < RT; ++rt) {
-                        const u32x4 qm = NH == 1 || (g >> 1) == h ? qx[rt][i] : u32x4{0, 0, 0, 0};
+                        const u32x4 qm = NH == 1 ? qx[rt][i] : qx[rt][i] & (h ? ~low : low);
                         acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ka, __builtin_bit_cast(bf16x8, qm), acc[rt], 0, 0, 0);
                     }
                     if constexpr (G != 0) {
@@ -455,21 +514,29 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                     for (int j = 0; j < 4; ++j) s[rt][ti][j] = acc[rt][j];
             }
         }
+        if constexpr (kLateV) load_v();
         // weights: e^(x - m) of the 64 keys, those that the row does not see 0
         const bool full = valid == ~0ull && k0 + 63 <= q.raw - q.n;
         uint32_t pw[RT][2][4], plo[RT][2][G == 0 ? 4 : 1];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
+            if (!full) {
+                const int see = last[rt] - k0 - 4 * g;    // keys 16 ti + j of this lane up to here
+#pragma unroll
+                for (int ti = 0; ti < 4; ++ti) {
+                    const uint32_t there = (uint32_t)(valid >> (16 * ti)) >> (4 * g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        s[rt][ti][j] = (16 * ti + j <= see && ((there >> j) & 1)) ? s[rt][ti][j] : kNone;
+                }
+            }
             float mx = kNone;
 #pragma unroll
             for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int k = 16 * ti + 4 * g + j;
-                    float x = s[rt][ti][j] * a.sl2e;
-                    if (!full && (k0 + k > last[rt] || !((valid >> k) & 1))) x = kNone;
-                    s[rt][ti][j] = x;
-                    mx = fmaxf(mx, x);
+                    s[rt][ti][j] *= a.sl2e;
+                    mx = fmaxf(mx, s[rt][ti][j]);
                 }
             mx = max_cols(mx);
             m[rt] = mx;
@@ -551,66 +618,94 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                 back[u] = __shfl(__uint_as_float((uint32_t)ex << 23), (l & 48) + 4 * g, 64);
             }
         }
-        auto pv = [&](uint64_t keys, int rt, f32x4 (&to)[E]) __attribute__((always_inline)) {
+        // V' of the given keys (others 0), both 32-key halves of a dim tile, into one product chain per column tile: added to
+        // o, or (single) to the columns that see the key
+        // the scale of this lane's dims at key j of the quad's four
+        auto key_scale = [&](const float (&v)[NS], int j) __attribute__((always_inline)) {
+            float x = quad_bcast(v[0], j);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                float vs8[8];
-                uint32_t keep[8];
+            for (int u = 1; u < NS; ++u) {
+                const float y = quad_bcast(v[u], j);  // (in every lane: a lane reads its neighbours')
+                x = (c & 3) >= u * (4 / NS) ? y : x;
+            }
+            return x;
+        };
+        auto pv = [&](uint64_t keys, auto single, int key) __attribute__((always_inline)) {
+            float vs[4][NS];
+            uint32_t keep[4] = {15, 15, 15, 15};
+            if constexpr (G != 0) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int ti = 2 * u + (j >> 2);
+                for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+                    for (int u = 0; u < NS; ++u) vs[ti][u] = vsc[ti][u] * fac[u];
+            }
+            if (keys != ~0ull) {
+#pragma unroll
+                for (int ti = 0; ti < 4; ++ti) {
+                    keep[ti] = (uint32_t)(keys >> (16 * ti)) >> (4 * g);
                     if constexpr (G != 0) {
-                        float sc[NS];
 #pragma unroll
-                        for (int v = 0; v < NS; ++v) sc[v] = quad_bcast(vsc[ti][v], j & 3);
-                        float x = sc[0] * fac[0];
-                        if constexpr (NS == 2) x = (c & 2) ? sc[1] * fac[1] : x;
-                        if constexpr (NS == 4) x = (c & 3) == 0 ? x : (c & 3) == 1 ? sc[1] * fac[1] : (c & 3) == 2 ? sc[2] * fac[2] : sc[3] * fac[3];
-                        vs8[j] = (keys >> (16 * ti + 4 * g + (j & 3))) & 1 ? x : 0.0f;
-                    } else {
-                        keep[j] = (keys >> (16 * ti + 4 * g + (j & 3))) & 1 ? 0xFFFFFFFFu : 0u;
+                        for (int u = 0; u < NS; ++u) vs[ti][u] = (keep[ti] >> (c & 3)) & 1 ? vs[ti][u] : 0.0f;
                     }
                 }
+                if constexpr (G == 0) {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
+                    for (int ti = 0; ti < 4; ++ti)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int u = 0; u < VW; ++u) vx[ti][j][u] = (keep[ti] >> j) & 1 ? vx[ti][j][u] : 0u;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                __builtin_amdgcn_sched_barrier(0);
+                f32x4 acc[RT];
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt] = single ? zero : o[rt][e];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
                     u32x4 va;
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         const int ti = 2 * u + (h >> 1), j = 2 * (h & 1);
                         if constexpr (G != 0) {
-                            va[h] = pack_f16(byte_f(vx[ti][j][e / 4], e & 3) * vs8[2 * h], byte_f(vx[ti][j + 1][e / 4], e & 3) * vs8[2 * h + 1]);
+                            va[h] = pack_f16(byte_f(vx[ti][j][e / 4], e & 3) * key_scale(vs[ti], j), byte_f(vx[ti][j + 1][e / 4], e & 3) * key_scale(vs[ti], j + 1));
                         } else {
-                            va[h] = __builtin_amdgcn_perm(vx[ti][j + 1][e / 2] & keep[2 * h + 1], vx[ti][j][e / 2] & keep[2 * h],
-                                                          (e & 1) ? 0x07060302u : 0x05040100u);
+                            va[h] = __builtin_amdgcn_perm(vx[ti][j + 1][e / 2], vx[ti][j][e / 2], (e & 1) ? 0x07060302u : 0x05040100u);
                         }
                     }
-                    const u32x4 pb = {pw[rt][u][0], pw[rt][u][1], pw[rt][u][2], pw[rt][u][3]};
-                    if constexpr (G != 0) {
-                        to[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, va), __builtin_bit_cast(f16x8, pb), to[e], 0, 0, 0);
-                    } else {
-                        const u32x4 pl = {plo[rt][u][0], plo[rt][u][1], plo[rt][u][2], plo[rt][u][3]};
-                        to[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb), to[e], 0, 0, 0);
-                        to[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pl), to[e], 0, 0, 0);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) {
+                        const u32x4 pb = {pw[rt][u][0], pw[rt][u][1], pw[rt][u][2], pw[rt][u][3]};
+                        if constexpr (G != 0) {
+                            acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, va), __builtin_bit_cast(f16x8, pb), acc[rt], 0, 0, 0);
+                        } else {
+                            const u32x4 pl = {plo[rt][u][0], plo[rt][u][1], plo[rt][u][2], plo[rt][u][3]};
+                            acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb), acc[rt], 0, 0, 0);
+                            acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pl), acc[rt], 0, 0, 0);
+                        }
                     }
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    if (!single) o[rt][e] = acc[rt];
+                    else if (key <= last[rt]) o[rt][e] = o[rt][e] + acc[rt];
                 }
             }
         };
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) pv(enter, rt, o[rt]);
+        pv(enter, std::false_type{}, 0);
         while (later) {
             const int k = __builtin_ctzll(later);
             later &= later - 1;
+            const vvec x = v_at(k);
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                f32x4 one[E];
+            for (int ti = 0; ti < 4; ++ti)
 #pragma unroll
-                for (int e = 0; e < E; ++e) one[e] = zero;
-                pv(1ull << k, rt, one);
-                if (k0 + k <= last[rt]) {
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int e = 0; e < E; ++e) o[rt][e] = o[rt][e] + one[e];
-                }
-            }
+                    for (int u = 0; u < VW; ++u) vx[ti][j][u] = k == 16 * ti + 4 * g + j ? x[u] : 0u;
+            pv(1ull << k, std::true_type{}, k0 + k);
         }
         if constexpr (G != 0) {
 #pragma unroll
@@ -664,6 +759,7 @@ __global__ __launch_bounds__(256) void k_paged_attn(PAttnArgs a) {
                 if (a.w && d < 4) a.pm64[(at * a.ns + sp) * 4 + d] = s_m[d][col];
             }
         }
+    }
     }
 }
 
@@ -730,16 +826,19 @@ static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weight
     return w;
 }
 
-template <int HD, int G>
-static int launch_split(const PAttnArgs& a, hipStream_t s) {
-    const int cols = a.max_rows * (a.nq / a.kv.nkv), rt = cols <= 16 ? 1 : 2;
-    const long long items = ((long long)a.kv.n_seq * a.ns + 7) / 8 * 8;
-    const long long blocks = items * a.kv.nkv * ((cols + 16 * rt - 1) / (16 * rt));
-    if (blocks > 0x7fffffffLL) { set_error("q27x_paged_attn_rows: %lld blocks", blocks); return Q27X_E_RANGE; }
-    if (rt == 1) hipLaunchKernelGGL((k_paged_attn<HD, G, 1>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_paged_attn<HD, G, 2>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+template <int HD, int G, int RT>
+static int launch_split_rt(const PAttnArgs& a, hipStream_t s) {
+    // as many blocks as fit at once, or fewer units: those of max_len keys in every sequence, in eights (one per XCD)
+    const int ncb = (a.max_rows * (a.nq / a.kv.nkv) + 16 * RT - 1) / (16 * RT);
+    const long long units = ((long long)a.kv.n_seq * a.ns + 7) / 8 * a.kv.nkv * ncb;
+    const long long most = (long long)kCUs / 8 * AttnOcc<HD, G, RT>::n;
+    hipLaunchKernelGGL((k_paged_attn<HD, G, RT>), dim3((unsigned)(8 * (units < most ? units : most))), dim3(256), 0, s, a);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
+}
+template <int HD, int G>
+static int launch_split(const PAttnArgs& a, hipStream_t s) {
+    return a.max_rows * (a.nq / a.kv.nkv) <= 16 ? launch_split_rt<HD, G, 1>(a, s) : launch_split_rt<HD, G, 2>(a, s);
 }
 static int launch_paged_attn(const PAttnArgs& a, hipStream_t s) {
     int rc;
