@@ -763,53 +763,139 @@ __global__ __launch_bounds__(256, (AttnOcc<HD, G, RT>::n)) void k_paged_attn(PAt
     }
 }
 
-// The splits of a (row, head) in split order; thread = dim. A sequence of one split was finished above: with weights, only
-// its maximum and sum are noted.
-template <int HD>
-__global__ __launch_bounds__(HD) void k_paged_combine(PAttnArgs a) {
-    const int head = blockIdx.x, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, d = threadIdx.x;
+// The splits of a (row, head) joined. Split s belongs to class s % 16; a class is added up in split order, the classes as
+// ((0 + 1) + (2 + 3)) and so on by fours, then the four fours in order: one order for both forms. X lanes hold 4 X dims of
+// a head, so wave w's lanes have 64 / X of its classes 4 w .. 4 w + 3 side by side and X / 16 each in a row. X = 16: a block
+// joins 64 dims with every class in lanes of its own, for few (row, head) pairs (24 heads of 126 splits: 4.8 us, 43 with one
+// thread per dim). X = hd/4: a block joins a head, fewer blocks of more work for many (48 rows of 24 heads and 17
+// splits: 20.8 us with X = 16). A thread's first eight splits are requested before the maximum is known.
+// A sequence of one split was finished above: with weights, only its maximum and sum are noted.
+template <int X>
+__global__ __launch_bounds__(256) void k_paged_combine(PAttnArgs a) {
+    constexpr int NA = X / 16, B = 8 / NA;            // classes of a lane, splits of each requested at a time
+    const int hd = a.kv.hd, parts = hd / (4 * X);
+    const int head = blockIdx.x / parts, d0 = (blockIdx.x % parts) * 4 * X, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows;
+    const int t = threadIdx.x, x = t % X, y = 4 * (t >> 6) + (t & 63) / X * NA;      // the lane's first class
     const SeqOf q = seq_of(a, b);
     if (i >= q.nr) return;
-    const int ns = q.len > 0 ? (q.len + kPSplit - 1) / kPSplit : 1;
-    if (ns == 1 && !a.w) return;
+    const int ns = splits_of(q);
+    if (ns == 1 && !(a.w && d0 == 0)) return;
     const size_t row = (size_t)(q.first + i), at = row * a.nq + head;
     const float* pm = a.pm + at * a.ns;
     const float* pl = a.pl + at * a.ns;
-    float M = -__builtin_huge_valf();
-    for (int s = d & 63; s < ns; s += 64) M = fmaxf(M, pm[s]);
+    const f32x4* po = (const f32x4*)(a.po + at * a.ns * hd + d0) + x;
+    __shared__ float s_red[4], s_l[4];
+    __shared__ float s_sum[4][4 * X];
+    f32x4 ov[B][NA];
+    float mv[B][NA], lv[B][NA], M = -__builtin_huge_valf();
+    auto batch = [&](int s0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) {
+                const int s = s0 + 16 * u + k;
+                mv[u][k] = s < ns ? pm[s] : -__builtin_huge_valf();
+                lv[u][k] = s < ns ? pl[s] : 0.0f;
+                ov[u][k] = s < ns && ns > 1 ? po[(size_t)s * (hd >> 2)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            }
+    };
+    batch(y);
+#pragma unroll
+    for (int u = 0; u < B; ++u)
+#pragma unroll
+        for (int k = 0; k < NA; ++k) M = fmaxf(M, mv[u][k]);
+    for (int s = 16 * B + t; s < ns; s += 256) M = fmaxf(M, pm[s]);
     M = max_xor(M, 64);
-    float L = 0.0f, o = 0.0f;
-    for (int s = 0; s < ns; ++s) {
-        const float f = weight_of(pm[s], M);
-        L = __builtin_fmaf(pl[s], f, L);
-        if (ns > 1) o = __builtin_fmaf(a.po[(at * a.ns + s) * HD + d], f, o);
+    if ((t & 63) == 0) s_red[t >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+    float L[NA] = {};
+    f32x4 o[NA] = {};
+    for (int s0 = y;; ) {
+#pragma unroll
+        for (int u = 0; u < B; ++u)
+#pragma unroll
+            for (int k = 0; k < NA; ++k) {
+                const float f = weight_of(mv[u][k], M);
+                L[k] = __builtin_fmaf(lv[u][k], f, L[k]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[k][e] = __builtin_fmaf(ov[u][k][e], f, o[k][e]);
+            }
+        s0 += 16 * B;
+        if (s0 - y >= ns) break;
+        batch(s0);
     }
-    if (ns > 1) put_out(a, HD, row, head, d, o, L);
-    if (a.w && d == 0) {
+#pragma unroll
+    for (int k = 1; k < NA; k *= 2)
+#pragma unroll
+        for (int n = 0; n < NA; n += 2 * k) {
+            L[n] = L[n] + L[n + k];
+            o[n] = o[n] + o[n + k];
+        }
+    if constexpr (X == 16) {
+        L[0] = L[0] + xor16(L[0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][e] = o[0][e] + xor16(o[0][e]);
+    }
+    if constexpr (X <= 32) {
+        L[0] = L[0] + xor32(L[0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[0][e] = o[0][e] + xor32(o[0][e]);
+    }
+    if ((t & 63) < X) {
+        *(f32x4*)&s_sum[t >> 6][4 * x] = o[0];
+        if (x == 0) s_l[t >> 6] = L[0];
+    }
+    __syncthreads();
+    if (t >= 4 * X) return;
+    const float l = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
+    if (ns > 1) put_out(a, hd, row, head, d0 + t, ((s_sum[0][t] + s_sum[1][t]) + s_sum[2][t]) + s_sum[3][t], l);
+    if (a.w && d0 == 0 && t == 0) {
         a.fin[2 * at] = M;
-        a.fin[2 * at + 1] = L;
+        a.fin[2 * at + 1] = l;
     }
 }
 
 // The weight that each key got from a row, summed over the query heads in order: w[row][key] = sum over h of
-// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of 64-key chunks. Keys up to the sequence's length are written (0
-// where the row does not see them), nothing behind.
+// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of 64-key chunks: one factor per (head, chunk), made first. Keys
+// up to the sequence's length are written (0 where the row does not see them), nothing behind. Bound by the 4 nq bytes
+// per key that it reads.
+constexpr int kWHeads = 64;
 __global__ __launch_bounds__(256) void k_paged_weights(PAttnArgs a) {
     const int sp = blockIdx.x, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, t = threadIdx.x;
     const SeqOf q = seq_of(a, b);
     const int key = sp * kPSplit + t;
-    if (i >= q.nr || key >= min(q.raw, a.max_len)) return;
-    const size_t row = (size_t)(q.first + i);
+    if (i >= q.nr || sp * kPSplit >= min(q.raw, a.max_len)) return;
+    const size_t at = (size_t)(q.first + i) * a.nq;
+    const bool live = sp * kPSplit < q.len;           // (behind the table's end nothing was split)
+    __shared__ float2 s_f[kWHeads][4];                // a chunk's factor, and what its sums are multiplied by where it has none
     float w = 0.0f;
-    for (int h = 0; h < a.nq && key < q.len; ++h) {
-        const size_t at = row * a.nq + h;
-        const float m = a.pm64[(at * a.ns + sp) * 4 + (t >> 6)], M = a.fin[2 * at], L = a.fin[2 * at + 1];
-        // (a chunk without a key that is there has no weights written; its share is 0, or not a number with the row's sum)
-        const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
-        w = __builtin_fmaf(m == -__builtin_huge_valf() ? 1.0f : a.pp[(at * a.ns + sp) * kPSplit + t], f, w);
+    for (int h0 = 0; h0 < a.nq && live; h0 += kWHeads) {
+        const int nh = min(kWHeads, a.nq - h0);
+        __syncthreads();
+        if (t < 4 * nh) {
+            const size_t r = at + h0 + (t >> 2);
+            const float m = a.pm64[(r * a.ns + sp) * 4 + (t & 3)], M = a.fin[2 * r], L = a.fin[2 * r + 1];
+            // (a chunk without a key that is there has no weights written: its share is 0, or not a number with the row's sum)
+            const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
+            s_f[t >> 2][t & 3] = make_float2(f, m == -__builtin_huge_valf() || f != f ? f : 0.0f);
+        }
+        __syncthreads();
+        const float* pp = a.pp + ((at + h0) * a.ns + sp) * kPSplit + t;
+        const size_t step = (size_t)a.ns * kPSplit;
+        for (int h = 0; h < nh; h += 8) {
+            float v[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) v[u] = h + u < nh ? pp[(h + u) * step] : 0.0f;
+#pragma unroll
+            for (int u = 0; u < 8; ++u)
+                if (h + u < nh) {
+                    const float2 f = s_f[h + u][t >> 6];
+                    w = f.x == 0.0f || f.x != f.x ? w + f.y : __builtin_fmaf(v[u], f.x, w);
+                }
+        }
     }
-    if (key > q.raw - q.n + i) w = 0.0f;
-    a.w[row * a.w_stride + key] = w;
+    if (key < min(q.raw, a.max_len)) a.w[(size_t)(q.first + i) * a.w_stride + key] = key > q.raw - q.n + i ? 0.0f : w;
 }
 
 struct WorkLayout { size_t po, pp, pm, pl, pm64, fin, total; };
@@ -853,12 +939,13 @@ static int launch_paged_attn(const PAttnArgs& a, hipStream_t s) {
         default: rc = launch_split<256, 64>(a, s); break;
     }
     if (rc || (a.ns == 1 && !a.w)) return rc;
-    const dim3 rows((unsigned)a.nq, (unsigned)(a.kv.n_seq * a.max_rows));
-    if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_combine<128>, rows, dim3(128), 0, s, a);
-    else hipLaunchKernelGGL(k_paged_combine<256>, rows, dim3(256), 0, s, a);
+    const unsigned rows = (unsigned)(a.kv.n_seq * a.max_rows);
+    if ((long long)rows * a.nq < 2 * kCUs) hipLaunchKernelGGL(k_paged_combine<16>, dim3((unsigned)(a.nq * (a.kv.hd / 64)), rows), dim3(256), 0, s, a);
+    else if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_combine<32>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(k_paged_combine<64>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
     Q27X_HIP(hipGetLastError());
     if (a.w) {
-        hipLaunchKernelGGL(k_paged_weights, dim3((unsigned)a.ns, rows.y), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(k_paged_weights, dim3((unsigned)a.ns, rows), dim3(256), 0, s, a);
         Q27X_HIP(hipGetLastError());
     }
     return Q27X_OK;
