@@ -109,6 +109,13 @@ __device__ __forceinline__ void lds_dma16(const void* g, uint32_t lds) {
                  "global_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
                  : "=&s"(save) : "s"(lds), "v"(g) : "memory");
 }
+// lds_dma16 of data that is read once (not kept in the caches)
+__device__ __forceinline__ void lds_dma16_nt(const void* g, uint32_t lds) {
+    uint32_t save;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\t"
+                 "global_load_lds_dwordx4 %2, off nt\n\ts_mov_b32 m0, %0"
+                 : "=&s"(save) : "s"(lds), "v"(g) : "memory");
+}
 
 // lds_dma16 from a wave-uniform base and a 32-bit offset per lane
 __device__ __forceinline__ void lds_dma16_at(const void* base, uint32_t off, uint32_t lds) {

@@ -372,6 +372,30 @@ def test_attention_bits_do_not_depend_on_the_batch(gpu, group):
             assert np.array_equal(one[3][0, :cache.lens[0]], w[r, :cache.lens[0]]), (b, i)
 
 
+@pytest.mark.parametrize("geom,group", [("4x1x128", 32), ("6x1x256", 32), ("4x1x128", 0), ("6x1x256", 16)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_attention_bits_of_a_large_batch(gpu, geom, group, rows):
+    """A batch of enough keys and rows for the other forms of the kernels: the bits of each sequence alone."""
+    rng = np.random.default_rng(16)
+    nq, nkv, hd = GEOMS[geom]
+    n = 100
+    lens = rng.integers(rows, 700, n)
+    lens[:4] = [rows, 256, 257, 1500]
+    cache = Cache(rng, lens, [rows] * n, nkv, hd, group, page=32)
+    q, gate = queries(rng, n * rows, nq, hd)
+    # max_len far above the lengths counts as much work: whole splits for a wave, a block per head in the join
+    out, xq, xs, w = run_attn(gpu, cache, q, gate, nq, max_len=256 * (1800 * 8 // n + 1))
+    table, start = cache.table, cache.row_start
+    for b in (0, 1, 2, 3, 50, 99):
+        cache.lens, cache.counts = lens[b:b + 1].astype(np.int32), np.array([rows], np.int32)
+        cache.row_start, cache.table = np.array([0, rows], np.int32), table[b:b + 1].copy()
+        r = slice(start[b], start[b] + rows)
+        one = run_attn(gpu, cache, q[r], gate[r], nq)
+        assert np.array_equal(one[0], out[r]) and np.array_equal(one[1], xq[r]) and np.array_equal(one[2], xs[r]), b
+        assert np.array_equal(one[3][:, :lens[b]], w[r, :lens[b]]), b
+        check_attn(cache, one, q[r], gate[r], nq)
+
+
 def test_attention_like_the_contiguous_entry(gpu):
     """q27x_attn_rows over the same cache, its pages counting up: both within their roundings of the float64 form."""
     X, rng = gpu, np.random.default_rng(14)
