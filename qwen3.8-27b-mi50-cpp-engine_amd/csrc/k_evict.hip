@@ -5,6 +5,8 @@
 // in all, ties to the lowest index. Attention does not care for the order of the keys, so nothing is shifted: the keys
 // behind `budget` that stay move into the places of those before it that go, both in ascending order, as many bytes as
 // can be. Source and target positions are disjoint, so the moves need no staging.
+#include <mutex>
+
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -18,12 +20,15 @@ struct EvictArgs {
     uint32_t* rank;                 // [n_seq][max_len] the keys' order: larger stays
     int2* pairs;                    // [n_seq][max_len / 2 + 1] (from, to)
     int32_t* npairs;                // [n_seq]
+    int fused;                      // the kernel that picks also moves
 };
 constexpr int kEvThreads = 1024, kEvWaves = kEvThreads / 64;
 
-// Floats as unsigned numbers of the same order: -0 as 0, what is not a number below all others; the newest above all.
+// Floats as unsigned numbers of the same order: -0 as 0, what is not a number below all others; the newest above all, and
+// 0 for a place without a key.
+constexpr uint32_t kNewest = 0xFFFFFFFFu, kNaN = 1u;
 __device__ __forceinline__ uint32_t rank_of(float x) {
-    if (x != x) return 0u;
+    if (x != x) return kNaN;
     const uint32_t u = __float_as_uint(x == 0.0f ? 0.0f : x);
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
@@ -73,7 +78,7 @@ __global__ __launch_bounds__(kEvThreads) void k_evict_pick(EvictArgs a) {
         int o = total + i - known;
         if (i < known) o = ord[i];
         else ord[i] = o;
-        if (over) rank[i] = o >= fresh ? 0xFFFFFFFFu : rank_of(x);
+        if (over) rank[i] = o >= fresh ? kNewest : rank_of(x);
     }
     __syncthreads();                                  // (known and total are read by every thread before they change)
     if (t == 0) {
@@ -148,29 +153,378 @@ __global__ __launch_bounds__(kEvThreads) void k_evict_pick(EvictArgs a) {
     }
 }
 
-// One wave a moved position: its key, its value and their scales.
-__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
-    const int b = blockIdx.y, l = threadIdx.x & 63;
-    const int i = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (i >= a.npairs[b]) return;
-    const int2 p = a.pairs[(size_t)b * (a.max_len / 2 + 1) + i];
-    const int from = paged_slot(a.kv, b, p.x), to = paged_slot(a.kv, b, p.y);
-    if (from < 0 || to < 0) return;
-    const size_t width = (size_t)a.kv.nkv * a.kv.hd * (a.kv.G ? 1 : 2);     // bytes, whole 128s
-    for (size_t x = 16 * (size_t)l; x < width; x += 1024) {
-        const uint4 k = *(const uint4*)((const char*)a.kv.k + (size_t)from * width + x);
-        const uint4 v = *(const uint4*)((const char*)a.kv.v + (size_t)from * width + x);
-        *(uint4*)((char*)a.kv.k + (size_t)to * width + x) = k;
-        *(uint4*)((char*)a.kv.v + (size_t)to * width + x) = v;
+// The sums of up to kTiles x 1024 keys of a sequence by one block, the keys' ranks in registers (thread t: keys t, t + 1024
+// ..), read once. The budget-th largest rank: a histogram of 2048 equal steps of the range between the smallest and the
+// largest, then of the step that holds it, three at most -- digits of the rank itself meet in a few counters, as sums share
+// their exponents, and LDS adds to one address come one after another (4097 keys: 53 us with eight bits a pass).
+// Bound by latency: loads, then about ten barriers a pass; with one block a sequence, not by memory.
+constexpr int kTiles = 32, kBins = 2048;
+
+// Exclusive prefix sum over the block's first n <= 1024 values, one a thread; the sum of all in `sum`.
+__device__ __forceinline__ uint32_t scan_block(uint32_t x, uint32_t* red, uint32_t& sum) {
+    const int l = threadIdx.x & 63, wv = threadIdx.x >> 6;
+    uint32_t y = x;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const uint32_t z = __shfl_up(y, o, 64);
+        y += l >= o ? z : 0u;
     }
-    if (a.kv.G) {
-        const int ng = a.kv.nkv * (a.kv.hd / a.kv.G);
-        for (int x = l; x < ng; x += 64) {
-            const float k = a.kv.ks[(size_t)from * ng + x], v = a.kv.vs[(size_t)from * ng + x];
-            a.kv.ks[(size_t)to * ng + x] = k;
-            a.kv.vs[(size_t)to * ng + x] = v;
+    __syncthreads();
+    if (l == 63) red[wv] = y;
+    __syncthreads();
+    uint32_t before = 0;
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < kEvWaves; ++i) {
+        const uint32_t z = red[i];
+        before += i < wv ? z : 0u;
+        sum += z;
+    }
+    return before + y - x;
+}
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// Moved positions by one wave: their keys, values and scales.
+template <int U>
+__device__ __forceinline__ void move_rows(const PagedArgs& kv, int b, const int2 (&p)[U], int n) {
+    const int l = threadIdx.x & 63;
+    const size_t width = (size_t)kv.nkv * kv.hd * (kv.G ? 1 : 2);           // bytes, whole 128s
+    const int ng = kv.G ? kv.nkv * (kv.hd / kv.G) : 0;
+    int from[U], to[U];                               // (where there is nothing to move, position 0 is read and not stored)
+    bool is[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        from[u] = u < n ? paged_slot(kv, b, p[u].x) : -1;
+        to[u] = u < n ? paged_slot(kv, b, p[u].y) : -1;
+        is[u] = from[u] >= 0 && to[u] >= 0;
+        from[u] = is[u] ? from[u] : 0;
+    }
+    for (size_t x = 16 * (size_t)l; x < width; x += 1024) {
+        u32x4 k[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = *(const u32x4*)((const char*)kv.k + (size_t)from[u] * width + x);
+            v[u] = *(const u32x4*)((const char*)kv.v + (size_t)from[u] * width + x);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (is[u]) {
+                *(u32x4*)((char*)kv.k + (size_t)to[u] * width + x) = k[u];
+                *(u32x4*)((char*)kv.v + (size_t)to[u] * width + x) = v[u];
+            }
+    }
+    for (int x = l; x < ng; x += 64) {
+        float k[U], v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            k[u] = kv.ks[(size_t)from[u] * ng + x];
+            v[u] = kv.vs[(size_t)from[u] * ng + x];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (is[u]) {
+                kv.ks[(size_t)to[u] * ng + x] = k[u];
+                kv.vs[(size_t)to[u] * ng + x] = v[u];
+            }
+    }
+}
+
+// A bounded cache's steady state: as many keys go as a step brought, found one after another as the smallest rank left (of
+// equal ones the highest place). The keys behind budget that stay are at most as many; one wave pairs them with the
+// places that fall free. 4097 keys of which one goes: 18.7 us by the histograms below, 8 here.
+constexpr int kFew = 8;
+__device__ __forceinline__ void few_go(const EvictArgs& a, const uint32_t (&key)[kTiles], int len, int tiles, float* acc, int32_t* ord, int2* pairs) {
+    const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    __shared__ uint32_t s_key[2][kEvWaves], s_at[2][kEvWaves];
+    __shared__ int s_gone[kFew], s_hole[kFew];
+    __shared__ int2 s_pair[kFew];
+    const int budget = a.budget, go = len - budget;
+    uint32_t gone = 0;                                // bit r: this thread's key of tile r went
+    for (int k = 0; k < go; ++k) {
+        uint32_t best = 0xFFFFFFFFu, at = 0xFFFFFFFFu;    // at: 2^31 - 1 - place, so that the highest is the least
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+            if (r < tiles) {
+                const int i = r * kEvThreads + t;
+                const bool take = i < len && !((gone >> r) & 1) && key[r] <= best;
+                best = take ? key[r] : best;
+                at = take ? 0x7FFFFFFFu - (uint32_t)i : at;
+            }
+        const uint32_t wbest = min_xor64(best);
+        const uint32_t wat = min_xor64(best == wbest ? at : 0xFFFFFFFFu);
+        if (l == 0) { s_key[k & 1][wv] = wbest; s_at[k & 1][wv] = wat; }
+        __syncthreads();
+        uint32_t mk = 0xFFFFFFFFu, ma = 0xFFFFFFFFu;
+#pragma unroll
+        for (int w = 0; w < kEvWaves; ++w) {
+            const uint32_t x = s_key[k & 1][w], y = s_at[k & 1][w];
+            ma = x < mk ? y : x == mk ? min(ma, y) : ma;
+            mk = min(mk, x);
+        }
+        const int place = (int)(0x7FFFFFFFu - ma);
+        if ((place & (kEvThreads - 1)) == t) gone |= 1u << (place / kEvThreads);
+        if (t == 0) s_gone[k] = place;
+    }
+    __syncthreads();
+    int moves = 0;
+    if (wv == 0) {
+        const int mine = l < go ? s_gone[l] : 0x7FFFFFFF;      // lane l: the l-th that went, and the l-th place behind budget
+        int rank = 0;
+        bool went = false;
+        for (int k = 0; k < go; ++k) {
+            rank += s_gone[k] < mine ? 1 : 0;
+            went = went || s_gone[k] == budget + l;
+        }
+        const uint64_t movers = __ballot(l < go && !went);
+        if (l < go && mine < budget) s_hole[rank] = mine;
+        __builtin_amdgcn_wave_barrier();
+        if ((movers >> l) & 1) {
+            const int m = __popcll(movers & ((1ull << l) - 1)), from = budget + l, to = s_hole[m];
+            s_pair[m] = make_int2(from, to);
+            pairs[m] = make_int2(from, to);
+            acc[to] = acc[from];
+            ord[to] = ord[from];
+        }
+        moves = __popcll(movers);
+        if (l == 0) a.npairs[b] = moves;
+    }
+    if (a.fused) {
+        if (l == 0) s_key[0][wv] = (uint32_t)moves;
+        __syncthreads();
+        moves = (int)s_key[0][0];
+        for (int i = wv; i < moves; i += kEvWaves) {
+            const int2 p[1] = {s_pair[i]};
+            move_rows<1>(a.kv, b, p, 1);
         }
     }
+}
+
+__global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
+    const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t count[kTiles * kEvWaves];
+    __shared__ uint32_t red[kEvWaves], red2[3][kEvWaves];
+    __shared__ uint32_t s_bin, s_left, s_same;
+    extern __shared__ int holes[];                    // the places that fall free, in order
+    int first, n;
+    paged_rows(a.kv, b, first, n);
+    const long long cap = paged_cap(a.kv);
+    int len = min(a.kv.lens[b], a.max_len);
+    len = len < cap ? len : (int)cap;
+    len = len < 0 ? 0 : len;
+    int known = a.state[2 * b], total = a.state[2 * b + 1];
+    known = min(known < 0 ? 0 : known, len);
+    const int now = total + len - known;
+    int rows = a.w ? min(n, a.nrows - first) : 0;
+    if (a.n_acc) rows = min(rows, a.n_acc[b]);
+    float* acc = a.acc + (size_t)b * a.stride;
+    int32_t* ord = a.ord + (size_t)b * a.stride;
+    const bool over = len > a.high;
+    const int fresh = now - a.recent;                 // the first of the newest keys
+    const int budget = a.budget;
+    uint32_t key[kTiles];
+    // eight keys a thread at a time, their loads together
+#pragma unroll
+    for (int r0 = 0; r0 < kTiles; r0 += 8) {
+        if (r0 * kEvThreads < len) {
+            float x[8];
+            int o[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = (r0 + u) * kEvThreads + t, j = min(i, len - 1);
+                x[u] = acc[j];
+                o[u] = ord[j];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = (r0 + u) * kEvThreads + t;
+                x[u] = i < known ? x[u] * a.decay : 0.0f;
+                o[u] = i < known ? o[u] : total + i - known;
+            }
+            for (int r = 0; r < rows; ++r) {
+                const float* w = a.w + (size_t)(first + r) * a.w_stride;
+                float y[8];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) y[u] = w[min((r0 + u) * kEvThreads + t, len - 1)];
+#pragma unroll
+                for (int u = 0; u < 8; ++u) x[u] += y[u];
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = (r0 + u) * kEvThreads + t;
+                if (i < len) {
+                    acc[i] = x[u];
+                    if (i >= known) ord[i] = o[u];
+                }
+                key[r0 + u] = i < len ? (o[u] >= fresh ? kNewest : rank_of(x[u])) : 0u;
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) key[r0 + u] = 0u;
+        }
+    }
+    __syncthreads();                                  // (known and total are read by every thread before they change)
+    if (t == 0) {
+        const int left = over ? budget : len;
+        a.new_lens[b] = left;
+        a.state[2 * b] = left;
+        a.state[2 * b + 1] = now;
+        if (!over) a.npairs[b] = 0;
+    }
+    if (!over) return;
+    const int tiles = (len + kEvThreads - 1) / kEvThreads;
+    int2* pairs = a.pairs + (size_t)b * (a.max_len / 2 + 1);
+    if (len - budget <= kFew) {
+        few_go(a, key, len, tiles, acc, ord, pairs);
+        return;
+    }
+    // the newest, counted, and the range of the others
+    uint32_t lo = kNewest, hi = 0, fixed = 0;
+#pragma unroll
+    for (int r = 0; r < kTiles; ++r) {
+        if (r < tiles) {
+            const uint32_t x = key[r];
+            fixed += (uint32_t)__popcll(__ballot(x == kNewest));
+            if (x != 0 && x != kNewest) {
+                lo = min(lo, x);
+                hi = max(hi, x);
+            }
+        }
+    }
+    lo = min_xor64(lo);
+    hi = ~min_xor64(~hi);
+    if (l == 0) { red2[0][wv] = fixed; red2[1][wv] = lo; red2[2][wv] = hi; }
+    __syncthreads();
+    fixed = 0; lo = kNewest; hi = 0;
+#pragma unroll
+    for (int i = 0; i < kEvWaves; ++i) {
+        fixed += red2[0][i];
+        lo = min(lo, red2[1][i]);
+        hi = max(hi, red2[2][i]);
+    }
+    // top: the budget-th largest rank; left: how many of that rank stay; same: how many there are
+    uint32_t top = kNewest, left = (uint32_t)budget, same = fixed;
+    if (fixed < (uint32_t)budget) {
+        left = (uint32_t)budget - fixed;
+        uint32_t span = hi - lo;
+        for (;;) {
+            const int bits = span ? 32 - __builtin_clz(span) : 0, shift = bits > 11 ? bits - 11 : 0;
+            hist[t] = 0;
+            hist[t + kEvThreads] = 0;
+            __syncthreads();
+#pragma unroll
+            for (int r = 0; r < kTiles; ++r)
+                if (r < tiles) {
+                    const uint32_t x = key[r] - lo;
+                    if (x <= span && key[r] != kNewest && key[r] != 0) atomicAdd(&hist[x >> shift], 1u);
+                }
+            __syncthreads();
+            const uint32_t h1 = hist[kBins - 1 - 2 * t], h0 = hist[kBins - 2 - 2 * t];     // from the top
+            uint32_t sum;
+            const uint32_t before = scan_block(h1 + h0, red, sum);
+            if (before < left && left <= before + h1 + h0) {
+                const bool second = left > before + h1;
+                s_bin = (uint32_t)(kBins - 1 - 2 * t - (second ? 1 : 0));
+                s_left = left - before - (second ? h1 : 0);
+                s_same = second ? h0 : h1;
+            }
+            __syncthreads();
+            lo += s_bin << shift;
+            left = s_left;
+            same = s_same;
+            if (shift == 0) break;
+            span = (1u << shift) - 1;
+        }
+        top = lo;
+    }
+    // which keys stay: bit r of `stays`; of those of rank `top` the lowest places, if not all do
+    uint32_t stays = 0, sum = 0;
+    const uint64_t below = (1ull << l) - 1;
+    if (same == left) {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r) stays |= key[r] >= top ? 1u << r : 0u;
+    } else {
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+            if (r < tiles) {
+                const uint64_t eq = __ballot(key[r] == top);
+                if (l == 0) count[r * kEvWaves + wv] = (uint32_t)__popcll(eq);
+            }
+        __syncthreads();
+        const uint32_t c = t < tiles * kEvWaves ? count[t] : 0u;
+        const uint32_t before = scan_block(c, red, sum);
+        if (t < tiles * kEvWaves) count[t] = before;
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kTiles; ++r)
+            if (r < tiles) {
+                const uint64_t eq = __ballot(key[r] == top);
+                const bool in = key[r] > top || (key[r] == top && count[r * kEvWaves + wv] + (uint32_t)__popcll(eq & below) < left);
+                stays |= in ? 1u << r : 0u;
+            }
+        __syncthreads();
+    }
+    // the places before budget that fall free (low half) and the keys behind it that stay (high half), counted in order
+#pragma unroll
+    for (int r = 0; r < kTiles; ++r)
+        if (r < tiles) {
+            const int i = r * kEvThreads + t;
+            const bool in = (stays >> r) & 1;
+            const uint64_t hole = __ballot(!in && i < budget && i < len), mover = __ballot(in && i >= budget);
+            if (l == 0) count[r * kEvWaves + wv] = (uint32_t)__popcll(hole) | ((uint32_t)__popcll(mover) << 16);
+        }
+    __syncthreads();
+    const uint32_t c = t < tiles * kEvWaves ? count[t] : 0u;
+    const uint32_t before = scan_block(c, red, sum);
+    if (t < tiles * kEvWaves) count[t] = before;
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kTiles; ++r)
+        if (r < tiles) {
+            const int i = r * kEvThreads + t;
+            const bool is = !((stays >> r) & 1) && i < budget && i < len;
+            const uint64_t hole = __ballot(is);
+            if (is) holes[(count[r * kEvWaves + wv] & 0xFFFFu) + (uint32_t)__popcll(hole & below)] = i;
+        }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kTiles; ++r)
+        if (r < tiles) {
+            const int i = r * kEvThreads + t;
+            const bool is = ((stays >> r) & 1) && i >= budget;
+            const uint64_t mover = __ballot(is);
+            if (is) {
+                const uint32_t m = (count[r * kEvWaves + wv] >> 16) + (uint32_t)__popcll(mover & below);
+                const int to = holes[m];
+                pairs[m] = make_int2(i, to);
+                acc[to] = acc[i];
+                ord[to] = ord[i];
+            }
+        }
+    const int moves = (int)(sum & 0xFFFFu);
+    if (t == 0) a.npairs[b] = moves;
+    if (a.fused) {                                    // a few moves at most: no second launch
+        __syncthreads();
+        for (int i = wv; i < moves; i += kEvWaves) {
+            const int2 p[1] = {pairs[i]};
+            move_rows<1>(a.kv, b, p, 1);
+        }
+    }
+}
+
+// The moved positions of a sequence, kMoves a wave. Bound by memory.
+constexpr int kMoves = 4;
+__global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
+    const int b = blockIdx.y;
+    const int i = (blockIdx.x * 4 + (threadIdx.x >> 6)) * kMoves, n = a.npairs[b] - i;
+    if (n <= 0) return;
+    const int2* pairs = a.pairs + (size_t)b * (a.max_len / 2 + 1) + i;
+    int2 p[kMoves];
+#pragma unroll
+    for (int u = 0; u < kMoves; ++u) p[u] = pairs[u < n ? u : 0];
+    move_rows<kMoves>(a.kv, b, p, n);
 }
 
 struct EvictWork { size_t rank, pairs, npairs, total; };      // bytes
@@ -212,11 +566,21 @@ extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w
     a.pairs = (int2*)((char*)work + ew.pairs);
     a.rank = (uint32_t*)((char*)work + ew.rank);
     a.npairs = (int32_t*)((char*)work + ew.npairs);
-    hipLaunchKernelGGL(k_evict_pick, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), 0, (hipStream_t)s, a);
+    const int most = max_len > high ? min(budget, max_len - budget) : 0;       // moves of a sequence
+    if (max_len <= kTiles * kEvThreads) {
+        static std::once_flag attr;
+        static hipError_t attr_e = hipSuccess;
+        std::call_once(attr, [] { attr_e = hipFuncSetAttribute((const void*)k_evict, hipFuncAttributeMaxDynamicSharedMemorySize, kTiles * kEvThreads * 2); });
+        Q27X_HIP(attr_e);
+        a.fused = most <= kEvWaves;
+        hipLaunchKernelGGL(k_evict, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), (size_t)most * 4, (hipStream_t)s, a);
+    } else {
+        hipLaunchKernelGGL(k_evict_pick, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), 0, (hipStream_t)s, a);
+    }
     Q27X_HIP(hipGetLastError());
-    if (max_len > high) {
-        const int most = min(budget, max_len - budget);
-        hipLaunchKernelGGL(k_evict_move, dim3((unsigned)((most + 3) / 4), (unsigned)a.kv.n_seq), dim3(256), 0, (hipStream_t)s, a);
+    if (most > 0 && !a.fused) {
+        const unsigned per = 4 * kMoves;
+        hipLaunchKernelGGL(k_evict_move, dim3((unsigned)((most + per - 1) / per), (unsigned)a.kv.n_seq), dim3(256), 0, (hipStream_t)s, a);
         Q27X_HIP(hipGetLastError());
     }
     return Q27X_OK;

@@ -529,6 +529,21 @@ def test_evict_more_than_a_block(gpu):
     ev.compare(ev.expect([9001, 3, 4096, 3500], [w[b:b + 1] for b in range(4)], 1.0, 3999, 3001, 500))
 
 
+@pytest.mark.parametrize("len_", [1024, 1025, 32768, 40001])
+def test_evict_lengths_of_the_kernels(gpu, len_):
+    """The ends of what a block holds in registers, and past it; sums that are all equal, and spread over many exponents; a
+    budget of one key less, whose move needs no launch of its own, and of few."""
+    X, rng = gpu, np.random.default_rng(len_)
+    for budget, spread in ((len_ - 1, 0), (len_ - 1, 1), (len_ - 8, 0), (len_ - 8, 2), (len_ - 9, 0), (len_ - 20, 1), (17, 2)):
+        cache = Cache(rng, [len_, 20], [1, 1], 1, 128, 64, page=16)
+        cache.push(X)
+        ev = Evictor(X, cache, len_)
+        w = np.ones((2, len_), np.float32) if spread == 0 else rng.random((2, len_)).astype(np.float32) ** (1 if spread == 1 else 40)
+        dw = X.DevBuf(array=w)
+        ev.call(dw.ptr, len_, None, 2, 1.0, budget, budget, 5, len_)
+        ev.compare(ev.expect([len_, 20], [w[:1], w[1:]], 1.0, budget, budget, 5))
+
+
 def test_evict_sums_that_are_not_numbers(gpu):
     """NaN goes first, infinity stays, -0 and 0 are equal, negative sums are ordered; no weights at all leaves the sums."""
     X, rng = gpu, np.random.default_rng(22)
