@@ -40,9 +40,11 @@ int paged_args(const q27x_paged_kv_t* kv, const char* who, PagedArgs* out) {
 // (as they are) go to the row's position in the pages, int8 codes with a scale per group (s = max|v| / 127, code =
 // rint(v / s)) or bf16.
 //
-// Block = (row, 16 heads of q | k | v), 16 lanes a head: a lane holds HD/16 neighbouring dims, so a group's maximum and the
-// head's sum of squares are a few DPP steps and four heads share a wave's root and division. The row's angles are read
-// once per block into LDS; the partner dims of a turn come through LDS too, so rot can be any even number.
+// Wave = 4 heads of q | k | v of a row, 16 lanes a head: a lane holds HD/16 neighbouring dims, so a group's maximum and the
+// head's sum of squares are a few DPP steps and four heads share a wave's root and division. Waves are independent: each
+// reads its row's angles into its own LDS (a row's are 2 rot floats, from L1 after the first wave), and the partner dims of
+// a turn come through LDS too, so rot can be any even number. Bound by latency (row -> sequence -> page and position -> angle are
+// chains of loads), so the row's values are requested before anything else and both chains run beside the norm.
 struct PrepArgs {
     const uint16_t* qkv; int qkv_stride;
     const uint16_t* q_norm_w; const uint16_t* k_norm_w;
@@ -67,6 +69,12 @@ __device__ __forceinline__ void ld_bf16(const uint16_t* p, float (&v)[E]) {
         }
     }
 }
+// two floats as bf16 (to nearest even, by the hardware)
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    const bf16x2 v = {(__bf16)lo, (__bf16)hi};
+    return __builtin_bit_cast(uint32_t, v);
+}
 template <int E>
 __device__ __forceinline__ void st_bf16(uint16_t* p, const float (&v)[E]) {
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4), aligned(2)));
@@ -74,7 +82,7 @@ __device__ __forceinline__ void st_bf16(uint16_t* p, const float (&v)[E]) {
     for (int i = 0; i < E / 8; ++i) {
         u32x4 x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) x[j] = (uint32_t)f2bf(v[8 * i + 2 * j]) | ((uint32_t)f2bf(v[8 * i + 2 * j + 1]) << 16);
+        for (int j = 0; j < 4; ++j) x[j] = pack_bf16(v[8 * i + 2 * j], v[8 * i + 2 * j + 1]);
         *(u32x4*)(p + 8 * i) = x;
     }
 }
@@ -126,33 +134,47 @@ __device__ __forceinline__ void st_kv(const PagedArgs& a, void* pool, float* sca
 template <int HD, int G>
 __global__ __launch_bounds__(256) void k_paged_prep(PrepArgs a) {
     constexpr int E = HD / 16;
-    const int r = blockIdx.x, t = threadIdx.x, c = t & 15, slotw = t >> 4;
+    const int r = blockIdx.x, t = threadIdx.x, l = t & 63, c = t & 15, wv = t >> 6, slotw = t >> 4;
     const int half = a.rot >> 1;
-    __shared__ float cs[2][HD / 2];
-    __shared__ float ex[16][HD];
-    // the row's angles: thread t < rot takes the cosine (t < half) or sine of pair t % half
-    if (t < a.rot) {
-        const int f = t < half ? t : t - half;
-        const int axis = (a.axes[f >> 4] >> (2 * (f & 15))) & 3;
-        int p = a.pos[(size_t)axis * a.pos_stride + r];
-        p = p < 0 ? 0 : (p >= a.n_pos ? a.n_pos - 1 : p);
-        cs[t >= half][f] = (t < half ? a.rope_cos : a.rope_sin)[(size_t)p * half + f];
-    }
-    const int b = seq_of_row(a.kv, r);
-    if (b < 0) return;                               // (the same in every wave: a row behind the last sequence)
+    __shared__ __attribute__((aligned(16))) float s_cs[4][2][HD / 2];
+    __shared__ __attribute__((aligned(16))) float s_ex[16][HD];
     const int u = blockIdx.y * 16 + slotw;           // q heads, then k, then v
     const bool isq = u < a.nq, isk = !isq && u < a.nq + a.kv.nkv, isv = !isq && !isk && u < a.nq + 2 * a.kv.nkv;
     const int head = isq ? u : isk ? u - a.nq : u - a.nq - a.kv.nkv;
     const int qw = a.gate ? 2 * HD : HD;
-    float y[E];
-    if (isq || isk || isv) {
-        const uint16_t* src = a.qkv + (size_t)r * a.qkv_stride +
-                              (isq ? (size_t)head * qw : (size_t)a.nq * qw + ((size_t)(isv ? a.kv.nkv : 0) + head) * HD) + E * c;
-        ld_bf16<E>(src, y);
+    float y[E], w[E];
+    // (lanes past the last head read the first one's)
+    const uint16_t* src = a.qkv + (size_t)r * a.qkv_stride + E * c +
+                          (isq ? (size_t)head * qw : isk || isv ? (size_t)a.nq * qw + ((size_t)(isv ? a.kv.nkv : 0) + head) * HD : 0);
+    ld_bf16<E>(src, y);
+    ld_bf16<E>((isq ? a.q_norm_w : a.k_norm_w) + E * c, w);
+    // the row's angles: lane l takes the cosines, then the sines of pairs l, l + 64 ..
+    int p[HD / 128];
+#pragma unroll
+    for (int i = 0; i < HD / 128; ++i) {
+        const int f = l + 64 * i < half ? l + 64 * i : 0;
+        const int axis = (a.axes[f >> 4] >> (2 * (f & 15))) & 3;
+        p[i] = a.pos[(size_t)axis * a.pos_stride + r];
     }
+    const int b = seq_of_row(a.kv, r);
+    if (b < 0) return;                               // (a row behind the last sequence)
+    int slot = -1;
+    if (isk || isv) {
+        int first, n;
+        paged_rows(a.kv, b, first, n);
+        slot = paged_slot(a.kv, b, a.kv.lens[b] - n + (r - first));
+    }
+#pragma unroll
+    for (int i = 0; i < HD / 128; ++i) {
+        const int f = l + 64 * i;
+        if (f < half) {
+            const int q = p[i] < 0 ? 0 : (p[i] >= a.n_pos ? a.n_pos - 1 : p[i]);
+            s_cs[wv][0][f] = a.rope_cos[(size_t)q * half + f];
+            s_cs[wv][1][f] = a.rope_sin[(size_t)q * half + f];
+        }
+    }
+    const bool turns = (isq || isk) && E * c < a.rot;
     if (isq || isk) {
-        float w[E];
-        ld_bf16<E>((isq ? a.q_norm_w : a.k_norm_w) + E * c, w);
         float ss = 0.0f;
 #pragma unroll
         for (int e = 0; e < E; ++e) ss = __builtin_fmaf(y[e], y[e], ss);
@@ -160,29 +182,41 @@ __global__ __launch_bounds__(256) void k_paged_prep(PrepArgs a) {
         const float inv = rsqrt_cr(ss * (1.0f / (float)HD) + a.eps);
 #pragma unroll
         for (int e = 0; e < E; ++e) y[e] = y[e] * inv * (1.0f + w[e]);
+        if (turns) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) ex[slotw][E * c + e] = y[e];
-    }
-    __syncthreads();
-    if ((isq || isk) && E * c < a.rot) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int d = E * c + e;
-            if (d >= a.rot) break;
-            const int f = d < half ? d : d - half;
-            const float o = ex[slotw][d < half ? d + half : d - half];
-            y[e] = d < half ? y[e] * cs[0][f] - o * cs[1][f] : y[e] * cs[0][f] + o * cs[1][f];
+            for (int e = 0; e < E; ++e) s_ex[slotw][E * c + e] = y[e];
         }
     }
-    if (isq) {
-        st_bf16<E>(a.qh + ((size_t)r * a.nq + head) * HD + E * c, y);
-    } else if (isk || isv) {
-        int first, n;
-        paged_rows(a.kv, b, first, n);
-        const int slot = paged_slot(a.kv, b, a.kv.lens[b] - n + (r - first));
-        if (slot < 0) return;
-        st_kv<HD, G>(a.kv, isk ? a.kv.k : a.kv.v, isk ? a.kv.ks : a.kv.vs, (size_t)slot, head, c, y);
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    if (turns && half % E == 0) {                    // a lane's dims are one half's, its partners and angles neighbours
+        const int d = E * c, f = d < half ? d : d - half;
+        const float4* o4 = (const float4*)&s_ex[slotw][d < half ? d + half : f];
+        const float4 *c4 = (const float4*)&s_cs[wv][0][f], *s4 = (const float4*)&s_cs[wv][1][f];
+        const float sign = d < half ? -1.0f : 1.0f;
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 o = o4[e / 4], k = c4[e / 4], n = s4[e / 4];
+            y[e] = __builtin_fmaf(sign * o.x, n.x, y[e] * k.x);
+            y[e + 1] = __builtin_fmaf(sign * o.y, n.y, y[e + 1] * k.y);
+            y[e + 2] = __builtin_fmaf(sign * o.z, n.z, y[e + 2] * k.z);
+            y[e + 3] = __builtin_fmaf(sign * o.w, n.w, y[e + 3] * k.w);
+        }
+    } else if (turns) {
+#pragma unroll 1
+        for (int e = 0; e < E; ++e) {
+            const int d = E * c + e, f = d < half ? d : d - half;
+            if (d < a.rot) {
+                const float o = s_ex[slotw][d < half ? d + half : f], k = s_cs[wv][1][f];
+                const float z = __builtin_fmaf(o, d < half ? -k : k, s_ex[slotw][d] * s_cs[wv][0][f]);
+#pragma unroll
+                for (int x = 0; x < E; ++x) y[x] = x == e ? z : y[x];
+            }
+        }
     }
+    if (isq) st_bf16<E>(a.qh + ((size_t)r * a.nq + head) * HD + E * c, y);
+    else if (slot >= 0) st_kv<HD, G>(a.kv, isk ? a.kv.k : a.kv.v, isk ? a.kv.ks : a.kv.vs, (size_t)slot, head, c, y);
 }
 
 static int launch_prep(const PrepArgs& a, hipStream_t s) {
