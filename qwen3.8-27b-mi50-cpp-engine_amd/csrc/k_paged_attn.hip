@@ -7,7 +7,7 @@
 // depends on its own keys alone, whatever else is in the batch. A wave takes a chunk for up to 16 RT columns, the pairs
 // of a row and a query head of its kv head: it has the chunk's scores before it needs their maximum, so the chunk has one
 // maximum and one exponential, and leaves (m, l, o). Chunks are joined in order, (m, l, o) <- (m', l e^(m - m') + l_c e^(m_c
-// - m'), ..), m' = max(m, m_c); k_paged_combine joins the splits. Two forms of the same arithmetic, the same bits:
+// - m'), ..), m' = max(m, m_c); k_paged_finish joins the splits. Two forms of the same arithmetic, the same bits:
 //   PAR: block = a split's chunks, one a wave, joined through LDS: as many waves as can be, for few keys.
 //   else: a wave walks a split's chunks and joins them in registers; waves are independent (no barrier), each with the
 //     next chunk's keys and values on their way, for many keys.
@@ -50,7 +50,7 @@ struct PAttnArgs {
     int nq, gate, max_len, max_rows, nrows, ns;      // ns: splits of max_len
     float sl2e;                                      // log2(e) / sqrt(hd)
     float* po; float* pm; float* pl;                 // splits' outputs [row][head][ns][hd], maxima and sums [row][head][ns]
-    float* pp; float* pmc; float* fin;               // with w: e^(x - m) [row][head][ns 256], chunk maxima [row][head][ns chunks], (M, l)
+    float* pp; float* pmc;                           // with w: e^(x - m) [row][head][ns 256], chunk maxima [row][head][ns chunks]
     uint16_t* out; int8_t* xq; float* xs;
     float* w; int w_stride;
     int par;                                         // the split kernel's form: PAR finishes sequences of one split
@@ -114,6 +114,19 @@ __device__ __forceinline__ SeqOf seq_of(const PAttnArgs& a, int b) {
     return q;
 }
 
+// The same of a sequence that all lanes ask for, by scalar loads.
+__device__ __forceinline__ SeqOf seq_of_all(const PAttnArgs& a, int b) {
+    SeqOf q;
+    q.first = a.kv.row_start ? ld_uniform(a.kv.row_start + b) : b;
+    q.n = a.kv.row_start ? ld_uniform(a.kv.row_start + b + 1) - q.first : 1;
+    if (q.n < 0 || q.first < 0) q.n = 0;
+    q.nr = min(min(q.n, a.max_rows), a.nrows - q.first);
+    q.raw = ld_uniform(a.kv.lens + b);
+    const long long cap = paged_cap(a.kv);
+    q.len = min(q.raw, a.max_len);
+    q.len = q.len < cap ? q.len : (int)cap;
+    return q;
+}
 __device__ __forceinline__ int splits_of(const SeqOf& q) {
     return q.nr <= 0 ? 0 : q.len <= kPSplit ? 1 : (q.len + kPSplit - 1) / kPSplit;
 }
@@ -161,8 +174,9 @@ struct AttnShape {
     static constexpr int kLds = kWaves * kWaveBytes + kJoinBytes;
     static constexpr int kXBytes = kWaves * CG * (HD + 4) * 4;                     // (the exchange lies over the keys)
     static_assert(!PAR || kXBytes <= kWaves * kWaveBytes, "exchange");
-    // waves of a SIMD that the registers are cut for
-static constexpr int kOcc = HD == 128 ? (RT == 1 ? (G || !PAR ? 3 : 2) : 2) : RT == 1 && G ? 2 : 1;
+    // Waves of a SIMD that the registers are cut for. More in flight is not more: 64 x 4000 keys on bf16 pages take 192 us
+    // with two waves a SIMD (not PAR), 207 with three; int8 PAR 89 with two, 85 with three, 98 with four.
+    static constexpr int kOcc = HD == 128 ? (RT == 1 && G && PAR ? 3 : 2) : RT == 1 && G ? 2 : 1;
 };
 
 // One wave's work on one chunk after another: the split's running (m, l, o) of its columns, and the chunk's K, V and scales.
@@ -269,8 +283,16 @@ struct Chunker {
 
     float s[RT][NT][4];
     // Scores of the chunk (times nothing yet). The caller has waited for K.
+    typedef uint32_t kvec __attribute__((ext_vector_type(G ? 2 : 4)));
+    // dims 32 i + 8 g .. of key r
+    __device__ __forceinline__ kvec k_at(int r, int i) const {
+        const char* row = keys + r * S::KB;
+        if constexpr (G == 0) return *(const kvec*)(row + 16 * place(r, 4 * i + g));
+        else return *(const kvec*)(row + 16 * place(r, 2 * i + (g >> 1)) + 8 * (g & 1));
+    }
     __device__ __forceinline__ void scores() {
         const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        kvec first = k_at(c, 0);
 #pragma unroll
         for (int ti = 0; ti < NT; ++ti) {
             __builtin_amdgcn_sched_barrier(0);        // (tiles widened ahead of their products spill)
@@ -280,7 +302,7 @@ struct Chunker {
             constexpr int NP = G == 16 ? 2 * NM : NM, PG = G == 0 ? NP : G == 16 ? 1 : G / 32;    // products, and of a group
             f32x4 acc[2][RT];
             u32x4 kb;
-            const char* row = keys + (16 * ti + c) * S::KB;
+            kvec x = first;
             auto scale = [&](int gr) __attribute__((always_inline)) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt)
@@ -295,14 +317,17 @@ struct Chunker {
                 const int i = G == 16 ? p / 2 : p, gr = p / PG;
                 if constexpr (G != 0) __builtin_amdgcn_sched_barrier(0);
                 if (G != 16 || p % 2 == 0) {
+                    // the operand after this one is requested first
+                    const kvec now = x;
+                    if (i + 1 < NM) x = k_at(16 * ti + c, i + 1);
+                    else if (ti + 1 < NT) first = k_at(16 * ti + 16 + c, 0);
                     if constexpr (G == 0) {
-                        kb = *(const u32x4*)(row + 16 * place(16 * ti + c, 4 * i + g));
+                        kb = now;
                     } else {
-                        const u32x2 x = *(const u32x2*)(row + 16 * place(16 * ti + c, 2 * i + (g >> 1)) + 8 * (g & 1));
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            kb[2 * h] = pack_bf(byte_f(x[h], 0), byte_f(x[h], 1));
-                            kb[2 * h + 1] = pack_bf(byte_f(x[h], 2), byte_f(x[h], 3));
+                            kb[2 * h] = pack_bf(byte_f(now[h], 0), byte_f(now[h], 1));
+                            kb[2 * h + 1] = pack_bf(byte_f(now[h], 2), byte_f(now[h], 3));
                         }
                     }
                 }
@@ -451,12 +476,23 @@ struct Chunker {
         for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
             for (int j = 0; j < 4; ++j) fb[rt][j] = G ? f2[rt] * back[j * NS / 4] : f2[rt];
+        // a dim tile's products are joined to o while the next tile's run
+        f32x4 acc[2][RT];
+        auto join = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = acc[e & 1][rt][j];
+                    if constexpr (!SINGLE) o[rt][e][j] = __builtin_fmaf(x, fb[rt][j], o[rt][e][j] * f1[rt]);
+                    else o[rt][e][j] = key <= last[rt] ? __builtin_fmaf(x, fb[rt][j], o[rt][e][j]) : o[rt][e][j];
+                }
+        };
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             __builtin_amdgcn_sched_barrier(0);
-            f32x4 acc[RT];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int rt = 0; rt < RT; ++rt) acc[e & 1][rt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 u32x4 va;
@@ -473,22 +509,17 @@ struct Chunker {
                 for (int rt = 0; rt < RT; ++rt) {
                     const u32x4 pb = {pw[rt][u][0], pw[rt][u][1], pw[rt][u][2], pw[rt][u][3]};
                     if constexpr (G != 0) {
-                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, va), __builtin_bit_cast(f16x8, pb), acc[rt], 0, 0, 0);
+                        acc[e & 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, va), __builtin_bit_cast(f16x8, pb), acc[e & 1][rt], 0, 0, 0);
                     } else {
                         const u32x4 pl = {plo[rt][u][0], plo[rt][u][1], plo[rt][u][2], plo[rt][u][3]};
-                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb), acc[rt], 0, 0, 0);
-                        acc[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pl), acc[rt], 0, 0, 0);
+                        acc[e & 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pb), acc[e & 1][rt], 0, 0, 0);
+                        acc[e & 1][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, pl), acc[e & 1][rt], 0, 0, 0);
                     }
                 }
             }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (!SINGLE) o[rt][e][j] = __builtin_fmaf(acc[rt][j], fb[rt][j], o[rt][e][j] * f1[rt]);
-                    else o[rt][e][j] = key <= last[rt] ? __builtin_fmaf(acc[rt][j], fb[rt][j], o[rt][e][j]) : o[rt][e][j];
-                }
+            if (e > 0) join(e - 1);
         }
+        join(E - 1);
     }
     // The chunk's values joined to o. Keys that are not there read something else, maybe not finite, and are left out. Keys
     // that only later rows see enter too (their weight is 0 in the rows before), unless they hold something that is not
@@ -576,7 +607,7 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShap
         int b, sp;
         if (!items.find(a, (int)(unit / (unsigned)per * 8u + (blockIdx.x & 7u)), b, sp)) return;
         const int kvh = sub % kv.nkv, col0 = sub / kv.nkv * 16 * RT;
-        const SeqOf q = seq_of(a, b);
+        const SeqOf q = seq_of_all(a, b);
         const int ncol = min(q.nr * grp - col0, 16 * RT);        // this unit's columns
         if (ncol <= 0) continue;
         int t;
@@ -719,16 +750,13 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShap
 // thread per dim). X = hd/4: a block joins a head, fewer blocks of more work for many (48 rows of 24 heads and 17
 // splits: 20.8 us with X = 16). A thread's first eight splits are requested before the maximum is known.
 template <int X>
-__global__ __launch_bounds__(256) void k_paged_combine(PAttnArgs a) {
+__device__ __forceinline__ void join_splits(const PAttnArgs& a, const SeqOf& q, int i) {
     constexpr int NA = X / 16, B = 8 / NA;            // classes of a lane, splits of each requested at a time
     const int hd = a.kv.hd, parts = hd / (4 * X);
-    const int head = blockIdx.x / parts, d0 = (blockIdx.x % parts) * 4 * X, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows;
+    const int head = blockIdx.x / parts, d0 = (blockIdx.x % parts) * 4 * X;
     const int t = threadIdx.x, x = t % X, y = 4 * (t >> 6) + (t & 63) / X * NA;      // the lane's first class
-    const SeqOf q = seq_of(a, b);
-    if (i >= q.nr) return;
     const int ns = splits_of(q);
-    const bool done = ns == 1 && a.par;               // (finished by the split kernel: with weights, its sum is noted)
-    if (done && !(a.w && d0 == 0)) return;
+    if (ns == 1 && a.par) return;                     // (finished by the split kernel)
     const size_t row = (size_t)(q.first + i), at = row * a.nq + head;
     const float* pm = a.pm + at * a.ns;
     const float* pl = a.pl + at * a.ns;
@@ -745,7 +773,7 @@ __global__ __launch_bounds__(256) void k_paged_combine(PAttnArgs a) {
                 const int s = s0 + 16 * u + k;
                 mv[u][k] = s < ns ? pm[s] : -__builtin_huge_valf();
                 lv[u][k] = s < ns ? pl[s] : 0.0f;
-                ov[u][k] = s < ns && !done ? po[(size_t)s * (hd >> 2)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                ov[u][k] = s < ns ? po[(size_t)s * (hd >> 2)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
     };
     batch(y);
@@ -798,57 +826,69 @@ __global__ __launch_bounds__(256) void k_paged_combine(PAttnArgs a) {
     __syncthreads();
     if (t >= 4 * X) return;
     const float l = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
-    if (!done) put_out(a, hd, row, head, d0 + t, ((s_sum[0][t] + s_sum[1][t]) + s_sum[2][t]) + s_sum[3][t], l);
-    if (a.w && d0 == 0 && t == 0) {
-        a.fin[2 * at] = M;
-        a.fin[2 * at + 1] = l;
-    }
+    put_out(a, hd, row, head, d0 + t, ((s_sum[0][t] + s_sum[1][t]) + s_sum[2][t]) + s_sum[3][t], l);
 }
 
-// The weight that each key got from a row, summed over the query heads in order: w[row][key] = sum over h of
-// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of its chunks: one factor per (head, chunk), made first. Keys
-// up to the sequence's length are written (0 where the row does not see them), nothing behind. Bound by the 4 nq bytes
-// per key that it reads.
-constexpr int kWHeads = 64;
-__global__ __launch_bounds__(256) void k_paged_weights(PAttnArgs a) {
-    const int sp = blockIdx.x, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, t = threadIdx.x;
-    const SeqOf q = seq_of(a, b);
-    const int key = sp * kPSplit + t;
-    if (i >= q.nr || sp * kPSplit >= min(q.raw, a.max_len)) return;
+// The weight that each key of split sp got from row i, summed over the query heads in order: w[row][key] = sum over h of
+// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of its chunks: one factor per (head, chunk), made first by 8 lanes a
+// head from the splits' maxima and sums. Keys up to the sequence's length are written (0 where the row does not see
+// them), nothing behind. Bound by the 4 nq bytes per key that it reads.
+constexpr int kWHeads = 32;
+__device__ __forceinline__ void key_weights(const PAttnArgs& a, const SeqOf& q, int i, int sp) {
+    const int t = threadIdx.x, key = sp * kPSplit + t;
+    if (sp * kPSplit >= min(q.raw, a.max_len)) return;
     const size_t at = (size_t)(q.first + i) * a.nq;
     const bool live = sp * kPSplit < q.len;           // (behind the table's end nothing was split)
-    constexpr int nc = kChunks, per = kChunk;
-    __shared__ float2 s_f[kWHeads][nc];                // a chunk's factor, and what its sums are multiplied by where it has none
+    const int ns = splits_of(q);
+    __shared__ float2 s_f[kWHeads][kChunks];          // a chunk's factor, and what is added where it has no weights
     float w = 0.0f;
     for (int h0 = 0; h0 < a.nq && live; h0 += kWHeads) {
         const int nh = min(kWHeads, a.nq - h0);
+        const int h = t >> 3, y = t & 7;
+        const size_t r = at + h0 + (h < nh ? h : 0);
+        const float* pm = a.pm + r * a.ns;
+        const float* pl = a.pl + r * a.ns;
+        const float m = a.pmc[(r * a.ns + sp) * kChunks + (y & 3)];
+        float M = -__builtin_huge_valf(), L = 0.0f;
+        for (int s = y; s < ns; s += 8) M = fmaxf(M, pm[s]);
+        M = max_xor(M, 8);
+        for (int s = y; s < ns; s += 8) L = __builtin_fmaf(pl[s], weight_of(pm[s], M), L);
+        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0xB1, 0xF, 0xF, false));
+        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0x4E, 0xF, 0xF, false));
+        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0x141, 0xF, 0xF, false));
+        // (a chunk without a key that is there has no weights written: its share is 0, or not a number with the row's sum)
+        const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
         __syncthreads();
-        for (int u = t; u < nc * nh; u += 256) {
-            const size_t r = at + h0 + u / nc;
-            const float m = a.pmc[(r * a.ns + sp) * nc + u % nc], M = a.fin[2 * r], L = a.fin[2 * r + 1];
-            // (a chunk without a key that is there has no weights written: its share is 0, or not a number with the row's sum)
-            const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
-            s_f[u / nc][u % nc] = make_float2(f, m == -__builtin_huge_valf() || f != f ? f : 0.0f);
-        }
+        if (y < kChunks && h < nh) s_f[h][y] = make_float2(f, m == -__builtin_huge_valf() || f != f ? f : 0.0f);
         __syncthreads();
         const float* pp = a.pp + ((at + h0) * a.ns + sp) * kPSplit + t;
         const size_t step = (size_t)a.ns * kPSplit;
-        for (int h = 0; h < nh; h += 8) {
+        for (int u0 = 0; u0 < nh; u0 += 8) {
             float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = h + u < nh ? pp[(h + u) * step] : 0.0f;
+            for (int u = 0; u < 8; ++u) v[u] = u0 + u < nh ? pp[(u0 + u) * step] : 0.0f;
 #pragma unroll
             for (int u = 0; u < 8; ++u)
-                if (h + u < nh) {
-                    const float2 f = s_f[h + u][t / per];
-                    w = f.x == 0.0f || f.x != f.x ? w + f.y : __builtin_fmaf(v[u], f.x, w);
+                if (u0 + u < nh) {
+                    const float2 k = s_f[u0 + u][t / kChunk];
+                    w = k.x == 0.0f || k.x != k.x ? w + k.y : __builtin_fmaf(v[u], k.x, w);
                 }
         }
     }
     if (key < min(q.raw, a.max_len)) a.w[(size_t)(q.first + i) * a.w_stride + key] = key > q.raw - q.n + i ? 0.0f : w;
 }
 
-struct WorkLayout { size_t po, pp, pm, pl, pmc, fin, total; };
+// What is left of a row after the splits: blocks x < nq hd / (4 X) join them, the others (with w) make the keys' weights.
+template <int X>
+__global__ __launch_bounds__(256) void k_paged_finish(PAttnArgs a) {
+    const int b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, joins = a.nq * (a.kv.hd / (4 * X));
+    const SeqOf q = seq_of_all(a, b);
+    if (i >= q.nr) return;
+    if ((int)blockIdx.x < joins) join_splits<X>(a, q, i);
+    else key_weights(a, q, i, (int)blockIdx.x - joins);
+}
+
+struct WorkLayout { size_t po, pp, pm, pl, pmc, total; };
 static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weights) {
     const size_t n = (size_t)nrows * nq, ns = ((size_t)max_len + kPSplit - 1) / kPSplit;
     WorkLayout w{};
@@ -857,8 +897,7 @@ static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weight
     w.pm = w.pp + (weights ? n * ns * kPSplit : 0);
     w.pl = w.pm + n * ns;
     w.pmc = w.pl + n * ns;
-    w.fin = w.pmc + (weights ? n * ns * kChunks : 0);
-    w.total = w.fin + (weights ? 2 * n : 0);
+    w.total = w.pmc + (weights ? n * ns * kChunks : 0);
     return w;
 }
 
@@ -884,7 +923,7 @@ static int launch_split_rt(PAttnArgs& a, hipStream_t s) {
     // Waves of their own need many splits to fill the CUs. Measured (PAR / not, us): 1 column tile, 128-wide heads: 68 units
     // of an XCD 12 / 23, 544 units 85 / 89, 2048 units 319 / 298; 256-wide: 63 units 31 / 40, 136 units 55 / 61. Two tiles
     // (the joins double, and a wave's registers): 136 units of 256-wide heads 126 / 96, 544 of 128-wide 201 / 137.
-    a.par = units < (RT == 1 ? 1792 : 96);
+    a.par = units < (RT == 2 ? 96 : G ? 1792 : 512);
     return a.par ? launch_split_form<HD, G, RT, true>(a, units, s) : launch_split_form<HD, G, RT, false>(a, units, s);
 }
 template <int HD, int G>
@@ -904,15 +943,12 @@ static int launch_paged_attn(PAttnArgs& a, hipStream_t s) {
         default: rc = launch_split<256, 64>(a, s); break;
     }
     if (rc || (a.ns == 1 && a.par && !a.w)) return rc;
-    const unsigned rows = (unsigned)(a.kv.n_seq * a.max_rows);
-    if ((long long)rows * a.nq < 2 * kCUs) hipLaunchKernelGGL(k_paged_combine<16>, dim3((unsigned)(a.nq * (a.kv.hd / 64)), rows), dim3(256), 0, s, a);
-    else if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_combine<32>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(k_paged_combine<64>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
+    const unsigned rows = (unsigned)(a.kv.n_seq * a.max_rows), more = a.w ? (unsigned)a.ns : 0;
+    if ((long long)rows * a.nq < 2 * kCUs)
+        hipLaunchKernelGGL(k_paged_finish<16>, dim3((unsigned)(a.nq * (a.kv.hd / 64)) + more, rows), dim3(256), 0, s, a);
+    else if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_finish<32>, dim3((unsigned)a.nq + more, rows), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL(k_paged_finish<64>, dim3((unsigned)a.nq + more, rows), dim3(256), 0, s, a);
     Q27X_HIP(hipGetLastError());
-    if (a.w) {
-        hipLaunchKernelGGL(k_paged_weights, dim3((unsigned)a.ns, rows), dim3(256), 0, s, a);
-        Q27X_HIP(hipGetLastError());
-    }
     return Q27X_OK;
 }
 
@@ -949,7 +985,7 @@ extern "C" int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate
     const WorkLayout wl = work_layout(nq, a.kv.hd, max_len, nrows, w != nullptr);
     float* p = (float*)work;
     a.po = p + wl.po; a.pm = p + wl.pm; a.pl = p + wl.pl;
-    if (w) { a.pp = p + wl.pp; a.pmc = p + wl.pmc; a.fin = p + wl.fin; }
+    if (w) { a.pp = p + wl.pp; a.pmc = p + wl.pmc; }
     a.out = out; a.xq = xq; a.xs = xs; a.w = w; a.w_stride = w_stride;
     return launch_paged_attn(a, (hipStream_t)s);
 }
