@@ -7,7 +7,7 @@
 // depends on its own keys alone, whatever else is in the batch. A wave takes a chunk for up to 16 RT columns, the pairs
 // of a row and a query head of its kv head: it has the chunk's scores before it needs their maximum, so the chunk has one
 // maximum and one exponential, and leaves (m, l, o). Chunks are joined in order, (m, l, o) <- (m', l e^(m - m') + l_c e^(m_c
-// - m'), ..), m' = max(m, m_c); k_paged_finish joins the splits. Two forms of the same arithmetic, the same bits:
+// - m'), ..), m' = max(m, m_c); k_paged_join joins the splits. Two forms of the same arithmetic, the same bits:
 //   PAR: block = a split's chunks, one a wave, joined through LDS: as many waves as can be, for few keys.
 //   else: a wave walks a split's chunks and joins them in registers; waves are independent (no barrier), each with the
 //     next chunk's keys and values on their way, for many keys.
@@ -50,7 +50,7 @@ struct PAttnArgs {
     int nq, gate, max_len, max_rows, nrows, ns;      // ns: splits of max_len
     float sl2e;                                      // log2(e) / sqrt(hd)
     float* po; float* pm; float* pl;                 // splits' outputs [row][head][ns][hd], maxima and sums [row][head][ns]
-    float* pp; float* pmc;                           // with w: e^(x - m) [row][head][ns 256], chunk maxima [row][head][ns chunks]
+    float* pp; float* pmc; float* fin;               // with w: e^(x - m) [row][head][ns 256], chunk maxima [row][head][ns chunks], (M, l)
     uint16_t* out; int8_t* xq; float* xs;
     float* w; int w_stride;
     int par;                                         // the split kernel's form: PAR finishes sequences of one split
@@ -750,13 +750,17 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShap
 // thread per dim). X = hd/4: a block joins a head, fewer blocks of more work for many (48 rows of 24 heads and 17
 // splits: 20.8 us with X = 16). A thread's first eight splits are requested before the maximum is known.
 template <int X>
-__device__ __forceinline__ void join_splits(const PAttnArgs& a, const SeqOf& q, int i) {
+__global__ __launch_bounds__(256) void k_paged_join(PAttnArgs a) {
+    const int b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows;
+    const SeqOf q = seq_of_all(a, b);
+    if (i >= q.nr) return;
     constexpr int NA = X / 16, B = 8 / NA;            // classes of a lane, splits of each requested at a time
     const int hd = a.kv.hd, parts = hd / (4 * X);
     const int head = blockIdx.x / parts, d0 = (blockIdx.x % parts) * 4 * X;
     const int t = threadIdx.x, x = t % X, y = 4 * (t >> 6) + (t & 63) / X * NA;      // the lane's first class
     const int ns = splits_of(q);
-    if (ns == 1 && a.par) return;                     // (finished by the split kernel)
+    const bool done = ns == 1 && a.par;               // (finished by the split kernel: with weights, its sums are noted)
+    if (done && !(a.w && d0 == 0)) return;
     const size_t row = (size_t)(q.first + i), at = row * a.nq + head;
     const float* pm = a.pm + at * a.ns;
     const float* pl = a.pl + at * a.ns;
@@ -770,10 +774,12 @@ __device__ __forceinline__ void join_splits(const PAttnArgs& a, const SeqOf& q, 
         for (int u = 0; u < B; ++u)
 #pragma unroll
             for (int k = 0; k < NA; ++k) {
-                const int s = s0 + 16 * u + k;
-                mv[u][k] = s < ns ? pm[s] : -__builtin_huge_valf();
-                lv[u][k] = s < ns ? pl[s] : 0.0f;
-                ov[u][k] = s < ns ? po[(size_t)s * (hd >> 2)] : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                const int s = s0 + 16 * u + k, r = s < ns ? s : 0;
+                const float m = pm[r], l = pl[r];
+                const f32x4 o = po[(unsigned)(r * (hd >> 2))];
+                mv[u][k] = s < ns ? m : -__builtin_huge_valf();
+                lv[u][k] = s < ns ? l : 0.0f;
+                ov[u][k] = s < ns ? o : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
             }
     };
     batch(y);
@@ -826,40 +832,36 @@ __device__ __forceinline__ void join_splits(const PAttnArgs& a, const SeqOf& q, 
     __syncthreads();
     if (t >= 4 * X) return;
     const float l = ((s_l[0] + s_l[1]) + s_l[2]) + s_l[3];
-    put_out(a, hd, row, head, d0 + t, ((s_sum[0][t] + s_sum[1][t]) + s_sum[2][t]) + s_sum[3][t], l);
+    if (!done) put_out(a, hd, row, head, d0 + t, ((s_sum[0][t] + s_sum[1][t]) + s_sum[2][t]) + s_sum[3][t], l);
+    if (a.w && d0 == 0 && t == 0) {
+        a.fin[2 * at] = M;
+        a.fin[2 * at + 1] = l;
+    }
 }
 
 // The weight that each key of split sp got from row i, summed over the query heads in order: w[row][key] = sum over h of
-// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of its chunks: one factor per (head, chunk), made first by 8 lanes a
-// head from the splits' maxima and sums. Keys up to the sequence's length are written (0 where the row does not see
-// them), nothing behind. Bound by the 4 nq bytes per key that it reads.
-constexpr int kWHeads = 32;
-__device__ __forceinline__ void key_weights(const PAttnArgs& a, const SeqOf& q, int i, int sp) {
-    const int t = threadIdx.x, key = sp * kPSplit + t;
-    if (sp * kPSplit >= min(q.raw, a.max_len)) return;
+// e^(x - M_h) / l_h, from the split kernel's e^(x - m) of its chunks: one factor per (head, chunk), made first. Keys up
+// to the sequence's length are written (0 where the row does not see them), nothing behind. Bound by the 4 nq bytes per key that it reads.
+constexpr int kWHeads = 64;
+__global__ __launch_bounds__(256) void k_paged_weights(PAttnArgs a) {
+    const int sp = blockIdx.x, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, t = threadIdx.x, key = sp * kPSplit + t;
+    const SeqOf q = seq_of_all(a, b);
+    if (i >= q.nr || sp * kPSplit >= min(q.raw, a.max_len)) return;
     const size_t at = (size_t)(q.first + i) * a.nq;
     const bool live = sp * kPSplit < q.len;           // (behind the table's end nothing was split)
-    const int ns = splits_of(q);
     __shared__ float2 s_f[kWHeads][kChunks];          // a chunk's factor, and what is added where it has no weights
     float w = 0.0f;
     for (int h0 = 0; h0 < a.nq && live; h0 += kWHeads) {
         const int nh = min(kWHeads, a.nq - h0);
-        const int h = t >> 3, y = t & 7;
-        const size_t r = at + h0 + (h < nh ? h : 0);
-        const float* pm = a.pm + r * a.ns;
-        const float* pl = a.pl + r * a.ns;
-        const float m = a.pmc[(r * a.ns + sp) * kChunks + (y & 3)];
-        float M = -__builtin_huge_valf(), L = 0.0f;
-        for (int s = y; s < ns; s += 8) M = fmaxf(M, pm[s]);
-        M = max_xor(M, 8);
-        for (int s = y; s < ns; s += 8) L = __builtin_fmaf(pl[s], weight_of(pm[s], M), L);
-        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0xB1, 0xF, 0xF, false));
-        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0x4E, 0xF, 0xF, false));
-        L += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(L), 0x141, 0xF, 0xF, false));
-        // (a chunk without a key that is there has no weights written: its share is 0, or not a number with the row's sum)
-        const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
         __syncthreads();
-        if (y < kChunks && h < nh) s_f[h][y] = make_float2(f, m == -__builtin_huge_valf() || f != f ? f : 0.0f);
+        if (t < kChunks * nh) {
+            const int h = t / kChunks, y = t % kChunks;
+            const size_t r = at + h0 + h;
+            const float m = a.pmc[(r * a.ns + sp) * kChunks + y], M = a.fin[2 * r], L = a.fin[2 * r + 1];
+            // (a chunk without a key that is there has no weights written: its share is 0, or not a number with the row's sum)
+            const float f = L == 0.0f ? 0.0f : weight_of(m, M) / L;
+            s_f[h][y] = make_float2(f, m == -__builtin_huge_valf() || f != f ? f : 0.0f);
+        }
         __syncthreads();
         const float* pp = a.pp + ((at + h0) * a.ns + sp) * kPSplit + t;
         const size_t step = (size_t)a.ns * kPSplit;
@@ -878,17 +880,7 @@ __device__ __forceinline__ void key_weights(const PAttnArgs& a, const SeqOf& q, 
     if (key < min(q.raw, a.max_len)) a.w[(size_t)(q.first + i) * a.w_stride + key] = key > q.raw - q.n + i ? 0.0f : w;
 }
 
-// What is left of a row after the splits: blocks x < nq hd / (4 X) join them, the others (with w) make the keys' weights.
-template <int X>
-__global__ __launch_bounds__(256) void k_paged_finish(PAttnArgs a) {
-    const int b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, joins = a.nq * (a.kv.hd / (4 * X));
-    const SeqOf q = seq_of_all(a, b);
-    if (i >= q.nr) return;
-    if ((int)blockIdx.x < joins) join_splits<X>(a, q, i);
-    else key_weights(a, q, i, (int)blockIdx.x - joins);
-}
-
-struct WorkLayout { size_t po, pp, pm, pl, pmc, total; };
+struct WorkLayout { size_t po, pp, pm, pl, pmc, fin, total; };
 static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weights) {
     const size_t n = (size_t)nrows * nq, ns = ((size_t)max_len + kPSplit - 1) / kPSplit;
     WorkLayout w{};
@@ -897,7 +889,8 @@ static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weight
     w.pm = w.pp + (weights ? n * ns * kPSplit : 0);
     w.pl = w.pm + n * ns;
     w.pmc = w.pl + n * ns;
-    w.total = w.pmc + (weights ? n * ns * kChunks : 0);
+    w.fin = w.pmc + (weights ? n * ns * kChunks : 0);
+    w.total = w.fin + (weights ? 2 * n : 0);
     return w;
 }
 
@@ -942,13 +935,18 @@ static int launch_paged_attn(PAttnArgs& a, hipStream_t s) {
         case 25632: rc = launch_split<256, 32>(a, s); break;
         default: rc = launch_split<256, 64>(a, s); break;
     }
-    if (rc || (a.ns == 1 && a.par && !a.w)) return rc;
-    const unsigned rows = (unsigned)(a.kv.n_seq * a.max_rows), more = a.w ? (unsigned)a.ns : 0;
-    if ((long long)rows * a.nq < 2 * kCUs)
-        hipLaunchKernelGGL(k_paged_finish<16>, dim3((unsigned)(a.nq * (a.kv.hd / 64)) + more, rows), dim3(256), 0, s, a);
-    else if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_finish<32>, dim3((unsigned)a.nq + more, rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL(k_paged_finish<64>, dim3((unsigned)a.nq + more, rows), dim3(256), 0, s, a);
-    Q27X_HIP(hipGetLastError());
+    if (rc) return rc;
+    const unsigned rows = (unsigned)(a.kv.n_seq * a.max_rows);
+    if (a.ns > 1 || !a.par || a.w) {
+        if ((long long)rows * a.nq < 2 * kCUs) hipLaunchKernelGGL(k_paged_join<16>, dim3((unsigned)(a.nq * (a.kv.hd / 64)), rows), dim3(256), 0, s, a);
+        else if (a.kv.hd == 128) hipLaunchKernelGGL(k_paged_join<32>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
+        else hipLaunchKernelGGL(k_paged_join<64>, dim3((unsigned)a.nq, rows), dim3(256), 0, s, a);
+        Q27X_HIP(hipGetLastError());
+    }
+    if (a.w) {
+        hipLaunchKernelGGL(k_paged_weights, dim3((unsigned)a.ns, rows), dim3(256), 0, s, a);
+        Q27X_HIP(hipGetLastError());
+    }
     return Q27X_OK;
 }
 
@@ -985,7 +983,7 @@ extern "C" int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate
     const WorkLayout wl = work_layout(nq, a.kv.hd, max_len, nrows, w != nullptr);
     float* p = (float*)work;
     a.po = p + wl.po; a.pm = p + wl.pm; a.pl = p + wl.pl;
-    if (w) { a.pp = p + wl.pp; a.pmc = p + wl.pmc; }
+    if (w) { a.pp = p + wl.pp; a.pmc = p + wl.pmc; a.fin = p + wl.fin; }
     a.out = out; a.xq = xq; a.xs = xs; a.w = w; a.w_stride = w_stride;
     return launch_paged_attn(a, (hipStream_t)s);
 }
