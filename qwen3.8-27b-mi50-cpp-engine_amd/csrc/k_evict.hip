@@ -33,132 +33,8 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive prefix sums over the block's waves of one count per wave; total in *sum
-__device__ __forceinline__ int scan_waves(int mine, int wv, int* red, int& sum) {
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[wv] = mine;
-    __syncthreads();
-    int before = 0;
-    sum = 0;
-    for (int i = 0; i < kEvWaves; ++i) {
-        const int x = red[i];
-        before += i < wv ? x : 0;
-        sum += x;
-    }
-    return before;
-}
-
-__global__ __launch_bounds__(kEvThreads) void k_evict_pick(EvictArgs a) {
-    const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
-    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-    __shared__ uint32_t hist[256];
-    __shared__ int red[kEvWaves];
-    __shared__ uint32_t s_digit;
-    __shared__ int s_left;
-    int first, n;
-    paged_rows(a.kv, b, first, n);
-    const long long cap = paged_cap(a.kv);
-    int len = min(a.kv.lens[b], a.max_len);
-    len = len < cap ? len : (int)cap;
-    len = len < 0 ? 0 : len;
-    int known = a.state[2 * b], total = a.state[2 * b + 1];
-    known = min(known < 0 ? 0 : known, len);
-    const int now = total + len - known;
-    int rows = a.w ? min(n, a.nrows - first) : 0;
-    if (a.n_acc) rows = min(rows, a.n_acc[b]);
-    float* acc = a.acc + (size_t)b * a.stride;
-    int32_t* ord = a.ord + (size_t)b * a.stride;
-    uint32_t* rank = a.rank + (size_t)b * a.max_len;
-    const bool over = len > a.high;
-    const int fresh = now - a.recent;                 // the first of the newest keys
-    for (int i = t; i < len; i += kEvThreads) {
-        float x = i < known ? acc[i] * a.decay : 0.0f;
-        for (int r = 0; r < rows; ++r) x += a.w[(size_t)(first + r) * a.w_stride + i];
-        acc[i] = x;
-        int o = total + i - known;
-        if (i < known) o = ord[i];
-        else ord[i] = o;
-        if (over) rank[i] = o >= fresh ? kNewest : rank_of(x);
-    }
-    __syncthreads();                                  // (known and total are read by every thread before they change)
-    if (t == 0) {
-        const int left = over ? a.budget : len;
-        a.new_lens[b] = left;
-        a.state[2 * b] = left;
-        a.state[2 * b + 1] = now;
-        if (!over) a.npairs[b] = 0;
-    }
-    if (!over) return;
-    // the budget-th largest rank, eight bits at a time; left: how many of that rank stay
-    uint32_t top = 0;
-    int left = a.budget;
-    for (int sh = 24; sh >= 0; sh -= 8) {
-        if (t < 256) hist[t] = 0;
-        __syncthreads();
-        for (int i = t; i < len; i += kEvThreads) {
-            const uint32_t x = rank[i];
-            if (sh == 24 || (x >> (sh + 8)) == (top >> (sh + 8))) atomicAdd(&hist[(x >> sh) & 255u], 1u);
-        }
-        __syncthreads();
-        if (t == 0) {
-            int d = 255, k = left;
-            while (d > 0 && (int)hist[d] < k) k -= (int)hist[d--];
-            s_digit = (uint32_t)d;
-            s_left = k;
-        }
-        __syncthreads();
-        top |= s_digit << sh;
-        left = s_left;
-    }
-    // Each wave walks a run of 64-key steps in order: how many of rank `top` come before it tells which of those stay;
-    // then the places that fall free before budget and the keys that stay behind it, each counted in order.
-    const int steps = (len + 63) / 64, run = (steps + kEvWaves - 1) / kEvWaves;
-    const int s0 = wv * run, s1 = min(s0 + run, steps);
-    int count = 0, sum = 0;
-    for (int s = s0; s < s1; ++s) {
-        const int i = 64 * s + l;
-        count += __popcll(__ballot(i < len && rank[i] == top));
-    }
-    const int eq0 = scan_waves(count, wv, red, sum);
-    const uint64_t below = (1ull << l) - 1;
-    int2* pairs = a.pairs + (size_t)b * (a.max_len / 2 + 1);
-    int holes = 0, movers = 0, h0 = 0, m0 = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        int eq = eq0, h = h0, m = m0;
-        for (int s = s0; s < s1; ++s) {
-            const int i = 64 * s + l;
-            const uint32_t x = i < len ? rank[i] : 0u;
-            const uint64_t same = __ballot(i < len && x == top);
-            const bool stays = i < len && (x > top || (x == top && eq + __popcll(same & below) < left));
-            eq += __popcll(same);
-            const uint64_t hole = __ballot(i < len && !stays && i < a.budget), mover = __ballot(stays && i >= a.budget);
-            if (pass) {
-                if ((hole >> l) & 1) pairs[h + __popcll(hole & below)].y = i;
-                if ((mover >> l) & 1) pairs[m + __popcll(mover & below)].x = i;
-            }
-            h += __popcll(hole);
-            m += __popcll(mover);
-        }
-        if (!pass) {
-            h0 = scan_waves(h, wv, red, holes);
-            m0 = scan_waves(m, wv, red, movers);
-        }
-    }
-    __syncthreads();
-    if (t == 0) a.npairs[b] = holes;
-    for (int i = t; i < holes; i += kEvThreads) {
-        const int2 p = pairs[i];
-        acc[p.y] = acc[p.x];
-        ord[p.y] = ord[p.x];
-    }
-}
-
-// The sums of up to kTiles x 1024 keys of a sequence by one block, the keys' ranks in registers (thread t: keys t, t + 1024
-// ..), read once. The budget-th largest rank: a histogram of 2048 equal steps of the range between the smallest and the
-// largest, then of the step that holds it, three at most -- digits of the rank itself meet in a few counters, as sums share
-// their exponents, and LDS adds to one address come one after another (4097 keys: 53 us with eight bits a pass).
-// Bound by latency: loads, then about ten barriers a pass; with one block a sequence, not by memory.
 constexpr int kTiles = 32, kBins = 2048;
+constexpr int kMaxKeys = 0x7fffffff - 16 * kEvThreads;     // (indexes run over by less than that)
 
 // Exclusive prefix sum over the block's first n <= 1024 values, one a thread; the sum of all in `sum`.
 __device__ __forceinline__ uint32_t scan_block(uint32_t x, uint32_t* red, uint32_t& sum) {
@@ -181,6 +57,137 @@ __device__ __forceinline__ uint32_t scan_block(uint32_t x, uint32_t* red, uint32
         sum += z;
     }
     return before + y - x;
+}
+
+// A block's sequence.
+struct EvictSeq {
+    int first, rows, len, known, total, now, fresh;   // its rows of w, keys, keys with a sum, arrivals before and now, the first of the newest
+    bool over;
+    float* acc;
+    int32_t* ord;
+    int2* pairs;
+};
+__device__ __forceinline__ EvictSeq evict_seq(const EvictArgs& a, int b) {
+    EvictSeq q;
+    int n;
+    paged_rows(a.kv, b, q.first, n);
+    const long long cap = paged_cap(a.kv);
+    int len = min(a.kv.lens[b], a.max_len);
+    len = len < cap ? len : (int)cap;
+    q.len = len < 0 ? 0 : len;
+    const int known = a.state[2 * b];
+    q.total = a.state[2 * b + 1];
+    q.known = min(known < 0 ? 0 : known, q.len);
+    q.now = q.total + q.len - q.known;
+    q.rows = a.w ? min(n, a.nrows - q.first) : 0;
+    if (a.n_acc) q.rows = min(q.rows, a.n_acc[b]);
+    q.over = q.len > a.high;
+    q.fresh = q.now - a.recent;
+    q.acc = a.acc + (size_t)b * a.stride;
+    q.ord = a.ord + (size_t)b * a.stride;
+    q.pairs = a.pairs + (size_t)b * (a.max_len / 2 + 1);
+    return q;
+}
+// The thread's sums of keys i, i + 1024 .. , eight with their loads together, and their ranks. q.len > 0.
+__device__ __forceinline__ void add_up(const EvictArgs& a, const EvictSeq& q, int i0, uint32_t (&key)[8]) {
+    float x[8];
+    int o[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int j = min(i0 + u * kEvThreads, q.len - 1);
+        x[u] = q.acc[j];
+        o[u] = q.ord[j];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kEvThreads;
+        x[u] = i < q.known ? x[u] * a.decay : 0.0f;
+        o[u] = i < q.known ? o[u] : q.total + i - q.known;
+    }
+    for (int r = 0; r < q.rows; ++r) {
+        const float* w = a.w + (size_t)(q.first + r) * a.w_stride;
+        float y[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) y[u] = w[min(i0 + u * kEvThreads, q.len - 1)];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) x[u] += y[u];
+    }
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        const int i = i0 + u * kEvThreads;
+        if (i < q.len) {
+            q.acc[i] = x[u];
+            if (i >= q.known) q.ord[i] = o[u];
+        }
+        key[u] = i < q.len ? (o[u] >= q.fresh ? kNewest : rank_of(x[u])) : 0u;
+    }
+}
+// The sequence's state after its sums; every thread has read what it was.
+__device__ __forceinline__ void set_state(const EvictArgs& a, const EvictSeq& q, int b) {
+    const int left = q.over ? a.budget : q.len;
+    a.new_lens[b] = left;
+    a.state[2 * b] = left;
+    a.state[2 * b + 1] = q.now;
+    if (!q.over) a.npairs[b] = 0;
+}
+
+// The budget-th largest of a block's ranks: a histogram of 2048 equal steps of the range between the smallest and the
+// largest, then of the step that holds it, three at most -- digits of the rank itself meet in a few counters, as sums share
+// their exponents, and LDS adds to one address come one after another (4097 keys: 53 us with eight bits a pass).
+struct Cut {
+    uint32_t top, left, same;       // that rank, how many of that rank stay, how many there are
+};
+// `each(f)`: f(rank) for every rank of this thread (0: no key); fixed, lo, hi: this thread's count of the newest (this
+// wave's, rather) and the smallest and largest of its other ranks.
+template <class Each>
+__device__ __forceinline__ Cut find_cut(int budget, uint32_t fixed, uint32_t lo, uint32_t hi, uint32_t* red, const Each& each) {
+    __shared__ uint32_t hist[kBins];
+    __shared__ uint32_t red2[3][kEvWaves];
+    __shared__ uint32_t s_bin, s_left, s_same;
+    const int t = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    lo = min_xor64(lo);
+    hi = ~min_xor64(~hi);
+    if ((t & 63) == 0) { red2[0][wv] = fixed; red2[1][wv] = lo; red2[2][wv] = hi; }
+    __syncthreads();
+    fixed = 0; lo = kNewest; hi = 0;
+#pragma unroll
+    for (int i = 0; i < kEvWaves; ++i) {
+        fixed += red2[0][i];
+        lo = min(lo, red2[1][i]);
+        hi = max(hi, red2[2][i]);
+    }
+    Cut cut{kNewest, (uint32_t)budget, fixed};
+    if (fixed >= (uint32_t)budget) return cut;
+    cut.left = (uint32_t)budget - fixed;
+    uint32_t span = hi - lo;
+    for (;;) {
+        const int bits = span ? 32 - __builtin_clz(span) : 0, shift = bits > 11 ? bits - 11 : 0;
+        hist[t] = 0;
+        hist[t + kEvThreads] = 0;
+        __syncthreads();
+        each([&](uint32_t key) __attribute__((always_inline)) {
+            const uint32_t x = key - lo;
+            if (x <= span && key != kNewest && key != 0) atomicAdd(&hist[x >> shift], 1u);
+        });
+        __syncthreads();
+        const uint32_t h1 = hist[kBins - 1 - 2 * t], h0 = hist[kBins - 2 - 2 * t];     // from the top
+        uint32_t sum;
+        const uint32_t before = scan_block(h1 + h0, red, sum);
+        if (before < cut.left && cut.left <= before + h1 + h0) {
+            const bool second = cut.left > before + h1;
+            s_bin = (uint32_t)(kBins - 1 - 2 * t - (second ? 1 : 0));
+            s_left = cut.left - before - (second ? h1 : 0);
+            s_same = second ? h0 : h1;
+        }
+        __syncthreads();
+        lo += s_bin << shift;
+        cut.left = s_left;
+        cut.same = s_same;
+        if (shift == 0) break;
+        span = (1u << shift) - 1;
+    }
+    cut.top = lo;
+    return cut;
 }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -300,87 +307,35 @@ __device__ __forceinline__ void few_go(const EvictArgs& a, const uint32_t (&key)
     }
 }
 
+// The sums of up to kTiles x 1024 keys of a sequence by one block, the keys' ranks in registers (thread t: keys t, t + 1024
+// ..), read once. Bound by latency: loads, then about ten barriers a pass; with one block a sequence, not by memory.
 __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
     const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-    __shared__ uint32_t hist[kBins];
     __shared__ uint32_t count[kTiles * kEvWaves];
-    __shared__ uint32_t red[kEvWaves], red2[3][kEvWaves];
-    __shared__ uint32_t s_bin, s_left, s_same;
+    __shared__ uint32_t red[kEvWaves];
     extern __shared__ int holes[];                    // the places that fall free, in order
-    int first, n;
-    paged_rows(a.kv, b, first, n);
-    const long long cap = paged_cap(a.kv);
-    int len = min(a.kv.lens[b], a.max_len);
-    len = len < cap ? len : (int)cap;
-    len = len < 0 ? 0 : len;
-    int known = a.state[2 * b], total = a.state[2 * b + 1];
-    known = min(known < 0 ? 0 : known, len);
-    const int now = total + len - known;
-    int rows = a.w ? min(n, a.nrows - first) : 0;
-    if (a.n_acc) rows = min(rows, a.n_acc[b]);
-    float* acc = a.acc + (size_t)b * a.stride;
-    int32_t* ord = a.ord + (size_t)b * a.stride;
-    const bool over = len > a.high;
-    const int fresh = now - a.recent;                 // the first of the newest keys
-    const int budget = a.budget;
+    const EvictSeq q = evict_seq(a, b);
+    const int len = q.len, budget = a.budget;
+    float* acc = q.acc;
+    int32_t* ord = q.ord;
     uint32_t key[kTiles];
-    // eight keys a thread at a time, their loads together
 #pragma unroll
     for (int r0 = 0; r0 < kTiles; r0 += 8) {
-        if (r0 * kEvThreads < len) {
-            float x[8];
-            int o[8];
+        uint32_t some[8] = {};
+        if (r0 * kEvThreads < len) add_up(a, q, r0 * kEvThreads + t, some);
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = (r0 + u) * kEvThreads + t, j = min(i, len - 1);
-                x[u] = acc[j];
-                o[u] = ord[j];
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = (r0 + u) * kEvThreads + t;
-                x[u] = i < known ? x[u] * a.decay : 0.0f;
-                o[u] = i < known ? o[u] : total + i - known;
-            }
-            for (int r = 0; r < rows; ++r) {
-                const float* w = a.w + (size_t)(first + r) * a.w_stride;
-                float y[8];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) y[u] = w[min((r0 + u) * kEvThreads + t, len - 1)];
-#pragma unroll
-                for (int u = 0; u < 8; ++u) x[u] += y[u];
-            }
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = (r0 + u) * kEvThreads + t;
-                if (i < len) {
-                    acc[i] = x[u];
-                    if (i >= known) ord[i] = o[u];
-                }
-                key[r0 + u] = i < len ? (o[u] >= fresh ? kNewest : rank_of(x[u])) : 0u;
-            }
-        } else {
-#pragma unroll
-            for (int u = 0; u < 8; ++u) key[r0 + u] = 0u;
-        }
+        for (int u = 0; u < 8; ++u) key[r0 + u] = some[u];
     }
-    __syncthreads();                                  // (known and total are read by every thread before they change)
-    if (t == 0) {
-        const int left = over ? budget : len;
-        a.new_lens[b] = left;
-        a.state[2 * b] = left;
-        a.state[2 * b + 1] = now;
-        if (!over) a.npairs[b] = 0;
-    }
-    if (!over) return;
+    __syncthreads();                                  // (the state is read by every thread before it changes)
+    if (t == 0) set_state(a, q, b);
+    if (!q.over) return;
     const int tiles = (len + kEvThreads - 1) / kEvThreads;
-    int2* pairs = a.pairs + (size_t)b * (a.max_len / 2 + 1);
+    int2* pairs = q.pairs;
     if (len - budget <= kFew) {
         few_go(a, key, len, tiles, acc, ord, pairs);
         return;
     }
-    // the newest, counted, and the range of the others
     uint32_t lo = kNewest, hi = 0, fixed = 0;
 #pragma unroll
     for (int r = 0; r < kTiles; ++r) {
@@ -393,52 +348,12 @@ __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
             }
         }
     }
-    lo = min_xor64(lo);
-    hi = ~min_xor64(~hi);
-    if (l == 0) { red2[0][wv] = fixed; red2[1][wv] = lo; red2[2][wv] = hi; }
-    __syncthreads();
-    fixed = 0; lo = kNewest; hi = 0;
+    const Cut cut = find_cut(budget, fixed, lo, hi, red, [&](auto f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kEvWaves; ++i) {
-        fixed += red2[0][i];
-        lo = min(lo, red2[1][i]);
-        hi = max(hi, red2[2][i]);
-    }
-    // top: the budget-th largest rank; left: how many of that rank stay; same: how many there are
-    uint32_t top = kNewest, left = (uint32_t)budget, same = fixed;
-    if (fixed < (uint32_t)budget) {
-        left = (uint32_t)budget - fixed;
-        uint32_t span = hi - lo;
-        for (;;) {
-            const int bits = span ? 32 - __builtin_clz(span) : 0, shift = bits > 11 ? bits - 11 : 0;
-            hist[t] = 0;
-            hist[t + kEvThreads] = 0;
-            __syncthreads();
-#pragma unroll
-            for (int r = 0; r < kTiles; ++r)
-                if (r < tiles) {
-                    const uint32_t x = key[r] - lo;
-                    if (x <= span && key[r] != kNewest && key[r] != 0) atomicAdd(&hist[x >> shift], 1u);
-                }
-            __syncthreads();
-            const uint32_t h1 = hist[kBins - 1 - 2 * t], h0 = hist[kBins - 2 - 2 * t];     // from the top
-            uint32_t sum;
-            const uint32_t before = scan_block(h1 + h0, red, sum);
-            if (before < left && left <= before + h1 + h0) {
-                const bool second = left > before + h1;
-                s_bin = (uint32_t)(kBins - 1 - 2 * t - (second ? 1 : 0));
-                s_left = left - before - (second ? h1 : 0);
-                s_same = second ? h0 : h1;
-            }
-            __syncthreads();
-            lo += s_bin << shift;
-            left = s_left;
-            same = s_same;
-            if (shift == 0) break;
-            span = (1u << shift) - 1;
-        }
-        top = lo;
-    }
+        for (int r = 0; r < kTiles; ++r)
+            if (r < tiles) f(key[r]);
+    });
+    const uint32_t top = cut.top, left = cut.left, same = cut.same;
     // which keys stay: bit r of `stays`; of those of rank `top` the lowest places, if not all do
     uint32_t stays = 0, sum = 0;
     const uint64_t below = (1ull << l) - 1;
@@ -514,6 +429,101 @@ __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
     }
 }
 
+// The same for longer sequences in two launches, the ranks in memory: sums and ranks by a block for every 8192 keys, then
+// the choice by one block a sequence, each wave walking a run of 64-key steps in order, 16 with their loads together.
+// 131071 keys of which one goes: 149 us, of which half go 156 (digits of eight bits and one launch: 343); bound by the one
+// block's LDS adds and its share of the L2. A limit above the budget has it done once in many steps.
+__global__ __launch_bounds__(kEvThreads) void k_evict_sums(EvictArgs a) {
+    const int b = blockIdx.y, i0 = (int)blockIdx.x * 8 * kEvThreads + (int)threadIdx.x;
+    const EvictSeq q = evict_seq(a, b);
+    if (i0 - (int)threadIdx.x >= q.len) return;
+    uint32_t* rank = a.rank + (size_t)b * a.max_len;
+    uint32_t key[8];
+    add_up(a, q, i0, key);
+    if (!q.over) return;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+        if (i0 + u * kEvThreads < q.len) rank[i0 + u * kEvThreads] = key[u];
+}
+__global__ __launch_bounds__(kEvThreads) void k_evict_long(EvictArgs a) {
+    const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    __shared__ uint32_t red[kEvWaves];
+    const EvictSeq q = evict_seq(a, b);
+    const int len = q.len, budget = a.budget;
+    const uint32_t* rank = a.rank + (size_t)b * a.max_len;
+    __syncthreads();                                  // (the state is read by every thread before it changes)
+    if (t == 0) set_state(a, q, b);
+    if (!q.over) return;
+    const int steps = (len + 63) / 64, run = (steps + kEvWaves - 1) / kEvWaves;
+    const int s0 = wv * run, s1 = min(s0 + run, steps);
+    constexpr int kDeep = 16;
+    // f(place, rank) for the keys of this wave's run in order; the rank is 0 where there is no key
+    auto walk = [&](auto f) __attribute__((always_inline)) {
+        for (int st = s0; st < s1; st += kDeep) {
+            uint32_t x[kDeep];
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) x[u] = rank[min(64 * (st + u) + l, len - 1)];
+#pragma unroll
+            for (int u = 0; u < kDeep; ++u) {
+                const int i = 64 * (st + u) + l;
+                f(i, st + u < s1 && i < len ? x[u] : 0u);
+            }
+        }
+    };
+    uint32_t lo = kNewest, hi = 0, fixed = 0;
+    walk([&](int, uint32_t x) __attribute__((always_inline)) {
+        fixed += (uint32_t)__popcll(__ballot(x == kNewest));
+        if (x != 0 && x != kNewest) {
+            lo = min(lo, x);
+            hi = max(hi, x);
+        }
+    });
+    const Cut cut = find_cut(budget, fixed, lo, hi, red, [&](auto f) __attribute__((always_inline)) {
+        walk([&](int, uint32_t x) __attribute__((always_inline)) { f(x); });
+    });
+    const uint32_t top = cut.top, left = cut.left;
+    // how many of rank `top` come before this wave's run tells which of those stay
+    const uint64_t below = (1ull << l) - 1;
+    uint32_t eq0 = 0, sum;
+    if (cut.same != left) {
+        uint32_t n = 0;
+        walk([&](int, uint32_t x) __attribute__((always_inline)) { n += (uint32_t)__popcll(__ballot(x == top)); });
+        eq0 = scan_block(l == 0 ? n : 0u, red, sum);
+        eq0 = __builtin_amdgcn_readfirstlane(eq0);
+    }
+    // the places that fall free before budget and the keys that stay behind it, counted and then written down in order
+    uint32_t holes = 0, h0 = 0, m0 = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {
+        uint32_t eq = eq0, h = h0, m = m0;
+        walk([&](int i, uint32_t x) __attribute__((always_inline)) {
+            const uint64_t same = __ballot(x == top);
+            const bool stays = x > top || (x == top && eq + (uint32_t)__popcll(same & below) < left);
+            eq += (uint32_t)__popcll(same);
+            const bool falls = x != 0 && !stays && i < budget, moves = stays && i >= budget;
+            const uint64_t hole = __ballot(falls), mover = __ballot(moves);
+            if (pass) {
+                if (falls) q.pairs[h + (uint32_t)__popcll(hole & below)].y = i;
+                if (moves) q.pairs[m + (uint32_t)__popcll(mover & below)].x = i;
+            }
+            h += (uint32_t)__popcll(hole);
+            m += (uint32_t)__popcll(mover);
+        });
+        if (!pass) {
+            h0 = __builtin_amdgcn_readfirstlane(scan_block(l == 0 ? h : 0u, red, holes));
+            m0 = __builtin_amdgcn_readfirstlane(scan_block(l == 0 ? m : 0u, red, sum));
+        }
+    }
+    __syncthreads();
+    if (t == 0) a.npairs[b] = (int)holes;
+    for (uint32_t i = (uint32_t)t; i < holes; i += kEvThreads) {
+        const int2 p = q.pairs[i];
+        q.acc[p.y] = q.acc[p.x];
+        q.ord[p.y] = q.ord[p.x];
+    }
+}
+
 // The moved positions of a sequence, kMoves a wave. Bound by memory.
 constexpr int kMoves = 4;
 __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
@@ -541,7 +551,7 @@ static EvictWork evict_work(int n_seq, int max_len) {
 
 using namespace q27x;
 extern "C" size_t q27x_paged_evict_work_bytes(int n_seq, int max_len) {
-    return n_seq >= 1 && n_seq <= 65535 && max_len >= 1 ? evict_work(n_seq, max_len).total : 0;
+    return n_seq >= 1 && n_seq <= 65535 && max_len >= 1 && max_len <= kMaxKeys ? evict_work(n_seq, max_len).total : 0;
 }
 extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc, int nrows,
                                 float decay, float* acc, int32_t* ord, int acc_stride, int32_t* state, int high, int budget,
@@ -551,7 +561,7 @@ extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w
     if (int rc = paged_args(kv, who, &a.kv)) return rc;
     if (!acc || !ord || !state || !work || !new_lens) { set_error("%s: null argument", who); return Q27X_E_ARG; }
     if ((uintptr_t)work & 15) { set_error("%s: work must be 16-byte aligned", who); return Q27X_E_ARG; }
-    if (max_len < 1 || max_len > 0x7fffffff - 64 || acc_stride < max_len || (w && (w_stride < max_len || nrows < 1))) {
+    if (max_len < 1 || max_len > kMaxKeys || acc_stride < max_len || (w && (w_stride < max_len || nrows < 1))) {
         set_error("%s: bad counts (max_len=%d acc_stride=%d w_stride=%d nrows=%d)", who, max_len, acc_stride, w_stride, nrows);
         return Q27X_E_ARG;
     }
@@ -575,7 +585,10 @@ extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w
         a.fused = most <= kEvWaves;
         hipLaunchKernelGGL(k_evict, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), (size_t)most * 4, (hipStream_t)s, a);
     } else {
-        hipLaunchKernelGGL(k_evict_pick, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), 0, (hipStream_t)s, a);
+        const unsigned per = 8 * kEvThreads;
+        hipLaunchKernelGGL(k_evict_sums, dim3(((unsigned)max_len + per - 1) / per, (unsigned)a.kv.n_seq), dim3(kEvThreads), 0, (hipStream_t)s, a);
+        Q27X_HIP(hipGetLastError());
+        hipLaunchKernelGGL(k_evict_long, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), 0, (hipStream_t)s, a);
     }
     Q27X_HIP(hipGetLastError());
     if (most > 0 && !a.fused) {

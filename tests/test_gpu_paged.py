@@ -544,6 +544,28 @@ def test_evict_lengths_of_the_kernels(gpu, len_):
         ev.compare(ev.expect([len_, 20], [w[:1], w[1:]], 1.0, budget, budget, 5))
 
 
+@pytest.mark.parametrize("max_len", [32769, 90000])
+def test_evict_long_sequences(gpu, max_len):
+    """Lengths past what a block holds beside short ones, ends of its tiles, many equal sums, two accepted rows of three, one
+    sequence between budget and limit; then calls that bring a few keys."""
+    X, rng = gpu, np.random.default_rng(max_len)
+    lens, counts = [max_len, 24577, 16384, 0, 16385, max_len - 1], [1, 3, 1, 1, 2, 0]
+    cache = Cache(rng, lens, counts, 1, 128, 64, page=64)
+    cache.push(X)
+    ev = Evictor(X, cache, max_len + 3)
+    n, n_acc = sum(counts), np.array([1, 2, 1, 1, 0, 1], np.int32)
+    da = X.DevBuf(array=n_acc)
+    for call, (high, budget, recent) in enumerate([(20000, 12301, 1000), (12301, 12301, 1000), (16384, 9000, 0)]):
+        w = (rng.integers(0, 40, (n, max_len)) ** 3 / 8).astype(np.float32)
+        now = [min(x, 12301 + 5 * b) if call else x for b, x in enumerate(lens)]
+        cache.lens = np.asarray(now, np.int32)
+        cache.d["lens"].upload(cache.lens)
+        dw = X.DevBuf(array=w)
+        ev.call(dw.ptr, max_len, da.ptr, n, 0.75, high, budget, recent, max_len)
+        rows = [w[cache.row_start[b]:cache.row_start[b] + min(counts[b], n_acc[b])] for b in range(len(lens))]
+        ev.compare(ev.expect(now, rows, 0.75, high, budget, recent))
+
+
 def test_evict_sums_that_are_not_numbers(gpu):
     """NaN goes first, infinity stays, -0 and 0 are equal, negative sums are ordered; no weights at all leaves the sums."""
     X, rng = gpu, np.random.default_rng(22)
