@@ -252,8 +252,9 @@ int q27x_attn_rows_noalloc(const uint16_t* qh, const uint16_t* qkv_gate, int qkv
  * page table[b][i / page]; keys on pages outside 0 .. n_pages-1 or behind the table are neither
  * read nor written. lens[b]: keys that sequence b holds, the call's rows included. Sequence b's rows
  * are row_start[b] .. row_start[b+1]-1 (not decreasing; NULL: row b), its last lens[b] - n .. lens[b]-1
- * keys. Rows behind the last sequence are left as they were. k, v 16-byte aligned; hd 128 or 256;
- * no two sequences that a call writes share a page. table, lens and row_start are device arrays:
+ * keys. Rows behind the last sequence are left as they were. k, v 16-byte aligned; hd 128 or 256.
+ * Attention may meet a page in several sequences (a shared prompt); a call that writes (prep: the new
+ * rows' pages; eviction: all pages of the sequence) must meet such a page once in the table. table, lens and row_start are device arrays:
  * a captured graph follows them. */
 typedef struct q27x_paged_kv {
     void* k; void* v;

@@ -841,7 +841,8 @@ __global__ __launch_bounds__(256) void k_paged_join(PAttnArgs a) {
 
 // The weight that each key of split sp got from row i, summed over the query heads in order: w[row][key] = sum over h of
 // e^(x - M_h) / l_h, from the split kernel's e^(x - m) of its chunks: one factor per (head, chunk), made first. Keys up
-// to the sequence's length are written (0 where the row does not see them), nothing behind. Bound by the 4 nq bytes per key that it reads.
+// to the sequence's length are written (0 where the row does not see them, or the table does not reach: such chunks left
+// nothing behind), nothing further. Bound by the 4 nq bytes per key that it reads.
 constexpr int kWHeads = 64;
 __global__ __launch_bounds__(256) void k_paged_weights(PAttnArgs a) {
     const int sp = blockIdx.x, b = blockIdx.y / a.max_rows, i = blockIdx.y % a.max_rows, t = threadIdx.x, key = sp * kPSplit + t;
@@ -877,7 +878,7 @@ __global__ __launch_bounds__(256) void k_paged_weights(PAttnArgs a) {
                 }
         }
     }
-    if (key < min(q.raw, a.max_len)) a.w[(size_t)(q.first + i) * a.w_stride + key] = key > q.raw - q.n + i ? 0.0f : w;
+    if (key < min(q.raw, a.max_len)) a.w[(size_t)(q.first + i) * a.w_stride + key] = key > q.raw - q.n + i || key >= q.len ? 0.0f : w;
 }
 
 struct WorkLayout { size_t po, pp, pm, pl, pmc, fin, total; };

@@ -313,6 +313,18 @@ def test_attention_keys_that_are_not_there(gpu, group):
     assert np.linalg.norm(bf2f(got[0]) - ref * sg) <= 2.0 ** -8 * np.linalg.norm(ref * sg)
 
 
+@pytest.mark.parametrize("max_len", [200, 24576])
+def test_attention_weights_behind_the_table(gpu, max_len):
+    """The table ends inside a split, chunks before the sequence's length: the keys behind it have no weight, in both forms of
+    the split kernel."""
+    rng = np.random.default_rng(24)
+    cache = Cache(rng, [200, 80, 60, 199], [3, 1, 2, 3], 2, 128, 32, page=16, cap=80)
+    q, gate = queries(rng, 9, 16, 128)
+    got = run_attn(gpu, cache, q, gate, 16, max_len=max_len)
+    check_attn(cache, got, q, gate, 16)
+    assert (got[3][:3, 80:200] == 0).all()
+
+
 @pytest.mark.parametrize("group", [0, 32])
 @pytest.mark.parametrize("hd", [128, 256])
 def test_attention_not_finite_stays_with_its_rows(gpu, group, hd):
