@@ -254,8 +254,8 @@ int q27x_attn_rows_noalloc(const uint16_t* qh, const uint16_t* qkv_gate, int qkv
  * are row_start[b] .. row_start[b+1]-1 (not decreasing; NULL: row b), its last lens[b] - n .. lens[b]-1
  * keys. Rows behind the last sequence are left as they were. k, v 16-byte aligned; hd 128 or 256.
  * Attention may meet a page in several sequences (a shared prompt); a call that writes (prep: the new
- * rows' pages; eviction: all pages of the sequence) must meet such a page once in the table. table, lens and row_start are device arrays:
- * a captured graph follows them. */
+ * rows' pages; eviction: all pages of the sequence) must meet such a page once in the table. table,
+ * lens and row_start are device arrays: a captured graph follows them. */
 typedef struct q27x_paged_kv {
     void* k; void* v;
     float* ks; float* vs;
@@ -309,7 +309,7 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
  * know, keys that ever came; zero state to begin a sequence, acc and ord need no start value. After a
  * rollback pass the shorter lens. new_lens may be kv->lens. A later q27x_paged_attn_rows needs no
  * positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
- * aligned. */
+ * aligned, not shared by calls that may overlap. */
 size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
 int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc,
                      int nrows, float decay, float* acc, int32_t* ord, int acc_stride, int32_t* state,

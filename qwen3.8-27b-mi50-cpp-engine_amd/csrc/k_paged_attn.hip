@@ -26,6 +26,11 @@
 // 8 bytes a lane over 16 rows 67 cycles, over 4 rows 18; 16 bytes a lane over 8 rows 21), so K comes by LDS DMA in whole
 // rows of a head, swizzled so that the operand reads of 16 rows meet distinct banks, and V in rows over 16 lanes. K read
 // straight into operands, 32 bytes of 16 rows at a time, held 64 x 8000 keys to 3.2 TB/s.
+//
+// Bound: bf16 pages by memory (64 x 4000 keys, 1.05 GB: 192 us, 5.5 TB/s; its loads without the arithmetic 188). int8 pages
+// by both sides, which overlap for the most part (32 x 4097 keys, 302 MB: 86 us; the loads alone 72, the arithmetic on
+// keys in the L2 65), two column tiles of 256-wide heads by the arithmetic (16 x 4099 keys, 3 rows: 92 us, alone 90): widening
+// the codes costs a conversion each and half a pack, 4 cycles a wave both, and a wave with two tiles has its SIMD to itself.
 #include <math.h>
 
 #include <mutex>
@@ -914,9 +919,11 @@ template <int HD, int G, int RT>
 static int launch_split_rt(PAttnArgs& a, hipStream_t s) {
     const int ncb = (a.max_rows * (a.nq / a.kv.nkv) + 16 * RT - 1) / (16 * RT);
     const long long units = ((long long)a.kv.n_seq * a.ns + 7) / 8 * a.kv.nkv * ncb;      // of an XCD, if all sequences have max_len keys
-    // Waves of their own need many splits to fill the CUs. Measured (PAR / not, us): 1 column tile, 128-wide heads: 68 units
-    // of an XCD 12 / 23, 544 units 85 / 89, 2048 units 319 / 298; 256-wide: 63 units 31 / 40, 136 units 55 / 61. Two tiles
-    // (the joins double, and a wave's registers): 136 units of 256-wide heads 126 / 96, 544 of 128-wide 201 / 137.
+    // Waves of their own need many splits to fill the CUs; the bound counts max_len keys of every sequence, of which a ragged
+    // batch has fewer. Measured (PAR / not, us), int8, 1 column tile, 128-wide heads: 68 units of an XCD 13 / 22, 544 units
+    // 85 / 82, 1536 by the bound with lengths from 8 to 8190 34 / 38, 2048 units 322 / 285; 256-wide: 63 units 30 / 39, 136
+    // units 55 / 61. bf16, 1024 units: 212 / 193. Two tiles (the joins double, and a wave's registers): 136 units of 256-wide
+    // heads 118 / 93, 544 of 128-wide 199 / 133.
     a.par = units < (RT == 2 ? 96 : G ? 1792 : 512);
     return a.par ? launch_split_form<HD, G, RT, true>(a, units, s) : launch_split_form<HD, G, RT, false>(a, units, s);
 }

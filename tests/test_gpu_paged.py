@@ -408,6 +408,74 @@ def test_attention_bits_of_a_large_batch(gpu, geom, group, rows):
         check_attn(cache, one, q[r], gate[r], nq)
 
 
+@pytest.mark.parametrize("group", [0, 16, 32, 64])
+@pytest.mark.parametrize("geom", list(GEOMS))
+def test_attention_with_room_for_many_keys(gpu, group, geom):
+    """The borders of tiles, chunks and splits under a max_len that stands for much work: waves that walk whole splits."""
+    rng = np.random.default_rng(70 + group)
+    nq, nkv, hd = GEOMS[geom]
+    counts = [1] * len(LENS) if nq // nkv < 20 else [1, 2, 1, 3, 1, 1, 2, 1, 1]
+    cache = Cache(rng, LENS, counts, nkv, hd, group, page=16)
+    q, gate = queries(rng, sum(counts), nq, hd)
+    got = run_attn(gpu, cache, q, gate, nq, max_len=256 * (1800 * 8 // (len(LENS) * nkv) + 1))
+    check_attn(cache, got, q, gate, nq)
+
+
+def test_attention_many_heads(gpu):
+    """More query heads than the weights' kernel takes at a time, and five column tiles of a kv head."""
+    rng = np.random.default_rng(25)
+    cache = Cache(rng, [300, 70], [2, 1], 2, 128, 32)
+    q, gate = queries(rng, 3, 160, 128)
+    check_attn(cache, run_attn(gpu, cache, q, gate, 160), q, gate, 160)
+
+
+def test_attention_shared_pages(gpu):
+    """Sequences that begin on the same pages, and one whose pages repeat: what each reads alone."""
+    rng = np.random.default_rng(26)
+    cache = Cache(rng, [150, 131, 90], [1, 2, 1], 2, 128, 32, page=16)
+    cache.table[1, :8] = cache.table[0, :8]
+    cache.table[2, :6] = cache.table[2, 0]
+    q, gate = queries(rng, 4, 8, 128)
+    check_attn(cache, run_attn(gpu, cache, q, gate, 8), q, gate, 8)
+
+
+@pytest.mark.parametrize("hd", [128, 256])
+def test_arguments_of_their_types_alignment(gpu, hd):
+    """Only the pages and the scratch memory are aligned to more than their type: everything else two bytes, or a float, on."""
+    X, rng = gpu, np.random.default_rng(27)
+    nq, nkv = 8, 2
+    cache = Cache(rng, [70, 9], [1, 2], nkv, hd, 32)
+    cache.push(X)
+    q, gate = queries(rng, 3, nq, hd)
+    want = run_attn(X, cache, q, gate, nq)
+    held = []
+
+    def shifted(a):
+        n = a.dtype.itemsize
+        b = X.DevBuf(array=np.concatenate([np.zeros(1, a.dtype), a.reshape(-1), np.zeros(1, a.dtype)]))
+        held.append(b)
+        return b.ptr + n
+
+    kv = cache.push(X)
+    kv.ks, kv.vs = shifted(cache.ks), shifted(cache.vs)
+    width = nq * 2 * hd + 2 * nkv * hd + 1
+    g = np.zeros((3, width), np.uint16)
+    g[:, :nq * 2 * hd].reshape(3, nq, 2, hd)[:, :, 1] = gate
+    out = X.DevBuf(array=np.zeros(3 * nq * hd + 1, np.uint16))
+    xq, xs = X.DevBuf(array=np.zeros(3 * nq * hd + 1, np.int8)), X.DevBuf(array=np.zeros(3 * nq * hd // 16 + 1, np.float32))
+    w = X.DevBuf(array=np.zeros(3 * 71 + 1, np.float32))
+    work = X.DevBuf(X.lib().q27x_paged_attn_work_bytes(nq, hd, 70, 3, 1))
+    X.call("q27x_paged_attn_rows", shifted(q), shifted(g), width, ctypes.byref(kv), nq, 1, 70, 2, 3, work.ptr, out.ptr + 2, xq.ptr + 1,
+           xs.ptr + 4, w.ptr + 4, 71, None)
+    X.call("q27x_device_sync")
+    assert np.array_equal(out.download(np.uint16, (3 * nq * hd + 1,))[1:], want[0].reshape(-1))
+    assert np.array_equal(xq.download(np.int8, (3 * nq * hd + 1,))[1:], want[1].reshape(-1))
+    assert np.array_equal(xs.download(np.float32, (3 * nq * hd // 16 + 1,))[1:], want[2].reshape(-1))
+    got = w.download(np.float32, (3 * 71 + 1,))[1:].reshape(3, 71)
+    for r, n in enumerate((70, 9, 9)):
+        assert np.array_equal(got[r, :n], want[3][r, :n])
+
+
 def test_attention_like_the_contiguous_entry(gpu):
     """q27x_attn_rows over the same cache, its pages counting up: both within their roundings of the float64 form."""
     X, rng = gpu, np.random.default_rng(14)
