@@ -312,9 +312,9 @@ __device__ __forceinline__ void few_go(const EvictArgs& a, const uint32_t (&key)
 __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
     const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
     const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
-    __shared__ uint32_t count[kTiles * kEvWaves];
+    __shared__ uint64_t s_stay[kTiles * kEvWaves], s_same[kTiles * kEvWaves];
     __shared__ uint32_t red[kEvWaves];
-    extern __shared__ int holes[];                    // the places that fall free, in order
+    extern __shared__ uint32_t holes[];               // the places that fall free, in order; above them the keys that move in
     const EvictSeq q = evict_seq(a, b);
     const int len = q.len, budget = a.budget;
     float* acc = q.acc;
@@ -353,73 +353,60 @@ __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
         for (int r = 0; r < kTiles; ++r)
             if (r < tiles) f(key[r]);
     });
-    const uint32_t top = cut.top, left = cut.left, same = cut.same;
-    // which keys stay: bit r of `stays`; of those of rank `top` the lowest places, if not all do
-    uint32_t stays = 0, sum = 0;
-    const uint64_t below = (1ull << l) - 1;
-    if (same == left) {
+    const uint32_t top = cut.top, left = cut.left;
+    // Which keys stay, a bit each: a tile's ballot is two words of 32 keys, word t then thread t's. Of the keys of rank `top`
+    // the lowest places stay, if not all do. (Ballots and counts per tile all the way: 16 us more at 32001 keys.)
 #pragma unroll
-        for (int r = 0; r < kTiles; ++r) stays |= key[r] >= top ? 1u << r : 0u;
+    for (int r = 0; r < kTiles; ++r)
+        if (r < tiles) {
+            const uint64_t more = __ballot(key[r] > top), as = __ballot(key[r] == top);
+            if (l == 0) {
+                s_stay[r * kEvWaves + wv] = more;
+                s_same[r * kEvWaves + wv] = as;
+            }
+        }
+    __syncthreads();
+    const bool mine = t < tiles * (kEvThreads / 32);
+    uint32_t stay = mine ? ((const uint32_t*)s_stay)[t] : 0u, eq = mine ? ((const uint32_t*)s_same)[t] : 0u, sum;
+    if (cut.same == left) {
+        stay |= eq;
     } else {
-#pragma unroll
-        for (int r = 0; r < kTiles; ++r)
-            if (r < tiles) {
-                const uint64_t eq = __ballot(key[r] == top);
-                if (l == 0) count[r * kEvWaves + wv] = (uint32_t)__popcll(eq);
-            }
-        __syncthreads();
-        const uint32_t c = t < tiles * kEvWaves ? count[t] : 0u;
-        const uint32_t before = scan_block(c, red, sum);
-        if (t < tiles * kEvWaves) count[t] = before;
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kTiles; ++r)
-            if (r < tiles) {
-                const uint64_t eq = __ballot(key[r] == top);
-                const bool in = key[r] > top || (key[r] == top && count[r * kEvWaves + wv] + (uint32_t)__popcll(eq & below) < left);
-                stays |= in ? 1u << r : 0u;
-            }
-        __syncthreads();
+        const uint32_t n = (uint32_t)__popc(eq), before = scan_block(n, red, sum);
+        for (uint32_t k = before < left ? min(n, left - before) : 0u; k > 0; --k) {
+            stay |= eq & (0u - eq);
+            eq &= eq - 1u;
+        }
     }
-    // the places before budget that fall free (low half) and the keys behind it that stay (high half), counted in order
-#pragma unroll
-    for (int r = 0; r < kTiles; ++r)
-        if (r < tiles) {
-            const int i = r * kEvThreads + t;
-            const bool in = (stays >> r) & 1;
-            const uint64_t hole = __ballot(!in && i < budget && i < len), mover = __ballot(in && i >= budget);
-            if (l == 0) count[r * kEvWaves + wv] = (uint32_t)__popcll(hole) | ((uint32_t)__popcll(mover) << 16);
-        }
+    // the places before budget that fall free and the keys behind it that stay, counted (low and high half) and listed in order
+    const int in = min(max(budget - 32 * t, 0), 32);              // keys of the word before budget
+    const uint32_t head = in == 32 ? ~0u : (1u << in) - 1u;
+    uint32_t hole = ~stay & head, mover = stay & ~head;
+    const uint32_t before = scan_block((uint32_t)__popc(hole) | ((uint32_t)__popc(mover) << 16), red, sum);
+    for (uint32_t m = before & 0xFFFFu; hole; ++m, hole &= hole - 1u) holes[m] = (uint32_t)(32 * t + __builtin_ctz(hole));
     __syncthreads();
-    const uint32_t c = t < tiles * kEvWaves ? count[t] : 0u;
-    const uint32_t before = scan_block(c, red, sum);
-    if (t < tiles * kEvWaves) count[t] = before;
+    for (uint32_t m = before >> 16; mover; ++m, mover &= mover - 1u) holes[m] |= (uint32_t)(32 * t + __builtin_ctz(mover)) << 16;
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kTiles; ++r)
-        if (r < tiles) {
-            const int i = r * kEvThreads + t;
-            const bool is = !((stays >> r) & 1) && i < budget && i < len;
-            const uint64_t hole = __ballot(is);
-            if (is) holes[(count[r * kEvWaves + wv] & 0xFFFFu) + (uint32_t)__popcll(hole & below)] = i;
-        }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kTiles; ++r)
-        if (r < tiles) {
-            const int i = r * kEvThreads + t;
-            const bool is = ((stays >> r) & 1) && i >= budget;
-            const uint64_t mover = __ballot(is);
-            if (is) {
-                const uint32_t m = (count[r * kEvWaves + wv] >> 16) + (uint32_t)__popcll(mover & below);
-                const int to = holes[m];
-                pairs[m] = make_int2(i, to);
-                acc[to] = acc[i];
-                ord[to] = ord[i];
-            }
-        }
     const int moves = (int)(sum & 0xFFFFu);
     if (t == 0) a.npairs[b] = moves;
+    for (int m0 = t; m0 < moves; m0 += 8 * kEvThreads) {
+        uint32_t p[8];
+        float x[8];
+        int o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            p[u] = holes[min(m0 + u * kEvThreads, moves - 1)];
+            x[u] = acc[p[u] >> 16];
+            o[u] = ord[p[u] >> 16];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (m0 + u * kEvThreads < moves) {
+                const int from = (int)(p[u] >> 16), to = (int)(p[u] & 0xFFFFu);
+                pairs[m0 + u * kEvThreads] = make_int2(from, to);
+                acc[to] = x[u];
+                ord[to] = o[u];
+            }
+    }
     if (a.fused) {                                    // a few moves at most: no second launch
         __syncthreads();
         for (int i = wv; i < moves; i += kEvWaves) {
