@@ -3,8 +3,8 @@
 // Row i of a sequence's n new rows sees keys 0 .. len - n + i of its cache. For every query head, with x = q.k / sqrt(hd):
 // out = sum e^(x - M) v / sum e^(x - M), M = max x, times sigmoid(gate); a row that sees nothing gets zeros.
 //
-// Keys are cut into fixed splits of 256 and these into chunks of 64, so a row's result
-// depends on its own keys alone, whatever else is in the batch. A wave takes a chunk for up to 16 RT columns, the pairs
+// Keys are cut into fixed splits of 256 and these into chunks of 64, so a row's result depends on its own keys alone,
+// whatever else is in the batch. A wave takes a chunk for up to 16 RT columns, the pairs
 // of a row and a query head of its kv head: it has the chunk's scores before it needs their maximum, so the chunk has one
 // maximum and one exponential, and leaves (m, l, o). Chunks are joined in order, (m, l, o) <- (m', l e^(m - m') + l_c e^(m_c
 // - m'), ..), m' = max(m, m_c); k_paged_join joins the splits. Two forms of the same arithmetic, the same bits:
@@ -27,10 +27,10 @@
 // rows of a head, swizzled so that the operand reads of 16 rows meet distinct banks, and V in rows over 16 lanes. K read
 // straight into operands, 32 bytes of 16 rows at a time, held 64 x 8000 keys to 3.2 TB/s.
 //
-// Bound: bf16 pages by memory (64 x 4000 keys, 1.05 GB: 192 us, 5.5 TB/s; its loads without the arithmetic 188). int8 pages
-// by both sides, which overlap for the most part (32 x 4097 keys, 302 MB: 86 us; the loads alone 72, the arithmetic on
-// keys in the L2 65), two column tiles of 256-wide heads by the arithmetic (16 x 4099 keys, 3 rows: 92 us, alone 90): widening
-// the codes costs a conversion each and half a pack, 4 cycles a wave both, and a wave with two tiles has its SIMD to itself.
+// Bound: bf16 pages by memory (64 x 4000 keys, 1.05 GB: 191 us, 5.5 TB/s; its loads without the arithmetic 189). int8 pages
+// by both sides, which overlap for the most part (32 x 4097 keys, 302 MB: 76 us; the loads alone 63, the arithmetic on
+// keys in the L2 59). Two column tiles of 256-wide heads by one wave's latencies (16 x 4099 keys, 3 rows, 151 MB: 78 us, the
+// arithmetic alone 74): it has its SIMD to itself, whose vector instructions fill 28% of the time, the matrix ones 18%.
 #include <math.h>
 
 #include <mutex>
@@ -42,6 +42,7 @@ namespace q27x {
 constexpr int kPSplit = 256;
 constexpr int kCUs = 256;             // compute units of an MI355X
 constexpr int kChunk = 64, kChunks = kPSplit / kChunk;
+constexpr int kCounted = 256;          // sequences whose splits the split kernel counts before it begins
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -58,7 +59,7 @@ struct PAttnArgs {
     float* pp; float* pmc; float* fin;               // with w: e^(x - m) [row][head][ns 256], chunk maxima [row][head][ns chunks], (M, l)
     uint16_t* out; int8_t* xq; float* xs;
     float* w; int w_stride;
-    int par;                                         // the split kernel's form: PAR finishes sequences of one split
+    int par;                                         // PAR throughout: sequences of one split are finished by it
 };
 
 // lane n of the 16-lane row, in every lane of it, and lane j of every quad in its four lanes (n, j constants after
@@ -166,6 +167,10 @@ struct Items {
     }
 };
 
+__host__ __device__ __forceinline__ int column_blocks(const PAttnArgs& a, int rt) {
+    return (a.max_rows * (a.nq / a.kv.nkv) + 16 * rt - 1) / (16 * rt);
+}
+
 template <int HD, int G, int RT, bool PAR>
 struct AttnShape {
     static constexpr int NCH = kChunks, CH = kChunk;
@@ -176,12 +181,19 @@ struct AttnShape {
     static constexpr int CG = HD == 128 ? 8 : 4;                                   // columns joined at a time (PAR)
     static constexpr int kWaveBytes = kKeyBytes + 8 * kOffs;
     static constexpr int kJoinBytes = PAR ? kWaves * 16 * RT * 8 : 0;
-    static constexpr int kLds = kWaves * kWaveBytes + kJoinBytes;
+    static constexpr int kLds = kWaves * kWaveBytes + kJoinBytes;                  // (not PAR: no less than PAR's)
     static constexpr int kXBytes = kWaves * CG * (HD + 4) * 4;                     // (the exchange lies over the keys)
     static_assert(!PAR || kXBytes <= kWaves * kWaveBytes, "exchange");
     // Waves of a SIMD that the registers are cut for. More in flight is not more: 64 x 4000 keys on bf16 pages take 192 us
-    // with two waves a SIMD (not PAR), 207 with three; int8 PAR 89 with two, 85 with three, 98 with four.
-    static constexpr int kOcc = HD == 128 ? (RT == 1 && G && PAR ? 3 : 2) : RT == 1 && G ? 2 : 1;
+    // with two waves a SIMD (not PAR), 207 with three; int8 PAR 89 with two, 85 with three, 98 with four. 256-wide heads (32 x
+    // 4099 keys, one, two waves): groups of 32 89 / 81, of 64 83 / 69; of 16 107 / 194, the second wave's registers spill.
+    static constexpr int kOcc = HD == 128 ? (RT == 1 && G && PAR ? 3 : 2) : RT == 1 && G && (G != 16 || PAR) ? 2 : 1;
+    static constexpr int kBlocks = kCUs / 8 * (160 * 1024 / kLds < 4 * kOcc / kWaves ? 160 * 1024 / kLds : 4 * kOcc / kWaves);    // an XCD's at once
+    // Units a block that are left to PAR at most, rather than a round of waves of their own. Measured (PAR / not, us, join
+    // and all): one tile, 128-wide int8, 64 blocks of an XCD: 136 units 30 / 36, 204 units 40 / 37; bf16 the same way, 136
+    // units 35 / 39, 204 units 46 / 43. A wave a SIMD (bf16, 256-wide), 32 blocks: 34 units 36 / 41, 68 units 53 / 44. Two
+    // tiles (the joins double, and a wave's registers), 256-wide, 32 blocks: 42 units left 102 / 94, 68 units 74 / 52.
+    static constexpr unsigned kTail = RT == 2 ? 1 : kOcc == 1 ? 2 : 3;
 };
 
 // One wave's work on one chunk after another: the split's running (m, l, o) of its columns, and the chunk's K, V and scales.
@@ -591,23 +603,16 @@ struct Chunker {
     }
 };
 
+// This block's (PAR) or wave's units from `unit` on, `step` apart, below `end`.
 template <int HD, int G, int RT, bool PAR>
-__global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShape<HD, G, RT, PAR>::kOcc)) void k_paged_attn(PAttnArgs a) {
+__device__ __forceinline__ void attn_units(const PAttnArgs& a, char* lds, Items& items, unsigned unit, unsigned step, unsigned end) {
     using S = AttnShape<HD, G, RT, PAR>;
     using C = Chunker<HD, G, RT, PAR>;
-    extern __shared__ __attribute__((aligned(16))) char lds[];
     const int wv = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const PagedArgs& kv = a.kv;
-    const int grp = a.nq / kv.nkv;
-    // Blocks j and j + 8 run on the same XCD: XCD x takes the pairs x, x + 8, .. with all their kv heads, which share the
-    // lines of the scales; its blocks (waves) take its (pair, head, columns) units in turn.
-    const int ncb = (a.max_rows * grp + 16 * RT - 1) / (16 * RT), per = kv.nkv * ncb;
-    unsigned unit = PAR ? blockIdx.x >> 3 : (blockIdx.x >> 3) * S::kWaves + (unsigned)wv;
-    const unsigned step = (gridDim.x >> 3) * (PAR ? 1 : S::kWaves);
+    const int grp = a.nq / kv.nkv, per = kv.nkv * column_blocks(a, RT);
     char* mine = lds + wv * S::kWaveBytes;
-    Items items;
-    items.load(a, 0, 0);
-    for (;; unit += step) {
+    for (; unit < end; unit += step) {
         const int sub = (int)(unit % (unsigned)per);
         int b, sp;
         if (!items.find(a, (int)(unit / (unsigned)per * 8u + (blockIdx.x & 7u)), b, sp)) return;
@@ -695,7 +700,7 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShap
             float* s_l = s_m + S::kWaves * 16 * RT;
             float* s_o = (float*)lds;
             constexpr int OS = HD + 4;
-            const bool whole = q.len <= kPSplit;      // the sequence has no other split: finished here
+            const bool whole = a.par && q.len <= kPSplit;      // the sequence has no other split: finished here
             if (g == 0) {
 #pragma unroll
                 for (int rt = 0; rt < RT; ++rt) {
@@ -745,6 +750,41 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, PAR>::kWaves), (AttnShap
                 }
             }
         }
+    }
+}
+
+// Blocks j and j + 8 run on the same XCD: XCD x takes the pairs x, x + 8, .. with all their kv heads, which share the lines
+// of the scales; its blocks (waves) take its (pair, head, columns) units in turn. ALL: every unit as PAR. Else the rounds
+// that fill every wave, then what is left as PAR, if that is kTail units a block or fewer, as one more round of waves
+// otherwise: 16 sequences of 4099 keys with 3 rows on 256-wide heads are 136 units for an XCD's 128 waves, 92 us in two rounds,
+// 78 with 8 units left to PAR; 32 of 4097 keys on 128-wide ones 544 for 256, 76 with 32 left, 87 all as PAR. A batch whose
+// units come to little more than two a block gains nothing (48 sequences of 8 to 8190 keys: 38, all as PAR 34, three waves a
+// SIMD).
+template <int HD, int G, int RT, bool ALL>
+__global__ __launch_bounds__((64 * AttnShape<HD, G, RT, ALL>::kWaves), (AttnShape<HD, G, RT, ALL>::kOcc)) void k_paged_attn(PAttnArgs a) {
+    using S = AttnShape<HD, G, RT, ALL>;
+    static_assert(S::kLds >= AttnShape<HD, G, RT, true>::kLds, "the tail's LDS");
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const unsigned xcd = blockIdx.x & 7u, block = blockIdx.x >> 3, blocks = gridDim.x >> 3;
+    Items items;
+    items.load(a, 0, 0);
+    if constexpr (ALL) {
+        attn_units<HD, G, RT, true>(a, lds, items, block, blocks, ~0u);
+    } else {
+        const unsigned wv = (unsigned)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blocks * S::kWaves;
+        unsigned tail = ~0u;
+        if (a.kv.n_seq <= kCounted) {                 // (more sequences are not worth their counting)
+            unsigned n = (unsigned)__builtin_amdgcn_readlane(items.upto, 63);
+            for (int b = 64; b < a.kv.n_seq; b += 64) {
+                Items more;
+                more.load(a, b, (int)n);
+                n = (unsigned)__builtin_amdgcn_readlane(more.upto, 63);
+            }
+            n = n > xcd ? (n - xcd + 7u) / 8u * (unsigned)(a.kv.nkv * column_blocks(a, RT)) : 0u;
+            if (n % waves <= S::kTail * blocks) tail = n - n % waves;
+        }
+        attn_units<HD, G, RT, false>(a, lds, items, block * S::kWaves + wv, waves, tail);
+        if (tail != ~0u) attn_units<HD, G, RT, true>(a, lds, items, tail + block, blocks, ~0u);
     }
 }
 
@@ -900,31 +940,24 @@ static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weight
     return w;
 }
 
-template <int HD, int G, int RT, bool PAR>
+template <int HD, int G, int RT, bool ALL>
 static int launch_split_form(const PAttnArgs& a, long long units, hipStream_t s) {
-    using S = AttnShape<HD, G, RT, PAR>;
+    using S = AttnShape<HD, G, RT, ALL>;
     static std::once_flag attr;
     static hipError_t attr_e = hipSuccess;
-    std::call_once(attr, [] { attr_e = hipFuncSetAttribute((const void*)k_paged_attn<HD, G, RT, PAR>, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds); });
+    std::call_once(attr, [] { attr_e = hipFuncSetAttribute((const void*)k_paged_attn<HD, G, RT, ALL>, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds); });
     Q27X_HIP(attr_e);
     // as many blocks as fit at once, or fewer units, in eights (one per XCD)
-    const int lds_fit = 160 * 1024 / S::kLds, reg_fit = 4 * S::kOcc / S::kWaves;
-    const long long most = (long long)kCUs / 8 * (lds_fit < reg_fit ? lds_fit : reg_fit);
-    const long long need = PAR ? units : (units + S::kWaves - 1) / S::kWaves;
-    hipLaunchKernelGGL((k_paged_attn<HD, G, RT, PAR>), dim3((unsigned)(8 * (need < most ? need : most))), dim3(64 * S::kWaves), S::kLds, s, a);
+    const long long need = ALL ? units : (units + S::kWaves - 1) / S::kWaves;
+    hipLaunchKernelGGL((k_paged_attn<HD, G, RT, ALL>), dim3((unsigned)(8 * (need < S::kBlocks ? need : S::kBlocks))), dim3(64 * S::kWaves), S::kLds, s, a);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
 }
 template <int HD, int G, int RT>
 static int launch_split_rt(PAttnArgs& a, hipStream_t s) {
-    const int ncb = (a.max_rows * (a.nq / a.kv.nkv) + 16 * RT - 1) / (16 * RT);
-    const long long units = ((long long)a.kv.n_seq * a.ns + 7) / 8 * a.kv.nkv * ncb;      // of an XCD, if all sequences have max_len keys
-    // Waves of their own need many splits to fill the CUs; the bound counts max_len keys of every sequence, of which a ragged
-    // batch has fewer. Measured (PAR / not, us), int8, 1 column tile, 128-wide heads: 68 units of an XCD 13 / 22, 544 units
-    // 85 / 82, 1536 by the bound with lengths from 8 to 8190 34 / 38, 2048 units 322 / 285; 256-wide: 63 units 30 / 39, 136
-    // units 55 / 61. bf16, 1024 units: 212 / 193. Two tiles (the joins double, and a wave's registers): 136 units of 256-wide
-    // heads 118 / 93, 544 of 128-wide 199 / 133.
-    a.par = units < (RT == 2 ? 96 : G ? 1792 : 512);
+    using S = AttnShape<HD, G, RT, false>;
+    const long long units = ((long long)a.kv.n_seq * a.ns + 7) / 8 * a.kv.nkv * column_blocks(a, RT);      // of an XCD, if all sequences have max_len keys
+    a.par = units <= S::kTail * S::kBlocks;
     return a.par ? launch_split_form<HD, G, RT, true>(a, units, s) : launch_split_form<HD, G, RT, false>(a, units, s);
 }
 template <int HD, int G>
