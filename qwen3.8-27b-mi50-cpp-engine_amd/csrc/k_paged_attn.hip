@@ -30,7 +30,7 @@
 // Bound: bf16 pages by memory (64 x 4000 keys, 1.05 GB: 191 us, 5.5 TB/s; its loads without the arithmetic 189). int8 pages
 // by both sides, which overlap for the most part (32 x 4097 keys, 302 MB: 76 us; the loads alone 63, the arithmetic on
 // keys in the L2 59). Two column tiles of 256-wide heads by one wave's latencies (16 x 4099 keys, 3 rows, 151 MB: 78 us, the
-// arithmetic alone 74): it has its SIMD to itself, whose vector instructions fill 28% of the time, the matrix ones 18%.
+// arithmetic alone 74): it has its SIMD to itself, and vector instructions fill half of its time, matrix ones a twelfth.
 #include <math.h>
 
 #include <mutex>
