@@ -313,34 +313,36 @@ def test_attention_keys_that_are_not_there(gpu, group):
     assert np.linalg.norm(bf2f(got[0]) - ref * sg) <= 2.0 ** -8 * np.linalg.norm(ref * sg)
 
 
-@pytest.mark.parametrize("max_len", [200, 24576])
-def test_attention_weights_behind_the_table(gpu, max_len):
+@pytest.mark.parametrize("max_len,times", [(200, 1), (24576, 1), (2048, 65)])
+def test_attention_weights_behind_the_table(gpu, max_len, times):
     """The table ends inside a split, chunks before the sequence's length: the keys behind it have no weight, in both forms of
     the split kernel."""
     rng = np.random.default_rng(24)
-    cache = Cache(rng, [200, 80, 60, 199], [3, 1, 2, 3], 2, 128, 32, page=16, cap=80)
-    q, gate = queries(rng, 9, 16, 128)
+    cache = Cache(rng, [200, 80, 60, 199] * times, [3, 1, 2, 3] * times, 2, 128, 32, page=16, cap=80)
+    q, gate = queries(rng, 9 * times, 16, 128)
     got = run_attn(gpu, cache, q, gate, 16, max_len=max_len)
     check_attn(cache, got, q, gate, 16)
     assert (got[3][:3, 80:200] == 0).all()
 
 
+@pytest.mark.parametrize("more", [0, 260])
 @pytest.mark.parametrize("group", [0, 32])
 @pytest.mark.parametrize("hd", [128, 256])
-def test_attention_not_finite_stays_with_its_rows(gpu, group, hd):
-    """A key that is not finite reaches the rows that see it and no other: the new rows before it are as they were."""
+def test_attention_not_finite_stays_with_its_rows(gpu, group, hd, more):
+    """A key that is not finite reaches the rows that see it and no other: the new rows before it are as they were. Alone, and
+    among as many sequences as have a wave walk each split."""
     rng = np.random.default_rng(11)
     for bad in (np.nan, np.inf):
-        cache = Cache(rng, [130, 70], [5, 2], 1, hd, group)
-        q, gate = queries(rng, 7, 4, hd)
-        clean = run_attn(gpu, cache, q, gate, 4)
+        cache = Cache(rng, [130, 70] + [3] * more, [5, 2] + [1] * more, 1, hd, group)
+        q, gate = queries(rng, 7 + more, 4, hd)
+        clean = run_attn(gpu, cache, q, gate, 4, max_len=2048)
         for b, key in ((0, 128), (1, 69)):             # row 3 of 5, row 1 of 2
             s = cache.slot(b, key)
             if group:
                 cache.vs[s], cache.ks[s] = bad, bad
             else:
                 cache.v[s], cache.k[s] = bf(np.full(hd, bad)), bf(np.full(hd, bad))
-        got = run_attn(gpu, cache, q, gate, 4)
+        got = run_attn(gpu, cache, q, gate, 4, max_len=2048)
         for r in (0, 1, 2, 5):
             a, b = bf2f(got[0][r]), bf2f(clean[0][r])
             assert (np.abs(a - b) <= 2.0 ** -7 * np.abs(b) + 2.0 ** -12).all()
@@ -419,6 +421,44 @@ def test_attention_with_room_for_many_keys(gpu, group, geom):
     q, gate = queries(rng, sum(counts), nq, hd)
     got = run_attn(gpu, cache, q, gate, nq, max_len=256 * (1800 * 8 // (len(LENS) * nkv) + 1))
     check_attn(cache, got, q, gate, nq)
+
+
+@pytest.mark.parametrize("group", [0, 16, 32, 64])
+@pytest.mark.parametrize("geom", list(GEOMS))
+def test_attention_many_sequences(gpu, group, geom):
+    """More sequences than are counted ahead: a wave walks each split."""
+    rng = np.random.default_rng(80 + group)
+    nq, nkv, hd = GEOMS[geom]
+    n = 260
+    lens = rng.integers(0, 300, n)
+    lens[:len(LENS)] = LENS
+    counts = rng.integers(0, 3, n) if nq // nkv < 20 else np.ones(n, np.int64)
+    cache = Cache(rng, lens, counts, nkv, hd, group, page=32)
+    q, gate = queries(rng, int(sum(counts)), nq, hd)
+    check_attn(cache, run_attn(gpu, cache, q, gate, nq, max_len=2048), q, gate, nq)
+
+
+@pytest.mark.parametrize("geom,group,rows", [("32x8x128", 32, 1), ("32x8x128", 0, 1), ("32x8x128", 16, 5), ("24x4x256", 0, 1), ("24x4x256", 32, 3),
+                                             ("24x4x256", 16, 1)])
+def test_attention_rounds_and_their_rest(gpu, geom, group, rows):
+    """A few units more than the waves take at once, the rest by whole blocks: within the tolerances, and the bits of a sequence
+    alone, the first, one in between and the last."""
+    rng = np.random.default_rng(90 + group + rows)
+    nq, nkv, hd = GEOMS[geom]
+    n = 130
+    lens = rng.integers(257, 320, n)
+    cache = Cache(rng, lens, [rows] * n, nkv, hd, group, page=32)
+    q, gate = queries(rng, n * rows, nq, hd)
+    got = run_attn(gpu, cache, q, gate, nq)
+    check_attn(cache, got, q, gate, nq)
+    table, start = cache.table, cache.row_start
+    for b in (0, 64, 127, 128, 129):
+        cache.lens, cache.counts = lens[b:b + 1].astype(np.int32), np.array([rows], np.int32)
+        cache.row_start, cache.table = np.array([0, rows], np.int32), table[b:b + 1].copy()
+        r = slice(start[b], start[b] + rows)
+        one = run_attn(gpu, cache, q[r], gate[r], nq)
+        assert np.array_equal(one[0], got[0][r]) and np.array_equal(one[1], got[1][r]) and np.array_equal(one[2], got[2][r]), b
+        assert np.array_equal(one[3][:, :lens[b]], got[3][r, :lens[b]]), b
 
 
 def test_attention_many_heads(gpu):
