@@ -5,8 +5,6 @@
 // in all, ties to the lowest index. Attention does not care for the order of the keys, so nothing is shifted: the keys
 // behind `budget` that stay move into the places of those before it that go, both in ascending order, as many bytes as
 // can be. Source and target positions are disjoint, so the moves need no staging.
-#include <mutex>
-
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -565,10 +563,7 @@ extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w
     a.npairs = (int32_t*)((char*)work + ew.npairs);
     const int most = max_len > high ? min(budget, max_len - budget) : 0;       // moves of a sequence
     if (max_len <= kTiles * kEvThreads) {
-        static std::once_flag attr;
-        static hipError_t attr_e = hipSuccess;
-        std::call_once(attr, [] { attr_e = hipFuncSetAttribute((const void*)k_evict, hipFuncAttributeMaxDynamicSharedMemorySize, kTiles * kEvThreads * 2); });
-        Q27X_HIP(attr_e);
+        Q27X_HIP(allow_lds<k_evict>(kTiles * kEvThreads * 2));
         a.fused = most <= kEvWaves;
         hipLaunchKernelGGL(k_evict, dim3((unsigned)a.kv.n_seq), dim3(kEvThreads), (size_t)most * 4, (hipStream_t)s, a);
     } else {

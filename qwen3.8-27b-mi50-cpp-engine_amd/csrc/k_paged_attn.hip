@@ -33,8 +33,6 @@
 // arithmetic alone 74): it has its SIMD to itself, and vector instructions fill half of its time, matrix ones a twelfth.
 #include <math.h>
 
-#include <mutex>
-
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -943,10 +941,7 @@ static WorkLayout work_layout(int nq, int hd, int max_len, int nrows, int weight
 template <int HD, int G, int RT, bool ALL>
 static int launch_split_form(const PAttnArgs& a, long long units, hipStream_t s) {
     using S = AttnShape<HD, G, RT, ALL>;
-    static std::once_flag attr;
-    static hipError_t attr_e = hipSuccess;
-    std::call_once(attr, [] { attr_e = hipFuncSetAttribute((const void*)k_paged_attn<HD, G, RT, ALL>, hipFuncAttributeMaxDynamicSharedMemorySize, S::kLds); });
-    Q27X_HIP(attr_e);
+    Q27X_HIP((allow_lds<k_paged_attn<HD, G, RT, ALL>>(S::kLds)));
     // as many blocks as fit at once, or fewer units, in eights (one per XCD)
     const long long need = ALL ? units : (units + S::kWaves - 1) / S::kWaves;
     hipLaunchKernelGGL((k_paged_attn<HD, G, RT, ALL>), dim3((unsigned)(8 * (need < S::kBlocks ? need : S::kBlocks))), dim3(64 * S::kWaves), S::kLds, s, a);

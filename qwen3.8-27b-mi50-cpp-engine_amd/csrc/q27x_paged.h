@@ -1,5 +1,7 @@
-// q27x_paged.h -- the paged cache as its kernels see it (k_paged.hip, k_evict.hip).
+// q27x_paged.h -- the paged cache as its kernels see it (k_paged.hip, k_paged_attn.hip, k_evict.hip).
 #pragma once
+#include <atomic>
+
 #include "q27x_dev.h"
 #include "q27x_int.h"
 
@@ -14,6 +16,18 @@ struct PagedArgs {
     const int32_t* lens; const int32_t* row_start;
     int n_seq;
 };
+// Lets kernel K have `bytes` of dynamic LDS on the current device: once per device.
+template <auto K>
+inline hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> known{0};
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (known.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    if (hipError_t e = hipFuncSetAttribute((const void*)K, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    known.fetch_or(bit, std::memory_order_relaxed);
+    return hipSuccess;
+}
 // the caller's handle, checked (negative: its status)
 int paged_args(const q27x_paged_kv_t* kv, const char* who, PagedArgs* out);
 
