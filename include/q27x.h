@@ -309,7 +309,7 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
  * know, keys that ever came; zero state to begin a sequence, acc and ord need no start value. After a
  * rollback pass the shorter lens. new_lens may be kv->lens. A later q27x_paged_attn_rows needs no
  * positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
- * aligned, not shared by calls that may overlap. */
+ * aligned, not shared by calls that may overlap. max_len at most 2^31 - 65537. */
 size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
 int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc,
                      int nrows, float decay, float* acc, int32_t* ord, int acc_stride, int32_t* state,

@@ -18,6 +18,8 @@ struct EvictArgs {
     uint32_t* rank;                 // [n_seq][max_len] the keys' order: larger stays
     int2* pairs;                    // [n_seq][max_len / 2 + 1] (from, to)
     int32_t* npairs;                // [n_seq]
+    uint32_t *parts;                // [n_seq][blocks of k_evict_sums][3] its newest keys, least and largest other rank
+    uint64_t *stay, *same;          // [n_seq][max_len / 64] a bit per key: above the cut, of the cut's rank
     int fused;                      // the kernel that picks also moves
 };
 constexpr int kEvThreads = 1024, kEvWaves = kEvThreads / 64;
@@ -32,7 +34,7 @@ __device__ __forceinline__ uint32_t rank_of(float x) {
 }
 
 constexpr int kTiles = 32, kBins = 2048;
-constexpr int kMaxKeys = 0x7fffffff - 16 * kEvThreads;     // (indexes run over by less than that)
+constexpr int kMaxKeys = 0x7fffffff - 64 * kEvThreads;     // (indexes run over by less than that)
 
 // Exclusive prefix sum over the block's first n <= 1024 values, one a thread; the sum of all in `sum`.
 __device__ __forceinline__ uint32_t scan_block(uint32_t x, uint32_t* red, uint32_t& sum) {
@@ -416,19 +418,45 @@ __global__ __launch_bounds__(kEvThreads) void k_evict(EvictArgs a) {
 
 // The same for longer sequences in two launches, the ranks in memory: sums and ranks by a block for every 8192 keys, then
 // the choice by one block a sequence, each wave walking a run of 64-key steps in order, 16 with their loads together.
-// 131071 keys of which one goes: 149 us, of which half go 156 (digits of eight bits and one launch: 343); bound by the one
-// block's LDS adds and its share of the L2. A limit above the budget has it done once in many steps.
+// 131071 keys of which one goes: 95 us, of which all but 16000 go 112 (sums in the one block, digits of eight bits: 343). Bound
+// by the one block's instructions, some 25 a step of 64 keys and walk, and its LDS adds. A limit above the budget has it done
+// once in many steps.
+__device__ __forceinline__ int sum_blocks(int max_len) { return (max_len + 8 * kEvThreads - 1) / (8 * kEvThreads); }
+__device__ __forceinline__ int mask_words(int max_len) { return (max_len + 63) / 64; }
 __global__ __launch_bounds__(kEvThreads) void k_evict_sums(EvictArgs a) {
-    const int b = blockIdx.y, i0 = (int)blockIdx.x * 8 * kEvThreads + (int)threadIdx.x;
+    const int b = blockIdx.y, t = threadIdx.x, i0 = (int)blockIdx.x * 8 * kEvThreads + t;
+    const int wv = __builtin_amdgcn_readfirstlane(t >> 6);
+    __shared__ uint32_t red[3][kEvWaves];
     const EvictSeq q = evict_seq(a, b);
-    if (i0 - (int)threadIdx.x >= q.len) return;
+    if (i0 - t >= q.len) return;
     uint32_t* rank = a.rank + (size_t)b * a.max_len;
     uint32_t key[8];
     add_up(a, q, i0, key);
     if (!q.over) return;
+    uint32_t lo = kNewest, hi = 0, fixed = 0;
 #pragma unroll
-    for (int u = 0; u < 8; ++u)
+    for (int u = 0; u < 8; ++u) {
         if (i0 + u * kEvThreads < q.len) rank[i0 + u * kEvThreads] = key[u];
+        fixed += (uint32_t)__popcll(__ballot(key[u] == kNewest));
+        if (key[u] != 0 && key[u] != kNewest) {
+            lo = min(lo, key[u]);
+            hi = max(hi, key[u]);
+        }
+    }
+    lo = min_xor64(lo);
+    hi = ~min_xor64(~hi);
+    if ((t & 63) == 0) { red[0][wv] = fixed; red[1][wv] = lo; red[2][wv] = hi; }
+    __syncthreads();
+    if (t == 0) {
+        fixed = 0; lo = kNewest; hi = 0;
+        for (int i = 0; i < kEvWaves; ++i) {
+            fixed += red[0][i];
+            lo = min(lo, red[1][i]);
+            hi = max(hi, red[2][i]);
+        }
+        uint32_t* part = a.parts + ((size_t)b * sum_blocks(a.max_len) + blockIdx.x) * 3;
+        part[0] = fixed; part[1] = lo; part[2] = hi;
+    }
 }
 __global__ __launch_bounds__(kEvThreads) void k_evict_long(EvictArgs a) {
     const int b = blockIdx.x, t = threadIdx.x, l = t & 63;
@@ -443,69 +471,78 @@ __global__ __launch_bounds__(kEvThreads) void k_evict_long(EvictArgs a) {
     const int steps = (len + 63) / 64, run = (steps + kEvWaves - 1) / kEvWaves;
     const int s0 = wv * run, s1 = min(s0 + run, steps);
     constexpr int kDeep = 16;
-    // f(place, rank) for the keys of this wave's run in order; the rank is 0 where there is no key
+    // f(step, rank) for the keys of this wave's run in order; the rank is 0 where there is no key
     auto walk = [&](auto f) __attribute__((always_inline)) {
         for (int st = s0; st < s1; st += kDeep) {
             uint32_t x[kDeep];
 #pragma unroll
             for (int u = 0; u < kDeep; ++u) x[u] = rank[min(64 * (st + u) + l, len - 1)];
 #pragma unroll
-            for (int u = 0; u < kDeep; ++u) {
-                const int i = 64 * (st + u) + l;
-                f(i, st + u < s1 && i < len ? x[u] : 0u);
-            }
+            for (int u = 0; u < kDeep; ++u) f(st + u, st + u < s1 && 64 * (st + u) + l < len ? x[u] : 0u);
         }
     };
-    uint32_t lo = kNewest, hi = 0, fixed = 0;
-    walk([&](int, uint32_t x) __attribute__((always_inline)) {
-        fixed += (uint32_t)__popcll(__ballot(x == kNewest));
-        if (x != 0 && x != kNewest) {
-            lo = min(lo, x);
-            hi = max(hi, x);
-        }
-    });
-    const Cut cut = find_cut(budget, fixed, lo, hi, red, [&](auto f) __attribute__((always_inline)) {
+    uint32_t lo = kNewest, hi = 0, fixed = 0, sum;
+    for (int i = t; i < sum_blocks(len); i += kEvThreads) {
+        const uint32_t* part = a.parts + ((size_t)b * sum_blocks(a.max_len) + i) * 3;
+        fixed += part[0];
+        lo = min(lo, part[1]);
+        hi = max(hi, part[2]);
+    }
+    scan_block(fixed, red, sum);
+    const Cut cut = find_cut(budget, wv == 0 ? sum : 0u, lo, hi, red, [&](auto f) __attribute__((always_inline)) {
         walk([&](int, uint32_t x) __attribute__((always_inline)) { f(x); });
     });
-    const uint32_t top = cut.top, left = cut.left;
-    // how many of rank `top` come before this wave's run tells which of those stay
-    const uint64_t below = (1ull << l) - 1;
-    uint32_t eq0 = 0, sum;
-    if (cut.same != left) {
-        uint32_t n = 0;
-        walk([&](int, uint32_t x) __attribute__((always_inline)) { n += (uint32_t)__popcll(__ballot(x == top)); });
-        eq0 = scan_block(l == 0 ? n : 0u, red, sum);
-        eq0 = __builtin_amdgcn_readfirstlane(eq0);
-    }
-    // the places that fall free before budget and the keys that stay behind it, counted and then written down in order
-    uint32_t holes = 0, h0 = 0, m0 = 0;
-#pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {
-        uint32_t eq = eq0, h = h0, m = m0;
-        walk([&](int i, uint32_t x) __attribute__((always_inline)) {
-            const uint64_t same = __ballot(x == top);
-            const bool stays = x > top || (x == top && eq + (uint32_t)__popcll(same & below) < left);
-            eq += (uint32_t)__popcll(same);
-            const bool falls = x != 0 && !stays && i < budget, moves = stays && i >= budget;
-            const uint64_t hole = __ballot(falls), mover = __ballot(moves);
-            if (pass) {
-                if (falls) q.pairs[h + (uint32_t)__popcll(hole & below)].y = i;
-                if (moves) q.pairs[m + (uint32_t)__popcll(mover & below)].x = i;
-            }
-            h += (uint32_t)__popcll(hole);
-            m += (uint32_t)__popcll(mover);
-        });
-        if (!pass) {
-            h0 = __builtin_amdgcn_readfirstlane(scan_block(l == 0 ? h : 0u, red, holes));
-            m0 = __builtin_amdgcn_readfirstlane(scan_block(l == 0 ? m : 0u, red, sum));
+    uint64_t *stays = a.stay + (size_t)b * mask_words(a.max_len), *sames = a.same + (size_t)b * mask_words(a.max_len);
+    walk([&](int st, uint32_t x) __attribute__((always_inline)) {
+        const uint64_t more = __ballot(x > cut.top), as = __ballot(x == cut.top);
+        if (l == 0 && st < s1) {
+            stays[st] = more;
+            sames[st] = as;
         }
+    });
+    __syncthreads();
+    // as in k_evict, 1024 words of 32 keys at a time: sames so far, places that fall free and keys that move
+    uint32_t eq0 = 0, h0 = 0, m0 = 0;
+    for (int w0 = 0; w0 < 2 * steps; w0 += kEvThreads) {
+        const int w = w0 + t;
+        uint32_t stay = w < 2 * steps ? ((const uint32_t*)stays)[w] : 0u, eq = w < 2 * steps ? ((const uint32_t*)sames)[w] : 0u;
+        if (cut.same == cut.left) {
+            stay |= eq;
+        } else {
+            const uint32_t n = (uint32_t)__popc(eq), before = eq0 + scan_block(n, red, sum);
+            eq0 += sum;
+            for (uint32_t k = before < cut.left ? min(n, cut.left - before) : 0u; k > 0; --k) {
+                stay |= eq & (0u - eq);
+                eq &= eq - 1u;
+            }
+        }
+        const int in = min(max(budget - 32 * w, 0), 32);
+        const uint32_t head = in == 32 ? ~0u : (1u << in) - 1u;
+        uint32_t hole = ~stay & head, mover = stay & ~head;
+        const uint32_t before = scan_block((uint32_t)__popc(hole) | ((uint32_t)__popc(mover) << 16), red, sum);
+        for (uint32_t h = h0 + (before & 0xFFFFu); hole; ++h, hole &= hole - 1u) q.pairs[h].y = 32 * w + __builtin_ctz(hole);
+        for (uint32_t m = m0 + (before >> 16); mover; ++m, mover &= mover - 1u) q.pairs[m].x = 32 * w + __builtin_ctz(mover);
+        h0 += sum & 0xFFFFu;
+        m0 += sum >> 16;
     }
     __syncthreads();
-    if (t == 0) a.npairs[b] = (int)holes;
-    for (uint32_t i = (uint32_t)t; i < holes; i += kEvThreads) {
-        const int2 p = q.pairs[i];
-        q.acc[p.y] = q.acc[p.x];
-        q.ord[p.y] = q.ord[p.x];
+    if (t == 0) a.npairs[b] = (int)h0;
+    for (uint32_t i0 = (uint32_t)t; i0 < h0; i0 += 8 * kEvThreads) {
+        int2 p[8];
+        float x[8];
+        int o[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            p[u] = q.pairs[min(i0 + u * kEvThreads, h0 - 1u)];
+            x[u] = q.acc[p[u].x];
+            o[u] = q.ord[p[u].x];
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (i0 + u * kEvThreads < h0) {
+                q.acc[p[u].y] = x[u];
+                q.ord[p[u].y] = o[u];
+            }
     }
 }
 
@@ -522,13 +559,17 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictArgs a) {
     move_rows<kMoves>(a.kv, b, p, n);
 }
 
-struct EvictWork { size_t rank, pairs, npairs, total; };      // bytes
+struct EvictWork { size_t pairs, stay, same, parts, rank, npairs, total; };      // bytes; those of longer sequences, if any may be
 static EvictWork evict_work(int n_seq, int max_len) {
+    const size_t n = (size_t)n_seq, more = max_len > kTiles * kEvThreads ? n : 0;
     EvictWork w{};
     w.pairs = 0;
-    w.rank = w.pairs + (size_t)n_seq * ((size_t)max_len / 2 + 1) * sizeof(int2);
-    w.npairs = w.rank + (size_t)n_seq * max_len * 4;
-    w.total = w.npairs + (size_t)n_seq * 4;
+    w.stay = w.pairs + n * ((size_t)max_len / 2 + 1) * sizeof(int2);
+    w.same = w.stay + more * (((size_t)max_len + 63) / 64) * 8;
+    w.parts = w.same + more * (((size_t)max_len + 63) / 64) * 8;
+    w.rank = w.parts + more * (((size_t)max_len + 8 * kEvThreads - 1) / (8 * kEvThreads)) * 12;
+    w.npairs = w.rank + more * max_len * 4;
+    w.total = w.npairs + n * 4;
     return w;
 }
 
@@ -560,6 +601,9 @@ extern "C" int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w
     const EvictWork ew = evict_work(a.kv.n_seq, max_len);
     a.pairs = (int2*)((char*)work + ew.pairs);
     a.rank = (uint32_t*)((char*)work + ew.rank);
+    a.parts = (uint32_t*)((char*)work + ew.parts);
+    a.stay = (uint64_t*)((char*)work + ew.stay);
+    a.same = (uint64_t*)((char*)work + ew.same);
     a.npairs = (int32_t*)((char*)work + ew.npairs);
     const int most = max_len > high ? min(budget, max_len - budget) : 0;       // moves of a sequence
     if (max_len <= kTiles * kEvThreads) {

@@ -99,3 +99,13 @@ def test_work_bytes(X):
     assert 0 < e(1, 100) < e(2, 100) and e(0, 100) == e(1, 0) == 0
     # sizes that pass 32 bits
     assert f(32, 128, 131072, 512, 1) > 1 << 33
+
+
+def test_lengths_that_indexes_cannot_run_over(X):
+    """The kernels' indexes go a tile past max_len: lengths within that of 2^31 are refused, the last ones before it not."""
+    big = 2 ** 31 - 65536
+    assert evict(X, cache(X), max_len=big, stride=big, ws=big) == ARG
+    e, f = X.lib().q27x_paged_evict_work_bytes, X.lib().q27x_paged_attn_work_bytes
+    assert e(1, big) == 0 and e(1, big - 1) > 1 << 33
+    assert f(32, 128, 2 ** 31 - 256, 1, 0) == 0 and f(32, 128, 2 ** 31 - 257, 1, 0) > 1 << 36
+    assert attn(X, cache(X), max_len=2 ** 31 - 256) == SHAPE
