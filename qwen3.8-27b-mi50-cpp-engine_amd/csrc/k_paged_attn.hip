@@ -755,9 +755,10 @@ __device__ __forceinline__ void attn_units(const PAttnArgs& a, char* lds, Items&
 // of the scales; its blocks (waves) take its (pair, head, columns) units in turn. ALL: every unit as PAR. Else the rounds
 // that fill every wave, then what is left as PAR, if that is kTail units a block or fewer, as one more round of waves
 // otherwise: 16 sequences of 4099 keys with 3 rows on 256-wide heads are 136 units for an XCD's 128 waves, 92 us in two rounds,
-// 78 with 8 units left to PAR; 32 of 4097 keys on 128-wide ones 544 for 256, 76 with 32 left, 87 all as PAR. A batch whose
-// units come to little more than two a block gains nothing (48 sequences of 8 to 8190 keys: 38, all as PAR 34, three waves a
-// SIMD).
+// 78 with 8 units left to PAR; 32 of 4097 keys on 128-wide ones 544 for 256, 76 with 32 left, 87 all as PAR. Where the rest is
+// two units a block and some, the some go to the waves of as many blocks as they need, in the time of the others' two: 48
+// sequences of 8 to 8190 keys, 128 or 136 units for 64 blocks, 35.5 us, 39 with a third round (a batch that is known to be that
+// small from max_len is better off as PAR with three, 136 units in bf16 34.7 / 38.9).
 template <int HD, int G, int RT, bool ALL>
 __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, ALL>::kWaves), (AttnShape<HD, G, RT, ALL>::kOcc)) void k_paged_attn(PAttnArgs a) {
     using S = AttnShape<HD, G, RT, ALL>;
@@ -770,7 +771,7 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, ALL>::kWaves), (AttnShap
         attn_units<HD, G, RT, true>(a, lds, items, block, blocks, ~0u);
     } else {
         const unsigned wv = (unsigned)__builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), waves = blocks * S::kWaves;
-        unsigned tail = ~0u;
+        unsigned tail = ~0u, wide = 0;                // the rest's first unit, and the blocks whose waves take one each of it
         if (a.kv.n_seq <= kCounted) {                 // (more sequences are not worth their counting)
             unsigned n = (unsigned)__builtin_amdgcn_readlane(items.upto, 63);
             for (int b = 64; b < a.kv.n_seq; b += 64) {
@@ -779,10 +780,13 @@ __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, ALL>::kWaves), (AttnShap
                 n = (unsigned)__builtin_amdgcn_readlane(more.upto, 63);
             }
             n = n > xcd ? (n - xcd + 7u) / 8u * (unsigned)(a.kv.nkv * column_blocks(a, RT)) : 0u;
-            if (n % waves <= S::kTail * blocks) tail = n - n % waves;
+            const unsigned rest = n % waves;
+            if (rest <= S::kTail * blocks) tail = n - rest;
+            if (S::kTail == 3 && tail != ~0u && rest > 2 * blocks) wide = (rest - 2 * blocks + 1) / 2;
         }
-        attn_units<HD, G, RT, false>(a, lds, items, block * S::kWaves + wv, waves, tail);
-        if (tail != ~0u) attn_units<HD, G, RT, true>(a, lds, items, tail + block, blocks, ~0u);
+        const unsigned first = tail + wide * S::kWaves;              // of the units that go as PAR
+        attn_units<HD, G, RT, false>(a, lds, items, block * S::kWaves + wv, waves, block < wide ? first : tail);
+        if (tail != ~0u && block >= wide) attn_units<HD, G, RT, true>(a, lds, items, first + block - wide, blocks - wide, ~0u);
     }
 }
 

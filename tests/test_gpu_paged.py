@@ -438,21 +438,23 @@ def test_attention_many_sequences(gpu, group, geom):
     check_attn(cache, run_attn(gpu, cache, q, gate, nq, max_len=2048), q, gate, nq)
 
 
-@pytest.mark.parametrize("geom,group,rows", [("32x8x128", 32, 1), ("32x8x128", 0, 1), ("32x8x128", 16, 5), ("24x4x256", 0, 1), ("24x4x256", 32, 3),
-                                             ("24x4x256", 16, 1)])
-def test_attention_rounds_and_their_rest(gpu, geom, group, rows):
-    """A few units more than the waves take at once, the rest by whole blocks: within the tolerances, and the bits of a sequence
-    alone, the first, one in between and the last."""
+@pytest.mark.parametrize("geom,group,rows,n,max_len", [("32x8x128", 32, 1, 130, None), ("32x8x128", 0, 1, 130, None),
+                                                       ("32x8x128", 16, 5, 130, None), ("24x4x256", 0, 1, 130, None),
+                                                       ("24x4x256", 32, 3, 130, None), ("24x4x256", 16, 1, 130, None),
+                                                       ("32x8x128", 32, 1, 70, 1024), ("32x8x128", 0, 2, 90, 1024),
+                                                       ("24x4x256", 64, 1, 150, 1024)])
+def test_attention_rounds_and_their_rest(gpu, geom, group, rows, n, max_len):
+    """A few units more than the waves take at once, the rest by whole blocks, or by blocks and some waves: within the tolerances,
+    and the bits of a sequence alone, the first, some in between and the last."""
     rng = np.random.default_rng(90 + group + rows)
     nq, nkv, hd = GEOMS[geom]
-    n = 130
     lens = rng.integers(257, 320, n)
     cache = Cache(rng, lens, [rows] * n, nkv, hd, group, page=32)
     q, gate = queries(rng, n * rows, nq, hd)
-    got = run_attn(gpu, cache, q, gate, nq)
+    got = run_attn(gpu, cache, q, gate, nq, max_len=max_len)
     check_attn(cache, got, q, gate, nq)
     table, start = cache.table, cache.row_start
-    for b in (0, 64, 127, 128, 129):
+    for b in (0, 3, 7, n // 2, n - 3, n - 2, n - 1):
         cache.lens, cache.counts = lens[b:b + 1].astype(np.int32), np.array([rows], np.int32)
         cache.row_start, cache.table = np.array([0, rows], np.int32), table[b:b + 1].copy()
         r = slice(start[b], start[b] + rows)
