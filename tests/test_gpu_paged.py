@@ -734,6 +734,53 @@ def test_evict_pages_that_are_not_there(gpu):
     ev.compare(ev.expect([100, 128], [w[:1], w[1:]], 1.0, 50, 50, 5))
 
 
+def test_writes_past_32_bits(gpu):
+    """Prep and eviction on pages whose bytes lie past 4 GiB of the pool: what they do on near ones."""
+    X, rng = gpu, np.random.default_rng(28)
+    nq, nkv, hd, page, n, rot = 8, 8, 256, 16, 5, 64
+    cache = Cache(rng, [100], [n], nkv, hd, 32, page=page, spare=0)
+    n_pages = (9 << 29) // (nkv * hd * page)                       # 4.5 GiB of codes
+    width = nq * hd + 2 * nkv * hd
+    x, qn, kn = bf(rng.standard_normal((n, width)) * 2), bf(rng.standard_normal(hd) * 0.2), bf(rng.standard_normal(hd) * 0.2)
+    cos, sin = tables(64, rot)
+    w = rng.random((n, 100)).astype(np.float32)
+    near = cache.push(X)
+    parts = (("k", nkv * hd), ("v", nkv * hd), ("ks", nkv * hd // 32 * 4), ("vs", nkv * hd // 32 * 4))
+    far = {name: X.DevBuf(n_pages * page * size) for name, size in parts}
+    table = (n_pages - 1 - np.arange(cache.table.shape[1], dtype=np.int32))[None]
+    for name, size in parts:
+        for j, p in enumerate(cache.table[0]):
+            rows = np.ascontiguousarray(getattr(cache, name)[p * page:(p + 1) * page])
+            X.call("q27x_memcpy_h2d", far[name].ptr + int(table[0, j]) * page * size, rows.ctypes.data, rows.nbytes, None)
+    dt = X.DevBuf(array=np.ascontiguousarray(table))
+    away = X.PagedKV(k=far["k"].ptr, v=far["v"].ptr, ks=far["ks"].ptr, vs=far["vs"].ptr, kv_group=32, nkv=nkv, hd=hd, n_pages=n_pages,
+                     page=page, page_stride=0, table=dt.ptr, table_stride=table.shape[1], lens=cache.d["lens"].ptr,
+                     row_start=cache.d["row_start"].ptr, n_seq=1)
+    dev = [X.DevBuf(array=a) for a in (x, qn, kn, cos, sin, np.arange(n, dtype=np.int32), w)]
+    work = X.DevBuf(X.lib().q27x_paged_evict_work_bytes(1, 100))
+    seen = []
+    for kv in (near, away):
+        qh, new = X.DevBuf(n * nq * hd * 2), X.DevBuf(4)
+        acc, order, state = X.DevBuf(400), X.DevBuf(400), X.DevBuf(array=np.zeros(2, np.int32))
+        X.call("q27x_paged_prep_rows", dev[0].ptr, width, dev[1].ptr, dev[2].ptr, dev[3].ptr, dev[4].ptr, rot, 64, dev[5].ptr, n, 1, None,
+               ctypes.byref(kv), qh.ptr, nq, 0, 1e-6, n, None)
+        X.call("q27x_paged_evict", ctypes.byref(kv), dev[6].ptr, 100, None, n, 1.0, acc.ptr, order.ptr, 100, state.ptr, 60, 50, 10, 100,
+               work.ptr, new.ptr, None)
+        X.call("q27x_device_sync")
+        seen.append([b.download(np.uint8, (b.nbytes,)) for b in (qh, new, acc, order, state)])
+    assert all(np.array_equal(a, b) for a, b in zip(*seen))
+    got = cache.pull()
+    for name, size in parts:
+        assert not np.array_equal(got[name], getattr(cache, name))
+        for j, p in enumerate(cache.table[0]):
+            want = got[name][p * page:(p + 1) * page]
+            back = np.empty_like(want)
+            X.call("q27x_memcpy_d2h", back.ctypes.data, far[name].ptr + int(table[0, j]) * page * size, back.nbytes, None)
+            assert np.array_equal(back.view(np.uint8), np.ascontiguousarray(want).view(np.uint8)), (name, j)
+    for b in far.values():
+        b.free()
+
+
 # ---------------------------------------------------------------- together
 def test_serving_steps(gpu):
     """Steps of a bounded batch as a server runs them: rows prepared into the pages, attention with weights, some verify
