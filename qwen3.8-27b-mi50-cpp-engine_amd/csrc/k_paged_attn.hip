@@ -19,8 +19,10 @@
 // P.V as V^T P^T: the columns' weights are already where the second product wants them (slots 8 g .. of column c: keys
 // 4 g .. of two tiles), and lane (c, g) loads dims c HD/16 .. of keys 4 g .. + 3, so V needs no transpose: byte t of the
 // eight keys is row c of dim tile t. A value is code x scale rounded to fp16, scales first brought to [1, 2) by the power
-// of two of the group's largest (undone in fp32), weights (at most 1) are rounded to fp16: 2^-11 each, below the bf16
-// output's 2^-8. bf16 pages: values exact, weights as two bf16 terms (2^-16).
+// of two of the largest in the chunk and group (undone in fp32), weights (at most 1) are rounded to fp16: 2^-11 each, below
+// the bf16 output's 2^-8, but 2^-25 of the chunk's largest weight or scale where less than 2^-14 of it is left. The chunk's
+// largest is that of the keys that a row sees: where a later row's key would change it so that it shows, the
+// rows' products run one after another. bf16 pages: values exact, weights as two bf16 terms (2^-16).
 //
 // Loads: a vector load costs the texture addresser about 2.3 to 4 cycles per row of the cache that it touches (measured:
 // 8 bytes a lane over 16 rows 67 cycles, over 4 rows 18; 16 bytes a lane over 8 rows 21), so K comes by LDS DMA in whole
@@ -460,9 +462,9 @@ struct Chunker {
         }
         return x;
     }
-    // V of the keys in `in` (others 0) times the weights, joined to o: `single`, added to what is joined, in the columns
-    // that see `key`.
-    template <bool SINGLE>
+    // V of the keys in `in` (others 0) times the weights, joined to o. ONE: added to what is joined, in the columns of the row
+    // whose last key is `key`.
+    template <bool ONE>
     __device__ __forceinline__ void product(uint64_t in, int key) {
         float vs[NT][NS];
         if constexpr (G != 0) {
@@ -499,8 +501,8 @@ struct Chunker {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float x = acc[e & 1][rt][j];
-                    if constexpr (!SINGLE) o[rt][e][j] = __builtin_fmaf(x, fb[rt][j], o[rt][e][j] * f1[rt]);
-                    else o[rt][e][j] = key <= last[rt] ? __builtin_fmaf(x, fb[rt][j], o[rt][e][j]) : o[rt][e][j];
+                    if constexpr (!ONE) o[rt][e][j] = __builtin_fmaf(x, fb[rt][j], o[rt][e][j] * f1[rt]);
+                    else o[rt][e][j] = key == last[rt] ? __builtin_fmaf(x, fb[rt][j], o[rt][e][j]) : o[rt][e][j];
                 }
         };
 #pragma unroll
@@ -536,67 +538,96 @@ struct Chunker {
         }
         join(E - 1);
     }
-    // The chunk's values joined to o. Keys that are not there read something else, maybe not finite, and are left out. Keys
-    // that only later rows see enter too (their weight is 0 in the rows before), unless they hold something that is not
-    // finite: those enter one by one, in the columns that see them.
-    __device__ __forceinline__ void values(const SeqOf& q, int k0, uint64_t valid, int k) {
-        uint64_t enter = valid, later = 0;
-        if (q.raw - q.n < k0 + S::CH - 1) {
-            const int from = q.raw - q.n + 1 - k0;    // the first key that row 0 does not see
-            later = from <= 0 ? valid : valid & ~((1ull << from) - 1);
+    // The largest finite scale among the keys in `in` of group u of the quad's dims.
+    __device__ __forceinline__ float top_scale(uint64_t in, int u) const {
+        float mx = 0.0f;
+#pragma unroll
+        for (int ti = 0; ti < NT; ++ti) {
+            const bool is = (in >> (16 * ti + 4 * g + (c & 3))) & 1;
+            mx = fmaxf(mx, is && finite_f(vsc[ti][u]) ? fabsf(vsc[ti][u]) : 0.0f);
         }
-        if (later) {
-            bool odd = false;
-#pragma unroll
-            for (int ti = 0; ti < NT; ++ti) {
-                if constexpr (G != 0) {
-                    if ((later >> (16 * ti + 4 * g + (c & 3))) & 1) {
-#pragma unroll
-                        for (int u = 0; u < NS; ++u) odd |= !finite_f(vsc[ti][u]);
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        if ((later >> (16 * ti + 4 * g + j)) & 1) {
-#pragma unroll
-                            for (int u = 0; u < VW; ++u)
-                                odd |= (vx[ti][j][u] & 0x7F80u) == 0x7F80u || (vx[ti][j][u] & 0x7F800000u) == 0x7F800000u;
-                        }
-                }
-            }
-            if (__ballot(odd)) enter &= ~later;
-            else later = 0;
-        }
-        // the power of two that brings the largest finite scale of each of the quad's groups to [1, 2), and its inverse
-        // for the output rows 4 g + j (the dims of quad g)
+        return max_cols(max_quad(mx));
+    }
+    __device__ __forceinline__ static int exponent_of(float x) {
+        const int ex = (int)(__float_as_uint(x) >> 23);
+        return ex < 1 ? 1 : ex > 253 ? 253 : ex;
+    }
+    // The power of two that brings the largest finite scale of each of the quad's groups to [1, 2), among the keys in `in`,
+    // and its inverse for the output rows 4 g + j (the dims of quad g).
+    __device__ __forceinline__ void factors(uint64_t in) {
         if constexpr (G != 0) {
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
-                float mx = 0.0f;
-#pragma unroll
-                for (int ti = 0; ti < NT; ++ti) {
-                    const bool in = (valid >> (16 * ti + 4 * g + (c & 3))) & 1;
-                    mx = fmaxf(mx, in && finite_f(vsc[ti][u]) ? fabsf(vsc[ti][u]) : 0.0f);
-                }
-                mx = max_cols(max_quad(mx));
-                int ex = (int)(__float_as_uint(mx) >> 23);
-                ex = ex < 1 ? 1 : ex > 253 ? 253 : ex;
+                const int ex = exponent_of(top_scale(in, u));
                 fac[u] = __uint_as_float((uint32_t)(254 - ex) << 23);
                 back[u] = __shfl(__uint_as_float((uint32_t)ex << 23), (l & 48) + 4 * g, 64);
             }
         }
-        product<false>(enter, 0);
-        while (later) {
-            const int kk = __builtin_ctzll(later);
-            later &= later - 1;
-            const vvec x = v_at(k + kk);
+    }
+    // Whether the rows of the call have to be taken one by one, because a key that only later rows see would change what
+    // the rows before it get. Its weight there is 0, but it counts where it is not finite, and where its scale changes the
+    // factor: powers of two change nothing by themselves, so that takes a value that the larger factor's fp16 holds with
+    // fewer bits (a scale below 2^-14 of the largest), or a factor of the join that fp32 does (from 2^-126 on; the bounds
+    // here are far above). `first`: the keys of the first row that sees any.
+    __device__ __forceinline__ bool apart(uint64_t valid, uint64_t first, uint64_t later) const {
+        bool odd = false;
+        if constexpr (G != 0) {
+            bool moved = false, low = false;
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                const int ex = exponent_of(top_scale(valid, u)), ex0 = exponent_of(top_scale(first, u));
+                moved = moved || ex != ex0;
+                low = low || (ex != ex0 && ex0 < 64);
+#pragma unroll
+                for (int ti = 0; ti < NT; ++ti) {
+                    const int bit = 16 * ti + 4 * g + (c & 3);
+                    const uint32_t x = __float_as_uint(vsc[ti][u]) & 0x7FFFFFFFu;
+                    odd = odd || (((later >> bit) & 1) && x >= 0x7F800000u);
+                    low = low || (ex != ex0 && ((valid >> bit) & 1) && x != 0 && (int)(x >> 23) < ex - 14);
+                }
+            }
+            if (__ballot(moved)) {
+                odd = odd || low;
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) odd = odd || (f2[rt] != 0.0f && f2[rt] < 0x1p-60f);
+            }
+        } else {
 #pragma unroll
             for (int ti = 0; ti < NT; ++ti)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
+                    if ((later >> (16 * ti + 4 * g + j)) & 1) {
 #pragma unroll
-                    for (int u = 0; u < VW; ++u) vx[ti][j][u] = kk == 16 * ti + 4 * g + j ? x[u] : 0u;
-            product<true>(1ull << kk, k0 + kk);
+                        for (int u = 0; u < VW; ++u)
+                            odd = odd || (vx[ti][j][u] & 0x7F80u) == 0x7F80u || (vx[ti][j][u] & 0x7F800000u) == 0x7F800000u;
+                    }
+        }
+        return __ballot(odd) != 0;
+    }
+    // The chunk's values joined to o: those of keys that are there (the others read something else, maybe not finite). All
+    // rows at once where that gives each what it would get alone; else o joins nothing and each row adds its own keys,
+    // values and scales read again: the same roundings, so a row's result is that of its own keys.
+    __device__ __forceinline__ void values(const SeqOf& q, int k0, uint64_t valid, int k) {
+        const int from = q.raw - q.n + 1 - k0;        // the first key that row 0 does not see
+        uint64_t enter = valid;
+        if (from < S::CH) {
+            const uint64_t first = from <= 0 ? valid & 1 : valid & ((1ull << from) - 1), later = from <= 0 ? valid : valid & ~first;
+            if (later && apart(valid, first, later)) enter = 0;
+        }
+        factors(enter);
+        product<false>(enter, 0);
+        if (enter == valid) return;
+#pragma unroll 1
+        for (int i = 0; i < q.nr; ++i) {
+            const int end = from - 1 + i;             // row i's last key of the chunk
+            if (end < 0) continue;
+            const uint64_t in = end >= S::CH - 1 ? valid : valid & ((2ull << end) - 1);
+            asm volatile("" : "+v"(k), "+v"(c), "+v"(g));     // (opaque: nothing is kept over the loop, which spills)
+            load_v(k);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (G != 0) v_here();
+            factors(in);
+            product<true>(in, k0 + end);
         }
     }
 };

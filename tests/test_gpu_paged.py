@@ -386,6 +386,58 @@ def test_attention_bits_do_not_depend_on_the_batch(gpu, group):
             assert np.array_equal(one[3][0, :cache.lens[0]], w[r, :cache.lens[0]]), (b, i)
 
 
+# (lengths, rows, the row of each whose own key is the large one): inside a chunk, across one's end, at one's first key, the
+# first key of a split, the last row, eight rows
+LARGE = [([130, 66, 65, 257, 40, 300], [3, 3, 2, 2, 3, 8], [1, 2, 1, 1, 2, 4]),
+         ([70, 129, 513, 20, 261, 8], [3, 2, 3, 5, 8, 8], [2, 1, 1, 3, 7, 2])]
+
+
+@pytest.mark.parametrize("factor", [2.0 ** 10, 2.0 ** 16, 2.0 ** 24, 2.0 ** 32, np.inf, np.nan])
+@pytest.mark.parametrize("more", [0, 260])
+@pytest.mark.parametrize("geom,group", [("4x1x128", 16), ("4x1x128", 32), ("4x1x128", 64), ("4x1x128", 0), ("6x1x256", 16),
+                                        ("6x1x256", 32), ("6x1x256", 64), ("6x1x256", 0)])
+def test_attention_values_of_later_keys(gpu, geom, group, more, factor):
+    """One of a call's rows has a value far above the others', or one that is not finite: every row has the bits of its single
+    step, and the rows that do not see it stay within the bound that their own keys' values give. Alone, and among as many
+    sequences as have a wave walk each split."""
+    nq, nkv, hd = GEOMS[geom]
+    for seed, (lens, counts, which) in enumerate(LARGE):
+        rng = np.random.default_rng(300 + seed)
+        few, n = len(lens), sum(counts)
+        cache = Cache(rng, lens + [3] * more, counts + [1] * more, nkv, hd, group, page=16)
+        part = slice(0, None if seed else 1)                        # (of the scales: one group, or all)
+        for b in range(few):
+            s = cache.slot(b, lens[b] - counts[b] + which[b])
+            if group:
+                cache.vs[s, part] *= np.float32(factor)
+            else:
+                with np.errstate(invalid="ignore"):
+                    cache.v[s, ::1 if seed else 32] = bf(bf2f(cache.v[s, ::1 if seed else 32]) * np.float32(factor))
+        q, gate = queries(rng, n + more, nq, hd)
+        out, xq, xs, w = run_attn(gpu, cache, q, gate, nq, max_len=2048)
+        table, start = cache.table, cache.row_start
+        for b in range(few):
+            for i in range(counts[b]):
+                r, m = start[b] + i, lens[b] - counts[b] + i + 1
+                cache.lens, cache.counts = np.array([m], np.int32), np.array([1], np.int32)
+                cache.row_start, cache.table = np.array([0, 1], np.int32), table[b:b + 1].copy()
+                one = run_attn(gpu, cache, q[r:r + 1], gate[r:r + 1], nq)
+                alike = (one[0][0] == out[r]) | (np.isnan(bf2f(one[0][0])) & np.isnan(bf2f(out[r])))
+                assert alike.all(), (b, i, int((~alike).sum()))
+                assert np.array_equal(one[3][0, :m], w[r, :m]), (b, i)
+                if i >= which[b] or m <= 0:
+                    continue
+                assert np.array_equal(one[1][0], xq[r]) and np.array_equal(one[2][0], xs[r])
+                ref, mag, _, big = attention(cache, bf2f(q[r:r + 1]).astype(np.float64), nq)
+                sg = sigmoid(bf2f(gate[r:r + 1]).astype(np.float64))
+                d = 2 * (hd + 8) * U * big[0]
+                rel = 2 * 2.0 ** -11 + 2 * d + (m + 64) * U + 2.0 ** -20
+                own = cache.rows(b=0, n=m)                          # (below 2^-14: 2^-25 of the largest value that the row sees)
+                small = 2.0 ** -24 * m * (np.abs(cache.vs[own]).max() * 127 if group else 0.0)
+                tol = 2.0 ** -8 * np.abs(ref * sg) + sg * (rel * mag + small)
+                assert (np.abs(bf2f(out[r:r + 1]) - ref * sg) <= tol).all(), (b, i)
+
+
 @pytest.mark.parametrize("geom,group", [("4x1x128", 32), ("6x1x256", 32), ("4x1x128", 0), ("6x1x256", 16)])
 @pytest.mark.parametrize("rows", [1, 5])
 def test_attention_bits_of_a_large_batch(gpu, geom, group, rows):
