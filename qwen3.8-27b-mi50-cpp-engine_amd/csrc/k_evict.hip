@@ -75,9 +75,9 @@ __device__ __forceinline__ EvictSeq evict_seq(const EvictArgs& a, int b) {
     int len = min(a.kv.lens[b], a.max_len);
     len = len < cap ? len : (int)cap;
     q.len = len < 0 ? 0 : len;
-    const int known = a.state[2 * b];
-    q.total = a.state[2 * b + 1];
-    q.known = min(known < 0 ? 0 : known, q.len);
+    const int known = max(a.state[2 * b], 0);
+    q.known = min(known, q.len);
+    q.total = a.state[2 * b + 1] - (known - q.known);         // (keys that were taken back came last: their numbers are free again)
     q.now = q.total + q.len - q.known;
     q.rows = a.w ? min(n, a.nrows - q.first) : 0;
     if (a.n_acc) q.rows = min(q.rows, a.n_acc[b]);

@@ -133,7 +133,8 @@ def attention(cache, q, nq, max_len=None):
 def evict(acc, ord_, state, n, w_rows, decay, high, budget, recent):
     """One sequence: acc, ord_ float32 / int32 rows, changed in place; w_rows the accepted rows' weights. Returns the new
     length and the moves [(from, to)]."""
-    known, total = min(max(int(state[0]), 0), n), int(state[1])
+    known = min(max(int(state[0]), 0), n)
+    total = int(state[1]) - (max(int(state[0]), 0) - known)        # (keys taken back are the last that came)
     now = total + n - known
     acc[:known] = acc[:known] * np.float32(decay)
     acc[known:n] = 0
@@ -144,7 +145,8 @@ def evict(acc, ord_, state, n, w_rows, decay, high, budget, recent):
     if n <= high:
         state[0] = n
         return n, []
-    new = ord_[:n] >= now - recent
+    new = np.zeros(n, bool)
+    new[np.argsort(-ord_[:n].astype(np.int64), kind="stable")[:recent]] = True
     key = [(-2, 0.0, i) if new[i] else (0, 0.0, i) if np.isnan(acc[i]) else (-1, -float(acc[i]), i) for i in range(n)]
     stays = np.zeros(n, bool)
     stays[[k[2] for k in sorted(key)[:budget]]] = True

@@ -772,6 +772,39 @@ def test_evict_after_a_rollback_and_lens_in_place(gpu):
         ev.compare(ev.expect(lens, [w[:1], w[1:]], 0.75, 64, 50, 9), new=cache.d["lens"])
 
 
+@pytest.mark.parametrize("known,left,budget,recent", [(60, 52, 40, 9), (60, 52, 48, 9), (60, 59, 58, 58), (1500, 1490, 20, 20),
+                                                      (40000, 39000, 30000, 5000), (40000, 39999, 39998, 7)])
+def test_evict_cut_after_a_rollback(gpu, known, left, budget, recent):
+    """Keys are taken back, then the cache is cut: of those that are left the newest stay, though the sums want them least, and
+    the keys that come next are numbered behind them."""
+    X, rng = gpu, np.random.default_rng(known + budget)
+    cache = Cache(rng, [known, 7], [1, 1], 1, 128, 64, page=64)
+    cache.push(X)
+    ev = Evictor(X, cache, known)
+    w = (rng.integers(1, 9, (2, known)) / 8).astype(np.float32)
+    w[0, left - recent - known // 8:] = 0
+    dw = X.DevBuf(array=w)
+    ev.call(dw.ptr, known, None, 2, 1.0, known, known, recent, known)
+    cache.d["lens"].upload(np.array([left, 7], np.int32))
+    ev.call(dw.ptr, known, None, 2, 1.0, budget, budget, recent, known)
+    # no cut before: key i is the i-th that came, and the sums are twice the weights
+    old = sorted(range(left - recent), key=lambda i: (-w[0, i], i))[:budget - recent]
+    stays = np.zeros(left, bool)
+    stays[old], stays[left - recent:] = True, True
+    want = np.arange(left)
+    want[np.flatnonzero(~stays[:budget])] = np.flatnonzero(stays[budget:]) + budget
+    got = ev.dev[1].download(np.int32, (2, known))[0, :budget]
+    assert np.array_equal(got, want[:budget])
+    assert np.array_equal(ev.dev[0].download(np.float32, (2, known))[0, :budget], 2 * w[0, want[:budget]])
+    k, first = cache.pull()["k"], cache.rows(0, left)
+    assert np.array_equal(k[first[:budget]], cache.k[first[want[:budget]]])
+    assert ev.new.download(np.int32, (2,)).tolist() == [budget, 7]
+    cache.d["lens"].upload(np.array([budget + 1, 7], np.int32))
+    ev.call(None, 0, None, 2, 1.0, budget + 1, budget, recent, known)
+    assert ev.dev[1].download(np.int32, (2, known))[0, budget] == left
+    assert ev.dev[2].download(np.int32, (2, 2)).tolist() == [[budget + 1, left + 1], [7, 7]]
+
+
 def test_evict_pages_that_are_not_there(gpu):
     """Keys on missing pages are summed and ordered like the others; their rows are not copied. A table that ends early cuts
     the sequence."""
