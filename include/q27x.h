@@ -306,10 +306,12 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
  * that stay move, with cache rows, acc and ord, into the places before it that fall free, both in
  * ascending order: the cache's order is not kept, what lies behind new_lens is left as it was.
  * ord [n_seq][acc_stride]: how many keys came before each; state [n_seq][2]: keys that acc and ord
- * know, keys that came; zero state to begin a sequence, acc and ord need no start value. Below state[b][0]
- * lens takes back keys that came since the sequence was last cut (none before a cut: the order has changed): the next
- * ones get their numbers. new_lens may be kv->lens. A later q27x_paged_attn_rows needs no
- * positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
+ * know, keys that came; zero state to begin a sequence, acc and ord need no start value. lens here is
+ * without the keys of rejected rows: attention's lens less those, of which a cut would make kept
+ * keys, the newest, that no shorter lens reaches. A lens below state[b][0] takes back keys that came
+ * since the sequence was last cut (none from before a cut: the order has changed); the next ones get
+ * their numbers. new_lens may be kv->lens where no other layer's call is still to read that. A later
+ * q27x_paged_attn_rows needs no positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
  * aligned, not shared by calls that may overlap. max_len at most 2^31 - 65537. */
 size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
 int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc,

@@ -907,6 +907,49 @@ def test_serving_steps(gpu):
         assert kv.n_seq == 3 and lens.max() <= 64
 
 
+def test_layers_of_a_step_with_rejected_rows(gpu):
+    """Two layers' caches on one table and one lens, verify rows of which some are rejected, a cut in most steps: the rejected
+    rows are out of lens before a layer's eviction, and the last layer's writes it. No cache keeps a rejected key."""
+    X, rng = gpu, np.random.default_rng(32)
+    nq, nkv, hd, rot, cap = 8, 2, 128, 32, 96
+    lens = np.array([58, 5, 33], np.int32)
+    layers = [Cache(rng, lens, [1, 1, 1], nkv, hd, 32, page=16, cap=cap) for _ in range(2)]
+    layers[1].table = layers[0].table
+    evs = []
+    for cache in layers:
+        cache.push(X)
+        evs.append(Evictor(X, cache, cap))
+    gone, cuts = [[], []], 0
+    for step in range(8):
+        counts = rng.integers(1, 6, 3).astype(np.int32)
+        taken = np.array([rng.integers(1, c + 1) for c in counts], np.int32)
+        start = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        kept, new = X.DevBuf(array=lens + taken), None
+        for i, (cache, ev) in enumerate(zip(layers, evs)):
+            cache.counts, cache.lens, cache.row_start = counts, lens + counts, start
+            q, got, ref = run_prep(X, cache, rng, (nq, nkv, hd), rot, 3, [j % 3 for j in range(16)], True)
+            for name, a in got.items():
+                setattr(cache, name, a)
+            gate = bf(rng.standard_normal(q.shape))
+            res = run_attn(X, cache, q, gate, nq)
+            check_attn(cache, res, q, gate, nq)
+            gone[i] += [cache.k[cache.slot(b, p)].copy() for b in range(3) for p in range(lens[b] + taken[b], lens[b] + counts[b])]
+            full = np.zeros((len(res[3]), cap), np.float32)
+            full[:, :res[3].shape[1]] = res[3][:, :cap]
+            cache.push(X).lens = kept.ptr
+            dw, da = X.DevBuf(array=full), X.DevBuf(array=taken)
+            ev.call(dw.ptr, cap, da.ptr, len(full), 1.0, 60, 56, 8, cap, new=kept.ptr if i == 1 else None)
+            rows = [full[start[b]:start[b] + taken[b]] for b in range(3)]
+            new = np.array(ev.expect(lens + taken, rows, 1.0, 60, 56, 8), np.int32)
+            ev.compare(new, new=kept if i == 1 else None)
+        cuts += int((new < lens + taken).sum())
+        lens = new
+        for cache, bad in zip(layers, gone):
+            held = np.concatenate([cache.k[cache.rows(b, lens[b])] for b in range(3)])
+            assert not any((held == x).all(1).any() for x in bad)
+    assert cuts >= 3
+
+
 class _Graph:
     """A captured sequence of calls (HIP's graph functions, from the runtime that the library runs on)."""
 
