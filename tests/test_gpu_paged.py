@@ -950,6 +950,42 @@ def test_layers_of_a_step_with_rejected_rows(gpu):
     assert cuts >= 3
 
 
+def test_prompts_in_steps_of_a_few_rows(gpu):
+    """Two prompts behind what is there, prepared by one call: their attention sequence by sequence, eight rows at a time, and
+    both together with the rows of a step side by side, has the same bits, within the bounds."""
+    X, rng = gpu, np.random.default_rng(34)
+    nq, nkv, hd, rot = 8, 2, 128, 32
+    past, rows = [10, 0], [37, 21]
+    cache = Cache(rng, [a + b for a, b in zip(past, rows)], rows, nkv, hd, 32, page=16)
+    q, got, ref = run_prep(X, cache, rng, (nq, nkv, hd), rot, 3, [i % 3 for i in range(16)], True)
+    check_prep(cache, q, got, ref, rot)
+    for name, a in got.items():
+        setattr(cache, name, a)
+    gate = bf(rng.standard_normal(q.shape))
+    table, start = cache.table, [0, rows[0]]
+
+    def attend(seqs, at):
+        """Rows at .. at + 7 of the sequences' prompts, those there are."""
+        cache.counts = np.array([min(max(rows[b] - at, 0), 8) for b in seqs], np.int32)
+        cache.lens = np.array([past[b] + min(rows[b], at + 8) for b in seqs], np.int32)
+        cache.row_start = np.concatenate([[0], np.cumsum(cache.counts)]).astype(np.int32)
+        cache.table = np.ascontiguousarray(table[seqs])
+        pick = np.concatenate([np.arange(start[b] + at, start[b] + at + n) for b, n in zip(seqs, cache.counts)]).astype(np.int64)
+        res = run_attn(X, cache, np.ascontiguousarray(q[pick]), np.ascontiguousarray(gate[pick]), nq, max_rows=8)
+        check_attn(cache, res, q[pick], gate[pick], nq)
+        return pick, res[0]
+
+    alone, both = np.zeros_like(q), np.zeros_like(q)
+    for b in (0, 1):
+        for at in range(0, rows[b], 8):
+            pick, out = attend([b], at)
+            alone[pick] = out
+    for at in range(0, max(rows), 8):
+        pick, out = attend([0, 1], at)
+        both[pick] = out
+    assert np.array_equal(alone, both)
+
+
 class _Graph:
     """A captured sequence of calls (HIP's graph functions, from the runtime that the library runs on)."""
 
