@@ -310,7 +310,9 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
  * without the keys of rejected rows: attention's lens less those, of which a cut would make kept
  * keys, the newest, that no shorter lens reaches. A lens below state[b][0] takes back keys that came
  * since the sequence was last cut (none from before a cut: the order has changed); the next ones get
- * their numbers. new_lens may be kv->lens where no other layer's call is still to read that. A later
+ * their numbers. new_lens may be kv->lens where no other layer's call is still to read that. A
+ * sequence that can be cut has every page below lens: a key on a missing page is summed and chosen
+ * like others, but its row is not copied, neither from there nor to there. A later
  * q27x_paged_attn_rows needs no positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
  * aligned, not shared by calls that may overlap. max_len at most 2^31 - 65537. */
 size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
