@@ -288,8 +288,13 @@ int q27x_paged_prep_rows(const uint16_t* qkv, int qkv_stride, const uint16_t* q_
  * quantization (nullable). A row that sees no key gets zeros. w (nullable): the weight that each
  * key got from the row, summed over its query heads, w[row][0 .. min(lens, max_len)-1] (0 where
  * the row does not see it; nothing behind is written), rows w_stride >= max_len apart: what q27x_paged_evict takes.
- * A row's bits depend on its own keys only, not on the batch or the rows beside it. work: scratch of
- * q27x_paged_attn_work_bytes bytes (weights: with w), 16-byte aligned, not shared by calls that may
+ * A row's bits depend on its own keys only, not on the batch or the rows beside it. Scores, softmax
+ * sums and the products' sums are fp32, as q27x_attn_rows has them; what enters P.V is rounded, which that
+ * call does not: over int8 pages the weights e^(x - m) and the values code * scale to fp16, 2^-11 each
+ * (of 64 neighbouring keys, a weight below 2^-14 of the largest by an absolute 2^-25 of it, a value
+ * below 2^-14 of the group's largest scale by 2^-25 of that), over bf16 pages the weights to 2^-16. work: scratch
+ * of q27x_paged_attn_work_bytes bytes (weights: with w), about 4 nrows nq (hd + 2) per 256 keys of
+ * max_len, and 4 nrows nq 260 more with weights; 16-byte aligned, not shared by calls that may
  * overlap; 0 for counts that the call refuses. */
 size_t q27x_paged_attn_work_bytes(int nq, int hd, int max_len, int nrows, int weights);
 int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_stride,
@@ -299,7 +304,8 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
 
 /* Eviction by accumulated attention weight, one layer's cache. For every sequence b and its keys
  * i < len = min(lens[b], max_len): acc[b][i] = ((decay*acc[b][i]) + w[r0][i]) + w[r1][i] ... over its
- * first n_acc[b] rows (NULL: all; w NULL: none; the rows that speculation rejected left out), in
+ * first n_acc[b] rows (NULL: all; w NULL: none; the rows that speculation rejected left out, and
+ * those that attention did not compute), in
  * fp32; keys that came since the last call start from 0. Where len > high, the `recent` newest keys
  * and the heaviest others stay, `budget` in all (recent <= budget <= high; ties to the lowest index,
  * a sum that is not a number below all others), and new_lens[b] = budget, else len. Keys behind budget

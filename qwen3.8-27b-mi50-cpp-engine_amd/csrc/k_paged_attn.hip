@@ -22,7 +22,10 @@
 // of two of the largest in the chunk and group (undone in fp32), weights (at most 1) are rounded to fp16: 2^-11 each, below
 // the bf16 output's 2^-8, but 2^-25 of the chunk's largest weight or scale where less than 2^-14 of it is left. The chunk's
 // largest is that of the keys that a row sees: where a later row's key would change it so that it shows, the
-// rows' products run one after another. bf16 pages: values exact, weights as two bf16 terms (2^-16).
+// rows' products run one after another. One fp16 term each is a choice: of 16 x 4099 keys the outputs are 1.662e-3 from
+// the 64-bit ones (relative, whole tensor), 1.646e-3 with two terms each, which is the bf16 output's own rounding; two cost
+// 14 to 19% (16 x 4099 keys, 3 rows, 256-wide 77 -> 91 us, 32 x 4097 keys, 128-wide 75.5 -> 89.7), and two for the weights alone
+// change next to nothing (1.659e-3, 77 -> 82 us). bf16 pages: values exact, weights as two bf16 terms (2^-16).
 //
 // Loads: a vector load costs the texture addresser about 2.3 to 4 cycles per row of the cache that it touches (measured:
 // 8 bytes a lane over 16 rows 67 cycles, over 4 rows 18; 16 bytes a lane over 8 rows 21), so K comes by LDS DMA in whole
@@ -167,6 +170,8 @@ struct Items {
     }
 };
 
+// Units side by side for a kv head's columns. More than 32 of them (16 RT at a time) read the keys again: 16 x 4099 keys of 24 / 4
+// heads take 55 us with one row (6 columns), 78 with three (18), 133 with eight (48, two units).
 __host__ __device__ __forceinline__ int column_blocks(const PAttnArgs& a, int rt) {
     return (a.max_rows * (a.nq / a.kv.nkv) + 16 * rt - 1) / (16 * rt);
 }
@@ -187,6 +192,10 @@ struct AttnShape {
     // Waves of a SIMD that the registers are cut for. More in flight is not more: 64 x 4000 keys on bf16 pages take 192 us
     // with two waves a SIMD (not PAR), 207 with three; int8 PAR 89 with two, 85 with three, 98 with four. 256-wide heads (32 x
     // 4099 keys, one, two waves): groups of 32 89 / 81, of 64 83 / 69; of 16 107 / 194, the second wave's registers spill.
+    // Some forms spill a little all the same, in bytes a lane (not PAR): two tiles of 256 dims by 16 368, of 128 dims by 16 116,
+    // of 128 dims bf16 32, one tile of 256 dims by 32 12. Their times beside groups that do not: 16 x 4099 keys, 3 rows,
+    // 256-wide by 16 113 us, by 32 78, by 64 72; 32 x 4097 keys, 8 rows, 128-wide by 16 145, by 32 124, bf16 155 (1.8 times
+    // the bytes).
     static constexpr int kOcc = HD == 128 ? (RT == 1 && G && PAR ? 3 : 2) : RT == 1 && G && (G != 16 || PAR) ? 2 : 1;
     static constexpr int kBlocks = kCUs / 8 * (160 * 1024 / kLds < 4 * kOcc / kWaves ? 160 * 1024 / kLds : 4 * kOcc / kWaves);    // an XCD's at once
     // Units a block that are left to PAR at most, rather than a round of waves of their own. Measured (PAR / not, us, join
@@ -788,7 +797,7 @@ __device__ __forceinline__ void attn_units(const PAttnArgs& a, char* lds, Items&
 // otherwise: 16 sequences of 4099 keys with 3 rows on 256-wide heads are 136 units for an XCD's 128 waves, 92 us in two rounds,
 // 78 with 8 units left to PAR; 32 of 4097 keys on 128-wide ones 544 for 256, 76 with 32 left, 87 all as PAR. Where the rest is
 // two units a block and some, the some go to the waves of as many blocks as they need, in the time of the others' two: 48
-// sequences of 8 to 8190 keys, 128 or 136 units for 64 blocks, 35.5 us, 39 with a third round (a batch that is known to be that
+// sequences of 8 to 8190 keys, 128 or 136 units for 64 blocks, 34.6 us, 39 with a third round (a batch that is known to be that
 // small from max_len is better off as PAR with three, 136 units in bf16 34.7 / 38.9).
 template <int HD, int G, int RT, bool ALL>
 __global__ __launch_bounds__((64 * AttnShape<HD, G, RT, ALL>::kWaves), (AttnShape<HD, G, RT, ALL>::kOcc)) void k_paged_attn(PAttnArgs a) {
