@@ -284,16 +284,17 @@ int q27x_paged_prep_rows(const uint16_t* qkv, int qkv_stride, const uint16_t* q_
 
 /* q27x_attn_rows for many sequences over their pages: row i of a sequence's n rows (1 .. max_rows,
  * at most 8; further ones are left as they were) sees keys 0 .. lens - n + i, of which those below
- * max_len are read; out = bf16(softmax(q.k/sqrt(hd)) v * sigmoid(gate)) [nrows][nq*hd]; xq/xs its per-16
- * quantization (nullable). A row that sees no key gets zeros. w (nullable): the weight that each
- * key got from the row, summed over its query heads, w[row][0 .. min(lens, max_len)-1] (0 where
- * the row does not see it; nothing behind is written), rows w_stride >= max_len apart: what q27x_paged_evict takes.
- * A row's bits depend on its own keys only, not on the batch or the rows beside it. Scores, softmax
- * sums and the products' sums are fp32, as q27x_attn_rows has them; what enters P.V is rounded, which that
- * call does not: over int8 pages the weights e^(x - m) and the values code * scale to fp16, 2^-11 each
- * (of 64 neighbouring keys, a weight below 2^-14 of the largest by an absolute 2^-25 of it, a value
- * below 2^-14 of the group's largest scale by 2^-25 of that), over bf16 pages the weights to 2^-16. work: scratch
- * of q27x_paged_attn_work_bytes bytes (weights: with w), about 4 nrows nq (hd + 2) per 256 keys of
+ * max_len are read; out = bf16(softmax(q.k/sqrt(hd)) v * sigmoid(gate)) [nrows][nq*hd]; xq/xs its
+ * per-16 quantization (nullable). A row that sees no key, or none above -inf, gets zeros. w
+ * (nullable): the weight that each key got from the row, summed over its query heads, w[row][0 ..
+ * min(lens, max_len)-1] (0 where the row does not see it; nothing behind is written), rows w_stride
+ * >= max_len apart: what q27x_paged_evict takes. A row's bits depend on its own keys only, not on
+ * the batch or the rows beside it. Scores, softmax sums and the products' sums are fp32, as
+ * q27x_attn_rows has them; what enters P.V is rounded, which that call does not: over int8 pages
+ * the weights e^(x - m) and the values code * scale to fp16, 2^-11 each (of 64 neighbouring keys, a
+ * weight below 2^-14 of the largest by an absolute 2^-25 of it, a value below 2^-14 of the group's
+ * largest scale by 2^-25 of that), over bf16 pages the weights to 2^-16. work: scratch of
+ * q27x_paged_attn_work_bytes bytes (weights: with w), about 4 nrows nq (hd + 2) per 256 keys of
  * max_len, and 4 nrows nq 260 more with weights; 16-byte aligned, not shared by calls that may
  * overlap; 0 for counts that the call refuses. */
 size_t q27x_paged_attn_work_bytes(int nq, int hd, int max_len, int nrows, int weights);
@@ -305,22 +306,22 @@ int q27x_paged_attn_rows(const uint16_t* qh, const uint16_t* qkv_gate, int qkv_s
 /* Eviction by accumulated attention weight, one layer's cache. For every sequence b and its keys
  * i < len = min(lens[b], max_len): acc[b][i] = ((decay*acc[b][i]) + w[r0][i]) + w[r1][i] ... over its
  * first n_acc[b] rows (NULL: all; w NULL: none; the rows that speculation rejected left out, and
- * those that attention did not compute), in
- * fp32; keys that came since the last call start from 0. Where len > high, the `recent` newest keys
- * and the heaviest others stay, `budget` in all (recent <= budget <= high; ties to the lowest index,
- * a sum that is not a number below all others), and new_lens[b] = budget, else len. Keys behind budget
- * that stay move, with cache rows, acc and ord, into the places before it that fall free, both in
- * ascending order: the cache's order is not kept, what lies behind new_lens is left as it was.
- * ord [n_seq][acc_stride]: how many keys came before each; state [n_seq][2]: keys that acc and ord
- * know, keys that came; zero state to begin a sequence, acc and ord need no start value. lens here is
- * without the keys of rejected rows: attention's lens less those, of which a cut would make kept
- * keys, the newest, that no shorter lens reaches. A lens below state[b][0] takes back keys that came
- * since the sequence was last cut (none from before a cut: the order has changed); the next ones get
- * their numbers. new_lens may be kv->lens where no other layer's call is still to read that. A
- * sequence that can be cut has every page below lens: a key on a missing page is summed and chosen
- * like others, but its row is not copied, neither from there nor to there. A later
- * q27x_paged_attn_rows needs no positions, since the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte
- * aligned, not shared by calls that may overlap. max_len at most 2^31 - 65537. */
+ * those that attention did not compute), in fp32; keys that came since the last call start from 0.
+ * Where len > high, the `recent` newest keys and the heaviest others stay, `budget` in all (recent
+ * <= budget <= high; ties to the lowest index, a sum that is not a number below all others), and
+ * new_lens[b] = budget, else len. Keys behind budget that stay move, with cache rows, acc and ord,
+ * into the places before it that fall free, both in ascending order: the cache's order is not kept,
+ * what lies behind new_lens is left as it was. ord [n_seq][acc_stride]: how many keys came before
+ * each; state [n_seq][2]: keys that acc and ord know, keys that came; zero state to begin a
+ * sequence, acc and ord need no start value. lens here is without the keys of rejected rows:
+ * attention's lens less those, of which a cut would make kept keys, the newest, that no shorter
+ * lens reaches. A lens below state[b][0] takes back keys that came since the sequence was last cut
+ * (none from before a cut: the order has changed); the next ones get their numbers. new_lens may be
+ * kv->lens where no other layer's call is still to read that. A sequence that can be cut has every
+ * page below lens: a key on a missing page is summed and chosen like others, but its row is not
+ * copied, neither from there nor to there. A later q27x_paged_attn_rows needs no positions, since
+ * the rotation is in the keys. work: q27x_paged_evict_work_bytes bytes, 16-byte aligned, not shared
+ * by calls that may overlap. max_len at most 2^31 - 65537. */
 size_t q27x_paged_evict_work_bytes(int n_seq, int max_len);
 int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, const int32_t* n_acc,
                      int nrows, float decay, float* acc, int32_t* ord, int acc_stride, int32_t* state,

@@ -351,6 +351,40 @@ def test_attention_not_finite_stays_with_its_rows(gpu, group, hd, more):
             assert not np.isfinite(bf2f(got[0][r])).any()
 
 
+@pytest.mark.parametrize("rows", [1, 4])
+def test_attention_scores_of_minus_infinity(gpu, rows):
+    """Keys whose score is -inf have no weight; a row that has no other gets zeros, in a chunk, a split and the whole."""
+    rng = np.random.default_rng(35)
+    lens = [300, 70, 600]
+    cache = Cache(rng, lens, [rows] * 3, 1, 128, 0, page=16)
+    q, gate = queries(rng, 3 * rows, 4, 128)
+    q[..., 0] = bf(np.float32(1.0))
+    low = [np.arange(300), np.arange(0, 70, 2), np.arange(0, 512)]
+    for b, keys in enumerate(low):
+        cache.k[cache.rows(b, lens[b])[keys], 0] = 0xFF80
+    out, _, _, w = run_attn(gpu, cache, q, gate, 4)
+    assert (bf2f(out[:rows]) == 0).all() and (w[:rows, :300] == 0).all()
+    for b in (1, 2):
+        slots = cache.rows(b, lens[b])
+        K, V = cache.values(0, slots)[:, 0], cache.values(1, slots)[:, 0]
+        for i in range(rows):
+            r = b * rows + i
+            see = np.setdiff1d(np.arange(lens[b] - rows + i + 1), low[b])
+            total = np.zeros(lens[b])
+            for h in range(4):
+                x = K[see] @ bf2f(q[r, h]).astype(np.float64) / np.sqrt(128)
+                p = np.exp(x - x.max())
+                p /= p.sum()
+                total[see] += p
+                sg = sigmoid(bf2f(gate[r, h]).astype(np.float64))
+                want, mag = p @ V[see] * sg, p @ np.abs(V[see]) * sg
+                # (128 + 8 fp32 roundings of a score of at most 60 in all, twice; 2^-16 for the weights' two terms)
+                rel = 4 * 136 * U * 60 + 2.0 ** -16
+                assert (np.abs(bf2f(out[r, h]) - want) <= 2.0 ** -8 * np.abs(want) + rel * mag).all()
+            assert (w[r, low[b]] == 0).all()
+            assert (np.abs(w[r, :lens[b]] - total) <= (4 * 136 * U * 60 + 2.0 ** -16) * total).all()
+
+
 def test_attention_value_scales_of_any_size(gpu):
     """Value scales far from 1, different by group: every group keeps its own precision."""
     rng = np.random.default_rng(12)
@@ -436,6 +470,30 @@ def test_attention_values_of_later_keys(gpu, geom, group, more, factor):
                 small = 2.0 ** -24 * m * (np.abs(cache.vs[own]).max() * 127 if group else 0.0)
                 tol = 2.0 ** -8 * np.abs(ref * sg) + sg * (rel * mag + small)
                 assert (np.abs(bf2f(out[r:r + 1]) - ref * sg) <= tol).all(), (b, i)
+
+
+@pytest.mark.parametrize("std", [1.5, 12.0])
+@pytest.mark.parametrize("size", [2.0 ** -110, 2.0 ** -70, 2.0 ** 90])
+@pytest.mark.parametrize("factor", [2.0 ** 7, 2.0 ** 11, 2.0 ** 13, 2.0 ** 14])
+def test_attention_values_of_later_keys_near_the_limits(gpu, factor, size, std):
+    """Ratios of scales around what one factor holds, with scales near the ends of what fp32 does, and weights down to none
+    beside an earlier chunk's: the rows have the bits of their single steps."""
+    rng = np.random.default_rng(310)
+    nq, nkv, hd = 6, 1, 256
+    lens, counts, which = LARGE[0]
+    cache = Cache(rng, lens, counts, nkv, hd, 32, page=16)
+    cache.vs *= np.float32(size)
+    for b in range(len(lens)):
+        cache.vs[cache.slot(b, lens[b] - counts[b] + which[b])] *= np.float32(factor)
+    q, gate = queries(rng, sum(counts), nq, hd, std=std)
+    out = run_attn(gpu, cache, q, gate, nq, max_len=2048)[0]
+    table, start = cache.table, cache.row_start
+    for b in range(len(lens)):
+        for i in range(counts[b]):
+            cache.lens, cache.counts = np.array([lens[b] - counts[b] + i + 1], np.int32), np.array([1], np.int32)
+            cache.row_start, cache.table = np.array([0, 1], np.int32), table[b:b + 1].copy()
+            r = start[b] + i
+            assert np.array_equal(run_attn(gpu, cache, q[r:r + 1], gate[r:r + 1], nq)[0][0], out[r]), (b, i)
 
 
 @pytest.mark.parametrize("geom,group", [("4x1x128", 32), ("6x1x256", 32), ("4x1x128", 0), ("6x1x256", 16)])
