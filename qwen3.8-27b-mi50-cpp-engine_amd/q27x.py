@@ -56,6 +56,12 @@ class I8G(ctypes.Structure):
                 ("rows", ctypes.c_int), ("K", ctypes.c_int)]
 
 
+class NVFP4(ctypes.Structure):
+    """q27x_nvfp4_t: E2M1 codes, two a byte, and an E4M3 scale per 16 (device pointers)."""
+    _fields_ = [("w", ctypes.c_void_p), ("s", ctypes.c_void_p), ("alpha", ctypes.c_float),
+                ("rows", ctypes.c_int), ("K", ctypes.c_int)]
+
+
 class PagedKV(ctypes.Structure):
     """q27x_paged_kv_t: a pool of pages and the sequences that lie on them (device pointers)."""
     _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("ks", ctypes.c_void_p), ("vs", ctypes.c_void_p),
@@ -84,6 +90,8 @@ _SIGS = {
     "q27x_quant_weights_i8g64": ([VP, I, I, VP, VP, VP], I),
     "q27x_proj_rows": ([VP, VP, I, VP, VP, I, I, VP, I, I, F, I, VP], I),
     "q27x_proj_partials": ([VP, VP, I, VP, I, VP], I),
+    "q27x_proj_nvfp4_rows": ([VP, VP, I, VP, VP, I, I, VP, I, I, F, I, VP], I),
+    "q27x_swiglu_nvfp4_rows": ([VP, VP, VP, I, VP, VP, VP, F, I, VP], I),
     "q27x_i8g64_to_grp": ([VP, VP, I, I, I, VP, VP, VP], I),
     "q27x_quant_tok_groups": ([VP, I, I, I, I, VP, VP, VP], I),
     "q27x_gemm_i8g": ([VP, VP, I, I, I, F, VP, VP, I, VP, I, VP, I, F, VP], I),
