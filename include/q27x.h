@@ -360,6 +360,24 @@ int q27x_paged_evict(const q27x_paged_kv_t* kv, const float* w, int w_stride, co
 int q27x_argmax_rows(const float* logits, int n, int ld, int nr, int32_t* idx, float* val,
                      q27x_stream_t s);
 
+/* A token a row from n logits (fp32, or bf16 with logits_bf16), where q27x_argmax_rows takes the largest (the reference's host
+ * sampler, src/q27_main.cpp:2975-3007, with given random numbers, for every row of a batch, on the device). In order of falling
+ * logits, equal ones by index, without those that are not finite, and with w = e^((l - l0) / temperature), l0 the largest:
+ *   top_k >= 1 keeps the first top_k; top_p < 1 of these the fewest first ones whose w reach top_p of their sum (one at least);
+ *   min_p > 0 of these those with w >= min_p (one at least); idx = the first token whose running sum of w passes u times the sum of
+ *   what is kept, prob (nullable) = its w over that sum.
+ * temperature, top_k, top_p, min_p, u: device [nr], read by the kernels (a captured graph follows them); each but u may be NULL
+ * (temperature 1, no cut). temperature not above 0: the largest logit, as q27x_argmax_rows (top_p, min_p then cut nothing). u in
+ * [0, 1); outside: the nearest token of the kept ones. No finite logit: idx 0, prob 0. Weights are whole multiples of 2^-44 (below
+ * 2^-45 of the largest: 0, never drawn) and their sums exact, so nr, other rows and the order of atomics change nothing.
+ * n <= 524288. Rows are ld elements apart. Sampled verify rows go into q27x_accept as they are: a draft kept where the token drawn
+ * from the row is that draft, and otherwise that token, is speculative sampling for greedy drafts. work:
+ * q27x_sample_work_bytes bytes, 16-byte aligned, not shared by calls that may overlap; 0 for counts that the call refuses. */
+size_t q27x_sample_work_bytes(int n, int nr);
+int q27x_sample_rows(const void* logits, int logits_bf16, int n, int ld, int nr, const float* temperature,
+                     const int32_t* top_k, const float* top_p, const float* min_p, const float* u, void* work,
+                     int32_t* idx, float* prob, q27x_stream_t s);
+
 /* R20 greedy acceptance on the device: nacc = longest prefix with nx[j] == dt[j] (j < k),
  * ncommit = nacc + 1, committed = nx[0..nacc] (src/q27_main.cpp:2811-2812, 2929-2932). */
 int q27x_accept(const int32_t* nx, const int32_t* dt, int k, int32_t* nacc_ncommit,

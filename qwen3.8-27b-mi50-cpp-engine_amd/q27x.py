@@ -113,6 +113,8 @@ _SIGS = {
     "q27x_paged_evict_work_bytes": ([I, I], SZ),
     "q27x_paged_evict": ([VP, VP, I, VP, I, F, VP, VP, I, VP, I, I, I, I, VP, VP, VP], I),
     "q27x_argmax_rows": ([VP, I, I, I, VP, VP, VP], I),
+    "q27x_sample_work_bytes": ([I, I], SZ),
+    "q27x_sample_rows": ([VP, I, I, I, I, VP, VP, VP, VP, VP, VP, VP, VP, VP], I),
     "q27x_accept": ([VP, VP, I, VP, VP, VP], I),
     "q27x_math_test": ([VP, VP, I, I, VP], I),
     "q27x_config_default": ([VP], I), "q27x_config_tiny": ([VP], I),
