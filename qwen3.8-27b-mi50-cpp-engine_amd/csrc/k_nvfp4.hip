@@ -5,14 +5,19 @@
 //   y[n][r] = alpha sum_s dot_s (ws[r][s] xs[n][s]),  dot_s = sum of 16 products code x code, exact (multiples of 1/2 below 2^14).
 //
 // The codes go into the matrix instructions as they lie in memory: v_mfma_scale_f32_16x16x128_f8f6f4 takes one operand in E2M1
-// and the other in E4M3. An int8 code is 16 h + l, l its low nibble (0 .. 15) and h = h' - 8: E4M3 reads a byte 0 .. 15 as that
-// many 2^-9 exactly (subnormals, then the first binade), so nibbles are operands without a conversion, the instruction's own
-// power of two per operand (E8M0) supplies 2^9 and the 16, and the -8 comes from a constant operand, -8 where the others
-// hold codes. A slab has scales of its own on both sides, so slabs may not be summed by the instruction: row 4 n + i of the
-// activation operand holds slab i of row n and zeros elsewhere, and the 16 x 16 result has the dots of 4 slabs of 4 rows with
-// 16 weight rows. A quarter of the operand's lanes hold something; the matrix cores have the time.
-#include "q27x_dev.h"
-#include "q27x_int.h"
+// and the other in E4M3. An int8 code is 16 h + l, l its low nibble (0 .. 15) and h = -8 .. 7: E4M3 reads a byte 0 .. 15 as that
+// many 2^-9 exactly (subnormals, then the first binade), so nibbles are operands without a conversion, h as sign and size, and the
+// instruction's own power of two per operand (E8M0) supplies 2^9 and the 16. A slab has scales of its own on both sides, so
+// slabs may not be summed by the instruction: row 8 n + i of the activation operand holds slab i of row n and zeros elsewhere, and the
+// 16 x 16 result has the dots of 8 slabs of a pair of rows with 16 weight rows. An eighth of the operand holds something; the
+// matrix cores have the time.
+//
+// Bound by memory for few rows: 62080 x 5120, 1 row, 179 MB in 30.6 us (5.85 TB/s; a kernel that only reads them so, 26.0). What it
+// takes: whole 128-byte lines of 8 rows a load, exchanged in registers (16 rows by 64 bytes, which are operands at once, read
+// at 5.0 TB/s and no more); scales of several steps in one load; blocks that stay and keep the activations, prepared, in LDS (a block
+// a tile: 49.5 us, a third of it spent on them); the next tile on its way while one is worked on. For 8 rows by the LDS reads of the
+// activation operands (20 of 16 bytes a lane for 4096 weights): 55 us.
+#include "q27x_paged.h"
 
 namespace q27x {
 
@@ -32,220 +37,388 @@ struct Nvfp4Args {
     int8_t* oq; float* os; float g;                              // SwiGLU: codes and scales of v / in_scale, g = 1 / in_scale
 };
 
-constexpr int kNvTile = 128;          // weights of a row that a matrix instruction takes
-constexpr int kNvWaves = 8;           // waves of a block at most; they share K
+constexpr int kNvStep = 256;          // weights of a row that a wave takes at a time: a 128-byte line of codes
+constexpr int kNvSteps = 5;           // steps of a wave in registers
+constexpr int kNvWaves = 16;          // waves of a block at most
+constexpr int kNvItems = 3;           // slabs of activations that a thread brings at a time
+constexpr int kNvLds = 160 * 1024;
+constexpr int kNvMaxK = 65536;        // (the slots' sums have room in LDS)
 
-// Tile kt's operands of a wave: lane (c, g) = (lane & 15, lane >> 4) has the codes 32 g .. of weight row c, the scales of that
-// row, slabs g and 4 + g of activation row c / 4 if c % 4 == g, and the scales of activation row g.
-template <int RT, int SETS>
-struct Nvfp4Tile {
-    u32x4 w[RT];
-    u32x2 ws[RT];
-    u32x4 x[SETS][2];
-    f32x4 xs[SETS][2];
-};
-
-template <int RT, int SETS, bool SWIGLU>
-struct Nvfp4Wave {
-    using Tile = Nvfp4Tile<RT, SETS>;
-    const uint8_t* w[RT]; const uint8_t* s[RT];
-    const int8_t* x[SETS]; const float* xs[SETS];
-    bool has[SETS];                                  // this lane holds activation codes
-    int g;
-    float acc[RT][SETS];                             // activation row g (of each four), weight row c
-
-    __device__ __forceinline__ void begin(const Nvfp4Args& a, int l) {
-        const int c = l & 15;
-        g = l >> 4;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            const int r = SWIGLU ? (int)blockIdx.x * 16 + c : ((int)blockIdx.x * RT + t) * 16 + c;
-            const size_t row = (size_t)(r < a.rows ? r : a.rows - 1);       // (rows past the last read it again)
-            w[t] = a.w[SWIGLU ? t : 0] + row * (size_t)(a.K >> 1);
-            s[t] = a.s[SWIGLU ? t : 0] + row * (size_t)(a.K >> 4);
-        }
-#pragma unroll
-        for (int u = 0; u < SETS; ++u) {
-            const int rx = 4 * u + (c >> 2), ry = 4 * u + g;
-            has[u] = (c & 3) == g && rx < a.nr;
-            x[u] = a.xq + (size_t)(rx < a.nr ? rx : 0) * a.xstride;
-            xs[u] = a.xs + (size_t)(ry < a.nr ? ry : 0) * (a.xstride >> 4);
-#pragma unroll
-            for (int t = 0; t < RT; ++t) acc[t][u] = 0.0f;
-        }
-    }
-    __device__ __forceinline__ void load(Tile& b, int kt) const {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            b.w[t] = __builtin_nontemporal_load((const u32x4u*)(w[t] + (size_t)kt * 64 + 16 * g));
-            b.ws[t] = *(const u32x2u*)(s[t] + (size_t)kt * 8);
-        }
-#pragma unroll
-        for (int u = 0; u < SETS; ++u) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                b.x[u][h] = u32x4{0, 0, 0, 0};
-                if (has[u]) b.x[u][h] = *(const u32x4u*)(x[u] + (size_t)kt * 128 + 64 * h + 16 * g);
-                b.xs[u][h] = *(const f32x4u*)(xs[u] + (size_t)kt * 8 + 4 * h);
-            }
-        }
-    }
-    // a last tile of n (1 to 7) slabs: zeros behind them
-    __device__ __forceinline__ void load_end(Tile& b, int kt, int n) const {
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                u32x2 v = {0, 0};
-                if (2 * g + h < n) v = *(const u32x2u*)(w[t] + (size_t)kt * 64 + 16 * g + 8 * h);
-                b.w[t][2 * h] = v[0];
-                b.w[t][2 * h + 1] = v[1];
-                uint32_t e = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (4 * h + j < n) e |= (uint32_t)s[t][(size_t)kt * 8 + 4 * h + j] << (8 * j);
-                b.ws[t][h] = e;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < SETS; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                b.x[u][h] = u32x4{0, 0, 0, 0};
-                if (has[u] && 4 * h + g < n) b.x[u][h] = *(const u32x4u*)(x[u] + (size_t)kt * 128 + 64 * h + 16 * g);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) b.xs[u][h][j] = 4 * h + j < n ? xs[u][(size_t)kt * 8 + 4 * h + j] : 0.0f;
-            }
-    }
-    static __device__ __forceinline__ f32x4 dots(const i32x8& x, const u32x4& w, const f32x4& c, int scale) {
-        const i32x8 b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 0, 4, 0, scale, 0, 127);
-    }
-    // slabs 0 .. 3 (H = 0) or 4 .. 7 of the activation operand: its first or second half
-    template <int H>
-    static __device__ __forceinline__ i32x8 half(const u32x4& v) {
-        if constexpr (H == 0) return i32x8{(int)v[0], (int)v[1], (int)v[2], (int)v[3], 0, 0, 0, 0};
-        else return i32x8{0, 0, 0, 0, (int)v[0], (int)v[1], (int)v[2], (int)v[3]};
-    }
-    template <int H>
-    __device__ __forceinline__ void add_half(const Tile& b, const float (&sc)[RT][8]) {
-        constexpr int kOne = 127 + 9, k16 = kOne + 4;               // bytes are 2^-9 each
-        i32x8 lo[SETS], hi[SETS], minus[SETS];
-#pragma unroll
-        for (int u = 0; u < SETS; ++u) {
-            const uint32_t eight = has[u] ? 0x08080808u : 0u;
-            u32x4 l4, h4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                l4[i] = b.x[u][H][i] & 0x0F0F0F0Fu;
-                h4[i] = ((b.x[u][H][i] >> 4) & 0x0F0F0F0Fu) ^ eight;
-            }
-            lo[u] = half<H>(l4);
-            hi[u] = half<H>(h4);
-            const uint32_t m = has[u] ? 0x88888888u : 0u;
-            minus[u] = half<H>(u32x4{m, m, m, m});
-        }
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int u = 0; u < SETS; ++u) {
-                f32x4 d = dots(minus[u], b.w[t], f32x4{0.0f, 0.0f, 0.0f, 0.0f}, k16);
-                d = dots(lo[u], b.w[t], d, kOne);
-                d = dots(hi[u], b.w[t], d, k16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[t][u] = __builtin_fmaf(d[j], sc[t][4 * H + j] * b.xs[u][H][j], acc[t][u]);
-            }
-    }
-    __device__ __forceinline__ void add(const Tile& b) {
-        float sc[RT][8];
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const auto p = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.ws[t][h], false), q = __builtin_amdgcn_cvt_pk_f32_fp8((int)b.ws[t][h], true);
-                sc[t][4 * h] = p[0]; sc[t][4 * h + 1] = p[1]; sc[t][4 * h + 2] = q[0]; sc[t][4 * h + 3] = q[1];
-            }
-        add_half<0>(b, sc);
-        add_half<1>(b, sc);
+// LDS of a block: activation nibbles of its rows as operands, [rows][steps][low | high][256], and their scales, [rows][16
+// steps]; before them what lanes without activation codes read; behind them the waves' scales, the sums, [2][groups]
+// [slots][32 PAIRS], and the weights of a last step that K does not fill, for each group codes [16][128] and scales [16][16].
+struct Nvfp4Lds {
+    static constexpr int kZeros = 512 * kNvSteps;
+    int row, xs, ws, sums, tail, total;
+    __host__ __device__ __forceinline__ Nvfp4Lds(int rows, int steps, int per, int groups, int waves, int slots, int outs, bool ends_inside) {
+        row = 512 * steps;
+        xs = kZeros + rows * row;
+        ws = xs + 64 * rows * steps;
+        sums = ws + 256 * (per | 1) * groups * waves;
+        tail = sums + 8 * groups * slots * outs;
+        total = tail + (ends_inside ? 2304 * groups : 0);
     }
 };
 
-// Block = 16 RT weight rows (SWIGLU: 16 of gate and the same 16 of up), its waves take K's tiles in turn and are summed in
-// wave order.
-template <int RT, int SETS, bool SWIGLU>
-__global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a) {
-    __shared__ float s_sum[kNvWaves][RT][SETS][64];
-    const int t = threadIdx.x, l = t & 63, wv = __builtin_amdgcn_readfirstlane(t >> 6), waves = (int)blockDim.x >> 6;
-    Nvfp4Wave<RT, SETS, SWIGLU> v;
-    v.begin(a, l);
-    const int full = a.K / kNvTile, rest = (a.K % kNvTile) >> 4;
-    typename Nvfp4Wave<RT, SETS, SWIGLU>::Tile cur, next;
-    if (wv < full) v.load(cur, wv);
-    for (int kt = wv; kt < full; kt += waves) {
-        if (kt + waves < full) v.load(next, kt + waves);
-        v.add(cur);
-        cur = next;
+// Loads from `bytes` bytes at p, the same in every lane; what lies behind them reads as 0, without a branch.
+struct Span {
+    __amdgpu_buffer_rsrc_t r;
+    __device__ __forceinline__ Span(const void* p, uint32_t bytes) {
+        const uint64_t x = (uint64_t)(uintptr_t)p;
+        const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)x), hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32));
+        r = __builtin_amdgcn_make_buffer_rsrc((void*)(uintptr_t)((uint64_t)hi << 32 | lo), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00027000);
     }
-    if (rest && wv == full % waves) {
-        v.load_end(cur, full, rest);
-        v.add(cur);
+    __device__ __forceinline__ u32x4 ld16(uint32_t at) const { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 0)); }
+    __device__ __forceinline__ u32x4 ld16_nt(uint32_t at) const { return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, (int)at, 0, 2)); }
+    __device__ __forceinline__ float ldf(uint32_t at) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0)); }
+};
+
+// A wave's codes: up to kNvSteps steps of 16 rows, as they come: lane l has the codes 128 (l / 4 % 2) + 32 (l / 16) .. of a
+// step of rows r and 8 + r, r = l % 4 + 4 (l / 8 % 2), so a load covers 8 rows of a whole line. Exchanged between lanes 4
+// apart, register h has codes 128 h + 32 (l / 16) .. of row row_of(l % 16): an operand. The scales of all steps come together,
+// 16 per bytes of a row after another, and go through the wave's own LDS, [16][16 (per | 1)] (an odd number of 16 bytes apart).
+__device__ __forceinline__ int nvfp4_row_of(int c) { return 8 * ((c >> 2) & 1) + 4 * ((c >> 3) & 1) + (c & 3); }
+struct Nvfp4Weights {
+    static constexpr int kScales = (16 * kNvSteps + 63) / 64;
+    u32x4 w[kNvSteps][2];
+    u32x4 s[kScales];
+    uint32_t at[2], sat[kScales], sto[kScales];      // this lane's bytes from the tile's beginning, and in LDS
+
+    __device__ __forceinline__ void begin(int K, int per) {
+        const int l = threadIdx.x & 63, r = (l & 3) + 4 * ((l >> 3) & 1), piece = 4 * ((l >> 2) & 1) + (l >> 4);
+        at[0] = (uint32_t)r * (uint32_t)(K >> 1) + 16 * piece;
+        at[1] = at[0] + 8 * (uint32_t)(K >> 1);
+#pragma unroll
+        for (int i = 0; i < kScales; ++i) {
+            const uint32_t k = (uint32_t)(l + 64 * i), row = k / (uint32_t)per, j = k - row * (uint32_t)per;
+            sat[i] = row < 16 ? row * (uint32_t)(K >> 4) + 16 * j : 0x40000000u;
+            sto[i] = row < 16 ? (row * (uint32_t)(per | 1) + j) * 16 : ~0u;
+        }
     }
+    struct Tile {
+        Span w, s;
+        __device__ __forceinline__ Tile(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile)
+            : w(w_ + (size_t)16 * tile * (size_t)(K >> 1), (uint32_t)max(0, min(16, rows - 16 * tile)) * (uint32_t)(K >> 1)),
+              s(s_ + (size_t)16 * tile * (size_t)(K >> 4), (uint32_t)max(0, min(16, rows - 16 * tile)) * (uint32_t)(K >> 4)) {}
+    };
+    // step st of the tile into place j, if `is` (rows behind the last are 0). Always the same loads: where there is no step they
+    // read nothing, so that the waits for others know how many are on their way.
+    __device__ __forceinline__ void load(const Tile& from, int j, int st, bool is) {
+        const uint32_t wo = is ? (uint32_t)st * 128 : 0x80000000u;
+        w[j][0] = from.w.ld16_nt(at[0] + wo);
+        w[j][1] = from.w.ld16_nt(at[1] + wo);
+    }
+    // the scales of steps st .. (those of whole steps: `most` bytes of a row are)
+    __device__ __forceinline__ void load_scales(const Tile& from, int st, int per, int full) {
+        const int l = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < kScales; ++i) {
+            const uint32_t k = (uint32_t)(l + 64 * i), j = k % (uint32_t)per;
+            s[i] = from.s.ld16(st + (int)j < full ? sat[i] + (uint32_t)st * 16 : 0x80000000u);
+        }
+    }
+    __device__ __forceinline__ void store_scales(char* lds) const {
 #pragma unroll
-        for (int u = 0; u < SETS; ++u) s_sum[wv][i][u][l] = v.acc[i][u];
-    __syncthreads();
-    constexpr int kOut = SWIGLU ? SETS * 64 : RT * SETS * 64;
-    for (int i = t; i < kOut; i += (int)blockDim.x) {
-        const int c = i & 15, n = (i >> 4) % (4 * SETS), tile = SWIGLU ? 0 : i / (64 * SETS);
-        auto total = [&](int tl) {
-            float y = 0.0f;
-            for (int k = 0; k < waves; ++k) y = y + s_sum[k][tl][n >> 2][(n & 3) * 16 + c];
-            return y;
-        };
-        if constexpr (SWIGLU) {
-            const float gate = a.alpha[0] * total(0), up = a.alpha[1] * total(1);
-            const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
-            const float sc = max_xor(fabsf(z), 16) * (1.0f / 127.0f);
-            const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-            if (n < a.nr) {
-                const size_t at = (size_t)n * a.rows + (size_t)blockIdx.x * 16 + c;
-                a.oq[at] = qcode(z, inv);
-                if (c == 0) a.os[at >> 4] = sc;
+        for (int i = 0; i < kScales; ++i)
+            if (sto[i] != ~0u) *(u32x4*)(lds + sto[i]) = s[i];
+    }
+    // the tile's last step, of `rest` slabs, into LDS by `threads` threads, and from there into place j
+    static __device__ void bring(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile, char* lds, int rest, int t, int threads) {
+        for (int i = t; i < 16 * 16; i += threads) {
+            const int k = i & 15, row = 16 * tile + (i >> 4);
+            u32x2 v = {0, 0};
+            uint8_t e = 0;
+            if (k < rest && row < rows) {
+                const size_t end = (size_t)(K >> 4) - rest;
+                v = *(const u32x2u*)(w_ + (size_t)row * (size_t)(K >> 1) + 8 * (end + k));
+                e = s_[(size_t)row * (size_t)(K >> 4) + end + k];
             }
-        } else {
-            const int r = ((int)blockIdx.x * RT + tile) * 16 + c;
-            if (n < a.nr && r < a.rows) {
-                float y = a.alpha[0] * total(tile);
+            *(u32x2*)(lds + 8 * i) = v;
+            lds[2048 + i] = (char)e;
+        }
+    }
+    __device__ __forceinline__ void take(const char* lds, int j) {
+        const int l = threadIdx.x & 63, r = (l & 3) + 4 * ((l >> 3) & 1), piece = 4 * ((l >> 2) & 1) + (l >> 4);
+        w[j][0] = *(const u32x4*)(lds + 128 * r + 16 * piece);
+        w[j][1] = *(const u32x4*)(lds + 128 * (8 + r) + 16 * piece);
+    }
+    __device__ __forceinline__ u32x4 operand(int j, int h) const {
+        u32x4 v;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int x = (int)w[j][0][i], y = (int)w[j][1][i];
+            v[i] = (uint32_t)(h == 0 ? __builtin_amdgcn_update_dpp(x, y, 0x114, 0xF, 0xA, false) : __builtin_amdgcn_update_dpp(y, x, 0x104, 0xF, 0x5, false));
+        }
+        return v;
+    }
+};
+
+// A thread's share of some activation rows: up to kNvItems slabs.
+struct Nvfp4Rows {
+    u32x4 x[kNvItems];
+    float xs[kNvItems];
+    // slabs first .. + count - 1 of rows r0 .. + n - 1 (zeros behind K and of rows that are not); items from `item` on
+    __device__ __forceinline__ void load(const Nvfp4Args& a, int r0, int n, int first, int count, int item) {
+        const Span xq_(a.xq, (uint32_t)(a.nr - 1) * (uint32_t)a.xstride + (uint32_t)a.K);
+        const Span xs_(a.xs, (uint32_t)(a.nr - 1) * (uint32_t)(a.xstride >> 2) + (uint32_t)(a.K >> 2));
+#pragma unroll
+        for (int i = 0; i < kNvItems; ++i) {
+            const uint32_t k = (uint32_t)(item + (int)threadIdx.x + i * (int)blockDim.x), r = k / (uint32_t)count, slab = first + (k - r * (uint32_t)count);
+            const bool there = (int)r < n && r0 + (int)r < a.nr && (int)slab < (a.K >> 4);
+            const uint32_t off = (uint32_t)(r0 + (int)r) * (uint32_t)a.xstride + slab * 16;
+            x[i] = xq_.ld16(there ? off : 0x80000000u);
+            xs[i] = xs_.ldf(there ? off >> 2 : 0x80000000u);
+        }
+    }
+    // codes 16 h + l: l = 0 .. 15, h = -8 .. 7 as sign and size
+    __device__ __forceinline__ void store(char* lds, const Nvfp4Lds& L, int n, int count, int item) const {
+#pragma unroll
+        for (int i = 0; i < kNvItems; ++i) {
+            const uint32_t k = (uint32_t)(item + (int)threadIdx.x + i * (int)blockDim.x), r = k / (uint32_t)count, slab = k - r * (uint32_t)count;
+            if ((int)r >= n) continue;
+            u32x4 lo, hi;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                lo[j] = x[i][j] & 0x0F0F0F0Fu;
+                const uint32_t h = (x[i][j] >> 4) & 0x0F0F0F0Fu, minus = h & 0x08080808u, one = minus >> 3;
+                hi[j] = ((h ^ ((minus << 1) - one)) + one) | (minus << 4);
+            }
+            char* to = lds + Nvfp4Lds::kZeros + r * L.row + (slab >> 4) * 512 + (slab & 15) * 16;
+            *(u32x4*)to = lo;
+            *(u32x4*)(to + 256) = hi;
+            *(float*)(lds + L.xs + 4 * k) = xs[i];
+        }
+    }
+};
+
+__device__ __forceinline__ f32x4 nvfp4_dots(const i32x8& x, const u32x4& w, const f32x4& c, int scale) {
+    const i32x8 b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 0, 4, 0, scale, 0, 127);
+}
+
+// A block goes through tiles of 16 weight rows, `groups` side by side (SWIGLU: a tile of gate beside one of up). K is cut into
+// `slots` of `per` steps; a group's waves take one each, `turn` steps together, then the next ones. Activation rows go in pairs.
+// RESIDENT: all of them are in LDS, once for all tiles; else a pair's turn is brought when it comes. The weights of the next turn or
+// tile are requested as this one's are used. An output is the sum of its slots in order, whatever the waves, so its bits do not
+// depend on nr.
+template <int PAIRS, bool SWIGLU, bool RESIDENT>
+__global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups, int waves, int per, int slots) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
+    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
+    const int tiles = (a.rows + 15) >> 4, wide = SWIGLU ? groups >> 1 : groups;
+    const Nvfp4Lds L(RESIDENT ? a.nr : min(a.nr, 2), held, per, groups, waves, slots, 32 * PAIRS, rest != 0);
+    const uint8_t* wp = SWIGLU && (grp & 1) ? a.w[1] : a.w[0];
+    const uint8_t* sp = SWIGLU && (grp & 1) ? a.s[1] : a.s[0];
+    const int mine = SWIGLU ? grp >> 1 : grp;        // this group's tile of `wide`
+    char* tail = lds + L.tail + 2304 * grp;
+    for (int i = 16 * t; i < Nvfp4Lds::kZeros; i += 16 * (int)blockDim.x) *(u32x4*)(lds + i) = u32x4{0, 0, 0, 0};
+    Nvfp4Rows x;
+    Nvfp4Weights w;
+    w.begin(a.K, per);
+    char* scales = lds + L.ws + 256 * (per | 1) * wave;
+    x.load(a, 0, RESIDENT ? a.nr : 2, 0, count, 0);
+    __builtin_amdgcn_sched_barrier(0);               // (requested first: loads come in order)
+    int tile = (int)blockIdx.x * wide + mine;
+    {
+        const Nvfp4Weights::Tile from(wp, sp, a.rows, a.K, tile);
+        w.load_scales(from, wv * per, per, full);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kNvSteps; ++j) w.load(from, j, wv * per + j, j < per && wv * per + j < full);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (RESIDENT) {
+        x.store(lds, L, a.nr, count, 0);
+        for (int item = kNvItems * (int)blockDim.x; item < a.nr * count; item += kNvItems * (int)blockDim.x) {
+            x.load(a, 0, a.nr, 0, count, item);
+            x.store(lds, L, a.nr, count, item);
+        }
+        __syncthreads();
+    }
+    // the operand's row c holds slab c % 8 of row c / 8, in lanes g = c % 4, in its first or second half
+    int opa[2];
+    bool has[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        has[h] = (c & 3) == g && ((c >> 2) & 1) == h;
+        opa[h] = has[h] ? Nvfp4Lds::kZeros + (c >> 3) * L.row + wv * per * 512 + (c & 7) * 16 : 0;
+    }
+    const int xsa = L.xs + 4 * ((g >> 1) * count + wv * per * 16 + 4 * (g & 1));
+    int parity = 0;
+    for (int unit = blockIdx.x; unit * wide < tiles; unit += (int)gridDim.x, parity ^= 1) {
+        const int after = tile + (int)gridDim.x * wide;
+        if (rest) {
+            if (!RESIDENT || parity || unit != (int)blockIdx.x) __syncthreads();
+            w.bring(wp, sp, a.rows, a.K, tile, tail, rest, t - 64 * grp * waves, 64 * waves);
+            __syncthreads();
+        }
+        float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * PAIRS;       // [group][slot][row][16], of two tiles in turn
+        for (int s0 = 0, slot = wv; s0 < steps; s0 += turn, slot += waves) {
+            float acc[PAIRS] = {};                   // row 2 p + g / 2, slabs 4 (g % 2) .. of each 128 weights, weight row of lane c
+            const bool last = s0 + turn >= steps;    // (of the tile)
+            const Nvfp4Weights::Tile next(wp, sp, a.rows, a.K, last ? after : tile);
+            const int from = last ? wv * per : s0 + turn + wv * per;   // the steps after these
+            const int sa = L.ws + 256 * (per | 1) * wave + 16 * (per | 1) * nvfp4_row_of(c) + 4 * (g & 1);
+            w.store_scales(scales);
+            int o0 = opa[0], o1 = opa[1], ox = xsa;
+            if constexpr (RESIDENT) {
+                o0 = has[0] ? o0 + 512 * s0 : 0;
+                o1 = has[1] ? o1 + 512 * s0 : 0;
+                ox += 64 * s0;
+            }
+            asm volatile("" : "+v"(o0), "+v"(o1), "+v"(ox));          // (opaque: operands kept over the loop would spill)
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                if (p + 1 == PAIRS && (a.nr & 1)) {   // (a row that is not: zeros, and some scales)
+                    o0 = c >> 3 ? 0 : o0;
+                    o1 = c >> 3 ? 0 : o1;
+                    ox = g >> 1 ? ox - 4 * count : ox;
+                }
+                if constexpr (!RESIDENT) {
+                    __syncthreads();                  // (the pair before is read)
+                    x.store(lds, L, min(a.nr, 2), count, 0);
+                    __syncthreads();
+                    if (p + 1 < PAIRS) x.load(a, 2 * (p + 1), 2, 16 * s0, count, 0);
+                    else x.load(a, 0, 2, last ? 0 : 16 * (s0 + turn), count, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (p + 1 == PAIRS) {
+                    w.load_scales(next, from, per, full);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+                for (int j = 0; j < kNvSteps; ++j) {
+                    const int st = s0 + wv * per + j;
+                    int sj = sa + 16 * j;
+                    if (j < per && st < steps) {
+                        if (st == full) {
+                            w.take(tail, j);
+                            sj = L.tail + 2304 * grp + 2048 + 16 * nvfp4_row_of(c) + 4 * (g & 1);
+                        }
+                        constexpr int kOne = 127 + 9, k16 = kOne + 4;       // bytes are 2^-9 each
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            auto operand = [&](int at) __attribute__((always_inline)) {
+                                const u32x4 y = *(const u32x4*)(lds + o0 + at), z = *(const u32x4*)(lds + o1 + at);
+                                return i32x8{(int)y[0], (int)y[1], (int)y[2], (int)y[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
+                            };
+                            const i32x8 lo = operand(512 * j + 128 * h), hi = operand(512 * j + 256 + 128 * h);
+                            const f32x4 xs = *(const f32x4*)(lds + ox + 64 * j + 32 * h);
+                            const u32x4 q = w.operand(j, h);
+                            const f32x4 d = nvfp4_dots(hi, q, nvfp4_dots(lo, q, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, kOne), k16);
+                            const int e = *(const int*)(lds + sj + 8 * h);
+                            const auto e0 = __builtin_amdgcn_cvt_pk_f32_fp8(e, false), e1 = __builtin_amdgcn_cvt_pk_f32_fp8(e, true);
+                            acc[p] = __builtin_fmaf(d[0], e0[0] * xs[0], acc[p]);
+                            acc[p] = __builtin_fmaf(d[1], e0[1] * xs[1], acc[p]);
+                            acc[p] = __builtin_fmaf(d[2], e1[0] * xs[2], acc[p]);
+                            acc[p] = __builtin_fmaf(d[3], e1[1] * xs[3], acc[p]);
+                        }
+                    }
+                    if (p + 1 == PAIRS) w.load(next, j, from + j, j < per && from + j < full);
+                }
+                if constexpr (RESIDENT) {
+                    o0 = has[0] ? o0 + 2 * L.row : 0;
+                    o1 = has[1] ? o1 + 2 * L.row : 0;
+                    ox += 8 * count;
+                }
+            }
+            if (slot < slots) {
+#pragma unroll
+                for (int p = 0; p < PAIRS; ++p) {
+                    const float y = acc[p] + xor16(acc[p]);
+                    if (!(g & 1)) sums[((grp * slots + slot) * 2 * PAIRS + 2 * p + (g >> 1)) * 16 + nvfp4_row_of(c)] = y;
+                }
+            }
+        }
+        __syncthreads();
+        const int outs = wide * 32 * PAIRS;
+        for (int i = t; i < (outs + 63) / 64 * 64; i += (int)blockDim.x) {
+            const int r16 = i & 15, n = (i >> 4) % (2 * PAIRS), k = min(i / (32 * PAIRS), wide - 1), row = (unit * wide + k) * 16 + r16;
+            auto total = [&](int gr) {
+                float y = 0.0f;
+                for (int v = 0; v < slots; ++v) y = y + sums[((gr * slots + v) * 2 * PAIRS + n) * 16 + r16];
+                return y;
+            };
+            const bool is = i < outs && n < a.nr && row < a.rows;
+            if constexpr (SWIGLU) {
+                const float gate = a.alpha[0] * total(2 * k), up = a.alpha[1] * total(2 * k + 1);
+                const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
+                const float sc = max_xor(fabsf(z), 16) * (1.0f / 127.0f);
+                const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+                if (is) {
+                    const size_t at = (size_t)n * a.rows + row;
+                    a.oq[at] = qcode(z, inv);
+                    if (r16 == 0) a.os[at >> 4] = sc;
+                }
+            } else if (is) {
+                float y = a.alpha[0] * total(k);
                 if (a.res) {
-                    const size_t at = (size_t)n * a.rstride + r;
+                    const size_t at = (size_t)n * a.rstride + row;
                     y = __builtin_fmaf(a.rs, a.res_bf16 ? bf2f(((const uint16_t*)a.res)[at]) : ((const float*)a.res)[at], y);
                 }
-                const size_t at = (size_t)n * a.ystride + r;
+                const size_t at = (size_t)n * a.ystride + row;
                 if (a.out_bf16) ((uint16_t*)a.y)[at] = f2bf(y);
                 else ((float*)a.y)[at] = y;
             }
         }
+        tile = after;
     }
 }
 
-template <int RT, bool SWIGLU>
-static int launch_nvfp4(const Nvfp4Args& a, hipStream_t s) {
-    const int tiles = (a.K + kNvTile - 1) / kNvTile;
-    int waves = kNvWaves;
-    while (waves > 1 && waves > tiles) waves >>= 1;
-    const dim3 grid((unsigned)(SWIGLU ? a.rows / 16 : (a.rows + 16 * RT - 1) / (16 * RT)));
-    if (a.nr <= 4) hipLaunchKernelGGL((k_nvfp4<RT, 1, SWIGLU>), grid, dim3(64 * waves), 0, s, a);
-    else hipLaunchKernelGGL((k_nvfp4<RT, 2, SWIGLU>), grid, dim3(64 * waves), 0, s, a);
+struct Nvfp4Plan { int per, slots, groups, waves, bytes; bool resident; };
+template <int PAIRS, bool SWIGLU, bool RESIDENT>
+static int launch_nvfp4_form(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
+    const int wide = SWIGLU ? p.groups / 2 : p.groups, units = ((a.rows + 15) / 16 + wide - 1) / wide;
+    int fit = kNvLds / p.bytes;                      // blocks of a compute unit
+    fit = fit < kNvWaves / (p.groups * p.waves) ? fit : kNvWaves / (p.groups * p.waves);
+    fit = fit < 1 ? 1 : fit;
+    const int grid = 256 * fit < units ? 256 * fit : units;
+    Q27X_HIP((allow_lds<k_nvfp4<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
+    hipLaunchKernelGGL((k_nvfp4<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.groups, p.waves, p.per, p.slots);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
+}
+template <int PAIRS, bool SWIGLU>
+static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
+    const int steps = (a.K + kNvStep - 1) / kNvStep, tiles = (a.rows + 15) / 16;
+    const bool ends_inside = a.K % kNvStep != 0;
+    constexpr int least = SWIGLU ? 2 : 1;
+    Nvfp4Plan p;
+    p.per = steps <= 4 ? 1 : steps <= 8 ? 2 : kNvSteps;
+    p.slots = (steps + p.per - 1) / p.per;
+    // all activations in LDS, tiles side by side that share them
+    p.groups = PAIRS == 1 ? 1 : PAIRS == 2 ? 2 : 4;
+    if (p.groups < least) p.groups = least;
+    while (p.groups > least && tiles * least < 256 * p.groups) p.groups >>= 1;         // (tiles for every compute unit)
+    for (;; p.groups >>= 1) {
+        const int most = kNvWaves / p.groups, turns = (p.slots + most - 1) / most;
+        p.waves = (p.slots + turns - 1) / turns;
+        p.bytes = Nvfp4Lds(a.nr, steps, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
+        if (p.bytes <= kNvLds) return launch_nvfp4_form<PAIRS, SWIGLU, true>(a, p, s);
+        if (p.groups == least) break;
+    }
+    const int most = kNvWaves / 2 / least, turns = (p.slots + most - 1) / most;
+    p.waves = (p.slots + turns - 1) / turns;
+    p.bytes = Nvfp4Lds(a.nr < 2 ? a.nr : 2, p.waves * p.per, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
+    return launch_nvfp4_form<PAIRS, SWIGLU, false>(a, p, s);
+}
+template <bool SWIGLU>
+static int launch_nvfp4(const Nvfp4Args& a, hipStream_t s) {
+    switch ((a.nr + 1) / 2) {
+        case 1: return launch_nvfp4_pairs<1, SWIGLU>(a, s);
+        case 2: return launch_nvfp4_pairs<2, SWIGLU>(a, s);
+        case 3: return launch_nvfp4_pairs<3, SWIGLU>(a, s);
+        default: return launch_nvfp4_pairs<4, SWIGLU>(a, s);
+    }
 }
 
 // the caller's matrix and rows, checked
 static int nvfp4_args(const q27x_nvfp4_t* w, const char* who, const int8_t* xq, int xstride, const float* xs, int nr) {
     if (!w || !w->w || !w->s || !xq || !xs) { set_error("%s: null argument", who); return Q27X_E_ARG; }
-    if (w->rows < 1 || w->rows > 0x7fffffff - 64 || w->K < 16 || (w->K & 15) || w->K > 0x7fffffff - kNvTile) {
-        set_error("%s: unsupported shape (rows=%d K=%d: K a multiple of 16)", who, w->rows, w->K);
+    if (w->rows < 1 || w->rows > 0x7fffffff - 64 || w->K < 16 || (w->K & 15) || w->K > kNvMaxK) {
+        set_error("%s: unsupported shape (rows=%d K=%d: K a multiple of 16 up to %d)", who, w->rows, w->K, kNvMaxK);
         return Q27X_E_SHAPE;
     }
     if (nr < 1 || nr > kMaxRows) { set_error("%s: nr=%d: 1 to %d rows", who, nr, kMaxRows); return Q27X_E_SHAPE; }
@@ -275,7 +448,7 @@ extern "C" int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int
     a.xq = xq; a.xstride = nr > 1 ? xstride : 0; a.xs = xs; a.nr = nr;
     a.y = y; a.ystride = nr > 1 ? ystride : 0; a.out_bf16 = out_bf16 ? 1 : 0;
     a.res = res; a.res_bf16 = res_bf16 ? 1 : 0; a.rstride = nr > 1 ? rstride : 0; a.rs = rs;
-    return launch_nvfp4<1, false>(a, (hipStream_t)s);
+    return launch_nvfp4<false>(a, (hipStream_t)s);
 }
 extern "C" int q27x_swiglu_nvfp4_rows(const q27x_nvfp4_t* gate, const q27x_nvfp4_t* up, const int8_t* xq, int xstride,
                                       const float* xs, int8_t* oq, float* os, float in_scale, int nr, q27x_stream_t s) {
@@ -293,5 +466,5 @@ extern "C" int q27x_swiglu_nvfp4_rows(const q27x_nvfp4_t* gate, const q27x_nvfp4
     a.rows = gate->rows; a.K = gate->K;
     a.xq = xq; a.xstride = nr > 1 ? xstride : 0; a.xs = xs; a.nr = nr;
     a.oq = oq; a.os = os; a.g = 1.0f / in_scale;
-    return launch_nvfp4<2, true>(a, (hipStream_t)s);
+    return launch_nvfp4<true>(a, (hipStream_t)s);
 }
