@@ -9,29 +9,31 @@
 // t, the power in fp64 to 2^-46): sums are exact, whatever their order, and nothing depends on atomics' order or on the grid. A
 // token of z >= 48 weighs 0 and is never drawn.
 //
-//   k_sample_max: the largest logit of each slice of 4096.
+//   k_sample_max: the largest logit of each 4096.
 //   k_sample_bins: bins of z (a 16th of a binary order up to 16 of them, a quarter up to 48): a slice's tokens by bin, and each
-//     bin's weight.
-//   k_sample_draw: a row's bins summed and searched; the bin that a search ends in is searched by (logit, index) in steps of 10 bits.
-#include "q27x_dev.h"
-#include "q27x_int.h"
+//     bin's weight; up to 16 slices a row.
+//   k_sample_draw: a row's bins summed and searched. Where all that can be drawn is 256 tokens or fewer, each of them counts and
+//     sums those before it, and the cuts and the draw are comparisons; else the bin that a search ends in is narrowed to 256 by
+//     (logit, index) in steps of 8 bits, and these are counted like that.
+#include "q27x_paged.h"
 
 namespace q27x {
 
 typedef unsigned long long u64;
-constexpr int kSlice = 4096, kBins = 384, kBinThreads = 512, kPer = kSlice / kBinThreads;
-constexpr int kOffs = kBins + 8;                  // a slice's list offsets by bin, in u16
-constexpr int kDrawThreads = 1024, kHeld = 2048;  // candidates that LDS holds
+constexpr int kMaxPart = 4096;                    // logits of a block of k_sample_max
+constexpr int kLeastSlice = 4096, kMostSlices = 16, kMostSlice = 32768, kPer = 8;
+constexpr int kBins = 384, kOffs = kBins + 8;     // a slice's list offsets by bin, in u16
+constexpr int kDrawThreads = 256, kFew = 256, kHeld = 2048;     // tokens counted among each other, and held in LDS
 constexpr u64 kUnit = 1ull << 44;                 // the weight of the largest logit
-constexpr int kMaxTokens = 1 << 19;               // (their weights' sum fits 64 bits)
+constexpr int kMaxTokens = 1 << 19;               // (their weights' sum fits 64 bits, 16 slices hold them)
 
 struct SampleArgs {
-    const void* logits; int bf16, n, ld, nr, ns;
+    const void* logits; int bf16, n, ld, nr, ns, slice, parts;
     const float* temperature; const int32_t* top_k; const float* top_p; const float* min_p; const float* u;
-    float* smax;                                  // [nr][ns] slices' largest logits, -inf without a finite one
+    float* smax;                                  // [nr][parts] their largest logits, -inf without a finite one
     u64* bw;                                      // [nr][ns][kBins] weights
     uint16_t* off;                                // [nr][ns][kOffs] where a bin begins in the slice's list, and its end
-    uint16_t* list;                               // [nr][ns][kSlice] tokens of the slice by bin
+    uint16_t* list;                               // [nr][ns][slice] tokens of the slice by bin
     int32_t* idx; float* prob;
 };
 
@@ -49,7 +51,7 @@ __device__ __forceinline__ double inv_temp(const SampleArgs& a, int row, bool& g
 // the row's largest logit, in every lane of the calling wave
 __device__ __forceinline__ float row_max(const SampleArgs& a, int row) {
     float m = -__builtin_huge_valf();
-    for (int s = threadIdx.x & 63; s < a.ns; s += 64) m = fmaxf(m, a.smax[(size_t)row * a.ns + s]);
+    for (int s = threadIdx.x & 63; s < a.parts; s += 64) m = fmaxf(m, a.smax[(size_t)row * a.parts + s]);
     return max_xor(m, 64);
 }
 __device__ __forceinline__ double order_of(float l, double l0, double c) { return (l0 - (double)l) * c; }
@@ -81,55 +83,87 @@ __device__ __forceinline__ u64 rank_of(float l, int i) {
     return (u64)~up << 32 | (uint32_t)i;
 }
 
-__global__ __launch_bounds__(256) void k_sample_max(SampleArgs a) {
-    const int s = blockIdx.x, row = blockIdx.y, end = min(a.n, (s + 1) * kSlice);
-    float m = -__builtin_huge_valf();
-    for (int i = s * kSlice + threadIdx.x; i < end; i += 256) {
-        const float l = logit_at(a, row, i);
-        m = is_finite(l) ? fmaxf(m, l) : m;
+// four logits from i on, those behind the row as NaN
+__device__ __forceinline__ void logits4(const SampleArgs& a, int row, int i, float (&v)[4]) {
+    typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+    typedef uint32_t u32x2h __attribute__((ext_vector_type(2), aligned(2)));
+    const size_t at = (size_t)row * a.ld + i;
+    if (i + 4 <= a.n) {
+        if (a.bf16) {
+            const u32x2h x = *(const u32x2h*)((const uint16_t*)a.logits + at);
+            v[0] = __uint_as_float(x[0] << 16); v[1] = __uint_as_float(x[0] & 0xFFFF0000u);
+            v[2] = __uint_as_float(x[1] << 16); v[3] = __uint_as_float(x[1] & 0xFFFF0000u);
+        } else {
+            const f32x4u x = *(const f32x4u*)((const float*)a.logits + at);
+            v[0] = x[0]; v[1] = x[1]; v[2] = x[2]; v[3] = x[3];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = i + j < a.n ? logit_at(a, row, i + j) : __builtin_nanf("");
     }
+}
+
+__global__ __launch_bounds__(256) void k_sample_max(SampleArgs a) {
+    const int s = blockIdx.x, row = blockIdx.y;
+    float v[kMaxPart / 1024][4], m = -__builtin_huge_valf();
+#pragma unroll
+    for (int j = 0; j < kMaxPart / 1024; ++j) logits4(a, row, s * kMaxPart + 1024 * j + 4 * (int)threadIdx.x, v[j]);
+#pragma unroll
+    for (int j = 0; j < kMaxPart / 1024; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = is_finite(v[j][k]) ? fmaxf(m, v[j][k]) : m;
     __shared__ float s_m[4];
     m = max_xor(m, 64);
     if ((threadIdx.x & 63) == 0) s_m[threadIdx.x >> 6] = m;
     __syncthreads();
-    if (threadIdx.x == 0) a.smax[(size_t)row * a.ns + s] = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    if (threadIdx.x == 0) a.smax[(size_t)row * a.parts + s] = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
 }
 
-__global__ __launch_bounds__(kBinThreads) void k_sample_bins(SampleArgs a) {
-    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * kSlice;
+// T threads with 8 tokens each, a slice of 8 T or 4 times that
+template <int T>
+__global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t s_list[];
+    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice;
     __shared__ u64 s_w[kBins];
-    __shared__ uint32_t s_n[kBins], s_at[kBins];
-    __shared__ uint32_t s_part[kBinThreads / 64];
-    __shared__ __attribute__((aligned(16))) uint16_t s_list[kSlice];
-    for (int b = t; b < kBins; b += kBinThreads) { s_w[b] = 0; s_n[b] = 0; }
+    __shared__ uint32_t s_n[kBins], s_at[kBins], s_part[kBins / 64];
+    for (int b = t; b < kBins; b += T) { s_w[b] = 0; s_n[b] = 0; }
     const float top = row_max(a, row);
     bool greedy;
     const double c = inv_temp(a, row, greedy), l0 = (double)top;
     __syncthreads();
-    int bin[kPer];
+    for (int i0 = 0; i0 < a.slice; i0 += kPer * T) {
+        float v[kPer / 4][4];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int i = begin + j * kBinThreads + t;
-        const float l = i < a.n ? logit_at(a, row, i) : __builtin_huge_valf();
-        const double z = order_of(l, l0, c);
-        bin[j] = is_finite(l) && z < 48.0 ? bin_of(z) : -1;
-        if (bin[j] >= 0) {
-            atomicAdd(&s_w[bin[j]], weight(z));
-            atomicAdd(&s_n[bin[j]], 1u);
+        for (int j = 0; j < kPer / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const float l = v[j / 4][j % 4];
+            const double z = order_of(l, l0, c);
+            if (is_finite(l) && z < 48.0) {
+                atomicAdd(&s_w[bin_of(z)], weight(z));
+                atomicAdd(&s_n[bin_of(z)], 1u);
+            }
         }
     }
     __syncthreads();
     // where each bin begins
     const size_t at = (size_t)row * a.ns + s;
     uint32_t n = t < kBins ? s_n[t] : 0, run = n;
+    if (t < kBins) {
 #pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const uint32_t y = __shfl_up(run, o, 64);
-        run += (t & 63) >= o ? y : 0;
+        for (int o = 1; o < 64; o *= 2) {
+            const uint32_t y = __shfl_up(run, o, 64);
+            run += (t & 63) >= o ? y : 0;
+        }
+        if ((t & 63) == 63) s_part[t >> 6] = run;
     }
-    if ((t & 63) == 63) s_part[t >> 6] = run;
     __syncthreads();
-    for (int k = 0; k < t >> 6; ++k) run += s_part[k];
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kBins / 64; ++k) {
+        run += k < t >> 6 ? s_part[k] : 0;
+        total += s_part[k];
+    }
     if (t < kBins) {
         s_at[t] = run - n;
         a.off[at * kOffs + t] = (uint16_t)(run - n);
@@ -137,101 +171,129 @@ __global__ __launch_bounds__(kBinThreads) void k_sample_bins(SampleArgs a) {
         if (t == kBins - 1) a.off[at * kOffs + kBins] = (uint16_t)run;
     }
     __syncthreads();
+    for (int i0 = 0; i0 < a.slice; i0 += kPer * T) {
+        float v[kPer / 4][4];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j)
-        if (bin[j] >= 0) s_list[atomicAdd(&s_at[bin[j]], 1u)] = (uint16_t)(j * kBinThreads + t);
+        for (int j = 0; j < kPer / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const float l = v[j / 4][j % 4];
+            const double z = order_of(l, l0, c);
+            if (is_finite(l) && z < 48.0) s_list[atomicAdd(&s_at[bin_of(z)], 1u)] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
+        }
+    }
     __syncthreads();
-    uint32_t total = 0;
-    for (int k = 0; k < kBinThreads / 64; ++k) total += s_part[k];
-    for (uint32_t i = 2 * t; i < total; i += 2 * kBinThreads) *(uint32_t*)(a.list + at * kSlice + i) = *(const uint32_t*)&s_list[i];
+    for (uint32_t i = 8 * t; i < total; i += 8 * T) *(uint4*)(a.list + at * a.slice + i) = *(const uint4*)&s_list[i];
 }
 
-// Exclusive running sums over the block's threads of a count and a weight.
 struct Sum { uint32_t n; u64 w; };
 __device__ __forceinline__ u64 shfl_up64(u64 x, int o) {
     const uint32_t lo = __shfl_up((uint32_t)x, o, 64), hi = __shfl_up((uint32_t)(x >> 32), o, 64);
     return (u64)hi << 32 | lo;
 }
-__device__ __forceinline__ Sum scan_block(Sum x, Sum* part) {
-    const int t = threadIdx.x, l = t & 63;
-    Sum run = x;
+__device__ __forceinline__ u64 shfl_xor64(u64 x, int o) {
+    const uint32_t lo = __shfl_xor((uint32_t)x, o, 64), hi = __shfl_xor((uint32_t)(x >> 32), o, 64);
+    return (u64)hi << 32 | lo;
+}
+// Inclusive running sums over the wave.
+__device__ __forceinline__ Sum scan_wave(Sum x) {
+    const int l = threadIdx.x & 63;
 #pragma unroll
     for (int o = 1; o < 64; o *= 2) {
-        const uint32_t n = __shfl_up(run.n, o, 64);
-        const u64 w = shfl_up64(run.w, o);
-        if (l >= o) { run.n += n; run.w += w; }
+        const uint32_t n = __shfl_up(x.n, o, 64);
+        const u64 w = shfl_up64(x.w, o);
+        if (l >= o) { x.n += n; x.w += w; }
     }
-    __syncthreads();                              // (the parts before are read)
-    if (l == 63) part[t >> 6] = run;
-    __syncthreads();
-    for (int k = 0; k < t >> 6; ++k) { run.n += part[k].n; run.w += part[k].w; }
-    run.n -= x.n;
-    run.w -= x.w;
-    return run;
+    return x;
 }
 
 struct DrawShared {
     u64 bw[kBins + 1];                            // running weights and counts of the row's bins
     uint32_t bn[kBins + 1];
-    Sum part[kDrawThreads / 64];
-    u64 hw[1024];                                 // a search step's digits
-    uint32_t hn[1024];
+    uint16_t off[kMostSlices][kOffs];             // the slices' lists by bin
+    Sum part[kBins / 64];
+    u64 hw[256];                                  // a narrowing step's digits
+    uint32_t hn[256];
     u64 q[kHeld], w[kHeld];                       // candidates
-    u64 lo, hi, found_q, found_w, found_before;
-    u64 before_w;
-    uint32_t held, before_n, digit, left;
+    u64 lo[4], hi[4], found_q, found_w, found_end, digit_w;
+    uint32_t held, digit, digit_n, left;
 };
 
+// The tokens of bins b0 .. b1 of the row, f(rank, weight) for each, the block's threads side by side.
+template <typename F>
+__device__ __forceinline__ void each_listed(const SampleArgs& a, const DrawShared& sh, int row, int b0, int b1, double l0, double c, F f) {
+    const int wv = threadIdx.x >> 6, l = threadIdx.x & 63;
+    for (int s = wv; s < a.ns; s += kDrawThreads / 64) {
+        const size_t at = (size_t)row * a.ns + s;
+        const int end = sh.off[s][b1 + 1];
+        for (int i = sh.off[s][b0] + l; i < end; i += 64) {
+            const int id = s * a.slice + a.list[at * a.slice + i];
+            const float x = logit_at(a, row, id);
+            f(rank_of(x, id), weight(order_of(x, l0, c)));
+        }
+    }
+}
+// The same tokens into LDS; how many.
+__device__ __forceinline__ uint32_t hold(const SampleArgs& a, DrawShared& sh, int row, int b0, int b1, double l0, double c) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.held = 0;
+    __syncthreads();
+    each_listed(a, sh, row, b0, b1, l0, c, [&](u64 q, u64 w) {
+        const uint32_t k = atomicAdd(&sh.held, 1u);
+        sh.q[k] = q;
+        sh.w[k] = w;
+    });
+    __syncthreads();
+    return sh.held;
+}
+// What comes before this thread's token (q) among the n held ones.
+__device__ __forceinline__ Sum before_of(const DrawShared& sh, uint32_t n, u64 q) {
+    Sum x = {0, 0};
+    for (uint32_t i = 0; i < n; ++i) {
+        const bool is = sh.q[i] < q;
+        x.n += is ? 1u : 0u;
+        x.w += is ? sh.w[i] : 0;
+    }
+    return x;
+}
+
 // The token of bin b at which the running count (BY_COUNT) or weight, from the bin's beginning on, reaches `target` (at least 1, at
-// most the bin's): its rank, its weight and the running weight before it, in sh.
+// most the bin's): its rank, its weight and the running weight up to it, in sh.
 template <bool BY_COUNT>
 __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 target, double l0, double c) {
-    const int t = threadIdx.x, wv = t >> 6, l = t & 63;
-    const uint32_t count = sh.bn[b + 1] - sh.bn[b];
-    const bool held = count <= kHeld;
-    // every token of the bin, slices to waves in turn
-    auto each_listed = [&](auto f) {
-        for (int s = wv; s < a.ns; s += kDrawThreads / 64) {
-            const size_t at = (size_t)row * a.ns + s;
-            const int end = a.off[at * kOffs + b + 1];
-            for (int i = a.off[at * kOffs + b] + l; i < end; i += 64) {
-                const int id = s * kSlice + a.list[at * kSlice + i];
-                const float x = logit_at(a, row, id);
-                f(rank_of(x, id), weight(order_of(x, l0, c)));
-            }
-        }
-    };
-    __syncthreads();
-    if (t == 0) { sh.held = 0; sh.lo = ~0ull; sh.hi = 0; }
-    __syncthreads();
-    u64 lo = ~0ull, hi = 0;
-    each_listed([&](u64 q, u64 w) {
-        lo = q < lo ? q : lo;
-        hi = q > hi ? q : hi;
-        if (held) {
-            const uint32_t k = atomicAdd(&sh.held, 1u);
-            sh.q[k] = q;
-            sh.w[k] = w;
-        }
-    });
-    atomicMin(&sh.lo, lo);
-    atomicMax(&sh.hi, hi);
-    __syncthreads();
-    lo = sh.lo;
-    hi = sh.hi;
+    const int t = threadIdx.x;
+    uint32_t n = sh.bn[b + 1] - sh.bn[b];
+    u64 before = 0;                               // weight before what is left
+    if (n <= kHeld) hold(a, sh, row, b, b, l0, c);
+    bool held = n <= kHeld;
+    u64 lo = 0, hi = ~0ull;
     auto each = [&](auto f) {
-        if (held) {
-            for (uint32_t i = t; i < count; i += kDrawThreads) f(sh.q[i], sh.w[i]);
-        } else {
-            each_listed(f);
-        }
+        if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.q[i], sh.w[i]);
+        else each_listed(a, sh, row, b, b, l0, c, f);
     };
-    u64 before = 0;                               // weight before the digits that are left
-    int shift = max(0, 64 - __builtin_clzll((hi - lo) | 1) - 10);
-    for (;;) {
+    while (n > kFew) {
+        // the range of what is left, in 256 parts
+        u64 least = ~0ull, most = 0;
+        each([&](u64 q, u64) {
+            if (q >= lo && q <= hi) {
+                least = q < least ? q : least;
+                most = q > most ? q : most;
+            }
+        });
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const u64 x = shfl_xor64(least, o), y = shfl_xor64(most, o);
+            least = x < least ? x : least;
+            most = y > most ? y : most;
+        }
+        __syncthreads();
+        if ((t & 63) == 0) { sh.lo[t >> 6] = least; sh.hi[t >> 6] = most; }
         sh.hw[t] = 0;
         sh.hn[t] = 0;
         __syncthreads();
+        lo = min(min(sh.lo[0], sh.lo[1]), min(sh.lo[2], sh.lo[3]));
+        hi = max(max(sh.hi[0], sh.hi[1]), max(sh.hi[2], sh.hi[3]));
+        const int shift = max(0, 64 - __builtin_clzll((hi - lo) | 1) - 8);
         each([&](u64 q, u64 w) {
             if (q >= lo && q <= hi) {
                 atomicAdd(&sh.hw[(q - lo) >> shift], w);
@@ -239,29 +301,74 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
             }
         });
         __syncthreads();
-        const Sum mine = {sh.hn[t], sh.hw[t]}, run = scan_block(mine, sh.part);
-        const bool here = BY_COUNT ? run.n < target && target <= run.n + mine.n : run.w < target && target <= run.w + mine.w;
-        if (here) {
-            sh.digit = t;
-            sh.before_n = run.n;
-            sh.before_w = run.w;
-            sh.left = mine.n;
+        if (t < 64) {                             // four parts a lane
+            Sum x = {0, 0};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) { x.n += sh.hn[4 * t + k]; x.w += sh.hw[4 * t + k]; }
+            Sum run = scan_wave(x);
+            run.n -= x.n;
+            run.w -= x.w;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t pn = sh.hn[4 * t + k];
+                const u64 pw = sh.hw[4 * t + k];
+                if (BY_COUNT ? run.n < target && target <= run.n + pn : run.w < target && target <= run.w + pw) {
+                    sh.digit = 4 * t + k;
+                    sh.digit_n = run.n;
+                    sh.digit_w = run.w;
+                    sh.left = pn;
+                }
+                run.n += pn;
+                run.w += pw;
+            }
+            if (t == 0) sh.held = 0;
         }
         __syncthreads();
-        const u64 first = lo + ((u64)sh.digit << shift);
-        before += sh.before_w;
-        target -= BY_COUNT ? sh.before_n : sh.before_w;
-        const bool last = sh.left == 1 || shift == 0;
-        lo = first;
-        hi = min(hi, first + ((1ull << shift) - 1));
-        if (last) break;
-        shift = max(0, shift - 10);
-        __syncthreads();                          // (the choice is read)
+        lo += (u64)sh.digit << shift;
+        hi = min(hi, lo + ((1ull << shift) - 1));
+        before += sh.digit_w;
+        target -= BY_COUNT ? sh.digit_n : sh.digit_w;
+        const uint32_t left = sh.left;
+        if (left <= kFew) {                       // these alone, at the front
+            u64 kq[kHeld / kDrawThreads], kw[kHeld / kDrawThreads];
+            if (held) {
+#pragma unroll
+                for (int k = 0; k < kHeld / kDrawThreads; ++k) {
+                    const uint32_t i = t + k * kDrawThreads;
+                    kq[k] = i < n ? sh.q[i] : 0;
+                    kw[k] = i < n ? sh.w[i] : 0;
+                    if (i >= n || kq[k] < lo || kq[k] > hi) kq[k] = ~0ull;
+                }
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < kHeld / kDrawThreads; ++k)
+                    if (kq[k] != ~0ull) {
+                        const uint32_t i = atomicAdd(&sh.held, 1u);
+                        sh.q[i] = kq[k];
+                        sh.w[i] = kw[k];
+                    }
+            } else {
+                each_listed(a, sh, row, b, b, l0, c, [&](u64 q, u64 w) {
+                    if (q >= lo && q <= hi) {
+                        const uint32_t i = atomicAdd(&sh.held, 1u);
+                        sh.q[i] = q;
+                        sh.w[i] = w;
+                    }
+                });
+            }
+            __syncthreads();
+            n = left;
+        }
     }
-    each([&](u64 q, u64 w) {
-        if (q >= lo && q <= hi) { sh.found_q = q; sh.found_w = w; }
-    });
-    if (t == 0) sh.found_before = before;
+    if ((uint32_t)t < n) {
+        const Sum x = before_of(sh, n, sh.q[t]);
+        const u64 w = sh.w[t];
+        if (BY_COUNT ? x.n + 1 == target : x.w < target && target <= x.w + w) {
+            sh.found_q = sh.q[t];
+            sh.found_w = w;
+            sh.found_end = before + x.w + w;
+        }
+    }
     __syncthreads();
 }
 
@@ -276,90 +383,149 @@ __device__ int bin_that_reaches(const DrawShared& sh, u64 target) {
     }
     return lo;
 }
+// the largest of a value over the block
+__device__ __forceinline__ u64 max_block(DrawShared& sh, u64 x) {
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) x = max(x, shfl_xor64(x, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.lo[threadIdx.x >> 6] = x;
+    __syncthreads();
+    return max(max(sh.lo[0], sh.lo[1]), max(sh.lo[2], sh.lo[3]));
+}
+// the whole number that a running weight has to reach to be at least (PASS: more than) share x kept, of 1 .. kept
+template <bool PASS>
+__device__ __forceinline__ u64 share_of(float share, u64 kept) {
+    const double want = share > 0.0f ? (double)share * (double)kept : 0.0;
+    if (!(want < (double)kept)) return kept;
+    const u64 x = PASS ? (u64)want + 1 : (u64)__builtin_ceil(want);
+    return min(max(x, (u64)1), kept);
+}
 
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const int row = blockIdx.x, t = threadIdx.x;
     __shared__ DrawShared sh;
     const float top = row_max(a, row);
+    bool greedy;
+    const double c = inv_temp(a, row, greedy), l0 = (double)top;
+    const int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
+    const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
+    // the slices' lists, and bins 2 t and 2 t + 1 of the row
+    for (int i = t; i < a.ns * (kOffs / 8); i += kDrawThreads)
+        *(uint4*)&sh.off[i / (kOffs / 8)][8 * (i % (kOffs / 8))] = *(const uint4*)(a.off + ((size_t)row * a.ns + i / (kOffs / 8)) * kOffs + 8 * (i % (kOffs / 8)));
+    u64 w0 = 0, w1 = 0;
+    if (t < kBins / 2)
+#pragma unroll 8
+        for (int s = 0; s < a.ns; ++s) {
+            const ulonglong2 x = *(const ulonglong2*)(a.bw + ((size_t)row * a.ns + s) * kBins + 2 * t);
+            w0 += x.x;
+            w1 += x.y;
+        }
     if (!is_finite(top)) {                        // (no finite logit)
         if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
     }
-    bool greedy;
-    const double c = inv_temp(a, row, greedy), l0 = (double)top;
-    Sum mine = {0, 0};
-    if (t < kBins)
+    __syncthreads();
+    if (t < kBins / 2) {
+        uint32_t n0 = 0, n1 = 0;
         for (int s = 0; s < a.ns; ++s) {
-            const size_t at = (size_t)row * a.ns + s;
-            mine.n += (uint32_t)a.off[at * kOffs + t + 1] - a.off[at * kOffs + t];
-            mine.w += a.bw[at * kBins + t];
+            const uint32_t o0 = sh.off[s][2 * t], o1 = sh.off[s][2 * t + 1], o2 = sh.off[s][2 * t + 2];
+            n0 += o1 - o0;
+            n1 += o2 - o1;
         }
-    const Sum run = scan_block(mine, sh.part);
-    if (t <= kBins) { sh.bn[t] = run.n; sh.bw[t] = run.w; }
+        const Sum mine = {n0 + n1, w0 + w1};
+        Sum run = scan_wave(mine);
+        if ((t & 63) == 63) sh.part[t >> 6] = run;
+        sh.bn[2 * t + 1] = run.n - n1;
+        sh.bn[2 * t + 2] = run.n;
+        sh.bw[2 * t + 1] = run.w - w1;
+        sh.bw[2 * t + 2] = run.w;
+        if (t == 0) { sh.bn[0] = 0; sh.bw[0] = 0; }
+    }
+    __syncthreads();
+    if (t >= 64 && t < kBins / 2) {
+        Sum x = sh.part[0];
+        if (t >= 128) { x.n += sh.part[1].n; x.w += sh.part[1].w; }
+        sh.bn[2 * t + 1] += x.n; sh.bn[2 * t + 2] += x.n;
+        sh.bw[2 * t + 1] += x.w; sh.bw[2 * t + 2] += x.w;
+    }
     __syncthreads();
     u64 kept = sh.bw[kBins];                      // the weight of what is kept
-    const int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
-    if (k >= 1 && (uint32_t)k < sh.bn[kBins]) {
-        const int b = bin_that_reaches<true>(sh, (u64)k);
-        if (sh.bn[b + 1] == (uint32_t)k) {
-            kept = sh.bw[b + 1];
+    const bool by_k = k >= 1 && (uint32_t)k < sh.bn[kBins], by_p = p < 1.0f, by_m = m > 0.0f;
+    const int bk = by_k ? bin_that_reaches<true>(sh, (u64)k) : kBins - 1;
+    const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
+    // bins that tokens of weight `least` are in (the logarithm is rounded)
+    const double zm = by_m && m < 1.0f ? -log2((double)m) : 0.0;
+    const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
+    const int upto = by_k ? bk : by_p ? bin_that_reaches<false>(sh, share_of<false>(p, kept)) : by_m ? bm1 : kBins - 1;
+    if (sh.bn[upto + 1] <= kFew) {
+        // a thread a token
+        const uint32_t n = hold(a, sh, row, 0, upto, l0, c);
+        const bool is = (uint32_t)t < n;
+        const u64 q = is ? sh.q[t] : ~0ull, w = is ? sh.w[t] : 0;
+        const Sum x = before_of(sh, n, q);
+        const u64 end = x.w + w;
+        if (by_k) kept = max_block(sh, is && x.n < (uint32_t)k ? end : 0);
+        u64 cut = kept;
+        if (by_p) {
+            const u64 target = share_of<false>(p, kept);
+            cut = max_block(sh, is && x.w < target ? min(end, kept) : 0);
+        }
+        if (by_m) cut = min(cut, max_block(sh, is && w >= least ? end : 0));
+        const u64 target = share_of<true>(u, cut);
+        if (is && x.w < target && target <= end) {
+            a.idx[row] = (int32_t)(uint32_t)q;
+            if (a.prob) a.prob[row] = (float)((double)w / (double)cut);
+        }
+        return;
+    }
+    if (by_k) {
+        if (sh.bn[bk + 1] == (uint32_t)k) {
+            kept = sh.bw[bk + 1];
         } else {
-            search<true>(a, sh, row, b, (u64)k - sh.bn[b], l0, c);
-            kept = sh.bw[b] + sh.found_before + sh.found_w;
+            search<true>(a, sh, row, bk, (u64)k - sh.bn[bk], l0, c);
+            kept = sh.bw[bk] + sh.found_end;
         }
     }
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    if (p < 1.0f) {
-        const double want = p > 0.0f ? (double)p * (double)kept : 0.0;
-        const u64 target = max((u64)1, (u64)__builtin_ceil(want));
+    u64 cut = kept;
+    if (by_p) {
+        const u64 target = share_of<false>(p, kept);
         const int b = bin_that_reaches<false>(sh, target);
         search<false>(a, sh, row, b, target - sh.bw[b], l0, c);
-        kept = min(kept, sh.bw[b] + sh.found_before + sh.found_w);
+        cut = min(cut, sh.bw[b] + sh.found_end);
     }
-    const float m = a.min_p ? a.min_p[row] : 0.0f;
-    if (m > 0.0f) {
-        const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
-        // the last bin that holds a weight of at least `least`: its tokens' share
+    if (by_m) {
+        u64 sum = 0;
+        each_listed(a, sh, row, bm0, bm1, l0, c, [&](u64, u64 w) { sum += w >= least ? w : 0; });
         __syncthreads();
         if (t == 0) sh.found_w = 0;
         __syncthreads();
-        const double z = m < 1.0f ? -log2((double)m) : 0.0;
-        const int bm = z < 48.0 ? bin_of(z) : kBins - 1;
-        const int b0 = bm > 0 ? bm - 1 : 0, b1 = bm + 1 < kBins ? bm + 1 : kBins - 1;     // (its logarithm is rounded)
-        u64 sum = 0;
-        for (int s = t >> 6; s < a.ns; s += kDrawThreads / 64) {
-            const size_t at = (size_t)row * a.ns + s;
-            const int end = a.off[at * kOffs + b1 + 1];
-            for (int i = a.off[at * kOffs + b0] + (t & 63); i < end; i += 64) {
-                const u64 w = weight(order_of(logit_at(a, row, s * kSlice + a.list[at * kSlice + i]), l0, c));
-                sum += w >= least ? w : 0;
-            }
-        }
         if (sum) atomicAdd(&sh.found_w, sum);
         __syncthreads();
-        kept = min(kept, sh.bw[b0] + sh.found_w);
+        cut = min(cut, sh.bw[bm0] + sh.found_w);
+        __syncthreads();
     }
-    const float u = a.u[row];
-    double want = u > 0.0f ? (double)u * (double)kept : 0.0;
-    if (!(want < (double)kept)) want = (double)kept;
-    const u64 target = min((u64)want + 1, kept);  // passes u S: reaches the next whole number
+    const u64 target = share_of<true>(u, cut);
     const int b = bin_that_reaches<false>(sh, target);
     search<false>(a, sh, row, b, target - sh.bw[b], l0, c);
     if (t == 0) {
         a.idx[row] = (int32_t)(uint32_t)sh.found_q;
-        if (a.prob) a.prob[row] = (float)((double)sh.found_w / (double)kept);
+        if (a.prob) a.prob[row] = (float)((double)sh.found_w / (double)cut);
     }
 }
 
-struct SampleLayout { size_t bw, smax, off, list, total; };
+struct SampleLayout { size_t bw, smax, off, list, total; int slice, ns, parts; };
 static SampleLayout sample_layout(int n, int nr) {
-    const size_t at = (size_t)nr * (((size_t)n + kSlice - 1) / kSlice);
     SampleLayout w{};
+    w.slice = kLeastSlice;
+    while ((n + w.slice - 1) / w.slice > kMostSlices) w.slice *= 2;
+    w.ns = (n + w.slice - 1) / w.slice;
+    w.parts = (n + kMaxPart - 1) / kMaxPart;
+    const size_t at = (size_t)nr * w.ns;
     w.bw = 0;
     w.list = w.bw + at * kBins * 8;
-    w.off = w.list + at * kSlice * 2;
+    w.off = w.list + at * w.slice * 2;
     w.smax = w.off + at * kOffs * 2;
-    w.total = w.smax + at * 4;
+    w.total = w.smax + (size_t)nr * w.parts * 4;
     return w;
 }
 static bool sample_shape(int n, int nr) { return n >= 1 && n <= kMaxTokens && nr >= 1 && nr <= 65535; }
@@ -380,14 +546,20 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     const SampleLayout wl = sample_layout(n, nr);
     char* p = (char*)work;
     SampleArgs a{};
-    a.logits = logits; a.bf16 = logits_bf16 ? 1 : 0; a.n = n; a.ld = nr > 1 ? ld : 0; a.nr = nr; a.ns = (n + kSlice - 1) / kSlice;
+    a.logits = logits; a.bf16 = logits_bf16 ? 1 : 0; a.n = n; a.ld = nr > 1 ? ld : 0; a.nr = nr;
+    a.ns = wl.ns; a.slice = wl.slice; a.parts = wl.parts;
     a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
     a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off); a.smax = (float*)(p + wl.smax);
     a.idx = idx; a.prob = prob;
     const dim3 grid((unsigned)a.ns, (unsigned)nr);
-    hipLaunchKernelGGL(k_sample_max, grid, dim3(256), 0, (hipStream_t)s, a);
+    hipLaunchKernelGGL(k_sample_max, dim3((unsigned)a.parts, (unsigned)nr), dim3(256), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
-    hipLaunchKernelGGL(k_sample_bins, grid, dim3(kBinThreads), 0, (hipStream_t)s, a);
+    if (a.slice == kLeastSlice) {
+        hipLaunchKernelGGL(k_sample_bins<kLeastSlice / kPer>, grid, dim3(kLeastSlice / kPer), 2 * a.slice, (hipStream_t)s, a);
+    } else {
+        Q27X_HIP(allow_lds<k_sample_bins<1024>>(2 * kMostSlice));
+        hipLaunchKernelGGL(k_sample_bins<1024>, grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
+    }
     Q27X_HIP(hipGetLastError());
     hipLaunchKernelGGL(k_sample_draw, dim3((unsigned)nr), dim3(kDrawThreads), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
