@@ -21,9 +21,10 @@ namespace q27x {
 
 typedef unsigned long long u64;
 constexpr int kMaxPart = 4096;                    // logits of a block of k_sample_max
-constexpr int kLeastSlice = 4096, kMostSlices = 16, kMostSlice = 32768, kPer = 8;
+constexpr int kLeastSlice = 4096, kMostSlices = 16, kMostSlice = 32768, kCopies = 4;
 constexpr int kBins = 384, kOffs = kBins + 8;     // a slice's list offsets by bin, in u16
-constexpr int kDrawThreads = 256, kFew = 256, kHeld = 2048;     // tokens counted among each other, and held in LDS
+constexpr int kDrawThreads = 256, kHeld = 2048;   // (tokens that LDS holds)
+constexpr int kFew = 256, kLeft = 64;             // tokens counted among each other at once, and at a search's end
 constexpr u64 kUnit = 1ull << 44;                 // the weight of the largest logit
 constexpr int kMaxTokens = 1 << 19;               // (their weights' sum fits 64 bits, 16 slices hold them)
 
@@ -119,67 +120,86 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleArgs a) {
     if (threadIdx.x == 0) a.smax[(size_t)row * a.parts + s] = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
 }
 
-// T threads with 8 tokens each, a slice of 8 T or 4 times that
-template <int T>
+// A slice of T PER tokens (ROUNDS of them where the slice is larger). Bins are kept four times, by lane, as a wave's 64 tokens
+// lie in some 70 bins at most: adding to one place waits for one another. Counting gives a token its place in its bin at once.
+template <int T, int PER, bool MANY>
 __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint16_t s_list[];
-    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice;
-    __shared__ u64 s_w[kBins];
-    __shared__ uint32_t s_n[kBins], s_at[kBins], s_part[kBins / 64];
-    for (int b = t; b < kBins; b += T) { s_w[b] = 0; s_n[b] = 0; }
+    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice, copy = t & (kCopies - 1);
+    __shared__ u64 s_w[kBins * kCopies];
+    __shared__ uint32_t s_n[kBins * kCopies], s_part[(kBins + 63) / 64];
+    for (int b = t; b < kBins * kCopies; b += T) { s_w[b] = 0; s_n[b] = 0; }
     const float top = row_max(a, row);
     bool greedy;
     const double c = inv_temp(a, row, greedy), l0 = (double)top;
+    uint32_t place[PER];                          // of a token: its bin's copy, and how many came before it there; ~0: left out
     __syncthreads();
-    for (int i0 = 0; i0 < a.slice; i0 += kPer * T) {
-        float v[kPer / 4][4];
+    auto take = [&](int i0, bool add) __attribute__((always_inline)) {
+        float v[PER / 4][4];
 #pragma unroll
-        for (int j = 0; j < kPer / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+        for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
+        for (int j = 0; j < PER; ++j) {
             const float l = v[j / 4][j % 4];
             const double z = order_of(l, l0, c);
+            place[j] = ~0u;
             if (is_finite(l) && z < 48.0) {
-                atomicAdd(&s_w[bin_of(z)], weight(z));
-                atomicAdd(&s_n[bin_of(z)], 1u);
+                const int b = bin_of(z) * kCopies + copy;
+                if (add) atomicAdd(&s_w[b], weight(z));
+                place[j] = (uint32_t)b << 16 | atomicAdd(&s_n[b], 1u);
             }
         }
-    }
+    };
+    for (int i0 = 0; i0 < a.slice; i0 += PER * T) take(i0, true);
     __syncthreads();
     // where each bin begins
     const size_t at = (size_t)row * a.ns + s;
-    uint32_t n = t < kBins ? s_n[t] : 0, run = n;
+    uint32_t n[kCopies], run = 0;
     if (t < kBins) {
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) {
+            n[k] = s_n[t * kCopies + k];
+            run += n[k];
+        }
+        const uint32_t mine = run;
 #pragma unroll
         for (int o = 1; o < 64; o *= 2) {
             const uint32_t y = __shfl_up(run, o, 64);
             run += (t & 63) >= o ? y : 0;
         }
-        if ((t & 63) == 63) s_part[t >> 6] = run;
+        if ((t & 63) == 63 || t == kBins - 1) s_part[t >> 6] = run;
+        run -= mine;
     }
     __syncthreads();
     uint32_t total = 0;
 #pragma unroll
-    for (int k = 0; k < kBins / 64; ++k) {
+    for (int k = 0; k < (kBins + 63) / 64; ++k) {
         run += k < t >> 6 ? s_part[k] : 0;
         total += s_part[k];
     }
     if (t < kBins) {
-        s_at[t] = run - n;
-        a.off[at * kOffs + t] = (uint16_t)(run - n);
-        a.bw[at * kBins + t] = s_w[t];
+        a.off[at * kOffs + t] = (uint16_t)run;
+        u64 w = 0;
+#pragma unroll
+        for (int k = 0; k < kCopies; ++k) {
+            w += s_w[t * kCopies + k];
+            s_n[t * kCopies + k] = run;
+            run += n[k];
+        }
+        a.bw[at * kBins + t] = w;
         if (t == kBins - 1) a.off[at * kOffs + kBins] = (uint16_t)run;
     }
     __syncthreads();
-    for (int i0 = 0; i0 < a.slice; i0 += kPer * T) {
-        float v[kPer / 4][4];
+    if constexpr (!MANY) {
 #pragma unroll
-        for (int j = 0; j < kPer / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+        for (int j = 0; j < PER; ++j)
+            if (place[j] != ~0u) s_list[s_n[place[j] >> 16] + (place[j] & 0xFFFFu)] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
+    } else {
+        for (int i0 = 0; i0 < a.slice; i0 += PER * T) {
+            take(i0, false);                      // (the bins' beginnings count on)
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const float l = v[j / 4][j % 4];
-            const double z = order_of(l, l0, c);
-            if (is_finite(l) && z < 48.0) s_list[atomicAdd(&s_at[bin_of(z)], 1u)] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
+            for (int j = 0; j < PER; ++j)
+                if (place[j] != ~0u) s_list[place[j] & 0xFFFFu] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
         }
     }
     __syncthreads();
@@ -214,7 +234,7 @@ struct DrawShared {
     Sum part[kBins / 64];
     u64 hw[256];                                  // a narrowing step's digits
     uint32_t hn[256];
-    u64 q[kHeld], w[kHeld];                       // candidates
+    ulonglong2 qw[kHeld];                         // candidates: rank, weight
     u64 lo[4], hi[4], found_q, found_w, found_end, digit_w;
     uint32_t held, digit, digit_n, left;
 };
@@ -240,19 +260,35 @@ __device__ __forceinline__ uint32_t hold(const SampleArgs& a, DrawShared& sh, in
     __syncthreads();
     each_listed(a, sh, row, b0, b1, l0, c, [&](u64 q, u64 w) {
         const uint32_t k = atomicAdd(&sh.held, 1u);
-        sh.q[k] = q;
-        sh.w[k] = w;
+        sh.qw[k] = make_ulonglong2(q, w);
     });
     __syncthreads();
     return sh.held;
 }
-// What comes before this thread's token (q) among the n held ones.
-__device__ __forceinline__ Sum before_of(const DrawShared& sh, uint32_t n, u64 q) {
-    Sum x = {0, 0};
-    for (uint32_t i = 0; i < n; ++i) {
-        const bool is = sh.q[i] < q;
-        x.n += is ? 1u : 0u;
-        x.w += is ? sh.w[i] : 0;
+// Four, two or one threads a token: the held token that this thread is one of, and what comes before it among the n held ones.
+struct Counted { bool is; u64 q, w; Sum before; };
+__device__ __forceinline__ Counted count_held(const DrawShared& sh, uint32_t n) {
+    const uint32_t t = threadIdx.x, parts = n <= 64 ? 4 : n <= 128 ? 2 : 1, i = t / parts;
+    Counted x;
+    x.is = i < n && t % parts == 0;
+    const ulonglong2 mine = sh.qw[i < n ? i : 0];
+    x.q = mine.x;
+    x.w = mine.y;
+    x.before = {0, 0};
+#pragma unroll 4
+    for (uint32_t j = t % parts; j < n; j += parts) {
+        const ulonglong2 y = sh.qw[j];
+        const bool first = y.x < x.q;
+        x.before.n += first ? 1u : 0u;
+        x.before.w += first ? y.y : 0;
+    }
+    if (parts >= 2) {
+        x.before.n += __shfl_xor(x.before.n, 1, 64);
+        x.before.w += shfl_xor64(x.before.w, 1);
+    }
+    if (parts == 4) {
+        x.before.n += __shfl_xor(x.before.n, 2, 64);
+        x.before.w += shfl_xor64(x.before.w, 2);
     }
     return x;
 }
@@ -268,10 +304,10 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
     bool held = n <= kHeld;
     u64 lo = 0, hi = ~0ull;
     auto each = [&](auto f) {
-        if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.q[i], sh.w[i]);
+        if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.qw[i].x, sh.qw[i].y);
         else each_listed(a, sh, row, b, b, l0, c, f);
     };
-    while (n > kFew) {
+    while (n > kLeft) {
         // the range of what is left, in 256 parts
         u64 least = ~0ull, most = 0;
         each([&](u64 q, u64) {
@@ -329,45 +365,34 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
         before += sh.digit_w;
         target -= BY_COUNT ? sh.digit_n : sh.digit_w;
         const uint32_t left = sh.left;
-        if (left <= kFew) {                       // these alone, at the front
-            u64 kq[kHeld / kDrawThreads], kw[kHeld / kDrawThreads];
+        if (held || left <= kHeld) {              // these alone, at the front
             if (held) {
+                ulonglong2 x[kHeld / kDrawThreads];
 #pragma unroll
                 for (int k = 0; k < kHeld / kDrawThreads; ++k) {
                     const uint32_t i = t + k * kDrawThreads;
-                    kq[k] = i < n ? sh.q[i] : 0;
-                    kw[k] = i < n ? sh.w[i] : 0;
-                    if (i >= n || kq[k] < lo || kq[k] > hi) kq[k] = ~0ull;
+                    x[k] = sh.qw[i];
+                    if (i >= n || x[k].x < lo || x[k].x > hi) x[k].x = ~0ull;
                 }
                 __syncthreads();
 #pragma unroll
                 for (int k = 0; k < kHeld / kDrawThreads; ++k)
-                    if (kq[k] != ~0ull) {
-                        const uint32_t i = atomicAdd(&sh.held, 1u);
-                        sh.q[i] = kq[k];
-                        sh.w[i] = kw[k];
-                    }
+                    if (x[k].x != ~0ull) sh.qw[atomicAdd(&sh.held, 1u)] = x[k];
             } else {
                 each_listed(a, sh, row, b, b, l0, c, [&](u64 q, u64 w) {
-                    if (q >= lo && q <= hi) {
-                        const uint32_t i = atomicAdd(&sh.held, 1u);
-                        sh.q[i] = q;
-                        sh.w[i] = w;
-                    }
+                    if (q >= lo && q <= hi) sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w);
                 });
+                held = true;
             }
             __syncthreads();
             n = left;
         }
     }
-    if ((uint32_t)t < n) {
-        const Sum x = before_of(sh, n, sh.q[t]);
-        const u64 w = sh.w[t];
-        if (BY_COUNT ? x.n + 1 == target : x.w < target && target <= x.w + w) {
-            sh.found_q = sh.q[t];
-            sh.found_w = w;
-            sh.found_end = before + x.w + w;
-        }
+    const Counted x = count_held(sh, n);
+    if (x.is && (BY_COUNT ? x.before.n + 1 == target : x.before.w < target && target <= x.before.w + x.w)) {
+        sh.found_q = x.q;
+        sh.found_w = x.w;
+        sh.found_end = before + x.before.w + x.w;
     }
     __syncthreads();
 }
@@ -458,23 +483,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
     const int upto = by_k ? bk : by_p ? bin_that_reaches<false>(sh, share_of<false>(p, kept)) : by_m ? bm1 : kBins - 1;
     if (sh.bn[upto + 1] <= kFew) {
-        // a thread a token
-        const uint32_t n = hold(a, sh, row, 0, upto, l0, c);
-        const bool is = (uint32_t)t < n;
-        const u64 q = is ? sh.q[t] : ~0ull, w = is ? sh.w[t] : 0;
-        const Sum x = before_of(sh, n, q);
-        const u64 end = x.w + w;
-        if (by_k) kept = max_block(sh, is && x.n < (uint32_t)k ? end : 0);
+        const Counted x = count_held(sh, hold(a, sh, row, 0, upto, l0, c));
+        const u64 end = x.before.w + x.w;
+        if (by_k) kept = max_block(sh, x.is && x.before.n < (uint32_t)k ? end : 0);
         u64 cut = kept;
         if (by_p) {
             const u64 target = share_of<false>(p, kept);
-            cut = max_block(sh, is && x.w < target ? min(end, kept) : 0);
+            cut = max_block(sh, x.is && x.before.w < target ? min(end, kept) : 0);
         }
-        if (by_m) cut = min(cut, max_block(sh, is && w >= least ? end : 0));
+        if (by_m) cut = min(cut, max_block(sh, x.is && x.w >= least ? end : 0));
         const u64 target = share_of<true>(u, cut);
-        if (is && x.w < target && target <= end) {
-            a.idx[row] = (int32_t)(uint32_t)q;
-            if (a.prob) a.prob[row] = (float)((double)w / (double)cut);
+        if (x.is && x.before.w < target && target <= end) {
+            a.idx[row] = (int32_t)(uint32_t)x.q;
+            if (a.prob) a.prob[row] = (float)((double)x.w / (double)cut);
         }
         return;
     }
@@ -554,11 +575,16 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     const dim3 grid((unsigned)a.ns, (unsigned)nr);
     hipLaunchKernelGGL(k_sample_max, dim3((unsigned)a.parts, (unsigned)nr), dim3(256), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
-    if (a.slice == kLeastSlice) {
-        hipLaunchKernelGGL(k_sample_bins<kLeastSlice / kPer>, grid, dim3(kLeastSlice / kPer), 2 * a.slice, (hipStream_t)s, a);
+    if (a.slice == 4096) {
+        hipLaunchKernelGGL((k_sample_bins<512, 8, false>), grid, dim3(512), 2 * a.slice, (hipStream_t)s, a);
+    } else if (a.slice == 8192) {
+        hipLaunchKernelGGL((k_sample_bins<1024, 8, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
+    } else if (a.slice == 16384) {
+        Q27X_HIP((allow_lds<k_sample_bins<1024, 16, false>>(2 * kMostSlice)));
+        hipLaunchKernelGGL((k_sample_bins<1024, 16, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
     } else {
-        Q27X_HIP(allow_lds<k_sample_bins<1024>>(2 * kMostSlice));
-        hipLaunchKernelGGL(k_sample_bins<1024>, grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
+        Q27X_HIP((allow_lds<k_sample_bins<1024, 16, true>>(2 * kMostSlice)));
+        hipLaunchKernelGGL((k_sample_bins<1024, 16, true>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
     }
     Q27X_HIP(hipGetLastError());
     hipLaunchKernelGGL(k_sample_draw, dim3((unsigned)nr), dim3(kDrawThreads), 0, (hipStream_t)s, a);
