@@ -25,6 +25,7 @@ constexpr int kLeastSlice = 4096, kMostSlices = 16, kMostSlice = 32768, kCopies 
 constexpr int kBins = 384, kOffs = kBins + 8;     // a slice's list offsets by bin, in u16
 constexpr int kDrawThreads = 256, kHeld = 2048;   // (tokens that LDS holds)
 constexpr int kFew = 256, kLeft = 64;             // tokens counted among each other at once, and at a search's end
+constexpr int kAhead = 64, kBatch = 8;            // tokens of each slice's list read ahead; held tokens compared at a time
 constexpr u64 kUnit = 1ull << 44;                 // the weight of the largest logit
 constexpr int kMaxTokens = 1 << 19;               // (their weights' sum fits 64 bits, 16 slices hold them)
 
@@ -128,16 +129,19 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice, copy = t & (kCopies - 1);
     __shared__ u64 s_w[kBins * kCopies];
     __shared__ uint32_t s_n[kBins * kCopies], s_part[(kBins + 63) / 64];
+    float v[PER / 4][4];
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+    };
+    load(0);                                      // (requested before the maximum that they wait for)
     for (int b = t; b < kBins * kCopies; b += T) { s_w[b] = 0; s_n[b] = 0; }
     const float top = row_max(a, row);
     bool greedy;
     const double c = inv_temp(a, row, greedy), l0 = (double)top;
     uint32_t place[PER];                          // of a token: its bin's copy, and how many came before it there; ~0: left out
     __syncthreads();
-    auto take = [&](int i0, bool add) __attribute__((always_inline)) {
-        float v[PER / 4][4];
-#pragma unroll
-        for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
+    auto take = [&](bool add) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
             const float l = v[j / 4][j % 4];
@@ -150,7 +154,12 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
             }
         }
     };
-    for (int i0 = 0; i0 < a.slice; i0 += PER * T) take(i0, true);
+    take(true);
+    if constexpr (MANY)
+        for (int i0 = PER * T; i0 < a.slice; i0 += PER * T) {
+            load(i0);
+            take(true);
+        }
     __syncthreads();
     // where each bin begins
     const size_t at = (size_t)row * a.ns + s;
@@ -196,7 +205,8 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
             if (place[j] != ~0u) s_list[s_n[place[j] >> 16] + (place[j] & 0xFFFFu)] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
     } else {
         for (int i0 = 0; i0 < a.slice; i0 += PER * T) {
-            take(i0, false);                      // (the bins' beginnings count on)
+            load(i0);
+            take(false);                          // (the bins' beginnings count on)
 #pragma unroll
             for (int j = 0; j < PER; ++j)
                 if (place[j] != ~0u) s_list[place[j] & 0xFFFFu] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
@@ -234,9 +244,10 @@ struct DrawShared {
     Sum part[kBins / 64];
     u64 hw[256];                                  // a narrowing step's digits
     uint32_t hn[256];
-    ulonglong2 qw[kHeld];                         // candidates: rank, weight
-    u64 lo[4], hi[4], found_q, found_w, found_end, digit_w;
-    uint32_t held, digit, digit_n, left;
+    ulonglong2 qw[kHeld + 4 * kBatch];            // candidates: rank, weight
+    u64 lo[4], hi[4], found_q, found_w, found_end, digit_w, end_k, end_p, end_m;
+    uint32_t held, digit, digit_n, left, heavy;
+    int bk, bp;
 };
 
 // The tokens of bins b0 .. b1 of the row, f(rank, weight) for each, the block's threads side by side.
@@ -265,7 +276,8 @@ __device__ __forceinline__ uint32_t hold(const SampleArgs& a, DrawShared& sh, in
     __syncthreads();
     return sh.held;
 }
-// Four, two or one threads a token: the held token that this thread is one of, and what comes before it among the n held ones.
+// Four, two or one threads a token: the held token that this thread is one of, and what comes before it among the n held ones
+// (a call's threads past the last one's batches have put ranks behind all others there).
 struct Counted { bool is; u64 q, w; Sum before; };
 __device__ __forceinline__ Counted count_held(const DrawShared& sh, uint32_t n) {
     const uint32_t t = threadIdx.x, parts = n <= 64 ? 4 : n <= 128 ? 2 : 1, i = t / parts;
@@ -275,12 +287,16 @@ __device__ __forceinline__ Counted count_held(const DrawShared& sh, uint32_t n) 
     x.q = mine.x;
     x.w = mine.y;
     x.before = {0, 0};
-#pragma unroll 4
-    for (uint32_t j = t % parts; j < n; j += parts) {
-        const ulonglong2 y = sh.qw[j];
-        const bool first = y.x < x.q;
-        x.before.n += first ? 1u : 0u;
-        x.before.w += first ? y.y : 0;
+    for (uint32_t j0 = t % parts; j0 < n; j0 += parts * kBatch) {
+        ulonglong2 y[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) y[k] = sh.qw[j0 + parts * k];       // (behind the n: ranks that come after all)
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+            const bool first = y[k].x < x.q;
+            x.before.n += first ? 1u : 0u;
+            x.before.w += first ? y[k].y : 0;
+        }
     }
     if (parts >= 2) {
         x.before.n += __shfl_xor(x.before.n, 1, 64);
@@ -388,6 +404,8 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
             n = left;
         }
     }
+    if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
+    __syncthreads();
     const Counted x = count_held(sh, n);
     if (x.is && (BY_COUNT ? x.before.n + 1 == target : x.before.w < target && target <= x.before.w + x.w)) {
         sh.found_q = x.q;
@@ -408,15 +426,6 @@ __device__ int bin_that_reaches(const DrawShared& sh, u64 target) {
     }
     return lo;
 }
-// the largest of a value over the block
-__device__ __forceinline__ u64 max_block(DrawShared& sh, u64 x) {
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) x = max(x, shfl_xor64(x, o));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.lo[threadIdx.x >> 6] = x;
-    __syncthreads();
-    return max(max(sh.lo[0], sh.lo[1]), max(sh.lo[2], sh.lo[3]));
-}
 // the whole number that a running weight has to reach to be at least (PASS: more than) share x kept, of 1 .. kept
 template <bool PASS>
 __device__ __forceinline__ u64 share_of(float share, u64 kept) {
@@ -434,9 +443,16 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const double c = inv_temp(a, row, greedy), l0 = (double)top;
     const int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-    // the slices' lists, and bins 2 t and 2 t + 1 of the row
+    // the slices' lists, bins 2 t and 2 t + 1 of the row, and the first tokens of each slice's list
     for (int i = t; i < a.ns * (kOffs / 8); i += kDrawThreads)
         *(uint4*)&sh.off[i / (kOffs / 8)][8 * (i % (kOffs / 8))] = *(const uint4*)(a.off + ((size_t)row * a.ns + i / (kOffs / 8)) * kOffs + 8 * (i % (kOffs / 8)));
+    constexpr int kAheadOf = kMostSlices * kAhead / kDrawThreads;
+    int id[kAheadOf];
+#pragma unroll
+    for (int j = 0; j < kAheadOf; ++j) {
+        const int s = (t >> 6) + 4 * j;           // (any entry of a list is read as a token of its slice: those behind its end are not used)
+        id[j] = s < a.ns ? min(s * a.slice + (int)a.list[((size_t)row * a.ns + s) * a.slice + (t & 63)], a.n - 1) : 0;
+    }
     u64 w0 = 0, w1 = 0;
     if (t < kBins / 2)
 #pragma unroll 8
@@ -445,53 +461,91 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
             w0 += x.x;
             w1 += x.y;
         }
+    float ahead[kAheadOf];
+#pragma unroll
+    for (int j = 0; j < kAheadOf; ++j) ahead[j] = logit_at(a, row, id[j]);
     if (!is_finite(top)) {                        // (no finite logit)
         if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
     }
+    if (t == 0) { sh.held = 0; sh.heavy = 0; sh.bk = sh.bp = kBins - 1; }
     __syncthreads();
+    uint32_t n0 = 0, n1 = 0;
+    Sum run = {0, 0};
     if (t < kBins / 2) {
-        uint32_t n0 = 0, n1 = 0;
         for (int s = 0; s < a.ns; ++s) {
             const uint32_t o0 = sh.off[s][2 * t], o1 = sh.off[s][2 * t + 1], o2 = sh.off[s][2 * t + 2];
             n0 += o1 - o0;
             n1 += o2 - o1;
         }
-        const Sum mine = {n0 + n1, w0 + w1};
-        Sum run = scan_wave(mine);
+        run = scan_wave({n0 + n1, w0 + w1});
         if ((t & 63) == 63) sh.part[t >> 6] = run;
-        sh.bn[2 * t + 1] = run.n - n1;
-        sh.bn[2 * t + 2] = run.n;
-        sh.bw[2 * t + 1] = run.w - w1;
-        sh.bw[2 * t + 2] = run.w;
-        if (t == 0) { sh.bn[0] = 0; sh.bw[0] = 0; }
     }
     __syncthreads();
-    if (t >= 64 && t < kBins / 2) {
-        Sum x = sh.part[0];
-        if (t >= 128) { x.n += sh.part[1].n; x.w += sh.part[1].w; }
-        sh.bn[2 * t + 1] += x.n; sh.bn[2 * t + 2] += x.n;
-        sh.bw[2 * t + 1] += x.w; sh.bw[2 * t + 2] += x.w;
+    const Sum all = {sh.part[0].n + sh.part[1].n + sh.part[2].n, sh.part[0].w + sh.part[1].w + sh.part[2].w};
+    static_assert(kBins / 128 == 3, "three waves of bins");
+    u64 kept = all.w;                             // the weight of what is kept
+    const bool by_k = k >= 1 && (uint32_t)k < all.n, by_p = p < 1.0f, by_m = m > 0.0f;
+    if (t < kBins / 2) {
+        if (t >= 64) { run.n += sh.part[0].n; run.w += sh.part[0].w; }
+        if (t >= 128) { run.n += sh.part[1].n; run.w += sh.part[1].w; }
+        const uint32_t na = run.n - n0 - n1, nb = run.n - n1;
+        const u64 wa = run.w - w0 - w1, wb = run.w - w1;
+        sh.bn[2 * t] = na;
+        sh.bn[2 * t + 1] = nb;
+        sh.bw[2 * t] = wa;
+        sh.bw[2 * t + 1] = wb;
+        if (t == kBins / 2 - 1) { sh.bn[kBins] = run.n; sh.bw[kBins] = run.w; }
+        // the bins in which the cuts end (by weight, of all)
+        if (by_k && na < (uint32_t)k && (uint32_t)k <= run.n) sh.bk = 2 * t + ((uint32_t)k > nb);
+        const u64 target = share_of<false>(p, kept);
+        if (by_p && wa < target && target <= run.w) sh.bp = 2 * t + (target > wb);
     }
     __syncthreads();
-    u64 kept = sh.bw[kBins];                      // the weight of what is kept
-    const bool by_k = k >= 1 && (uint32_t)k < sh.bn[kBins], by_p = p < 1.0f, by_m = m > 0.0f;
-    const int bk = by_k ? bin_that_reaches<true>(sh, (u64)k) : kBins - 1;
+    const int bk = sh.bk;
     const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
     // bins that tokens of weight `least` are in (the logarithm is rounded)
     const double zm = by_m && m < 1.0f ? -log2((double)m) : 0.0;
     const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
-    const int upto = by_k ? bk : by_p ? bin_that_reaches<false>(sh, share_of<false>(p, kept)) : by_m ? bm1 : kBins - 1;
+    const int upto = by_k ? bk : by_p ? sh.bp : by_m ? bm1 : kBins - 1;
     if (sh.bn[upto + 1] <= kFew) {
-        const Counted x = count_held(sh, hold(a, sh, row, 0, upto, l0, c));
-        const u64 end = x.before.w + x.w;
-        if (by_k) kept = max_block(sh, x.is && x.before.n < (uint32_t)k ? end : 0);
-        u64 cut = kept;
-        if (by_p) {
-            const u64 target = share_of<false>(p, kept);
-            cut = max_block(sh, x.is && x.before.w < target ? min(end, kept) : 0);
+        // the tokens that can be drawn, into LDS: what was read ahead, and the rest of a longer list
+        for (int s = t >> 6, j = 0; s < a.ns; s += 4, ++j) {
+            const size_t at = (size_t)row * a.ns + s;
+            const int end = sh.off[s][upto + 1];
+            for (int i = t & 63; i < end; i += 64) {
+                int of = 0;
+                float x = 0.0f;
+                if (i < kAhead) {
+#pragma unroll
+                    for (int y = 0; y < kAheadOf; ++y) {
+                        of = y == j ? id[y] : of;
+                        x = y == j ? ahead[y] : x;
+                    }
+                } else {
+                    of = s * a.slice + a.list[at * a.slice + i];
+                    x = logit_at(a, row, of);
+                }
+                sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(rank_of(x, of), weight(order_of(x, l0, c)));
+            }
         }
-        if (by_m) cut = min(cut, max_block(sh, x.is && x.w >= least ? end : 0));
+        const uint32_t n = sh.bn[upto + 1];
+        if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
+        __syncthreads();
+        const Counted x = count_held(sh, n);
+        const u64 end = x.before.w + x.w;
+        if (by_k && x.is && x.before.n + 1 == (uint32_t)k) sh.end_k = end;
+        const uint32_t heavy = (uint32_t)__popcll(__ballot(x.is && x.w >= least));
+        if ((t & 63) == 0 && heavy) atomicAdd(&sh.heavy, heavy);
+        __syncthreads();
+        if (by_k) kept = sh.end_k;
+        const u64 want = share_of<false>(p, kept);
+        if (by_p && x.is && x.before.w < want && want <= end) sh.end_p = end;
+        if (by_m && x.is && x.before.n + 1 == sh.heavy) sh.end_m = end;
+        __syncthreads();
+        u64 cut = kept;
+        if (by_p) cut = min(cut, sh.end_p);
+        if (by_m) cut = min(cut, sh.end_m);
         const u64 target = share_of<true>(u, cut);
         if (x.is && x.before.w < target && target <= end) {
             a.idx[row] = (int32_t)(uint32_t)x.q;
