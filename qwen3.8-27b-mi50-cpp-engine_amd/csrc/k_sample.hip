@@ -26,6 +26,7 @@ constexpr int kBins = 384, kOffs = kBins + 8;     // a slice's list offsets by b
 constexpr int kDrawThreads = 256, kHeld = 2048;   // (tokens that LDS holds)
 constexpr int kFew = 256, kLeft = 64;             // tokens counted among each other at once, and at a search's end
 constexpr int kAhead = 64, kBatch = 8;            // tokens of each slice's list read ahead; held tokens compared at a time
+constexpr int kAheadOf = kMostSlices * kAhead / kDrawThreads, kOffLoads = (kMostSlices * kOffs / 8 + kDrawThreads - 1) / kDrawThreads;    // of a thread
 constexpr u64 kUnit = 1ull << 44;                 // the weight of the largest logit
 constexpr int kMaxTokens = 1 << 19;               // (their weights' sum fits 64 bits, 16 slices hold them)
 
@@ -121,7 +122,24 @@ __global__ __launch_bounds__(256) void k_sample_max(SampleArgs a) {
     if (threadIdx.x == 0) a.smax[(size_t)row * a.parts + s] = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
 }
 
-// A slice of T PER tokens (ROUNDS of them where the slice is larger). Bins are kept four times, by lane, as a wave's 64 tokens
+// Inclusive running sum over the wave, by DPP: the 16 lanes of a row, then the rows' ends.
+__device__ __forceinline__ uint32_t scan_wave(uint32_t x) {
+#define Q27X_STEP(CTRL, ROWS) x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true)
+    Q27X_STEP(0x111, 0xF); Q27X_STEP(0x112, 0xF); Q27X_STEP(0x114, 0xF); Q27X_STEP(0x118, 0xF);
+    Q27X_STEP(0x142, 0xA); Q27X_STEP(0x143, 0xC);
+#undef Q27X_STEP
+    return x;
+}
+__device__ __forceinline__ u64 scan_wave(u64 x) {
+#define Q27X_STEP(CTRL, ROWS) x += (u64)(uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xF, true) << 32 | \
+                                   (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xF, true)
+    Q27X_STEP(0x111, 0xF); Q27X_STEP(0x112, 0xF); Q27X_STEP(0x114, 0xF); Q27X_STEP(0x118, 0xF);
+    Q27X_STEP(0x142, 0xA); Q27X_STEP(0x143, 0xC);
+#undef Q27X_STEP
+    return x;
+}
+
+// A slice of T PER tokens (MANY: some times that). Bins are kept four times, by lane, as a wave's 64 tokens
 // lie in some 70 bins at most: adding to one place waits for one another. Counting gives a token its place in its bin at once.
 template <int T, int PER, bool MANY>
 __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
@@ -171,11 +189,7 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
             run += n[k];
         }
         const uint32_t mine = run;
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const uint32_t y = __shfl_up(run, o, 64);
-            run += (t & 63) >= o ? y : 0;
-        }
+        run = scan_wave(run);
         if ((t & 63) == 63 || t == kBins - 1) s_part[t >> 6] = run;
         run -= mine;
     }
@@ -217,30 +231,15 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
 }
 
 struct Sum { uint32_t n; u64 w; };
-__device__ __forceinline__ u64 shfl_up64(u64 x, int o) {
-    const uint32_t lo = __shfl_up((uint32_t)x, o, 64), hi = __shfl_up((uint32_t)(x >> 32), o, 64);
-    return (u64)hi << 32 | lo;
-}
 __device__ __forceinline__ u64 shfl_xor64(u64 x, int o) {
     const uint32_t lo = __shfl_xor((uint32_t)x, o, 64), hi = __shfl_xor((uint32_t)(x >> 32), o, 64);
     return (u64)hi << 32 | lo;
-}
-// Inclusive running sums over the wave.
-__device__ __forceinline__ Sum scan_wave(Sum x) {
-    const int l = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const uint32_t n = __shfl_up(x.n, o, 64);
-        const u64 w = shfl_up64(x.w, o);
-        if (l >= o) { x.n += n; x.w += w; }
-    }
-    return x;
 }
 
 struct DrawShared {
     u64 bw[kBins + 1];                            // running weights and counts of the row's bins
     uint32_t bn[kBins + 1];
-    uint16_t off[kMostSlices][kOffs];             // the slices' lists by bin
+    __attribute__((aligned(16))) uint16_t off[kMostSlices][kOffs];    // the slices' lists by bin
     Sum part[kBins / 64];
     u64 hw[256];                                  // a narrowing step's digits
     uint32_t hn[256];
@@ -357,9 +356,7 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
             Sum x = {0, 0};
 #pragma unroll
             for (int k = 0; k < 4; ++k) { x.n += sh.hn[4 * t + k]; x.w += sh.hw[4 * t + k]; }
-            Sum run = scan_wave(x);
-            run.n -= x.n;
-            run.w -= x.w;
+            Sum run = {scan_wave(x.n) - x.n, scan_wave(x.w) - x.w};
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t pn = sh.hn[4 * t + k];
@@ -438,32 +435,46 @@ __device__ __forceinline__ u64 share_of(float share, u64 kept) {
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const int row = blockIdx.x, t = threadIdx.x;
     __shared__ DrawShared sh;
+    const size_t first = (size_t)row * a.ns;
+    // Requested at once, as each is a trip to memory: the first tokens of each slice's list, its offsets, bins 2 t and 2 t + 1
+    // of each; then these tokens' logits. (Any entry of a list is read as a token of its slice: those behind its end are not used.)
+    int id[kAheadOf];
+    uint4 off[kOffLoads];
+    ulonglong2 bw[kMostSlices];
+#pragma unroll
+    for (int j = 0; j < kAheadOf; ++j) {
+        const int s = min((t >> 6) + 4 * j, a.ns - 1);
+        id[j] = s * a.slice + (int)a.list[(first + s) * a.slice + (t & 63)];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < kOffLoads; ++j) off[j] = ((const uint4*)(a.off + first * kOffs))[min(t + j * kDrawThreads, a.ns * (kOffs / 8) - 1)];
+#pragma unroll
+    for (int s = 0; s < kMostSlices; ++s)
+        bw[s] = *(const ulonglong2*)(a.bw + (first + min(s, a.ns - 1)) * kBins + 2 * min(t, kBins / 2 - 1));
+    __builtin_amdgcn_sched_barrier(0);
     const float top = row_max(a, row);
     bool greedy;
     const double c = inv_temp(a, row, greedy), l0 = (double)top;
     const int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
     const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-    // the slices' lists, bins 2 t and 2 t + 1 of the row, and the first tokens of each slice's list
-    for (int i = t; i < a.ns * (kOffs / 8); i += kDrawThreads)
-        *(uint4*)&sh.off[i / (kOffs / 8)][8 * (i % (kOffs / 8))] = *(const uint4*)(a.off + ((size_t)row * a.ns + i / (kOffs / 8)) * kOffs + 8 * (i % (kOffs / 8)));
-    constexpr int kAheadOf = kMostSlices * kAhead / kDrawThreads;
-    int id[kAheadOf];
-#pragma unroll
-    for (int j = 0; j < kAheadOf; ++j) {
-        const int s = (t >> 6) + 4 * j;           // (any entry of a list is read as a token of its slice: those behind its end are not used)
-        id[j] = s < a.ns ? min(s * a.slice + (int)a.list[((size_t)row * a.ns + s) * a.slice + (t & 63)], a.n - 1) : 0;
-    }
-    u64 w0 = 0, w1 = 0;
-    if (t < kBins / 2)
-#pragma unroll 8
-        for (int s = 0; s < a.ns; ++s) {
-            const ulonglong2 x = *(const ulonglong2*)(a.bw + ((size_t)row * a.ns + s) * kBins + 2 * t);
-            w0 += x.x;
-            w1 += x.y;
-        }
+    const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
+    // bins that tokens of weight `least` are in (the logarithm is rounded)
+    const double zm = m < 1.0f ? -(double)__builtin_amdgcn_logf(m) : 0.0;
+    const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
     float ahead[kAheadOf];
 #pragma unroll
-    for (int j = 0; j < kAheadOf; ++j) ahead[j] = logit_at(a, row, id[j]);
+    for (int j = 0; j < kAheadOf; ++j) ahead[j] = logit_at(a, row, min(id[j], a.n - 1));
+#pragma unroll
+    for (int j = 0; j < kOffLoads; ++j)
+        if (t + j * kDrawThreads < kMostSlices * (kOffs / 8)) ((uint4*)sh.off)[t + j * kDrawThreads] = off[j];
+    u64 w0 = 0, w1 = 0;
+#pragma unroll
+    for (int s = 0; s < kMostSlices; ++s)
+        if (s < a.ns) {
+            w0 += bw[s].x;
+            w1 += bw[s].y;
+        }
     if (!is_finite(top)) {                        // (no finite logit)
         if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
@@ -478,7 +489,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
             n0 += o1 - o0;
             n1 += o2 - o1;
         }
-        run = scan_wave({n0 + n1, w0 + w1});
+        run = {scan_wave(n0 + n1), scan_wave(w0 + w1)};
         if ((t & 63) == 63) sh.part[t >> 6] = run;
     }
     __syncthreads();
@@ -503,10 +514,6 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     }
     __syncthreads();
     const int bk = sh.bk;
-    const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
-    // bins that tokens of weight `least` are in (the logarithm is rounded)
-    const double zm = by_m && m < 1.0f ? -log2((double)m) : 0.0;
-    const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
     const int upto = by_k ? bk : by_p ? sh.bp : by_m ? bm1 : kBins - 1;
     if (sh.bn[upto + 1] <= kFew) {
         // the tokens that can be drawn, into LDS: what was read ahead, and the rest of a longer list
