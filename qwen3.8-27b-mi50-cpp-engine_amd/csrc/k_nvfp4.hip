@@ -44,15 +44,14 @@ constexpr int kNvItems = 3;           // slabs of activations that a thread brin
 constexpr int kNvLds = 160 * 1024;
 constexpr int kNvMaxK = 65536;        // (the slots' sums have room in LDS)
 
-// LDS of a block: activation nibbles of its rows as operands, [rows][steps][low | high][256], and their scales, [rows][16
-// steps]; before them what lanes without activation codes read; behind them the waves' scales, the sums, [2][groups]
+// LDS of a block: activation nibbles of its rows as operands, [steps][rows][low | high][256], and their scales, [steps][rows]
+// [16]; before them what lanes without activation codes read; behind them the waves' scales, the sums, [2][groups]
 // [slots][32 PAIRS], and the weights of a last step that K does not fill, for each group codes [16][128] and scales [16][16].
 struct Nvfp4Lds {
-    static constexpr int kZeros = 512 * kNvSteps;
-    int row, xs, ws, sums, tail, total;
+    static constexpr int kZeros = 1024 * (kMaxRows / 2 - 1) + 512;
+    int xs, ws, sums, tail, total;
     __host__ __device__ __forceinline__ Nvfp4Lds(int rows, int steps, int per, int groups, int waves, int slots, int outs, bool ends_inside) {
-        row = 512 * steps;
-        xs = kZeros + rows * row;
+        xs = kZeros + 512 * rows * steps;
         ws = xs + 64 * rows * steps;
         sums = ws + 256 * (per | 1) * groups * waves;
         tail = sums + 8 * groups * slots * outs;
@@ -183,10 +182,11 @@ struct Nvfp4Rows {
                 const uint32_t h = (x[i][j] >> 4) & 0x0F0F0F0Fu, minus = h & 0x08080808u, one = minus >> 3;
                 hi[j] = ((h ^ ((minus << 1) - one)) + one) | (minus << 4);
             }
-            char* to = lds + Nvfp4Lds::kZeros + r * L.row + (slab >> 4) * 512 + (slab & 15) * 16;
+            const uint32_t at = (slab >> 4) * (uint32_t)n + r;
+            char* to = lds + Nvfp4Lds::kZeros + at * 512 + (slab & 15) * 16;
             *(u32x4*)to = lo;
             *(u32x4*)(to + 256) = hi;
-            *(float*)(lds + L.xs + 4 * k) = xs[i];
+            *(float*)(lds + L.xs + at * 64 + 4 * (slab & 15)) = xs[i];
         }
     }
 };
@@ -237,15 +237,18 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
         }
         __syncthreads();
     }
-    // the operand's row c holds slab c % 8 of row c / 8, in lanes g = c % 4, in its first or second half
-    int opa[2];
-    bool has[2];
+    // the operand's row c holds slab c % 8 of row c / 8 of a pair, in lanes g = c % 4, in its first or second half; the other lanes
+    // read zeros (an odd last row's neighbour reads what lies behind it, for outputs that are not)
+    const int rows_held = RESIDENT ? a.nr : min(a.nr, 2);
+    int opa[2], per_step[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        has[h] = (c & 3) == g && ((c >> 2) & 1) == h;
-        opa[h] = has[h] ? Nvfp4Lds::kZeros + (c >> 3) * L.row + wv * per * 512 + (c & 7) * 16 : 0;
+        const bool has = (c & 3) == g && ((c >> 2) & 1) == h;
+        opa[h] = has ? Nvfp4Lds::kZeros + 512 * (wv * per * rows_held + (c >> 3)) + (c & 7) * 16 : 0;
+        per_step[h] = has ? 512 * rows_held : 0;
     }
-    const int xsa = L.xs + 4 * ((g >> 1) * count + wv * per * 16 + 4 * (g & 1));
+    const int xsa = L.xs + 64 * (wv * per * rows_held + (g >> 1)) + 16 * (g & 1);
+    constexpr int kPasses = RESIDENT ? 1 : PAIRS, kIn = RESIDENT ? PAIRS : 1;        // over the weights, and pairs of each
     int parity = 0;
     for (int unit = blockIdx.x; unit * wide < tiles; unit += (int)gridDim.x, parity ^= 1) {
         const int after = tile + (int)gridDim.x * wide;
@@ -262,20 +265,15 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
             const int from = last ? wv * per : s0 + turn + wv * per;   // the steps after these
             const int sa = L.ws + 256 * (per | 1) * wave + 16 * (per | 1) * nvfp4_row_of(c) + 4 * (g & 1);
             w.store_scales(scales);
-            int o0 = opa[0], o1 = opa[1], ox = xsa;
-            if constexpr (RESIDENT) {
-                o0 = has[0] ? o0 + 512 * s0 : 0;
-                o1 = has[1] ? o1 + 512 * s0 : 0;
-                ox += 64 * s0;
-            }
-            asm volatile("" : "+v"(o0), "+v"(o1), "+v"(ox));          // (opaque: operands kept over the loop would spill)
 #pragma unroll
-            for (int p = 0; p < PAIRS; ++p) {
-                if (p + 1 == PAIRS && (a.nr & 1)) {   // (a row that is not: zeros, and some scales)
-                    o0 = c >> 3 ? 0 : o0;
-                    o1 = c >> 3 ? 0 : o1;
-                    ox = g >> 1 ? ox - 4 * count : ox;
+            for (int p = 0; p < kPasses; ++p) {
+                int o0 = opa[0], o1 = opa[1], ox = xsa;
+                if constexpr (RESIDENT) {
+                    o0 += per_step[0] * s0;
+                    o1 += per_step[1] * s0;
+                    ox += 64 * rows_held * s0;
                 }
+                asm volatile("" : "+v"(o0), "+v"(o1), "+v"(ox));      // (opaque: operands kept over the loop would spill)
                 if constexpr (!RESIDENT) {
                     __syncthreads();                  // (the pair before is read)
                     x.store(lds, L, min(a.nr, 2), count, 0);
@@ -284,7 +282,7 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
                     else x.load(a, 0, 2, last ? 0 : 16 * (s0 + turn), count, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                if (p + 1 == PAIRS) {
+                if (p + 1 == kPasses) {
                     w.load_scales(next, from, per, full);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -300,28 +298,30 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
                         constexpr int kOne = 127 + 9, k16 = kOne + 4;       // bytes are 2^-9 each
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            auto operand = [&](int at) __attribute__((always_inline)) {
-                                const u32x4 y = *(const u32x4*)(lds + o0 + at), z = *(const u32x4*)(lds + o1 + at);
-                                return i32x8{(int)y[0], (int)y[1], (int)y[2], (int)y[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
-                            };
-                            const i32x8 lo = operand(512 * j + 128 * h), hi = operand(512 * j + 256 + 128 * h);
-                            const f32x4 xs = *(const f32x4*)(lds + ox + 64 * j + 32 * h);
                             const u32x4 q = w.operand(j, h);
-                            const f32x4 d = nvfp4_dots(hi, q, nvfp4_dots(lo, q, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, kOne), k16);
                             const int e = *(const int*)(lds + sj + 8 * h);
                             const auto e0 = __builtin_amdgcn_cvt_pk_f32_fp8(e, false), e1 = __builtin_amdgcn_cvt_pk_f32_fp8(e, true);
-                            acc[p] = __builtin_fmaf(d[0], e0[0] * xs[0], acc[p]);
-                            acc[p] = __builtin_fmaf(d[1], e0[1] * xs[1], acc[p]);
-                            acc[p] = __builtin_fmaf(d[2], e1[0] * xs[2], acc[p]);
-                            acc[p] = __builtin_fmaf(d[3], e1[1] * xs[3], acc[p]);
+#pragma unroll
+                            for (int i = 0; i < kIn; ++i) {
+                                auto operand = [&](int at) __attribute__((always_inline)) {
+                                    const u32x4 y = *(const u32x4*)(lds + o0 + at), z = *(const u32x4*)(lds + o1 + at);
+                                    return i32x8{(int)y[0], (int)y[1], (int)y[2], (int)y[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
+                                };
+                                const i32x8 lo = operand(1024 * i + 128 * h), hi = operand(1024 * i + 256 + 128 * h);
+                                const f32x4 xs = *(const f32x4*)(lds + ox + 128 * i + 32 * h);
+                                const f32x4 d = nvfp4_dots(hi, q, nvfp4_dots(lo, q, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, kOne), k16);
+                                float& y = acc[RESIDENT ? i : p];
+                                y = __builtin_fmaf(d[0], e0[0] * xs[0], y);
+                                y = __builtin_fmaf(d[1], e0[1] * xs[1], y);
+                                y = __builtin_fmaf(d[2], e1[0] * xs[2], y);
+                                y = __builtin_fmaf(d[3], e1[1] * xs[3], y);
+                            }
                         }
                     }
-                    if (p + 1 == PAIRS) w.load(next, j, from + j, j < per && from + j < full);
-                }
-                if constexpr (RESIDENT) {
-                    o0 = has[0] ? o0 + 2 * L.row : 0;
-                    o1 = has[1] ? o1 + 2 * L.row : 0;
-                    ox += 8 * count;
+                    o0 += per_step[0];
+                    o1 += per_step[1];
+                    ox += 64 * rows_held;
+                    if (p + 1 == kPasses) w.load(next, j, from + j, j < per && from + j < full);
                 }
             }
             if (slot < slots) {
