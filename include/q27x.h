@@ -127,8 +127,8 @@ typedef struct q27x_nvfp4 {
 /* q27x_proj_rows on NVFP4 weights as they are, nothing requantized (the reference's q27_proj_nvfp4_down_nr and lm_head forms,
  * include/q27_nr.h:14-19; src/q27_nvfp4.hip:4337-4544):
  *   y[n][r] = alpha * sum over 16-slabs s of (dot of the slab's codes, exact) * (ws[r][s] * xs[n][s])  (+ rs * res[n][r])
- * in fp32. Arguments as q27x_proj_rows; any rows, K % 16 == 0; with nr > 1 xstride % 16 == 0. Row n's bits do not depend on the
- * other rows or on nr. */
+ * in fp32. Arguments as q27x_proj_rows; any rows, K % 16 == 0 up to 57344; with nr > 1 xstride % 16 == 0. Row n's bits
+ * do not depend on the other rows or on nr. */
 int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int xstride, const float* xs,
                          void* y, int ystride, int out_bf16, const void* res, int res_bf16,
                          int rstride, float rs, int nr, q27x_stream_t s);
@@ -136,7 +136,7 @@ int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int xstride, c
 /* Gate and up of an MLP on NVFP4 weights, and q27x_swiglu_quant_rows of them, in one launch (the reference's fused
  * q27_proj_nvfp4_gu_nr, include/q27_nr.h:14-19): gate and up [rows][K] as q27x_proj_nvfp4_rows computes them, fp32, then
  *   v = (g/(1+e^-g)) * u * (1/in_scale); per 16: s = mx/127; q = clamp(rint(v/s)) -> oq [nr][rows], os [nr][rows/16].
- * rows % 16 == 0, K % 16 == 0; in_scale is that of the projection that reads oq. */
+ * rows % 16 == 0, K as there; in_scale is that of the projection that reads oq. */
 int q27x_swiglu_nvfp4_rows(const q27x_nvfp4_t* gate, const q27x_nvfp4_t* up, const int8_t* xq, int xstride,
                            const float* xs, int8_t* oq, float* os, float in_scale, int nr, q27x_stream_t s);
 

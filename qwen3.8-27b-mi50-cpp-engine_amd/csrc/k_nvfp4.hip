@@ -40,9 +40,8 @@ struct Nvfp4Args {
 constexpr int kNvStep = 256;          // weights of a row that a wave takes at a time: a 128-byte line of codes
 constexpr int kNvSteps = 5;           // steps of a wave in registers
 constexpr int kNvWaves = 16;          // waves of a block at most
-constexpr int kNvItems = 3;           // slabs of activations that a thread brings at a time
 constexpr int kNvLds = 160 * 1024;
-constexpr int kNvMaxK = 65536;        // (the slots' sums have room in LDS)
+constexpr int kNvMaxK = 57344;        // (45 slots: their sums of gate and up, 8 rows, have room in LDS beside 20 steps of 4 rows: 157 KB)
 
 // LDS of a block: activation nibbles of its rows as operands, [steps][rows][low | high][256], and their scales, [steps][rows]
 // [16]; before them what lanes without activation codes read; behind them the waves' scales, the sums, [2][groups]
@@ -152,16 +151,17 @@ struct Nvfp4Weights {
     }
 };
 
-// A thread's share of some activation rows: up to kNvItems slabs.
+// A thread's share of some activation rows: up to ITEMS slabs.
+template <int ITEMS>
 struct Nvfp4Rows {
-    u32x4 x[kNvItems];
-    float xs[kNvItems];
+    u32x4 x[ITEMS];
+    float xs[ITEMS];
     // slabs first .. + count - 1 of rows r0 .. + n - 1 (zeros behind K and of rows that are not); items from `item` on
     __device__ __forceinline__ void load(const Nvfp4Args& a, int r0, int n, int first, int count, int item) {
         const Span xq_(a.xq, (uint32_t)(a.nr - 1) * (uint32_t)a.xstride + (uint32_t)a.K);
         const Span xs_(a.xs, (uint32_t)(a.nr - 1) * (uint32_t)(a.xstride >> 2) + (uint32_t)(a.K >> 2));
 #pragma unroll
-        for (int i = 0; i < kNvItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             const uint32_t k = (uint32_t)(item + (int)threadIdx.x + i * (int)blockDim.x), r = k / (uint32_t)count, slab = first + (k - r * (uint32_t)count);
             const bool there = (int)r < n && r0 + (int)r < a.nr && (int)slab < (a.K >> 4);
             const uint32_t off = (uint32_t)(r0 + (int)r) * (uint32_t)a.xstride + slab * 16;
@@ -172,7 +172,7 @@ struct Nvfp4Rows {
     // codes 16 h + l: l = 0 .. 15, h = -8 .. 7 as sign and size
     __device__ __forceinline__ void store(char* lds, const Nvfp4Lds& L, int n, int count, int item) const {
 #pragma unroll
-        for (int i = 0; i < kNvItems; ++i) {
+        for (int i = 0; i < ITEMS; ++i) {
             const uint32_t k = (uint32_t)(item + (int)threadIdx.x + i * (int)blockDim.x), r = k / (uint32_t)count, slab = k - r * (uint32_t)count;
             if ((int)r >= n) continue;
             u32x4 lo, hi;
@@ -202,23 +202,26 @@ __device__ __forceinline__ f32x4 nvfp4_dots(const i32x8& x, const u32x4& w, cons
 // tile are requested as this one's are used. An output is the sum of its slots in order, whatever the waves, so its bits do not
 // depend on nr.
 template <int PAIRS, bool SWIGLU, bool RESIDENT>
-__global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups, int waves, int per, int slots) {
+__global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups, int waves, int per, int slots) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
     const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
     const int tiles = (a.rows + 15) >> 4, wide = SWIGLU ? groups >> 1 : groups;
-    const Nvfp4Lds L(RESIDENT ? a.nr : min(a.nr, 2), held, per, groups, waves, slots, 32 * PAIRS, rest != 0);
+    constexpr int kIn = RESIDENT || PAIRS == 1 ? PAIRS : 2, kPasses = (PAIRS + kIn - 1) / kIn;        // pairs of a pass over the weights, and passes
+    constexpr int kItems = RESIDENT ? 3 : 5;
+    const int rows_held = RESIDENT ? a.nr : min(a.nr, 2 * kIn);
+    const Nvfp4Lds L(rows_held, held, per, groups, waves, slots, 32 * PAIRS, rest != 0);
     const uint8_t* wp = SWIGLU && (grp & 1) ? a.w[1] : a.w[0];
     const uint8_t* sp = SWIGLU && (grp & 1) ? a.s[1] : a.s[0];
     const int mine = SWIGLU ? grp >> 1 : grp;        // this group's tile of `wide`
     char* tail = lds + L.tail + 2304 * grp;
     for (int i = 16 * t; i < Nvfp4Lds::kZeros; i += 16 * (int)blockDim.x) *(u32x4*)(lds + i) = u32x4{0, 0, 0, 0};
-    Nvfp4Rows x;
+    Nvfp4Rows<kItems> x;
     Nvfp4Weights w;
     w.begin(a.K, per);
     char* scales = lds + L.ws + 256 * (per | 1) * wave;
-    x.load(a, 0, RESIDENT ? a.nr : 2, 0, count, 0);
+    x.load(a, 0, rows_held, 0, count, 0);
     __builtin_amdgcn_sched_barrier(0);               // (requested first: loads come in order)
     int tile = (int)blockIdx.x * wide + mine;
     {
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
     __builtin_amdgcn_sched_barrier(0);
     if constexpr (RESIDENT) {
         x.store(lds, L, a.nr, count, 0);
-        for (int item = kNvItems * (int)blockDim.x; item < a.nr * count; item += kNvItems * (int)blockDim.x) {
+        for (int item = kItems * (int)blockDim.x; item < a.nr * count; item += kItems * (int)blockDim.x) {
             x.load(a, 0, a.nr, 0, count, item);
             x.store(lds, L, a.nr, count, item);
         }
@@ -239,7 +242,6 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
     }
     // the operand's row c holds slab c % 8 of row c / 8 of a pair, in lanes g = c % 4, in its first or second half; the other lanes
     // read zeros (an odd last row's neighbour reads what lies behind it, for outputs that are not)
-    const int rows_held = RESIDENT ? a.nr : min(a.nr, 2);
     int opa[2], per_step[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -248,7 +250,6 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
         per_step[h] = has ? 512 * rows_held : 0;
     }
     const int xsa = L.xs + 64 * (wv * per * rows_held + (g >> 1)) + 16 * (g & 1);
-    constexpr int kPasses = RESIDENT ? 1 : PAIRS, kIn = RESIDENT ? PAIRS : 1;        // over the weights, and pairs of each
     int parity = 0;
     for (int unit = blockIdx.x; unit * wide < tiles; unit += (int)gridDim.x, parity ^= 1) {
         const int after = tile + (int)gridDim.x * wide;
@@ -275,11 +276,15 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
                 }
                 asm volatile("" : "+v"(o0), "+v"(o1), "+v"(ox));      // (opaque: operands kept over the loop would spill)
                 if constexpr (!RESIDENT) {
-                    __syncthreads();                  // (the pair before is read)
-                    x.store(lds, L, min(a.nr, 2), count, 0);
+                    __syncthreads();                  // (the rows before are read)
+                    x.store(lds, L, rows_held, count, 0);
+                    for (int item = kItems * (int)blockDim.x; item < rows_held * count; item += kItems * (int)blockDim.x) {
+                        x.load(a, 2 * kIn * p, rows_held, 16 * s0, count, item);
+                        x.store(lds, L, rows_held, count, item);
+                    }
                     __syncthreads();
-                    if (p + 1 < PAIRS) x.load(a, 2 * (p + 1), 2, 16 * s0, count, 0);
-                    else x.load(a, 0, 2, last ? 0 : 16 * (s0 + turn), count, 0);
+                    if (p + 1 < kPasses) x.load(a, 2 * kIn * (p + 1), rows_held, 16 * s0, count, 0);
+                    else x.load(a, 0, rows_held, last ? 0 : 16 * (s0 + turn), count, 0);
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (p + 1 == kPasses) {
@@ -303,6 +308,7 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
                             const auto e0 = __builtin_amdgcn_cvt_pk_f32_fp8(e, false), e1 = __builtin_amdgcn_cvt_pk_f32_fp8(e, true);
 #pragma unroll
                             for (int i = 0; i < kIn; ++i) {
+                                if (p * kIn + i >= PAIRS) continue;
                                 auto operand = [&](int at) __attribute__((always_inline)) {
                                     const u32x4 y = *(const u32x4*)(lds + o0 + at), z = *(const u32x4*)(lds + o1 + at);
                                     return i32x8{(int)y[0], (int)y[1], (int)y[2], (int)y[3], (int)z[0], (int)z[1], (int)z[2], (int)z[3]};
@@ -310,7 +316,7 @@ __global__ __launch_bounds__(64 * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups
                                 const i32x8 lo = operand(1024 * i + 128 * h), hi = operand(1024 * i + 256 + 128 * h);
                                 const f32x4 xs = *(const f32x4*)(lds + ox + 128 * i + 32 * h);
                                 const f32x4 d = nvfp4_dots(hi, q, nvfp4_dots(lo, q, f32x4{0.0f, 0.0f, 0.0f, 0.0f}, kOne), k16);
-                                float& y = acc[RESIDENT ? i : p];
+                                float& y = acc[p * kIn + i];
                                 y = __builtin_fmaf(d[0], e0[0] * xs[0], y);
                                 y = __builtin_fmaf(d[1], e0[1] * xs[1], y);
                                 y = __builtin_fmaf(d[2], e1[0] * xs[2], y);
@@ -372,7 +378,8 @@ template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_form(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
     const int wide = SWIGLU ? p.groups / 2 : p.groups, units = ((a.rows + 15) / 16 + wide - 1) / wide;
     int fit = kNvLds / p.bytes;                      // blocks of a compute unit
-    fit = fit < kNvWaves / (p.groups * p.waves) ? fit : kNvWaves / (p.groups * p.waves);
+    const int room = (RESIDENT ? kNvWaves : kNvWaves / 2) / (p.groups * p.waves);
+    fit = fit < room ? fit : room;
     fit = fit < 1 ? 1 : fit;
     const int grid = 256 * fit < units ? 256 * fit : units;
     Q27X_HIP((allow_lds<k_nvfp4<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
@@ -401,7 +408,8 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
     }
     const int most = kNvWaves / 2 / least, turns = (p.slots + most - 1) / most;
     p.waves = (p.slots + turns - 1) / turns;
-    p.bytes = Nvfp4Lds(a.nr < 2 ? a.nr : 2, p.waves * p.per, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
+    p.bytes = Nvfp4Lds(a.nr < 4 ? a.nr : 4, p.waves * p.per, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
+    if (p.bytes > kNvLds) { set_error("nvfp4: K=%d: %d bytes of LDS", a.K, p.bytes); return Q27X_E_SHAPE; }
     return launch_nvfp4_form<PAIRS, SWIGLU, false>(a, p, s);
 }
 template <bool SWIGLU>
@@ -426,6 +434,7 @@ static int nvfp4_args(const q27x_nvfp4_t* w, const char* who, const int8_t* xq, 
         set_error("%s: xstride=%d: at least K=%d, a multiple of 16", who, xstride, w->K);
         return Q27X_E_ARG;
     }
+    if ((long long)(nr - 1) * (nr > 1 ? xstride : 0) + w->K > 0x7fffffffLL) { set_error("%s: rows of activations over more than 2^31 - 1 bytes", who); return Q27X_E_RANGE; }
     return Q27X_OK;
 }
 

@@ -256,6 +256,28 @@ def test_swiglu(gpu, rows, K, nr):
     check_swiglu(q, s, gate, up, xq, xs, 0.6)
 
 
+@pytest.mark.parametrize("K", [17408, 20480, 57344, 57328])
+def test_activations_that_do_not_fit_together(gpu, K):
+    """Rows too long for LDS at once, up to the longest: brought in turns, alone and eight together, a ragged end."""
+    rng = np.random.default_rng(K)
+    gate, up = (Matrix(gpu, rng, 48, K, alpha=a / np.sqrt(K)) for a in (0.05, 0.03))
+    for nr in (1, 4, 7, 8):
+        xq, xs = rows_of(rng, nr, K)
+        check(project(gpu, gate, xq, xs), gate, xq, xs)
+        q, s = swiglu(gpu, gate, up, xq, xs, 0.6)
+        check_swiglu(q, s, gate, up, xq, xs, 0.6)
+
+
+@pytest.mark.parametrize("rows,K", [(16 * 1100, 336), (16 * 2300 + 5, 160)])
+def test_proj_more_tiles_than_blocks(gpu, rows, K):
+    """Blocks that go through several tiles, the last round not full; a step that K does not fill in each."""
+    rng = np.random.default_rng(rows)
+    m = Matrix(gpu, rng, rows, K)
+    for nr in (1, 4, 8):
+        xq, xs = rows_of(rng, nr, K)
+        check(project(gpu, m, xq, xs), m, xq, xs)
+
+
 def test_swiglu_large_gates_and_zero_groups(gpu):
     """Gates far outside what e^-g holds in fp32, and a group whose outputs are all zero."""
     X, rng = gpu, np.random.default_rng(8)

@@ -30,7 +30,7 @@ def swiglu(X, w, up=None, **kw):
 
 @pytest.mark.parametrize("kw,rc", [(dict(w=None), ARG), (dict(s=None), ARG), (dict(rows=0), SHAPE), (dict(rows=-5), SHAPE),
                                    (dict(rows=2 ** 31 - 1), SHAPE), (dict(K=0), SHAPE), (dict(K=8), SHAPE), (dict(K=250), SHAPE),
-                                   (dict(K=2 ** 31 - 16), SHAPE)])
+                                   (dict(K=57360), SHAPE), (dict(K=2 ** 31 - 16), SHAPE)])
 @pytest.mark.parametrize("call", [proj, swiglu])
 def test_matrices_refused(X, call, kw, rc):
     assert call(X, matrix(X, **kw), xstride=2 ** 31 - 16) == rc
@@ -42,6 +42,12 @@ def test_matrices_refused(X, call, kw, rc):
 @pytest.mark.parametrize("call", [proj, swiglu])
 def test_rows_refused(X, call, kw, rc):
     assert call(X, matrix(X), **kw) == rc
+
+
+@pytest.mark.parametrize("call", [proj, swiglu])
+def test_rows_past_2_31_bytes_refused(X, call):
+    assert call(X, matrix(X), xstride=1 << 30, nr=3) == -6
+    assert call(X, matrix(X), xstride=(1 << 31) - 16, nr=2) == -6
 
 
 @pytest.mark.parametrize("call", [proj, swiglu])
