@@ -139,38 +139,43 @@ __device__ __forceinline__ u64 scan_wave(u64 x) {
     return x;
 }
 
-// A slice of T PER tokens (MANY: some times that). Bins are kept four times, by lane, as a wave's 64 tokens
-// lie in some 70 bins at most: adding to one place waits for one another. Counting gives a token its place in its bin at once.
+struct BinShared {
+    u64 w[kBins * kCopies];
+    uint32_t n[kBins * kCopies], part[(kBins + 63) / 64];
+};
+// A slice of T PER tokens (MANY: some times that) from `begin` on by bin: list, where each bin begins in it (off, and its end behind the
+// last), the bins' weights; how many there are. x: the slice's first logits, 4 (j T + t) .. + 3 of this thread.
+// Bins are kept four times, by lane, as a wave's 64 tokens lie in some 70 bins at most: adding to one place waits for one another.
+// Counting gives a token its place in its bin at once. From z = 16 on a slice's weights of a bin are below 2^43: the count has room
+// above them, one addition for both.
 template <int T, int PER, bool MANY>
-__global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
-    extern __shared__ __attribute__((aligned(16))) uint16_t s_list[];
-    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice, copy = t & (kCopies - 1);
-    __shared__ u64 s_w[kBins * kCopies];
-    __shared__ uint32_t s_n[kBins * kCopies], s_part[(kBins + 63) / 64];
-    float v[PER / 4][4];
-    auto load = [&](int i0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), v[j]);
-    };
-    load(0);                                      // (requested before the maximum that they wait for)
-    for (int b = t; b < kBins * kCopies; b += T) { s_w[b] = 0; s_n[b] = 0; }
-    const float top = row_max(a, row);
-    bool greedy;
-    const double c = inv_temp(a, row, greedy), l0 = (double)top;
+__device__ __forceinline__ uint32_t bins_of(const SampleArgs& a, BinShared& sh, uint16_t* list, int row, int begin, float (&x)[PER / 4][4], double l0,
+                                            double c, uint16_t* off, u64* bw) {
+    constexpr int kTail = 256 * kCopies;          // places of z >= 16
+    const int t = threadIdx.x, copy = t & (kCopies - 1);
     uint32_t place[PER];                          // of a token: its bin's copy, and how many came before it there; ~0: left out
-    __syncthreads();
     auto take = [&](bool add) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) {
-            const float l = v[j / 4][j % 4];
+            const float l = x[j / 4][j % 4];
             const double z = order_of(l, l0, c);
             place[j] = ~0u;
             if (is_finite(l) && z < 48.0) {
                 const int b = bin_of(z) * kCopies + copy;
-                if (add) atomicAdd(&s_w[b], weight(z));
-                place[j] = (uint32_t)b << 16 | atomicAdd(&s_n[b], 1u);
+                uint32_t before;
+                if (add && b >= kTail) {
+                    before = (uint32_t)(atomicAdd(&sh.w[b], weight(z) | 1ull << 48) >> 48);
+                } else {
+                    if (add) atomicAdd(&sh.w[b], weight(z));
+                    before = atomicAdd(&sh.n[b], 1u);
+                }
+                place[j] = (uint32_t)b << 16 | before;
             }
         }
+    };
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + i0 + 4 * (j * T + t), x[j]);
     };
     take(true);
     if constexpr (MANY)
@@ -180,53 +185,78 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
         }
     __syncthreads();
     // where each bin begins
-    const size_t at = (size_t)row * a.ns + s;
-    uint32_t n[kCopies], run = 0;
-    if (t < kBins) {
+    constexpr int kEach = (kBins + T - 1) / T;    // bins of a thread
+    uint32_t n[kEach][kCopies], run = 0;
+    if (t * kEach < kBins) {
 #pragma unroll
-        for (int k = 0; k < kCopies; ++k) {
-            n[k] = s_n[t * kCopies + k];
-            run += n[k];
-        }
-        const uint32_t mine = run;
-        run = scan_wave(run);
-        if ((t & 63) == 63 || t == kBins - 1) s_part[t >> 6] = run;
-        run -= mine;
+        for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) {
+                const int at = (t * kEach + e) * kCopies + k;
+                n[e][k] = at >= kTail ? (uint32_t)(sh.w[at] >> 48) : sh.n[at];
+                run += n[e][k];
+            }
     }
+    const uint32_t mine = run;
+    run = scan_wave(run);
+    if ((t & 63) == 63 && t * kEach < kBins + 64 * kEach) sh.part[t >> 6] = run;
+    run -= mine;
     __syncthreads();
+    constexpr int kWaves = (kBins + 64 * kEach - 1) / (64 * kEach);
     uint32_t total = 0;
 #pragma unroll
-    for (int k = 0; k < (kBins + 63) / 64; ++k) {
-        run += k < t >> 6 ? s_part[k] : 0;
-        total += s_part[k];
+    for (int k = 0; k < kWaves; ++k) {
+        run += k < t >> 6 ? sh.part[k] : 0;
+        total += sh.part[k];
     }
-    if (t < kBins) {
-        a.off[at * kOffs + t] = (uint16_t)run;
-        u64 w = 0;
+    if (t * kEach < kBins) {
 #pragma unroll
-        for (int k = 0; k < kCopies; ++k) {
-            w += s_w[t * kCopies + k];
-            s_n[t * kCopies + k] = run;
-            run += n[k];
+        for (int e = 0; e < kEach; ++e) {
+            const int bin = t * kEach + e;
+            off[bin] = (uint16_t)run;
+            u64 w = 0;
+#pragma unroll
+            for (int k = 0; k < kCopies; ++k) {
+                const u64 wk = sh.w[bin * kCopies + k];
+                w += bin * kCopies >= kTail ? wk & ((1ull << 48) - 1) : wk;
+                sh.n[bin * kCopies + k] = run;
+                run += n[e][k];
+            }
+            bw[bin] = w;
+            if (bin == kBins - 1) off[kBins] = (uint16_t)run;
         }
-        a.bw[at * kBins + t] = w;
-        if (t == kBins - 1) a.off[at * kOffs + kBins] = (uint16_t)run;
     }
     __syncthreads();
     if constexpr (!MANY) {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (place[j] != ~0u) s_list[s_n[place[j] >> 16] + (place[j] & 0xFFFFu)] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
+            if (place[j] != ~0u) list[sh.n[place[j] >> 16] + (place[j] & 0xFFFFu)] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
     } else {
         for (int i0 = 0; i0 < a.slice; i0 += PER * T) {
             load(i0);
             take(false);                          // (the bins' beginnings count on)
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                if (place[j] != ~0u) s_list[place[j] & 0xFFFFu] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
+                if (place[j] != ~0u) list[place[j] & 0xFFFFu] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
         }
     }
     __syncthreads();
+    return total;
+}
+template <int T, int PER, bool MANY>
+__global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint16_t s_list[];
+    __shared__ BinShared sh;
+    const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice;
+    float x[PER / 4][4];
+#pragma unroll
+    for (int j = 0; j < PER / 4; ++j) logits4(a, row, begin + 4 * (j * T + t), x[j]);       // (requested before the maximum that they wait for)
+    for (int b = t; b < kBins * kCopies; b += T) { sh.w[b] = 0; sh.n[b] = 0; }
+    bool greedy;
+    const double l0 = (double)row_max(a, row), c = inv_temp(a, row, greedy);
+    __syncthreads();
+    const size_t at = (size_t)row * a.ns + s;
+    const uint32_t total = bins_of<T, PER, MANY>(a, sh, s_list, row, begin, x, l0, c, a.off + at * kOffs, a.bw + at * kBins);
     for (uint32_t i = 8 * t; i < total; i += 8 * T) *(uint4*)(a.list + at * a.slice + i) = *(const uint4*)&s_list[i];
 }
 
@@ -236,11 +266,12 @@ __device__ __forceinline__ u64 shfl_xor64(u64 x, int o) {
     return (u64)hi << 32 | lo;
 }
 
+template <int SLICES>
 struct DrawShared {
     u64 bw[kBins + 1];                            // running weights and counts of the row's bins
     uint32_t bn[kBins + 1];
-    __attribute__((aligned(16))) uint16_t off[kMostSlices][kOffs];    // the slices' lists by bin
-    Sum part[kBins / 64];
+    __attribute__((aligned(16))) uint16_t off[SLICES][kOffs];         // the slices' lists by bin
+    Sum part[kBins / 128];
     u64 hw[256];                                  // a narrowing step's digits
     uint32_t hn[256];
     ulonglong2 qw[kHeld + 4 * kBatch];            // candidates: rank, weight
@@ -249,36 +280,40 @@ struct DrawShared {
     int bk, bp;
 };
 
-// The tokens of bins b0 .. b1 of the row, f(rank, weight) for each, the block's threads side by side.
-template <typename F>
-__device__ __forceinline__ void each_listed(const SampleArgs& a, const DrawShared& sh, int row, int b0, int b1, double l0, double c, F f) {
-    const int wv = threadIdx.x >> 6, l = threadIdx.x & 63;
-    for (int s = wv; s < a.ns; s += kDrawThreads / 64) {
-        const size_t at = (size_t)row * a.ns + s;
-        const int end = sh.off[s][b1 + 1];
-        for (int i = sh.off[s][b0] + l; i < end; i += 64) {
-            const int id = s * a.slice + a.list[at * a.slice + i];
-            const float x = logit_at(a, row, id);
-            f(rank_of(x, id), weight(order_of(x, l0, c)));
+// The row's tokens by bin: in the slices' lists, or (ONE) a single list and its logits in LDS.
+template <bool ONE>
+struct Lists {
+    const SampleArgs& a;
+    int row;
+    const uint16_t* list;
+    const float* x;
+    double l0, c;
+    // f(rank, weight) for each of bins b0 .. b1, the block's threads side by side
+    template <typename SH, typename F>
+    __device__ __forceinline__ void each(const SH& sh, int b0, int b1, F f) const {
+        if constexpr (ONE) {
+            for (int i = sh.off[0][b0] + (int)threadIdx.x; i < sh.off[0][b1 + 1]; i += kDrawThreads) {
+                const int id = list[i];
+                f(rank_of(x[id], id), weight(order_of(x[id], l0, c)));
+            }
+        } else {
+            for (int s = threadIdx.x >> 6; s < a.ns; s += kDrawThreads / 64) {
+                const size_t at = ((size_t)row * a.ns + s) * a.slice;
+                const int end = sh.off[s][b1 + 1];
+                for (int i = sh.off[s][b0] + (int)(threadIdx.x & 63); i < end; i += 64) {
+                    const int id = s * a.slice + a.list[at + i];
+                    const float l = logit_at(a, row, id);
+                    f(rank_of(l, id), weight(order_of(l, l0, c)));
+                }
+            }
         }
     }
-}
-// The same tokens into LDS; how many.
-__device__ __forceinline__ uint32_t hold(const SampleArgs& a, DrawShared& sh, int row, int b0, int b1, double l0, double c) {
-    __syncthreads();
-    if (threadIdx.x == 0) sh.held = 0;
-    __syncthreads();
-    each_listed(a, sh, row, b0, b1, l0, c, [&](u64 q, u64 w) {
-        const uint32_t k = atomicAdd(&sh.held, 1u);
-        sh.qw[k] = make_ulonglong2(q, w);
-    });
-    __syncthreads();
-    return sh.held;
-}
+};
 // Four, two or one threads a token: the held token that this thread is one of, and what comes before it among the n held ones
 // (a call's threads past the last one's batches have put ranks behind all others there).
 struct Counted { bool is; u64 q, w; Sum before; };
-__device__ __forceinline__ Counted count_held(const DrawShared& sh, uint32_t n) {
+template <typename SH>
+__device__ __forceinline__ Counted count_held(const SH& sh, uint32_t n) {
     const uint32_t t = threadIdx.x, parts = n <= 64 ? 4 : n <= 128 ? 2 : 1, i = t / parts;
     Counted x;
     x.is = i < n && t % parts == 0;
@@ -308,19 +343,25 @@ __device__ __forceinline__ Counted count_held(const DrawShared& sh, uint32_t n) 
     return x;
 }
 
-// The token of bin b at which the running count (BY_COUNT) or weight, from the bin's beginning on, reaches `target` (at least 1, at
+// The token of bin b at which the running count (by_count) or weight, from the bin's beginning on, reaches `target` (at least 1, at
 // most the bin's): its rank, its weight and the running weight up to it, in sh.
-template <bool BY_COUNT>
-__device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 target, double l0, double c) {
+template <typename SH, typename LISTS>
+__device__ __forceinline__ void search(SH& sh, const LISTS& lists, bool by_count, int b, u64 target) {
     const int t = threadIdx.x;
     uint32_t n = sh.bn[b + 1] - sh.bn[b];
     u64 before = 0;                               // weight before what is left
-    if (n <= kHeld) hold(a, sh, row, b, b, l0, c);
     bool held = n <= kHeld;
+    __syncthreads();
+    if (held) {
+        if (t == 0) sh.held = 0;
+        __syncthreads();
+        lists.each(sh, b, b, [&](u64 q, u64 w) { sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w); });
+        __syncthreads();
+    }
     u64 lo = 0, hi = ~0ull;
     auto each = [&](auto f) {
         if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.qw[i].x, sh.qw[i].y);
-        else each_listed(a, sh, row, b, b, l0, c, f);
+        else lists.each(sh, b, b, f);
     };
     while (n > kLeft) {
         // the range of what is left, in 256 parts
@@ -361,7 +402,7 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
             for (int k = 0; k < 4; ++k) {
                 const uint32_t pn = sh.hn[4 * t + k];
                 const u64 pw = sh.hw[4 * t + k];
-                if (BY_COUNT ? run.n < target && target <= run.n + pn : run.w < target && target <= run.w + pw) {
+                if (by_count ? run.n < target && target <= run.n + pn : run.w < target && target <= run.w + pw) {
                     sh.digit = 4 * t + k;
                     sh.digit_n = run.n;
                     sh.digit_w = run.w;
@@ -376,7 +417,7 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
         lo += (u64)sh.digit << shift;
         hi = min(hi, lo + ((1ull << shift) - 1));
         before += sh.digit_w;
-        target -= BY_COUNT ? sh.digit_n : sh.digit_w;
+        target -= by_count ? sh.digit_n : sh.digit_w;
         const uint32_t left = sh.left;
         if (held || left <= kHeld) {              // these alone, at the front
             if (held) {
@@ -392,7 +433,7 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
                 for (int k = 0; k < kHeld / kDrawThreads; ++k)
                     if (x[k].x != ~0ull) sh.qw[atomicAdd(&sh.held, 1u)] = x[k];
             } else {
-                each_listed(a, sh, row, b, b, l0, c, [&](u64 q, u64 w) {
+                lists.each(sh, b, b, [&](u64 q, u64 w) {
                     if (q >= lo && q <= hi) sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w);
                 });
                 held = true;
@@ -404,7 +445,7 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
     if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
     __syncthreads();
     const Counted x = count_held(sh, n);
-    if (x.is && (BY_COUNT ? x.before.n + 1 == target : x.before.w < target && target <= x.before.w + x.w)) {
+    if (x.is && (by_count ? x.before.n + 1 == target : x.before.w < target && target <= x.before.w + x.w)) {
         sh.found_q = x.q;
         sh.found_w = x.w;
         sh.found_end = before + x.before.w + x.w;
@@ -412,14 +453,13 @@ __device__ void search(const SampleArgs& a, DrawShared& sh, int row, int b, u64 
     __syncthreads();
 }
 
-// The bin in which the running count or weight of the row reaches `target`.
-template <bool BY_COUNT>
-__device__ int bin_that_reaches(const DrawShared& sh, u64 target) {
+// The bin in which the running weight of the row reaches `target`.
+template <typename SH>
+__device__ __forceinline__ int bin_that_reaches(const SH& sh, u64 target) {
     int lo = 0, hi = kBins - 1;
     while (lo < hi) {
         const int mid = (lo + hi) / 2;
-        const u64 upto = BY_COUNT ? (u64)sh.bn[mid + 1] : sh.bw[mid + 1];
-        if (upto >= target) hi = mid; else lo = mid + 1;
+        if (sh.bw[mid + 1] >= target) hi = mid; else lo = mid + 1;
     }
     return lo;
 }
@@ -432,9 +472,130 @@ __device__ __forceinline__ u64 share_of(float share, u64 kept) {
     return min(max(x, (u64)1), kept);
 }
 
+// A row's settings.
+struct Cuts {
+    int k;
+    float p, m, u;
+    double c;
+    u64 least;                                    // the weight that min_p asks for
+    int bm0, bm1;                                 // bins around those that tokens of this weight are in (the logarithm is rounded)
+    __device__ __forceinline__ Cuts(const SampleArgs& a, int row) {
+        bool greedy;
+        c = inv_temp(a, row, greedy);
+        k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
+        p = a.top_p ? a.top_p[row] : 1.0f;
+        m = a.min_p ? a.min_p[row] : 0.0f;
+        u = a.u[row];
+        least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
+        const double z = m < 1.0f ? -(double)__builtin_amdgcn_logf(m) : 0.0;
+        const int bm = z < 48.0 ? bin_of(z) : kBins - 1;
+        bm0 = bm > 0 ? bm - 1 : 0;
+        bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
+    }
+};
+
+// The row's token, from its bins: this thread's are 2 t and 2 t + 1, of n0, n1 tokens and weights w0, w1. push(upto): the tokens of
+// bins 0 .. upto into sh.qw.
+template <typename SH, typename LISTS, typename PUSH>
+__device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, const LISTS& lists, const Cuts& cuts, uint32_t n0, uint32_t n1, u64 w0, u64 w1, PUSH push) {
+    const int t = threadIdx.x;
+    Sum run = {0, 0};
+    if (t < kBins / 2) {
+        run = {scan_wave(n0 + n1), scan_wave(w0 + w1)};
+        if ((t & 63) == 63) sh.part[t >> 6] = run;
+    }
+    if (t == 0) { sh.held = 0; sh.heavy = 0; sh.bk = sh.bp = kBins - 1; }
+    __syncthreads();
+    const Sum all = {sh.part[0].n + sh.part[1].n + sh.part[2].n, sh.part[0].w + sh.part[1].w + sh.part[2].w};
+    static_assert(kBins / 128 == 3, "three waves of bins");
+    u64 kept = all.w;                             // the weight of what is kept
+    const int k = cuts.k;
+    const bool by_k = k >= 1 && (uint32_t)k < all.n, by_p = cuts.p < 1.0f, by_m = cuts.m > 0.0f;
+    if (t < kBins / 2) {
+        if (t >= 64) { run.n += sh.part[0].n; run.w += sh.part[0].w; }
+        if (t >= 128) { run.n += sh.part[1].n; run.w += sh.part[1].w; }
+        const uint32_t na = run.n - n0 - n1, nb = run.n - n1;
+        const u64 wa = run.w - w0 - w1, wb = run.w - w1;
+        sh.bn[2 * t] = na;
+        sh.bn[2 * t + 1] = nb;
+        sh.bw[2 * t] = wa;
+        sh.bw[2 * t + 1] = wb;
+        if (t == kBins / 2 - 1) { sh.bn[kBins] = run.n; sh.bw[kBins] = run.w; }
+        // the bins in which the cuts end (by weight, of all)
+        if (by_k && na < (uint32_t)k && (uint32_t)k <= run.n) sh.bk = 2 * t + ((uint32_t)k > nb);
+        const u64 target = share_of<false>(cuts.p, kept);
+        if (by_p && wa < target && target <= run.w) sh.bp = 2 * t + (target > wb);
+    }
+    __syncthreads();
+    const int bk = sh.bk, upto = by_k ? bk : by_p ? sh.bp : by_m ? cuts.bm1 : kBins - 1;
+    const uint32_t n = sh.bn[upto + 1];
+    if (n <= kFew) {
+        push(upto);                               // (all that can be drawn)
+        if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
+        __syncthreads();
+        const Counted x = count_held(sh, n);
+        const u64 end = x.before.w + x.w;
+        if (by_k && x.is && x.before.n + 1 == (uint32_t)k) sh.end_k = end;
+        const uint32_t heavy = (uint32_t)__popcll(__ballot(x.is && x.w >= cuts.least));
+        if ((t & 63) == 0 && heavy) atomicAdd(&sh.heavy, heavy);
+        __syncthreads();
+        if (by_k) kept = sh.end_k;
+        const u64 want = share_of<false>(cuts.p, kept);
+        if (by_p && x.is && x.before.w < want && want <= end) sh.end_p = end;
+        if (by_m && x.is && x.before.n + 1 == sh.heavy) sh.end_m = end;
+        __syncthreads();
+        u64 cut = kept;
+        if (by_p) cut = min(cut, sh.end_p);
+        if (by_m) cut = min(cut, sh.end_m);
+        const u64 target = share_of<true>(cuts.u, cut);
+        if (x.is && x.before.w < target && target <= end) {
+            a.idx[row] = (int32_t)(uint32_t)x.q;
+            if (a.prob) a.prob[row] = (float)((double)x.w / (double)cut);
+        }
+        return;
+    }
+    u64 cut = 0;
+#pragma unroll 1
+    for (int stage = 0; stage < 3; ++stage) {     // top-k, top-p, the draw (behind min-p): searches in one bin each
+        u64 target;
+        int b = bk;
+        if (stage == 0) {
+            if (!by_k) continue;
+            if (sh.bn[bk + 1] == (uint32_t)k) { kept = sh.bw[bk + 1]; continue; }
+            target = (u64)k - sh.bn[bk];
+        } else {
+            if (stage == 1) {
+                cut = kept;
+                if (!by_p) continue;
+            } else if (by_m) {
+                u64 sum = 0;
+                lists.each(sh, cuts.bm0, cuts.bm1, [&](u64, u64 w) { sum += w >= cuts.least ? w : 0; });
+                __syncthreads();
+                if (t == 0) sh.found_w = 0;
+                __syncthreads();
+                if (sum) atomicAdd(&sh.found_w, sum);
+                __syncthreads();
+                cut = min(cut, sh.bw[cuts.bm0] + sh.found_w);
+                __syncthreads();
+            }
+            target = stage == 1 ? share_of<false>(cuts.p, kept) : share_of<true>(cuts.u, cut);
+            b = bin_that_reaches(sh, target);
+            target -= sh.bw[b];
+        }
+        search(sh, lists, stage == 0, b, target);
+        const u64 end = sh.bw[b] + sh.found_end;
+        if (stage == 0) kept = end;
+        else if (stage == 1) cut = min(cut, end);
+    }
+    if (t == 0) {
+        a.idx[row] = (int32_t)(uint32_t)sh.found_q;
+        if (a.prob) a.prob[row] = (float)((double)sh.found_w / (double)cut);
+    }
+}
+
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const int row = blockIdx.x, t = threadIdx.x;
-    __shared__ DrawShared sh;
+    __shared__ DrawShared<kMostSlices> sh;
     const size_t first = (size_t)row * a.ns;
     // Requested at once, as each is a trip to memory: the first tokens of each slice's list, its offsets, bins 2 t and 2 t + 1
     // of each; then these tokens' logits. (Any entry of a list is read as a token of its slice: those behind its end are not used.)
@@ -454,14 +615,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
         bw[s] = *(const ulonglong2*)(a.bw + (first + min(s, a.ns - 1)) * kBins + 2 * min(t, kBins / 2 - 1));
     __builtin_amdgcn_sched_barrier(0);
     const float top = row_max(a, row);
-    bool greedy;
-    const double c = inv_temp(a, row, greedy), l0 = (double)top;
-    const int k = greedy ? 1 : a.top_k ? a.top_k[row] : 0;
-    const float p = a.top_p ? a.top_p[row] : 1.0f, m = a.min_p ? a.min_p[row] : 0.0f, u = a.u[row];
-    const u64 least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
-    // bins that tokens of weight `least` are in (the logarithm is rounded)
-    const double zm = m < 1.0f ? -(double)__builtin_amdgcn_logf(m) : 0.0;
-    const int bm = zm < 48.0 ? bin_of(zm) : kBins - 1, bm0 = bm > 0 ? bm - 1 : 0, bm1 = bm + 1 < kBins ? bm + 1 : kBins - 1;
+    const Cuts cuts(a, row);
     float ahead[kAheadOf];
 #pragma unroll
     for (int j = 0; j < kAheadOf; ++j) ahead[j] = logit_at(a, row, min(id[j], a.n - 1));
@@ -479,46 +633,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
         if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
     }
-    if (t == 0) { sh.held = 0; sh.heavy = 0; sh.bk = sh.bp = kBins - 1; }
     __syncthreads();
     uint32_t n0 = 0, n1 = 0;
-    Sum run = {0, 0};
-    if (t < kBins / 2) {
+    if (t < kBins / 2)
         for (int s = 0; s < a.ns; ++s) {
             const uint32_t o0 = sh.off[s][2 * t], o1 = sh.off[s][2 * t + 1], o2 = sh.off[s][2 * t + 2];
             n0 += o1 - o0;
             n1 += o2 - o1;
         }
-        run = {scan_wave(n0 + n1), scan_wave(w0 + w1)};
-        if ((t & 63) == 63) sh.part[t >> 6] = run;
-    }
-    __syncthreads();
-    const Sum all = {sh.part[0].n + sh.part[1].n + sh.part[2].n, sh.part[0].w + sh.part[1].w + sh.part[2].w};
-    static_assert(kBins / 128 == 3, "three waves of bins");
-    u64 kept = all.w;                             // the weight of what is kept
-    const bool by_k = k >= 1 && (uint32_t)k < all.n, by_p = p < 1.0f, by_m = m > 0.0f;
-    if (t < kBins / 2) {
-        if (t >= 64) { run.n += sh.part[0].n; run.w += sh.part[0].w; }
-        if (t >= 128) { run.n += sh.part[1].n; run.w += sh.part[1].w; }
-        const uint32_t na = run.n - n0 - n1, nb = run.n - n1;
-        const u64 wa = run.w - w0 - w1, wb = run.w - w1;
-        sh.bn[2 * t] = na;
-        sh.bn[2 * t + 1] = nb;
-        sh.bw[2 * t] = wa;
-        sh.bw[2 * t + 1] = wb;
-        if (t == kBins / 2 - 1) { sh.bn[kBins] = run.n; sh.bw[kBins] = run.w; }
-        // the bins in which the cuts end (by weight, of all)
-        if (by_k && na < (uint32_t)k && (uint32_t)k <= run.n) sh.bk = 2 * t + ((uint32_t)k > nb);
-        const u64 target = share_of<false>(p, kept);
-        if (by_p && wa < target && target <= run.w) sh.bp = 2 * t + (target > wb);
-    }
-    __syncthreads();
-    const int bk = sh.bk;
-    const int upto = by_k ? bk : by_p ? sh.bp : by_m ? bm1 : kBins - 1;
-    if (sh.bn[upto + 1] <= kFew) {
-        // the tokens that can be drawn, into LDS: what was read ahead, and the rest of a longer list
+    const Lists<false> lists = {a, row, nullptr, nullptr, (double)top, cuts.c};
+    draw_row(a, sh, row, lists, cuts, n0, n1, w0, w1, [&](int upto) {
+        // what was read ahead, and the rest of a longer list
         for (int s = t >> 6, j = 0; s < a.ns; s += 4, ++j) {
-            const size_t at = (size_t)row * a.ns + s;
+            const size_t at = (first + s) * a.slice;
             const int end = sh.off[s][upto + 1];
             for (int i = t & 63; i < end; i += 64) {
                 int of = 0;
@@ -530,69 +657,62 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
                         x = y == j ? ahead[y] : x;
                     }
                 } else {
-                    of = s * a.slice + a.list[at * a.slice + i];
+                    of = s * a.slice + a.list[at + i];
                     x = logit_at(a, row, of);
                 }
-                sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(rank_of(x, of), weight(order_of(x, l0, c)));
+                sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(rank_of(x, of), weight(order_of(x, lists.l0, lists.c)));
             }
         }
-        const uint32_t n = sh.bn[upto + 1];
-        if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
-        __syncthreads();
-        const Counted x = count_held(sh, n);
-        const u64 end = x.before.w + x.w;
-        if (by_k && x.is && x.before.n + 1 == (uint32_t)k) sh.end_k = end;
-        const uint32_t heavy = (uint32_t)__popcll(__ballot(x.is && x.w >= least));
-        if ((t & 63) == 0 && heavy) atomicAdd(&sh.heavy, heavy);
-        __syncthreads();
-        if (by_k) kept = sh.end_k;
-        const u64 want = share_of<false>(p, kept);
-        if (by_p && x.is && x.before.w < want && want <= end) sh.end_p = end;
-        if (by_m && x.is && x.before.n + 1 == sh.heavy) sh.end_m = end;
-        __syncthreads();
-        u64 cut = kept;
-        if (by_p) cut = min(cut, sh.end_p);
-        if (by_m) cut = min(cut, sh.end_m);
-        const u64 target = share_of<true>(u, cut);
-        if (x.is && x.before.w < target && target <= end) {
-            a.idx[row] = (int32_t)(uint32_t)x.q;
-            if (a.prob) a.prob[row] = (float)((double)x.w / (double)cut);
-        }
+    });
+}
+
+// Rows of one slice: all three steps by a block, the bins and the list in LDS.
+struct OneShared {
+    DrawShared<1> draw;
+    BinShared bins;
+    u64 bw[kBins];
+    float x[kLeastSlice];
+    uint16_t list[kLeastSlice];
+    float m[4];
+};
+__global__ __launch_bounds__(kDrawThreads) void k_sample_one(SampleArgs a) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    OneShared& sh = *(OneShared*)lds;
+    constexpr int kPer = kLeastSlice / kDrawThreads;
+    const int row = blockIdx.x, t = threadIdx.x;
+    float x[kPer / 4][4], top = -__builtin_huge_valf();
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j) logits4(a, row, 4 * (j * kDrawThreads + t), x[j]);
+    const Cuts cuts(a, row);
+    for (int b = t; b < kBins * kCopies; b += kDrawThreads) { sh.bins.w[b] = 0; sh.bins.n[b] = 0; }
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) top = is_finite(x[j][k]) ? fmaxf(top, x[j][k]) : top;
+        *(float4*)&sh.x[4 * (j * kDrawThreads + t)] = make_float4(x[j][0], x[j][1], x[j][2], x[j][3]);
+    }
+    top = max_xor(top, 64);
+    if ((t & 63) == 0) sh.m[t >> 6] = top;
+    __syncthreads();
+    top = fmaxf(fmaxf(sh.m[0], sh.m[1]), fmaxf(sh.m[2], sh.m[3]));
+    if (!is_finite(top)) {                        // (no finite logit)
+        if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
     }
-    if (by_k) {
-        if (sh.bn[bk + 1] == (uint32_t)k) {
-            kept = sh.bw[bk + 1];
-        } else {
-            search<true>(a, sh, row, bk, (u64)k - sh.bn[bk], l0, c);
-            kept = sh.bw[bk] + sh.found_end;
-        }
+    bins_of<kDrawThreads, kPer, false>(a, sh.bins, sh.list, row, 0, x, (double)top, cuts.c, sh.draw.off[0], sh.bw);
+    uint32_t n0 = 0, n1 = 0;
+    u64 w0 = 0, w1 = 0;
+    if (t < kBins / 2) {
+        const uint32_t o0 = sh.draw.off[0][2 * t], o1 = sh.draw.off[0][2 * t + 1], o2 = sh.draw.off[0][2 * t + 2];
+        n0 = o1 - o0;
+        n1 = o2 - o1;
+        w0 = sh.bw[2 * t];
+        w1 = sh.bw[2 * t + 1];
     }
-    u64 cut = kept;
-    if (by_p) {
-        const u64 target = share_of<false>(p, kept);
-        const int b = bin_that_reaches<false>(sh, target);
-        search<false>(a, sh, row, b, target - sh.bw[b], l0, c);
-        cut = min(cut, sh.bw[b] + sh.found_end);
-    }
-    if (by_m) {
-        u64 sum = 0;
-        each_listed(a, sh, row, bm0, bm1, l0, c, [&](u64, u64 w) { sum += w >= least ? w : 0; });
-        __syncthreads();
-        if (t == 0) sh.found_w = 0;
-        __syncthreads();
-        if (sum) atomicAdd(&sh.found_w, sum);
-        __syncthreads();
-        cut = min(cut, sh.bw[bm0] + sh.found_w);
-        __syncthreads();
-    }
-    const u64 target = share_of<true>(u, cut);
-    const int b = bin_that_reaches<false>(sh, target);
-    search<false>(a, sh, row, b, target - sh.bw[b], l0, c);
-    if (t == 0) {
-        a.idx[row] = (int32_t)(uint32_t)sh.found_q;
-        if (a.prob) a.prob[row] = (float)((double)sh.found_w / (double)cut);
-    }
+    const Lists<true> lists = {a, row, sh.list, sh.x, (double)top, cuts.c};
+    draw_row(a, sh.draw, row, lists, cuts, n0, n1, w0, w1, [&](int upto) {
+        lists.each(sh.draw, 0, upto, [&](u64 q, u64 w) { sh.draw.qw[atomicAdd(&sh.draw.held, 1u)] = make_ulonglong2(q, w); });
+    });
 }
 
 struct SampleLayout { size_t bw, smax, off, list, total; int slice, ns, parts; };
@@ -633,10 +753,16 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
     a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off); a.smax = (float*)(p + wl.smax);
     a.idx = idx; a.prob = prob;
+    if (a.ns == 1) {
+        Q27X_HIP(allow_lds<k_sample_one>((int)sizeof(OneShared)));
+        hipLaunchKernelGGL(k_sample_one, dim3((unsigned)nr), dim3(kDrawThreads), sizeof(OneShared), (hipStream_t)s, a);
+        Q27X_HIP(hipGetLastError());
+        return Q27X_OK;
+    }
     const dim3 grid((unsigned)a.ns, (unsigned)nr);
     hipLaunchKernelGGL(k_sample_max, dim3((unsigned)a.parts, (unsigned)nr), dim3(256), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
-    if (a.slice == 4096) {
+    if (a.slice == kLeastSlice) {
         hipLaunchKernelGGL((k_sample_bins<512, 8, false>), grid, dim3(512), 2 * a.slice, (hipStream_t)s, a);
     } else if (a.slice == 8192) {
         hipLaunchKernelGGL((k_sample_bins<1024, 8, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
