@@ -297,14 +297,26 @@ struct Lists {
                 f(rank_of(x[id], id), weight(order_of(x[id], l0, c)));
             }
         } else {
-            for (int s = threadIdx.x >> 6; s < a.ns; s += kDrawThreads / 64) {
-                const size_t at = ((size_t)row * a.ns + s) * a.slice;
-                const int end = sh.off[s][b1 + 1];
-                for (int i = sh.off[s][b0] + (int)(threadIdx.x & 63); i < end; i += 64) {
-                    const int id = s * a.slice + a.list[at + i];
-                    const float l = logit_at(a, row, id);
-                    f(rank_of(l, id), weight(order_of(l, l0, c)));
+            // a wave's slices, 64 tokens of each requested at once (those behind a list's end are read as some token, and left out)
+            constexpr int kOf = kMostSlices * 64 / kDrawThreads;
+            const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+            for (int i0 = 0;; i0 += 64) {
+                int id[kOf];
+                float l[kOf];
+                bool is[kOf], any = false;
+#pragma unroll
+                for (int j = 0; j < kOf; ++j) {
+                    const int s = min(wave + j * (kDrawThreads / 64), a.ns - 1), i = sh.off[s][b0] + i0 + lane;
+                    is[j] = wave + j * (kDrawThreads / 64) < a.ns && i < sh.off[s][b1 + 1];
+                    any |= is[j];
+                    id[j] = s * a.slice + a.list[((size_t)row * a.ns + s) * a.slice + min(i, a.slice - 1)];
                 }
+                if (!__ballot(any)) break;
+#pragma unroll
+                for (int j = 0; j < kOf; ++j) l[j] = logit_at(a, row, min(id[j], a.n - 1));
+#pragma unroll
+                for (int j = 0; j < kOf; ++j)
+                    if (is[j]) f(rank_of(l[j], id[j]), weight(order_of(l[j], l0, c)));
             }
         }
     }
@@ -671,7 +683,7 @@ struct OneShared {
     DrawShared<1> draw;
     BinShared bins;
     u64 bw[kBins];
-    float x[kLeastSlice];
+    __attribute__((aligned(16))) float x[kLeastSlice];
     uint16_t list[kLeastSlice];
     float m[4];
 };
