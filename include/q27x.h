@@ -127,8 +127,8 @@ typedef struct q27x_nvfp4 {
 /* q27x_proj_rows on NVFP4 weights as they are, nothing requantized (the reference's q27_proj_nvfp4_down_nr and lm_head forms,
  * include/q27_nr.h:14-19; src/q27_nvfp4.hip:4337-4544):
  *   y[n][r] = alpha * sum over 16-slabs s of (dot of the slab's codes, exact) * (ws[r][s] * xs[n][s])  (+ rs * res[n][r])
- * in fp32. Arguments as q27x_proj_rows; any rows, K % 16 == 0 up to 57344; with nr > 1 xstride % 16 == 0. Row n's bits
- * do not depend on the other rows or on nr. */
+ * in fp32. Arguments as q27x_proj_rows; up to 2^31 - 1 - 2^19 rows, K % 16 == 0 up to 57344; with nr > 1 xstride % 16 == 0. y may be res (of one
+ * type and stride) and else overlaps nothing that is read. Row n's bits do not depend on the other rows or on nr. */
 int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int xstride, const float* xs,
                          void* y, int ystride, int out_bf16, const void* res, int res_bf16,
                          int rstride, float rs, int nr, q27x_stream_t s);

@@ -41,6 +41,7 @@ constexpr int kNvStep = 256;          // weights of a row that a wave takes at a
 constexpr int kNvSteps = 5;           // steps of a wave in registers
 constexpr int kNvWaves = 16;          // waves of a block at most
 constexpr int kNvLds = 160 * 1024;
+constexpr int kNvMaxRows = 0x7fffffff - (1 << 19);      // (a block's next tile, and its rows, keep in 31 bits: 256 x 16 blocks of 4 tiles)
 constexpr int kNvMaxK = 57344;        // (45 slots: their sums of gate and up, 8 rows, have room in LDS beside 20 steps of 4 rows: 157 KB)
 
 // LDS of a block: activation nibbles of its rows as operands, [steps][rows][low | high][256], and their scales, [steps][rows]
@@ -425,7 +426,7 @@ static int launch_nvfp4(const Nvfp4Args& a, hipStream_t s) {
 // the caller's matrix and rows, checked
 static int nvfp4_args(const q27x_nvfp4_t* w, const char* who, const int8_t* xq, int xstride, const float* xs, int nr) {
     if (!w || !w->w || !w->s || !xq || !xs) { set_error("%s: null argument", who); return Q27X_E_ARG; }
-    if (w->rows < 1 || w->rows > 0x7fffffff - 64 || w->K < 16 || (w->K & 15) || w->K > kNvMaxK) {
+    if (w->rows < 1 || w->rows > kNvMaxRows || w->K < 16 || (w->K & 15) || w->K > kNvMaxK) {
         set_error("%s: unsupported shape (rows=%d K=%d: K a multiple of 16 up to %d)", who, w->rows, w->K, kNvMaxK);
         return Q27X_E_SHAPE;
     }

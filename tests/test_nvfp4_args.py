@@ -29,7 +29,7 @@ def swiglu(X, w, up=None, **kw):
 
 
 @pytest.mark.parametrize("kw,rc", [(dict(w=None), ARG), (dict(s=None), ARG), (dict(rows=0), SHAPE), (dict(rows=-5), SHAPE),
-                                   (dict(rows=2 ** 31 - 1), SHAPE), (dict(K=0), SHAPE), (dict(K=8), SHAPE), (dict(K=250), SHAPE),
+                                   (dict(rows=2 ** 31 - 1), SHAPE), (dict(rows=2 ** 31 - (1 << 19)), SHAPE), (dict(K=0), SHAPE), (dict(K=8), SHAPE), (dict(K=250), SHAPE),
                                    (dict(K=57360), SHAPE), (dict(K=2 ** 31 - 16), SHAPE)])
 @pytest.mark.parametrize("call", [proj, swiglu])
 def test_matrices_refused(X, call, kw, rc):
