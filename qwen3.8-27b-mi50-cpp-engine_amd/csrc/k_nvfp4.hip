@@ -12,11 +12,16 @@
 // 16 x 16 result has the dots of 8 slabs of a pair of rows with 16 weight rows. An eighth of the operand holds something; the
 // matrix cores have the time.
 //
-// Bound by memory for few rows: 62080 x 5120, 1 row, 179 MB in 30.6 us (5.85 TB/s; a kernel that only reads them so, 26.0). What it
+// Up to 4 rows the bound is memory: 62080 x 5120, 1 row, 179 MB in 30.6 us (5.85 TB/s; a kernel that only reads them so, 26.0). What it
 // takes: whole 128-byte lines of 8 rows a load, exchanged in registers (16 rows by 64 bytes, which are operands at once, read
-// at 5.0 TB/s and no more); scales of several steps in one load; blocks that stay and keep the activations, prepared, in LDS (a block
-// a tile: 49.5 us, a third of it spent on them); the next tile on its way while one is worked on. For 8 rows by the LDS reads of the
-// activation operands (20 of 16 bytes a lane for 4096 weights): 55 us.
+// at 5.0 TB/s and no more); scales of several steps in one load (one a step: +9 us of 39); blocks that stay and keep the
+// activations, prepared, in LDS (a block a tile: 49.5 us, a third of it spent on them); the next tile on its way while one is worked on.
+// Chunks of K shorter than 5 steps: 33 us (3), 39 (2), 58 (1).
+//
+// From 5 rows on tiles of 32 weight rows, and v_mfma_scale_f32_32x32x64_f8f6f4 with the nibbles in E2M3, whose codes 0 .. 15 are as many
+// eighths: row 4 n + i of the operand holds slab i of row n, so one instruction serves 8 rows. It takes 40 cycles, the 16 x 16 x 128
+// with E4M3, two rows, 42: 8 rows 37 us, where those tiles take 45 to 48. Left are the scales' products and sums (2 operations a slab, row
+// and weight row) and the masks of the operands: without the sums 33.8 us; without preparing the activations 36.9.
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -72,6 +77,30 @@ struct Span {
     __device__ __forceinline__ float ldf(uint32_t at) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0)); }
 };
 
+// ROWS rows of a matrix from ROWS tile on; those that are not read as 0.
+template <int ROWS>
+struct Nvfp4Tile {
+    Span w, s;
+    __device__ __forceinline__ Nvfp4Tile(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile)
+        : w(w_ + (size_t)ROWS * tile * (size_t)(K >> 1), (uint32_t)max(0, min(ROWS, rows - ROWS * tile)) * (uint32_t)(K >> 1)),
+          s(s_ + (size_t)ROWS * tile * (size_t)(K >> 4), (uint32_t)max(0, min(ROWS, rows - ROWS * tile)) * (uint32_t)(K >> 4)) {}
+    // its last step, of `rest` slabs, into LDS by `threads` threads: codes [ROWS][128], scales [ROWS][16], zeros behind K
+    static __device__ void bring(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile, char* lds, int rest, int t, int threads) {
+        for (int i = t; i < ROWS * 16; i += threads) {
+            const int k = i & 15, row = ROWS * tile + (i >> 4);
+            u32x2 v = {0, 0};
+            uint8_t e = 0;
+            if (k < rest && row < rows) {
+                const size_t end = (size_t)(K >> 4) - rest;
+                v = *(const u32x2u*)(w_ + (size_t)row * (size_t)(K >> 1) + 8 * (end + k));
+                e = s_[(size_t)row * (size_t)(K >> 4) + end + k];
+            }
+            *(u32x2*)(lds + 8 * i) = v;
+            lds[ROWS * 128 + i] = (char)e;
+        }
+    }
+};
+
 // A wave's codes: up to kNvSteps steps of 16 rows, as they come: lane l has the codes 128 (l / 4 % 2) + 32 (l / 16) .. of a
 // step of rows r and 8 + r, r = l % 4 + 4 (l / 8 % 2), so a load covers 8 rows of a whole line. Exchanged between lanes 4
 // apart, register h has codes 128 h + 32 (l / 16) .. of row row_of(l % 16): an operand. The scales of all steps come together,
@@ -94,21 +123,15 @@ struct Nvfp4Weights {
             sto[i] = row < 16 ? (row * (uint32_t)(per | 1) + j) * 16 : ~0u;
         }
     }
-    struct Tile {
-        Span w, s;
-        __device__ __forceinline__ Tile(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile)
-            : w(w_ + (size_t)16 * tile * (size_t)(K >> 1), (uint32_t)max(0, min(16, rows - 16 * tile)) * (uint32_t)(K >> 1)),
-              s(s_ + (size_t)16 * tile * (size_t)(K >> 4), (uint32_t)max(0, min(16, rows - 16 * tile)) * (uint32_t)(K >> 4)) {}
-    };
     // step st of the tile into place j, if `is` (rows behind the last are 0). Always the same loads: where there is no step they
     // read nothing, so that the waits for others know how many are on their way.
-    __device__ __forceinline__ void load(const Tile& from, int j, int st, bool is) {
+    __device__ __forceinline__ void load(const Nvfp4Tile<16>& from, int j, int st, bool is) {
         const uint32_t wo = is ? (uint32_t)st * 128 : 0x80000000u;
         w[j][0] = from.w.ld16_nt(at[0] + wo);
         w[j][1] = from.w.ld16_nt(at[1] + wo);
     }
     // the scales of steps st .. (those of whole steps: `most` bytes of a row are)
-    __device__ __forceinline__ void load_scales(const Tile& from, int st, int per, int full) {
+    __device__ __forceinline__ void load_scales(const Nvfp4Tile<16>& from, int st, int per, int full) {
         const int l = threadIdx.x & 63;
 #pragma unroll
         for (int i = 0; i < kScales; ++i) {
@@ -120,21 +143,6 @@ struct Nvfp4Weights {
 #pragma unroll
         for (int i = 0; i < kScales; ++i)
             if (sto[i] != ~0u) *(u32x4*)(lds + sto[i]) = s[i];
-    }
-    // the tile's last step, of `rest` slabs, into LDS by `threads` threads, and from there into place j
-    static __device__ void bring(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile, char* lds, int rest, int t, int threads) {
-        for (int i = t; i < 16 * 16; i += threads) {
-            const int k = i & 15, row = 16 * tile + (i >> 4);
-            u32x2 v = {0, 0};
-            uint8_t e = 0;
-            if (k < rest && row < rows) {
-                const size_t end = (size_t)(K >> 4) - rest;
-                v = *(const u32x2u*)(w_ + (size_t)row * (size_t)(K >> 1) + 8 * (end + k));
-                e = s_[(size_t)row * (size_t)(K >> 4) + end + k];
-            }
-            *(u32x2*)(lds + 8 * i) = v;
-            lds[2048 + i] = (char)e;
-        }
     }
     __device__ __forceinline__ void take(const char* lds, int j) {
         const int l = threadIdx.x & 63, r = (l & 3) + 4 * ((l >> 3) & 1), piece = 4 * ((l >> 2) & 1) + (l >> 4);
@@ -190,11 +198,72 @@ struct Nvfp4Rows {
             *(float*)(lds + L.xs + at * 64 + 4 * (slab & 15)) = xs[i];
         }
     }
+    // the same in E2M3: 6 bits a code, 12 bytes a slab
+    __device__ __forceinline__ void store_e2m3(char* codes, char* scales, int n, int count, int item) const {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const uint32_t k = (uint32_t)(item + (int)threadIdx.x + i * (int)blockDim.x), r = k / (uint32_t)count, slab = k - r * (uint32_t)count;
+            if ((int)r >= n) continue;
+            uint32_t lo[4], hi[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t h = (x[i][j] >> 4) & 0x0F0F0F0Fu, minus = h & 0x08080808u, one = minus >> 3;
+                lo[j] = six(x[i][j] & 0x0F0F0F0Fu);
+                hi[j] = six(((h ^ ((minus << 1) - one)) + one) | (minus << 2));
+            }
+            const uint32_t at = (slab >> 2) * (uint32_t)n + r;
+            char* to = codes + ((slab >> 2) * (uint32_t)n + at) * 64 + (slab & 3) * 16;
+            *(u32x4*)to = u32x4{lo[0] | lo[1] << 24, lo[1] >> 8 | lo[2] << 16, lo[2] >> 16 | lo[3] << 8, 0};
+            *(u32x4*)(to + 64 * n) = u32x4{hi[0] | hi[1] << 24, hi[1] >> 8 | hi[2] << 16, hi[2] >> 16 | hi[3] << 8, 0};
+            *(float*)(scales + at * 16 + 4 * (slab & 3)) = xs[i];
+        }
+    }
+    static __device__ __forceinline__ uint32_t six(uint32_t v) {           // four bytes below 64 as 24 bits
+        const uint32_t u = (v & 0x003F003Fu) | ((v >> 2) & 0x0FC00FC0u);
+        return (u & 0xFFFu) | ((u >> 4) & 0xFFF000u);
+    }
 };
 
 __device__ __forceinline__ f32x4 nvfp4_dots(const i32x8& x, const u32x4& w, const f32x4& c, int scale) {
     const i32x8 b = {(int)w[0], (int)w[1], (int)w[2], (int)w[3], 0, 0, 0, 0};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 0, 4, 0, scale, 0, 127);
+}
+
+// What a block's sums [group][slot][row][COLS] come to: `wide` tiles of ROWS outputs, tile, tile + stride ... With SWIGLU gate and up are groups
+// in turn, or the halves of a group's columns.
+template <int PAIRS, bool SWIGLU, int ROWS, int COLS>
+__device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* sums, int tile, int stride, int wide, int slots) {
+    const int outs = wide * 2 * PAIRS * ROWS;
+    constexpr bool kHalves = SWIGLU && COLS != ROWS;
+    for (int i = threadIdx.x; i < (outs + 63) / 64 * 64; i += (int)blockDim.x) {
+        const int r = i % ROWS, n = i / ROWS % (2 * PAIRS), k = min(i / (2 * PAIRS * ROWS), wide - 1), row = (tile + k * stride) * ROWS + r;
+        auto total = [&](int gr, int at = 0) {
+            float y = 0.0f;
+            for (int v = 0; v < slots; ++v) y = y + sums[((gr * slots + v) * 2 * PAIRS + n) * COLS + at + r];
+            return y;
+        };
+        const bool is = i < outs && n < a.nr && row < a.rows;
+        if constexpr (SWIGLU) {
+            const float gate = a.alpha[0] * (kHalves ? total(k) : total(2 * k)), up = a.alpha[1] * (kHalves ? total(k, ROWS) : total(2 * k + 1));
+            const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
+            const float sc = max_xor(fabsf(z), 16) * (1.0f / 127.0f);
+            const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
+            if (is) {
+                const size_t at = (size_t)n * a.rows + row;
+                a.oq[at] = qcode(z, inv);
+                if ((r & 15) == 0) a.os[at >> 4] = sc;
+            }
+        } else if (is) {
+            float y = a.alpha[0] * total(k);
+            if (a.res) {
+                const size_t at = (size_t)n * a.rstride + row;
+                y = __builtin_fmaf(a.rs, a.res_bf16 ? bf2f(((const uint16_t*)a.res)[at]) : ((const float*)a.res)[at], y);
+            }
+            const size_t at = (size_t)n * a.ystride + row;
+            if (a.out_bf16) ((uint16_t*)a.y)[at] = f2bf(y);
+            else ((float*)a.y)[at] = y;
+        }
+    }
 }
 
 // A block goes through tiles of 16 weight rows, `groups` side by side (SWIGLU: a tile of gate beside one of up). K is cut into
@@ -224,9 +293,9 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     char* scales = lds + L.ws + 256 * (per | 1) * wave;
     x.load(a, 0, rows_held, 0, count, 0);
     __builtin_amdgcn_sched_barrier(0);               // (requested first: loads come in order)
-    int tile = (int)blockIdx.x * wide + mine;
+    int tile = (int)blockIdx.x + mine * (int)gridDim.x;
     {
-        const Nvfp4Weights::Tile from(wp, sp, a.rows, a.K, tile);
+        const Nvfp4Tile<16> from(wp, sp, a.rows, a.K, tile);
         w.load_scales(from, wv * per, per, full);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -252,18 +321,17 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     }
     const int xsa = L.xs + 64 * (wv * per * rows_held + (g >> 1)) + 16 * (g & 1);
     int parity = 0;
-    for (int unit = blockIdx.x; unit * wide < tiles; unit += (int)gridDim.x, parity ^= 1) {
+    for (int first = blockIdx.x; first < tiles; first += (int)gridDim.x * wide, parity ^= 1) {
         const int after = tile + (int)gridDim.x * wide;
         if (rest) {
-            if (!RESIDENT || parity || unit != (int)blockIdx.x) __syncthreads();
-            w.bring(wp, sp, a.rows, a.K, tile, tail, rest, t - 64 * grp * waves, 64 * waves);
+            Nvfp4Tile<16>::bring(wp, sp, a.rows, a.K, tile, tail, rest, t - 64 * grp * waves, 64 * waves);
             __syncthreads();
         }
         float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * PAIRS;       // [group][slot][row][16], of two tiles in turn
         for (int s0 = 0, slot = wv; s0 < steps; s0 += turn, slot += waves) {
             float acc[PAIRS] = {};                   // row 2 p + g / 2, slabs 4 (g % 2) .. of each 128 weights, weight row of lane c
             const bool last = s0 + turn >= steps;    // (of the tile)
-            const Nvfp4Weights::Tile next(wp, sp, a.rows, a.K, last ? after : tile);
+            const Nvfp4Tile<16> next(wp, sp, a.rows, a.K, last ? after : tile);
             const int from = last ? wv * per : s0 + turn + wv * per;   // the steps after these
             const int sa = L.ws + 256 * (per | 1) * wave + 16 * (per | 1) * nvfp4_row_of(c) + 4 * (g & 1);
             w.store_scales(scales);
@@ -340,41 +408,221 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
             }
         }
         __syncthreads();
-        const int outs = wide * 32 * PAIRS;
-        for (int i = t; i < (outs + 63) / 64 * 64; i += (int)blockDim.x) {
-            const int r16 = i & 15, n = (i >> 4) % (2 * PAIRS), k = min(i / (32 * PAIRS), wide - 1), row = (unit * wide + k) * 16 + r16;
-            auto total = [&](int gr) {
-                float y = 0.0f;
-                for (int v = 0; v < slots; ++v) y = y + sums[((gr * slots + v) * 2 * PAIRS + n) * 16 + r16];
-                return y;
-            };
-            const bool is = i < outs && n < a.nr && row < a.rows;
-            if constexpr (SWIGLU) {
-                const float gate = a.alpha[0] * total(2 * k), up = a.alpha[1] * total(2 * k + 1);
-                const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
-                const float sc = max_xor(fabsf(z), 16) * (1.0f / 127.0f);
-                const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
-                if (is) {
-                    const size_t at = (size_t)n * a.rows + row;
-                    a.oq[at] = qcode(z, inv);
-                    if (r16 == 0) a.os[at >> 4] = sc;
-                }
-            } else if (is) {
-                float y = a.alpha[0] * total(k);
-                if (a.res) {
-                    const size_t at = (size_t)n * a.rstride + row;
-                    y = __builtin_fmaf(a.rs, a.res_bf16 ? bf2f(((const uint16_t*)a.res)[at]) : ((const float*)a.res)[at], y);
-                }
-                const size_t at = (size_t)n * a.ystride + row;
-                if (a.out_bf16) ((uint16_t*)a.y)[at] = f2bf(y);
-                else ((float*)a.y)[at] = y;
-            }
-        }
+        nvfp4_finish<PAIRS, SWIGLU, 16, 16>(a, sums, first, (int)gridDim.x, wide, slots);
         tile = after;
     }
 }
 
-struct Nvfp4Plan { int per, slots, groups, waves, bytes; bool resident; };
+// ---- Tiles of 32 weight rows (SWIGLU: 16 of gate and 16 of up, side by side: with tiles of both in groups of their own a block has half as
+// many, and the last round of 17408 rows is longer, 30.7 us against 29.0). 8 waves, for the registers: 80 hold weights on their way.
+// The operands are read 64 weights ahead, in a place for each row whether it is or not, so that their offsets are constants.
+constexpr int kNvWideWaves = 8, kWidePairs = 3;
+struct Nvfp4WideLds {                 // operands [4 steps][low | high][rows][4 slabs][12, 4 unused]; scales [4 steps][rows][4]; then as Nvfp4Lds
+    int xs, ws, sums, tail, total;
+    __host__ __device__ __forceinline__ Nvfp4WideLds(int rows, int steps, int per, int groups, int waves, int slots, bool ends_inside) {
+        xs = 512 * rows * steps;
+        ws = xs + 64 * rows * steps;
+        sums = ws + 512 * (per | 1) * groups * waves;
+        tail = sums + 8 * groups * slots * 32 * rows;
+        total = tail + (ends_inside ? 4608 * groups : 0);
+    }
+};
+// As Nvfp4Weights, of 32 rows: lane l's loads are of rows 8 i + l % 8, codes 32 (2 (l / 8 % 4) + l / 32) ..; exchanged between lanes 16 and 8
+// apart, register q has codes 64 q + 32 (l / 32) .. of row l % 32.
+template <int MATS>
+struct Nvfp4WideWeights {
+    static constexpr int kRows = 32 / MATS, kScales = (kRows * kNvSteps + 63) / 64;
+    u32x4 w[kNvSteps][4], s[MATS][kScales];
+    uint32_t at, rows8, sat[kScales], sto[kScales];
+
+    __device__ __forceinline__ void begin(int K, int per) {
+        const int l = threadIdx.x & 63;
+        rows8 = 8 * (uint32_t)(K >> 1);
+        at = (uint32_t)(l & 7) * (uint32_t)(K >> 1) + 16 * (2 * ((l >> 3) & 3) + (l >> 5));
+#pragma unroll
+        for (int i = 0; i < kScales; ++i) {
+            const uint32_t k = (uint32_t)(l + 64 * i), row = k / (uint32_t)per, j = k - row * (uint32_t)per;
+            sat[i] = row < kRows ? row * (uint32_t)(K >> 4) + 16 * j : 0x40000000u;
+            sto[i] = row < kRows ? (row * (uint32_t)(per | 1) + j) * 16 : ~0u;
+        }
+    }
+    template <typename TILES>
+    __device__ __forceinline__ void load(const TILES& from, int j, int st, bool is) {
+        const uint32_t wo = is ? at + (uint32_t)st * 128 : 0x80000000u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[j][i] = from[i * MATS / 4].w.ld16_nt(wo + (i * 8 % kRows / 8) * rows8);
+    }
+    template <typename TILES>
+    __device__ __forceinline__ void load_scales(const TILES& from, int st, int per, int full) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < kScales; ++i) {
+            const uint32_t k = (uint32_t)(l + 64 * i), j = k % (uint32_t)per;
+#pragma unroll
+            for (int m = 0; m < MATS; ++m) s[m][i] = from[m].s.ld16(st + (int)j < full ? sat[i] + (uint32_t)st * 16 : 0x80000000u);
+        }
+    }
+    __device__ __forceinline__ void store_scales(char* lds, int per) const {
+#pragma unroll
+        for (int i = 0; i < kScales; ++i)
+#pragma unroll
+            for (int m = 0; m < MATS; ++m)
+                if (sto[i] != ~0u) *(u32x4*)(lds + m * kRows * (per | 1) * 16 + sto[i]) = s[m][i];
+    }
+    __device__ __forceinline__ void take(const char* lds, int j) {
+        const int l = threadIdx.x & 63;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            w[j][i] = *(const u32x4*)(lds + i * MATS / 4 * (kRows * 144) + 128 * (i * 8 % kRows + (l & 7)) + 16 * (2 * ((l >> 3) & 3) + (l >> 5)));
+    }
+    __device__ __forceinline__ void operands(int j, u32x4 (&q)[4]) const {
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+            const auto x = __builtin_amdgcn_permlane16_swap(w[j][0][d], w[j][2][d], false, false), y = __builtin_amdgcn_permlane16_swap(w[j][1][d], w[j][3][d], false, false);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                q[2 * h][d] = (uint32_t)__builtin_amdgcn_update_dpp((int)x[h], (int)y[h], 0x118, 0xF, 0xC, false);
+                q[2 * h + 1][d] = (uint32_t)__builtin_amdgcn_update_dpp((int)y[h], (int)x[h], 0x108, 0xF, 0x3, false);
+            }
+        }
+    }
+};
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+template <int PAIRS, bool SWIGLU>
+__global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, int groups, int waves, int per, int slots) {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    constexpr int kMats = SWIGLU ? 2 : 1, kRows = 32 / kMats, kIn = 2 * PAIRS, kItems = 5;
+    using Weights = Nvfp4WideWeights<kMats>;
+    using Tile = Nvfp4Tile<kRows>;
+    const int t = threadIdx.x, l = t & 63, c = l & 31, g = l >> 5;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
+    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, count = 16 * steps;
+    const int tiles = (a.rows + kRows - 1) / kRows;
+    const Nvfp4WideLds L(kIn, steps, per, groups, waves, slots, rest != 0);
+    char* tail = lds + L.tail + 4608 * grp;
+    Nvfp4Rows<kItems> x;
+    Weights w;
+    w.begin(a.K, per);
+    char* scales = lds + L.ws + 512 * (per | 1) * wave;
+    x.load(a, 0, kIn, 0, count, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    int tile = (int)blockIdx.x + grp * (int)gridDim.x;
+    {
+        const Tile from[2] = {Tile(a.w[0], a.s[0], a.rows, a.K, tile), Tile(a.w[kMats - 1], a.s[kMats - 1], a.rows, a.K, tile)};
+        w.load_scales(from, wv * per, per, full);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < kNvSteps; ++j) w.load(from, j, wv * per + j, j < per && wv * per + j < full);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    x.store_e2m3(lds, lds + L.xs, kIn, count, 0);
+    for (int item = kItems * (int)blockDim.x; item < kIn * count; item += kItems * (int)blockDim.x) {
+        x.load(a, 0, kIn, 0, count, item);
+        x.store_e2m3(lds, lds + L.xs, kIn, count, item);
+    }
+    __syncthreads();
+    // row c of the operand holds slab c % 4 of row c / 4, in lanes g = c % 4 / 2, in its first or second half; zeros elsewhere
+    const bool has = ((c >> 1) & 1) == g && (c >> 2) < kIn;
+    const uint32_t even = has && !(c & 1) ? ~0u : 0, odd = has && (c & 1) ? ~0u : 0;
+    const int opa = 512 * kIn * wv * per + 16 * (c & (4 * kIn - 1 < 16 ? 4 * kIn - 1 : 31)), xsa = L.xs + 64 * kIn * wv * per + 16 * g;
+    int parity = 0;
+    for (int first = blockIdx.x; first < tiles; first += (int)gridDim.x * groups, parity ^= 1) {
+        const int after = tile + (int)gridDim.x * groups;
+        if (rest) {
+#pragma unroll
+            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.rows, a.K, tile, tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
+            __syncthreads();
+        }
+        float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * kIn;
+        for (int s0 = 0, slot = wv; s0 < steps; s0 += turn, slot += waves) {
+            float acc[PAIRS][2] = {};                // row 2 p + g; even and odd 64 weights
+            const bool last = s0 + turn >= steps;
+            const int from = last ? wv * per : s0 + turn + wv * per, to = last ? after : tile;
+            const Tile next[2] = {Tile(a.w[0], a.s[0], a.rows, a.K, to), Tile(a.w[kMats - 1], a.s[kMats - 1], a.rows, a.K, to)};
+            w.store_scales(scales, per);
+            int o = opa + 512 * kIn * s0, ox = xsa + 64 * kIn * s0, sa = L.ws + 512 * (per | 1) * wave + 16 * (per | 1) * c;
+            asm volatile("" : "+v"(o), "+v"(ox));
+            w.load_scales(next, from, per, full);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < kNvSteps; ++j) {
+                const int st = s0 + wv * per + j;
+                if (j < per && st < steps) {
+                    int sj = sa + 16 * j;
+                    if (st == full) {
+                        w.take(tail, j);
+                        sj = L.tail + 4608 * grp + c / kRows * (kRows * 144) + kRows * 128 + 16 * (c % kRows);
+                    }
+                    constexpr int kOne = 127 + 3, k16 = kOne + 4;       // codes are eighths
+                    u32x4 y[2][2];                   // 64 weights' operands ahead
+                    f32x4 xs[2][PAIRS];
+                    auto bring = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) y[i & 1][h] = *(const u32x4*)(lds + o + (2 * i + h) * 64 * kIn);
+                    };
+                    auto bring_scales = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int p = 0; p < PAIRS; ++p) xs[i & 1][p] = *(const f32x4*)(lds + ox + 16 * kIn * i + 32 * p);
+                    };
+                    auto operand = [&](const u32x4& v) __attribute__((always_inline)) {
+                        return i32x8{(int)(v[0] & even), (int)(v[1] & even), (int)(v[2] & even), (int)(v[0] & odd), (int)(v[1] & odd), (int)(v[2] & odd), 0, 0};
+                    };
+                    f32x16 d[2];
+                    bring(0);
+                    const u32x4 e = *(const u32x4*)(lds + sj);
+                    bring_scales(0);
+                    u32x4 q[4];
+                    w.operands(j, q);
+                    auto sum = [&](int i) __attribute__((always_inline)) {
+                        const auto e0 = __builtin_amdgcn_cvt_pk_f32_fp8((int)e[i], false), e1 = __builtin_amdgcn_cvt_pk_f32_fp8((int)e[i], true);
+#pragma unroll
+                        for (int p = 0; p < PAIRS; ++p) {
+                            const f32x4& z = xs[i & 1][p];
+                            float& r = acc[p][i & 1];
+                            r = __builtin_fmaf(d[i & 1][4 * p], e0[0] * z[0], r);
+                            r = __builtin_fmaf(d[i & 1][4 * p + 1], e0[1] * z[1], r);
+                            r = __builtin_fmaf(d[i & 1][4 * p + 2], e1[0] * z[2], r);
+                            r = __builtin_fmaf(d[i & 1][4 * p + 3], e1[1] * z[3], r);
+                        }
+                    };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const i32x8 b = {(int)q[i][0], (int)q[i][1], (int)q[i][2], (int)q[i][3], 0, 0, 0, 0};
+                        const i32x8 lo = operand(y[i & 1][0]), hi = operand(y[i & 1][1]);
+                        if (i < 3) bring(i + 1);
+                        d[i & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(lo, b, f32x16{}, 2, 4, 0, kOne, 0, 127);
+                        d[i & 1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(hi, b, d[i & 1], 2, 4, 0, k16, 0, 127);
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (i > 0) sum(i - 1);
+                        if (i < 3) bring_scales(i + 1);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    sum(3);
+                    o += 512 * kIn;
+                    ox += 64 * kIn;
+                }
+                w.load(next, j, from + j, j < per && from + j < full);
+            }
+            if (slot < slots) {
+#pragma unroll
+                for (int p = 0; p < PAIRS; ++p) sums[((grp * slots + slot) * kIn + 2 * p + g) * 32 + c] = acc[p][0] + acc[p][1];
+            }
+        }
+        __syncthreads();
+        nvfp4_finish<PAIRS, SWIGLU, kRows, 32>(a, sums, first, (int)gridDim.x, groups, slots);
+        tile = after;
+    }
+}
+
+struct Nvfp4Plan { int per, slots, groups, waves, bytes; };
+template <int PAIRS, bool SWIGLU>
+static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
+    const int tiles = SWIGLU ? a.rows / 16 : (a.rows + 31) / 32, units = (tiles + p.groups - 1) / p.groups, grid = units < 256 ? units : 256;
+    Q27X_HIP((allow_lds<k_nvfp4_wide<PAIRS, SWIGLU>>(kNvLds)));
+    hipLaunchKernelGGL((k_nvfp4_wide<PAIRS, SWIGLU>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.groups, p.waves, p.per, p.slots);
+    Q27X_HIP(hipGetLastError());
+    return Q27X_OK;
+}
 template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_form(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
     const int wide = SWIGLU ? p.groups / 2 : p.groups, units = ((a.rows + 15) / 16 + wide - 1) / wide;
@@ -396,6 +644,17 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
     Nvfp4Plan p;
     p.per = steps <= 4 ? 1 : steps <= 8 ? 2 : kNvSteps;
     p.slots = (steps + p.per - 1) / p.per;
+    // 5 rows and more: tiles of 32 weight rows, where there are enough of them. Against those of 16: 62080 x 5120, 8 rows 37 us (45), 5
+    // rows 36 (39); gate | up 17408 x 5120 29.6 (36.8), 29 (32); 5120 x 5120 11.9 (15.3), 11.6 (11.5); with fewer tiles than here
+    // 1024 x 768 5.6 (4.8), and 9001 x 5136, 5 rows 19.8 (18.0); 3 rows 33.4 (33.2) and 26.8 (24.8).
+    if constexpr (PAIRS >= kWidePairs) {
+        const int tiles32 = SWIGLU ? tiles : (tiles + 1) / 2;
+        p.groups = tiles32 < 512 ? 1 : 2;            // (tiles for every compute unit)
+        const int most = kNvWideWaves / p.groups, turns = (p.slots + most - 1) / most;
+        p.waves = (p.slots + turns - 1) / turns;
+        p.bytes = Nvfp4WideLds(2 * PAIRS, steps, p.per, p.groups, p.waves, p.slots, ends_inside).total;
+        if (tiles32 >= (PAIRS == 4 ? 160 : 512) && p.bytes <= kNvLds) return launch_nvfp4_wide<PAIRS, SWIGLU>(a, p, s);
+    }
     // all activations in LDS, tiles side by side that share them
     p.groups = PAIRS == 1 ? 1 : PAIRS == 2 ? 2 : 4;
     if (p.groups < least) p.groups = least;
