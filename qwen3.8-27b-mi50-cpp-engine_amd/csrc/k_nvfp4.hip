@@ -77,23 +77,23 @@ struct Span {
     __device__ __forceinline__ float ldf(uint32_t at) const { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(r, (int)at, 0, 0)); }
 };
 
-// ROWS rows of a matrix from ROWS tile on; those that are not read as 0.
+// Rows first .. first + ROWS - 1 of a matrix, of which those from `end` on are read as 0.
 template <int ROWS>
 struct Nvfp4Tile {
     Span w, s;
-    __device__ __forceinline__ Nvfp4Tile(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile)
-        : w(w_ + (size_t)ROWS * tile * (size_t)(K >> 1), (uint32_t)max(0, min(ROWS, rows - ROWS * tile)) * (uint32_t)(K >> 1)),
-          s(s_ + (size_t)ROWS * tile * (size_t)(K >> 4), (uint32_t)max(0, min(ROWS, rows - ROWS * tile)) * (uint32_t)(K >> 4)) {}
+    __device__ __forceinline__ Nvfp4Tile(const uint8_t* w_, const uint8_t* s_, int K, int first, int end)
+        : w(w_ + (size_t)first * (size_t)(K >> 1), (uint32_t)max(0, min(ROWS, end - first)) * (uint32_t)(K >> 1)),
+          s(s_ + (size_t)first * (size_t)(K >> 4), (uint32_t)max(0, min(ROWS, end - first)) * (uint32_t)(K >> 4)) {}
     // its last step, of `rest` slabs, into LDS by `threads` threads: codes [ROWS][128], scales [ROWS][16], zeros behind K
-    static __device__ void bring(const uint8_t* w_, const uint8_t* s_, int rows, int K, int tile, char* lds, int rest, int t, int threads) {
+    static __device__ void bring(const uint8_t* w_, const uint8_t* s_, int K, int first, int end, char* lds, int rest, int t, int threads) {
         for (int i = t; i < ROWS * 16; i += threads) {
-            const int k = i & 15, row = ROWS * tile + (i >> 4);
+            const int k = i & 15, row = first + (i >> 4);
             u32x2 v = {0, 0};
             uint8_t e = 0;
-            if (k < rest && row < rows) {
-                const size_t end = (size_t)(K >> 4) - rest;
-                v = *(const u32x2u*)(w_ + (size_t)row * (size_t)(K >> 1) + 8 * (end + k));
-                e = s_[(size_t)row * (size_t)(K >> 4) + end + k];
+            if (k < rest && row < end) {
+                const size_t slab = (size_t)(K >> 4) - rest + k;
+                v = *(const u32x2u*)(w_ + (size_t)row * (size_t)(K >> 1) + 8 * slab);
+                e = s_[(size_t)row * (size_t)(K >> 4) + slab];
             }
             *(u32x2*)(lds + 8 * i) = v;
             lds[ROWS * 128 + i] = (char)e;
@@ -229,20 +229,20 @@ __device__ __forceinline__ f32x4 nvfp4_dots(const i32x8& x, const u32x4& w, cons
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, b, c, 0, 4, 0, scale, 0, 127);
 }
 
-// What a block's sums [group][slot][row][COLS] come to: `wide` tiles of ROWS outputs, tile, tile + stride ... With SWIGLU gate and up are groups
-// in turn, or the halves of a group's columns.
+// What a block's sums [group][slot][row][COLS] come to: `wide` tiles of `each` of ROWS outputs, the first ones `first`, first + stride .. With SWIGLU
+// gate and up are groups in turn, or the halves of a group's columns.
 template <int PAIRS, bool SWIGLU, int ROWS, int COLS>
-__device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* sums, int tile, int stride, int wide, int slots) {
+__device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* sums, int first, int each, int stride, int wide, int slots) {
     const int outs = wide * 2 * PAIRS * ROWS;
     constexpr bool kHalves = SWIGLU && COLS != ROWS;
     for (int i = threadIdx.x; i < (outs + 63) / 64 * 64; i += (int)blockDim.x) {
-        const int r = i % ROWS, n = i / ROWS % (2 * PAIRS), k = min(i / (2 * PAIRS * ROWS), wide - 1), row = (tile + k * stride) * ROWS + r;
+        const int r = i % ROWS, n = i / ROWS % (2 * PAIRS), k = min(i / (2 * PAIRS * ROWS), wide - 1), row = first + k * stride + r;
         auto total = [&](int gr, int at = 0) {
             float y = 0.0f;
             for (int v = 0; v < slots; ++v) y = y + sums[((gr * slots + v) * 2 * PAIRS + n) * COLS + at + r];
             return y;
         };
-        const bool is = i < outs && n < a.nr && row < a.rows;
+        const bool is = i < outs && n < a.nr && r < each && row < a.rows;
         if constexpr (SWIGLU) {
             const float gate = a.alpha[0] * (kHalves ? total(k) : total(2 * k)), up = a.alpha[1] * (kHalves ? total(k, ROWS) : total(2 * k + 1));
             const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
@@ -266,18 +266,18 @@ __device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* su
     }
 }
 
-// A block goes through tiles of 16 weight rows, `groups` side by side (SWIGLU: a tile of gate beside one of up). K is cut into
+// A block goes through tiles of up to 16 weight rows, `groups` side by side (SWIGLU: 16 of gate beside 16 of up). K is cut into
 // `slots` of `per` steps; a group's waves take one each, `turn` steps together, then the next ones. Activation rows go in pairs.
 // RESIDENT: all of them are in LDS, once for all tiles; else a pair's turn is brought when it comes. The weights of the next turn or
 // tile are requested as this one's are used. An output is the sum of its slots in order, whatever the waves, so its bits do not
 // depend on nr.
 template <int PAIRS, bool SWIGLU, bool RESIDENT>
-__global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4Args a, int groups, int waves, int per, int slots) {
+__global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4Args a, int tile_rows, int groups, int waves, int per, int slots) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
     const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
-    const int tiles = (a.rows + 15) >> 4, wide = SWIGLU ? groups >> 1 : groups;
+    const int wide = SWIGLU ? groups >> 1 : groups, each = SWIGLU ? 16 : tile_rows;
     constexpr int kIn = RESIDENT || PAIRS == 1 ? PAIRS : 2, kPasses = (PAIRS + kIn - 1) / kIn;        // pairs of a pass over the weights, and passes
     constexpr int kItems = RESIDENT ? 3 : 5;
     const int rows_held = RESIDENT ? a.nr : min(a.nr, 2 * kIn);
@@ -293,9 +293,10 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     char* scales = lds + L.ws + 256 * (per | 1) * wave;
     x.load(a, 0, rows_held, 0, count, 0);
     __builtin_amdgcn_sched_barrier(0);               // (requested first: loads come in order)
-    int tile = (int)blockIdx.x + mine * (int)gridDim.x;
+    const int stride = (int)gridDim.x * each, turn_rows = stride * wide;
+    int row = (int)blockIdx.x * each + mine * stride;        // of the tile
     {
-        const Nvfp4Tile<16> from(wp, sp, a.rows, a.K, tile);
+        const Nvfp4Tile<16> from(wp, sp, a.K, row, min(row + each, a.rows));
         w.load_scales(from, wv * per, per, full);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -321,17 +322,17 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     }
     const int xsa = L.xs + 64 * (wv * per * rows_held + (g >> 1)) + 16 * (g & 1);
     int parity = 0;
-    for (int first = blockIdx.x; first < tiles; first += (int)gridDim.x * wide, parity ^= 1) {
-        const int after = tile + (int)gridDim.x * wide;
+    for (int first = (int)blockIdx.x * each; first < a.rows; first += turn_rows, parity ^= 1) {
         if (rest) {
-            Nvfp4Tile<16>::bring(wp, sp, a.rows, a.K, tile, tail, rest, t - 64 * grp * waves, 64 * waves);
+            Nvfp4Tile<16>::bring(wp, sp, a.K, row, min(row + each, a.rows), tail, rest, t - 64 * grp * waves, 64 * waves);
             __syncthreads();
         }
         float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * PAIRS;       // [group][slot][row][16], of two tiles in turn
         for (int s0 = 0, slot = wv; s0 < steps; s0 += turn, slot += waves) {
             float acc[PAIRS] = {};                   // row 2 p + g / 2, slabs 4 (g % 2) .. of each 128 weights, weight row of lane c
             const bool last = s0 + turn >= steps;    // (of the tile)
-            const Nvfp4Tile<16> next(wp, sp, a.rows, a.K, last ? after : tile);
+            const int to = last ? row + turn_rows : row;
+            const Nvfp4Tile<16> next(wp, sp, a.K, to, min(to + each, a.rows));
             const int from = last ? wv * per : s0 + turn + wv * per;   // the steps after these
             const int sa = L.ws + 256 * (per | 1) * wave + 16 * (per | 1) * nvfp4_row_of(c) + 4 * (g & 1);
             w.store_scales(scales);
@@ -408,8 +409,8 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
             }
         }
         __syncthreads();
-        nvfp4_finish<PAIRS, SWIGLU, 16, 16>(a, sums, first, (int)gridDim.x, wide, slots);
-        tile = after;
+        nvfp4_finish<PAIRS, SWIGLU, 16, 16>(a, sums, first, each, stride, wide, slots);
+        row += turn_rows;
     }
 }
 
@@ -497,7 +498,6 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     const int t = threadIdx.x, l = t & 63, c = l & 31, g = l >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
     const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, count = 16 * steps;
-    const int tiles = (a.rows + kRows - 1) / kRows;
     const Nvfp4WideLds L(kIn, steps, per, groups, waves, slots, rest != 0);
     char* tail = lds + L.tail + 4608 * grp;
     Nvfp4Rows<kItems> x;
@@ -506,9 +506,10 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     char* scales = lds + L.ws + 512 * (per | 1) * wave;
     x.load(a, 0, kIn, 0, count, 0);
     __builtin_amdgcn_sched_barrier(0);
-    int tile = (int)blockIdx.x + grp * (int)gridDim.x;
+    const int stride = (int)gridDim.x * kRows, turn_rows = stride * groups;
+    int row = (int)blockIdx.x * kRows + grp * stride;        // of the tile
     {
-        const Tile from[2] = {Tile(a.w[0], a.s[0], a.rows, a.K, tile), Tile(a.w[kMats - 1], a.s[kMats - 1], a.rows, a.K, tile)};
+        const Tile from[2] = {Tile(a.w[0], a.s[0], a.K, row, a.rows), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, row, a.rows)};
         w.load_scales(from, wv * per, per, full);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -526,19 +527,18 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     const uint32_t even = has && !(c & 1) ? ~0u : 0, odd = has && (c & 1) ? ~0u : 0;
     const int opa = 512 * kIn * wv * per + 16 * (c & (4 * kIn - 1 < 16 ? 4 * kIn - 1 : 31)), xsa = L.xs + 64 * kIn * wv * per + 16 * g;
     int parity = 0;
-    for (int first = blockIdx.x; first < tiles; first += (int)gridDim.x * groups, parity ^= 1) {
-        const int after = tile + (int)gridDim.x * groups;
+    for (int first = (int)blockIdx.x * kRows; first < a.rows; first += turn_rows, parity ^= 1) {
         if (rest) {
 #pragma unroll
-            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.rows, a.K, tile, tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
+            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.K, row, a.rows, tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
             __syncthreads();
         }
         float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * kIn;
         for (int s0 = 0, slot = wv; s0 < steps; s0 += turn, slot += waves) {
             float acc[PAIRS][2] = {};                // row 2 p + g; even and odd 64 weights
             const bool last = s0 + turn >= steps;
-            const int from = last ? wv * per : s0 + turn + wv * per, to = last ? after : tile;
-            const Tile next[2] = {Tile(a.w[0], a.s[0], a.rows, a.K, to), Tile(a.w[kMats - 1], a.s[kMats - 1], a.rows, a.K, to)};
+            const int from = last ? wv * per : s0 + turn + wv * per, to = last ? row + turn_rows : row;
+            const Tile next[2] = {Tile(a.w[0], a.s[0], a.K, to, a.rows), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, to, a.rows)};
             w.store_scales(scales, per);
             int o = opa + 512 * kIn * s0, ox = xsa + 64 * kIn * s0, sa = L.ws + 512 * (per | 1) * wave + 16 * (per | 1) * c;
             asm volatile("" : "+v"(o), "+v"(ox));
@@ -609,12 +609,12 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
             }
         }
         __syncthreads();
-        nvfp4_finish<PAIRS, SWIGLU, kRows, 32>(a, sums, first, (int)gridDim.x, groups, slots);
-        tile = after;
+        nvfp4_finish<PAIRS, SWIGLU, kRows, 32>(a, sums, first, kRows, stride, groups, slots);
+        row += turn_rows;
     }
 }
 
-struct Nvfp4Plan { int per, slots, groups, waves, bytes; };
+struct Nvfp4Plan { int per, slots, groups, waves, bytes, tile_rows, tiles; };
 template <int PAIRS, bool SWIGLU>
 static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
     const int tiles = SWIGLU ? a.rows / 16 : (a.rows + 31) / 32, units = (tiles + p.groups - 1) / p.groups, grid = units < 256 ? units : 256;
@@ -625,14 +625,14 @@ static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t
 }
 template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_form(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
-    const int wide = SWIGLU ? p.groups / 2 : p.groups, units = ((a.rows + 15) / 16 + wide - 1) / wide;
+    const int wide = SWIGLU ? p.groups / 2 : p.groups, units = (p.tiles + wide - 1) / wide;
     int fit = kNvLds / p.bytes;                      // blocks of a compute unit
     const int room = (RESIDENT ? kNvWaves : kNvWaves / 2) / (p.groups * p.waves);
     fit = fit < room ? fit : room;
     fit = fit < 1 ? 1 : fit;
     const int grid = 256 * fit < units ? 256 * fit : units;
     Q27X_HIP((allow_lds<k_nvfp4<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
-    hipLaunchKernelGGL((k_nvfp4<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.groups, p.waves, p.per, p.slots);
+    hipLaunchKernelGGL((k_nvfp4<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows, p.groups, p.waves, p.per, p.slots);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
 }
@@ -655,10 +655,15 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
         p.bytes = Nvfp4WideLds(2 * PAIRS, steps, p.per, p.groups, p.waves, p.slots, ends_inside).total;
         if (tiles32 >= (PAIRS == 4 ? 160 : 512) && p.bytes <= kNvLds) return launch_nvfp4_wide<PAIRS, SWIGLU>(a, p, s);
     }
+    // tiles of fewer rows where that gives every compute unit as many (5120 x 17408, 1 row: 10 of 16 rows 14.2 us, all 16 16.1; 5120 x
+    // 5120, 3 rows 8.4 and 9.7; where a compute unit has one at most it is no gain: 1024 x 768 4.2 and 3.9)
+    const int n = SWIGLU || tiles <= 256 ? 0 : (tiles + 255) / 256;
+    p.tile_rows = n ? (a.rows - 1) / (256 * n) + 1 : 16;
+    p.tiles = (a.rows + p.tile_rows - 1) / p.tile_rows;
     // all activations in LDS, tiles side by side that share them
     p.groups = PAIRS == 1 ? 1 : PAIRS == 2 ? 2 : 4;
     if (p.groups < least) p.groups = least;
-    while (p.groups > least && tiles * least < 256 * p.groups) p.groups >>= 1;         // (tiles for every compute unit)
+    while (p.groups > least && p.tiles * least < 256 * p.groups) p.groups >>= 1;         // (tiles for every compute unit)
     for (;; p.groups >>= 1) {
         const int most = kNvWaves / p.groups, turns = (p.slots + most - 1) / most;
         p.waves = (p.slots + turns - 1) / turns;

@@ -87,3 +87,14 @@ def test_not_finite_stays_with_its_rows(gpu):
     rest = np.setdiff1d(np.arange(rows), at)
     keep = [n for n in range(nr) if n != 4]
     assert np.array_equal(got[np.ix_(keep, rest)], clean[np.ix_(keep, rest)])
+
+
+@pytest.mark.parametrize("rows,K", [(4097, 272), (4113, 1040), (5120, 784), (8193, 144), (9001, 1296), (12295, 16)])
+def test_tiles_of_fewer_rows(gpu, rows, K):
+    """More tiles than compute units, in even shares: all outputs of 1 to 4 rows, with residual, nothing beside them."""
+    rng = np.random.default_rng(rows * K)
+    m = Matrix(gpu, rng, rows, K, alpha=-0.03)
+    for nr in (1, 2, 3, 4):
+        xq, xs = rows_of(rng, nr, K, K + 16)
+        res = rng.standard_normal((nr, rows + 2)).astype(np.float32)
+        check(project(gpu, m, xq, xs, res=res, rs=0.5, pad=7), m, xq, xs, res, 0.5)
