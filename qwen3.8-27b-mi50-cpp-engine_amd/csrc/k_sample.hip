@@ -15,6 +15,13 @@
 //   k_sample_draw: a row's bins summed and searched. Where all that can be drawn is 256 tokens or fewer, each of them counts and
 //     sums those before it, and the cuts and the draw are comparisons; else the bin that a search ends in is narrowed to 256 by
 //     (logit, index) in steps of 8 bits, and these are counted like that.
+//   k_sample_one: all of that by one block, for rows of up to 4096 logits (7.8 us for 300, 8 to 11 for 4000, by the settings).
+//
+// Bound by latency: 62080 logits, 1 row, 17.0 us, of which k_sample_max has 2.4, k_sample_bins 6.4, k_sample_draw 8 (2.9 to read, 2.2 to
+// sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 36 to 38 us: 4.9, 13.4 (the exponentials and the
+// atomics 2.6 each), 20 for the slowest row, whose cuts and draw are searches of about 5 us each, three trips to memory and some
+// ten barriers. All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000. A search down to 128
+// or 256 tokens in place of 64: 25.9 and 28.3 us. One copy of the bins: atomics of a wave wait for one another.
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -37,6 +44,7 @@ struct SampleArgs {
     u64* bw;                                      // [nr][ns][kBins] weights
     uint16_t* off;                                // [nr][ns][kOffs] where a bin begins in the slice's list, and its end
     uint16_t* list;                               // [nr][ns][slice] tokens of the slice by bin
+    float* ahead;                                 // [nr][ns][kAhead] logits of the first of them
     int32_t* idx; float* prob;
 };
 
@@ -144,13 +152,13 @@ struct BinShared {
     uint32_t n[kBins * kCopies], part[(kBins + 63) / 64];
 };
 // A slice of T PER tokens (MANY: some times that) from `begin` on by bin: list, where each bin begins in it (off, and its end behind the
-// last), the bins' weights; how many there are. x: the slice's first logits, 4 (j T + t) .. + 3 of this thread.
+// last), the bins' weights, the first tokens' logits (if `ahead`); how many there are. x: the slice's first logits, 4 (j T + t) .. + 3 of this thread.
 // Bins are kept four times, by lane, as a wave's 64 tokens lie in some 70 bins at most: adding to one place waits for one another.
 // Counting gives a token its place in its bin at once. From z = 16 on a slice's weights of a bin are below 2^43: the count has room
 // above them, one addition for both.
 template <int T, int PER, bool MANY>
 __device__ __forceinline__ uint32_t bins_of(const SampleArgs& a, BinShared& sh, uint16_t* list, int row, int begin, float (&x)[PER / 4][4], double l0,
-                                            double c, uint16_t* off, u64* bw) {
+                                            double c, uint16_t* off, u64* bw, float* ahead) {
     constexpr int kTail = 256 * kCopies;          // places of z >= 16
     const int t = threadIdx.x, copy = t & (kCopies - 1);
     uint32_t place[PER];                          // of a token: its bin's copy, and how many came before it there; ~0: left out
@@ -230,14 +238,22 @@ __device__ __forceinline__ uint32_t bins_of(const SampleArgs& a, BinShared& sh, 
     if constexpr (!MANY) {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-            if (place[j] != ~0u) list[sh.n[place[j] >> 16] + (place[j] & 0xFFFFu)] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
+            if (place[j] != ~0u) {
+                const uint32_t at = sh.n[place[j] >> 16] + (place[j] & 0xFFFFu);
+                list[at] = (uint16_t)(4 * (j / 4 * T + t) + j % 4);
+                if (ahead && at < kAhead) ahead[at] = x[j / 4][j % 4];
+            }
     } else {
         for (int i0 = 0; i0 < a.slice; i0 += PER * T) {
             load(i0);
             take(false);                          // (the bins' beginnings count on)
 #pragma unroll
             for (int j = 0; j < PER; ++j)
-                if (place[j] != ~0u) list[place[j] & 0xFFFFu] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
+                if (place[j] != ~0u) {
+                    const uint32_t at = place[j] & 0xFFFFu;
+                    list[at] = (uint16_t)(i0 + 4 * (j / 4 * T + t) + j % 4);
+                    if (ahead && at < kAhead) ahead[at] = x[j / 4][j % 4];
+                }
         }
     }
     __syncthreads();
@@ -247,6 +263,7 @@ template <int T, int PER, bool MANY>
 __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint16_t s_list[];
     __shared__ BinShared sh;
+    __shared__ float s_ahead[kAhead];
     const int s = blockIdx.x, row = blockIdx.y, t = threadIdx.x, begin = s * a.slice;
     float x[PER / 4][4];
 #pragma unroll
@@ -256,7 +273,8 @@ __global__ __launch_bounds__(T) void k_sample_bins(SampleArgs a) {
     const double l0 = (double)row_max(a, row), c = inv_temp(a, row, greedy);
     __syncthreads();
     const size_t at = (size_t)row * a.ns + s;
-    const uint32_t total = bins_of<T, PER, MANY>(a, sh, s_list, row, begin, x, l0, c, a.off + at * kOffs, a.bw + at * kBins);
+    const uint32_t total = bins_of<T, PER, MANY>(a, sh, s_list, row, begin, x, l0, c, a.off + at * kOffs, a.bw + at * kBins, s_ahead);
+    if (t < kAhead) a.ahead[at * kAhead + t] = s_ahead[t];       // (behind the list's end: anything)
     for (uint32_t i = 8 * t; i < total; i += 8 * T) *(uint4*)(a.list + at * a.slice + i) = *(const uint4*)&s_list[i];
 }
 
@@ -609,15 +627,17 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     const int row = blockIdx.x, t = threadIdx.x;
     __shared__ DrawShared<kMostSlices> sh;
     const size_t first = (size_t)row * a.ns;
-    // Requested at once, as each is a trip to memory: the first tokens of each slice's list, its offsets, bins 2 t and 2 t + 1
-    // of each; then these tokens' logits. (Any entry of a list is read as a token of its slice: those behind its end are not used.)
+    // Requested at once, as each is a trip to memory: the first tokens of each slice's list and their logits, its offsets, bins 2 t and
+    // 2 t + 1 of each. (What lies behind a list's end is read too, and not used.)
     int id[kAheadOf];
+    float ahead[kAheadOf];
     uint4 off[kOffLoads];
     ulonglong2 bw[kMostSlices];
 #pragma unroll
     for (int j = 0; j < kAheadOf; ++j) {
         const int s = min((t >> 6) + 4 * j, a.ns - 1);
         id[j] = s * a.slice + (int)a.list[(first + s) * a.slice + (t & 63)];
+        ahead[j] = a.ahead[(first + s) * kAhead + (t & 63)];
     }
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -628,9 +648,6 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(SampleArgs a) {
     __builtin_amdgcn_sched_barrier(0);
     const float top = row_max(a, row);
     const Cuts cuts(a, row);
-    float ahead[kAheadOf];
-#pragma unroll
-    for (int j = 0; j < kAheadOf; ++j) ahead[j] = logit_at(a, row, min(id[j], a.n - 1));
 #pragma unroll
     for (int j = 0; j < kOffLoads; ++j)
         if (t + j * kDrawThreads < kMostSlices * (kOffs / 8)) ((uint4*)sh.off)[t + j * kDrawThreads] = off[j];
@@ -711,7 +728,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_one(SampleArgs a) {
         if (t == 0) { a.idx[row] = 0; if (a.prob) a.prob[row] = 0.0f; }
         return;
     }
-    bins_of<kDrawThreads, kPer, false>(a, sh.bins, sh.list, row, 0, x, (double)top, cuts.c, sh.draw.off[0], sh.bw);
+    bins_of<kDrawThreads, kPer, false>(a, sh.bins, sh.list, row, 0, x, (double)top, cuts.c, sh.draw.off[0], sh.bw, nullptr);
     uint32_t n0 = 0, n1 = 0;
     u64 w0 = 0, w1 = 0;
     if (t < kBins / 2) {
@@ -727,7 +744,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_one(SampleArgs a) {
     });
 }
 
-struct SampleLayout { size_t bw, smax, off, list, total; int slice, ns, parts; };
+struct SampleLayout { size_t bw, smax, off, list, ahead, total; int slice, ns, parts; };
 static SampleLayout sample_layout(int n, int nr) {
     SampleLayout w{};
     w.slice = kLeastSlice;
@@ -738,7 +755,8 @@ static SampleLayout sample_layout(int n, int nr) {
     w.bw = 0;
     w.list = w.bw + at * kBins * 8;
     w.off = w.list + at * w.slice * 2;
-    w.smax = w.off + at * kOffs * 2;
+    w.ahead = w.off + at * kOffs * 2;
+    w.smax = w.ahead + at * kAhead * 4;
     w.total = w.smax + (size_t)nr * w.parts * 4;
     return w;
 }
@@ -763,7 +781,7 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     a.logits = logits; a.bf16 = logits_bf16 ? 1 : 0; a.n = n; a.ld = nr > 1 ? ld : 0; a.nr = nr;
     a.ns = wl.ns; a.slice = wl.slice; a.parts = wl.parts;
     a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
-    a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off); a.smax = (float*)(p + wl.smax);
+    a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off); a.ahead = (float*)(p + wl.ahead); a.smax = (float*)(p + wl.smax);
     a.idx = idx; a.prob = prob;
     if (a.ns == 1) {
         Q27X_HIP(allow_lds<k_sample_one>((int)sizeof(OneShared)));
