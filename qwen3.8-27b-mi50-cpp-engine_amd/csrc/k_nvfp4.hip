@@ -279,7 +279,7 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
     const int wide = SWIGLU ? groups >> 1 : groups, each = SWIGLU ? 16 : tile_rows;
     constexpr int kIn = RESIDENT || PAIRS == 1 ? PAIRS : 2, kPasses = (PAIRS + kIn - 1) / kIn;        // pairs of a pass over the weights, and passes
-    constexpr int kItems = RESIDENT ? 3 : 5;
+    constexpr int kItems = !RESIDENT ? 5 : PAIRS <= 2 ? 4 : 3;       // (3 rows of 17408 at once: 18.6 us, by 3 items 19.5)
     const int rows_held = RESIDENT ? a.nr : min(a.nr, 2 * kIn);
     const Nvfp4Lds L(rows_held, held, per, groups, waves, slots, 32 * PAIRS, rest != 0);
     const uint8_t* wp = SWIGLU && (grp & 1) ? a.w[1] : a.w[0];
@@ -489,16 +489,17 @@ struct Nvfp4WideWeights {
     }
 };
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-template <int PAIRS, bool SWIGLU>
-__global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, int groups, int waves, int per, int slots) {
+template <int PAIRS, bool SWIGLU, bool RESIDENT>
+__global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, int tile_rows, int groups, int waves, int per, int slots) {
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    constexpr int kMats = SWIGLU ? 2 : 1, kRows = 32 / kMats, kIn = 2 * PAIRS, kItems = 5;
+    constexpr int kMats = SWIGLU ? 2 : 1, kRows = 32 / kMats, kIn = 2 * PAIRS, kItems = RESIDENT ? 5 : 2;       // (5 spill there: 38.8 us, 34.7)
     using Weights = Nvfp4WideWeights<kMats>;
     using Tile = Nvfp4Tile<kRows>;
     const int t = threadIdx.x, l = t & 63, c = l & 31, g = l >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
-    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, count = 16 * steps;
-    const Nvfp4WideLds L(kIn, steps, per, groups, waves, slots, rest != 0);
+    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
+    const int each = SWIGLU ? kRows : tile_rows;
+    const Nvfp4WideLds L(kIn, held, per, groups, waves, slots, rest != 0);
     char* tail = lds + L.tail + 4608 * grp;
     Nvfp4Rows<kItems> x;
     Weights w;
@@ -506,31 +507,34 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     char* scales = lds + L.ws + 512 * (per | 1) * wave;
     x.load(a, 0, kIn, 0, count, 0);
     __builtin_amdgcn_sched_barrier(0);
-    const int stride = (int)gridDim.x * kRows, turn_rows = stride * groups;
-    int row = (int)blockIdx.x * kRows + grp * stride;        // of the tile
+    const int stride = (int)gridDim.x * each, turn_rows = stride * groups;
+    int row = (int)blockIdx.x * each + grp * stride;        // of the tile
     {
-        const Tile from[2] = {Tile(a.w[0], a.s[0], a.K, row, a.rows), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, row, a.rows)};
+        const Tile from[2] = {Tile(a.w[0], a.s[0], a.K, row, min(row + each, a.rows)), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, row, min(row + each, a.rows))};
         w.load_scales(from, wv * per, per, full);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < kNvSteps; ++j) w.load(from, j, wv * per + j, j < per && wv * per + j < full);
     }
     __builtin_amdgcn_sched_barrier(0);
-    x.store_e2m3(lds, lds + L.xs, kIn, count, 0);
-    for (int item = kItems * (int)blockDim.x; item < kIn * count; item += kItems * (int)blockDim.x) {
-        x.load(a, 0, kIn, 0, count, item);
-        x.store_e2m3(lds, lds + L.xs, kIn, count, item);
-    }
-    __syncthreads();
+    auto store = [&](int slab) __attribute__((always_inline)) {        // what x has, and the rest of these rows
+        x.store_e2m3(lds, lds + L.xs, kIn, count, 0);
+        for (int item = kItems * (int)blockDim.x; item < kIn * count; item += kItems * (int)blockDim.x) {
+            x.load(a, 0, kIn, slab, count, item);
+            x.store_e2m3(lds, lds + L.xs, kIn, count, item);
+        }
+        __syncthreads();
+    };
+    if constexpr (RESIDENT) store(0);
     // row c of the operand holds slab c % 4 of row c / 4, in lanes g = c % 4 / 2, in its first or second half; zeros elsewhere
     const bool has = ((c >> 1) & 1) == g && (c >> 2) < kIn;
     const uint32_t even = has && !(c & 1) ? ~0u : 0, odd = has && (c & 1) ? ~0u : 0;
     const int opa = 512 * kIn * wv * per + 16 * (c & (4 * kIn - 1 < 16 ? 4 * kIn - 1 : 31)), xsa = L.xs + 64 * kIn * wv * per + 16 * g;
     int parity = 0;
-    for (int first = (int)blockIdx.x * kRows; first < a.rows; first += turn_rows, parity ^= 1) {
+    for (int first = (int)blockIdx.x * each; first < a.rows; first += turn_rows, parity ^= 1) {
         if (rest) {
 #pragma unroll
-            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.K, row, a.rows, tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
+            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.K, row, min(row + each, a.rows), tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
             __syncthreads();
         }
         float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * kIn;
@@ -538,10 +542,16 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
             float acc[PAIRS][2] = {};                // row 2 p + g; even and odd 64 weights
             const bool last = s0 + turn >= steps;
             const int from = last ? wv * per : s0 + turn + wv * per, to = last ? row + turn_rows : row;
-            const Tile next[2] = {Tile(a.w[0], a.s[0], a.K, to, a.rows), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, to, a.rows)};
+            const Tile next[2] = {Tile(a.w[0], a.s[0], a.K, to, min(to + each, a.rows)), Tile(a.w[kMats - 1], a.s[kMats - 1], a.K, to, min(to + each, a.rows))};
             w.store_scales(scales, per);
-            int o = opa + 512 * kIn * s0, ox = xsa + 64 * kIn * s0, sa = L.ws + 512 * (per | 1) * wave + 16 * (per | 1) * c;
+            int o = opa + (RESIDENT ? 512 * kIn * s0 : 0), ox = xsa + (RESIDENT ? 64 * kIn * s0 : 0), sa = L.ws + 512 * (per | 1) * wave + 16 * (per | 1) * c;
             asm volatile("" : "+v"(o), "+v"(ox));
+            if constexpr (!RESIDENT) {
+                __syncthreads();                      // (the turn before is read)
+                store(16 * s0);
+                x.load(a, 0, kIn, last ? 0 : 16 * (s0 + turn), count, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             w.load_scales(next, from, per, full);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -609,17 +619,18 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
             }
         }
         __syncthreads();
-        nvfp4_finish<PAIRS, SWIGLU, kRows, 32>(a, sums, first, kRows, stride, groups, slots);
+        nvfp4_finish<PAIRS, SWIGLU, kRows, 32>(a, sums, first, each, stride, groups, slots);
         row += turn_rows;
     }
 }
 
 struct Nvfp4Plan { int per, slots, groups, waves, bytes, tile_rows, tiles; };
-template <int PAIRS, bool SWIGLU>
+template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
-    const int tiles = SWIGLU ? a.rows / 16 : (a.rows + 31) / 32, units = (tiles + p.groups - 1) / p.groups, grid = units < 256 ? units : 256;
-    Q27X_HIP((allow_lds<k_nvfp4_wide<PAIRS, SWIGLU>>(kNvLds)));
-    hipLaunchKernelGGL((k_nvfp4_wide<PAIRS, SWIGLU>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.groups, p.waves, p.per, p.slots);
+    const int tiles = (a.rows + p.tile_rows - 1) / p.tile_rows, units = (tiles + p.groups - 1) / p.groups, grid = units < 256 ? units : 256;
+    Q27X_HIP((allow_lds<k_nvfp4_wide<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
+    hipLaunchKernelGGL((k_nvfp4_wide<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows, p.groups, p.waves,
+                       p.per, p.slots);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
 }
@@ -644,16 +655,20 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
     Nvfp4Plan p;
     p.per = steps <= 4 ? 1 : steps <= 8 ? 2 : kNvSteps;
     p.slots = (steps + p.per - 1) / p.per;
+    const int tiles32 = SWIGLU ? tiles : (tiles + 1) / 2;
+    auto fits_wide = [&](int most, bool resident) {
+        const int turns = (p.slots + most - 1) / most;
+        p.waves = (p.slots + turns - 1) / turns;
+        p.bytes = Nvfp4WideLds(2 * PAIRS, resident ? steps : p.waves * p.per, p.per, p.groups, p.waves, p.slots, ends_inside).total;
+        return p.bytes <= kNvLds;
+    };
     // 5 rows and more: tiles of 32 weight rows, where there are enough of them. Against those of 16: 62080 x 5120, 8 rows 37 us (45), 5
     // rows 36 (39); gate | up 17408 x 5120 29.6 (36.8), 29 (32); 5120 x 5120 11.9 (15.3), 11.6 (11.5); with fewer tiles than here
     // 1024 x 768 5.6 (4.8), and 9001 x 5136, 5 rows 19.8 (18.0); 3 rows 33.4 (33.2) and 26.8 (24.8).
     if constexpr (PAIRS >= kWidePairs) {
-        const int tiles32 = SWIGLU ? tiles : (tiles + 1) / 2;
         p.groups = tiles32 < 512 ? 1 : 2;            // (tiles for every compute unit)
-        const int most = kNvWideWaves / p.groups, turns = (p.slots + most - 1) / most;
-        p.waves = (p.slots + turns - 1) / turns;
-        p.bytes = Nvfp4WideLds(2 * PAIRS, steps, p.per, p.groups, p.waves, p.slots, ends_inside).total;
-        if (tiles32 >= (PAIRS == 4 ? 160 : 512) && p.bytes <= kNvLds) return launch_nvfp4_wide<PAIRS, SWIGLU>(a, p, s);
+        p.tile_rows = SWIGLU ? 16 : 32;
+        if (tiles32 >= (PAIRS == 4 ? 160 : 512) && fits_wide(kNvWideWaves / p.groups, true)) return launch_nvfp4_wide<PAIRS, SWIGLU, true>(a, p, s);
     }
     // tiles of fewer rows where that gives every compute unit as many (5120 x 17408, 1 row: 10 of 16 rows 14.2 us, all 16 16.1; 5120 x
     // 5120, 3 rows 8.4 and 9.7; where a compute unit has one at most it is no gain: 1024 x 768 4.2 and 3.9)
@@ -670,6 +685,20 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
         p.bytes = Nvfp4Lds(a.nr, steps, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
         if (p.bytes <= kNvLds) return launch_nvfp4_form<PAIRS, SWIGLU, true>(a, p, s);
         if (p.groups == least) break;
+    }
+    // activations in turns: 32 weight rows where that is a tile for each compute unit at most, or 5 or 6 rows, or gate | up; and 4 waves have
+    // room beside the sums. Against 16: 5120 x 17408, 5 rows 24.9 us (34.3), 8 rows 34.7 (37.6), 9001 x 17408 42 (49), 63 (54), gate |
+    // up 17408 x 12288 96 (112), 115 (122), 5120 x 57344 81 (92), 170 (101; 2 waves)
+    if constexpr (PAIRS >= kWidePairs) {
+        if (tiles32 >= 160 && (PAIRS == 3 || SWIGLU || tiles32 <= 256)) {
+            const Nvfp4Plan narrow = p;
+            p.groups = 1;
+            const int shares = (tiles32 + 255) / 256;
+            p.tile_rows = SWIGLU ? 16 : (a.rows - 1) / (256 * shares) + 1;
+            for (int most = kNvWideWaves; most >= 4; --most)
+                if (fits_wide(most, false)) return launch_nvfp4_wide<PAIRS, SWIGLU, false>(a, p, s);
+            p = narrow;
+        }
     }
     const int most = kNvWaves / 2 / least, turns = (p.slots + most - 1) / most;
     p.waves = (p.slots + turns - 1) / turns;

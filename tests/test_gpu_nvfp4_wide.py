@@ -98,3 +98,31 @@ def test_tiles_of_fewer_rows(gpu, rows, K):
         xq, xs = rows_of(rng, nr, K, K + 16)
         res = rng.standard_normal((nr, rows + 2)).astype(np.float32)
         check(project(gpu, m, xq, xs, res=res, rs=0.5, pad=7), m, xq, xs, res, 0.5)
+
+
+@pytest.mark.parametrize("rows,K,nrs", [(5120, 17408, (5, 6, 8)), (5137, 12304, (7, 8)), (8195, 17424, (5, 8)), (5121, 57344, (5, 8))])
+def test_activations_in_turns(gpu, rows, K, nrs):
+    """Rows that LDS does not hold at once, even shares of weight rows: the ends against float64, every output against fewer rows' bits."""
+    rng = np.random.default_rng(rows + K)
+    m = Matrix(gpu, rng, rows, K, alpha=-0.02)
+    xq, xs = rows_of(rng, 8, K, K + 16)
+    alone = [project(gpu, m, xq[n:n + 1], xs[n:n + 1])[0] for n in range(8)]
+    part = [(0, 100), (rows - 100, rows), (2550, 2650)]
+    for nr in nrs:
+        got = project(gpu, m, xq[:nr], xs[:nr], pad=1)
+        assert np.array_equal(got.view(np.uint32), np.array(alone[:nr]).view(np.uint32))
+    for lo, hi in part:
+        check(got[:, lo:hi], _last(m, hi - lo, lo), xq[:nr], xs[:nr])
+
+
+@pytest.mark.parametrize("nr", [5, 8])
+def test_swiglu_in_turns(gpu, nr):
+    rng = np.random.default_rng(nr)
+    rows, K = 2592, 12304
+    gate, up = (Matrix(gpu, rng, rows, K, alpha=a / np.sqrt(K)) for a in (0.05, -0.03))
+    xq, xs = rows_of(rng, nr, K)
+    q, s = swiglu(gpu, gate, up, xq, xs, 0.6)
+    check_swiglu(q[:, -96:], s[:, -6:], _last(gate, 96), _last(up, 96), xq, xs, 0.6)
+    for n in range(nr):
+        q1, s1 = swiglu(gpu, gate, up, xq[n:n + 1], xs[n:n + 1], 0.6)
+        assert np.array_equal(q1[0], q[n]) and np.array_equal(s1[0], s[n])
