@@ -136,7 +136,7 @@ int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int xstride, c
 /* Gate and up of an MLP on NVFP4 weights, and q27x_swiglu_quant_rows of them, in one launch (the reference's fused
  * q27_proj_nvfp4_gu_nr, include/q27_nr.h:14-19): gate and up [rows][K] as q27x_proj_nvfp4_rows computes them, fp32, then
  *   v = (g/(1+e^-g)) * u * (1/in_scale); per 16: s = mx/127; q = clamp(rint(v/s)) -> oq [nr][rows], os [nr][rows/16].
- * rows % 16 == 0, K as there; in_scale is that of the projection that reads oq. */
+ * rows % 16 == 0, K as there; in_scale is that of the projection that reads oq; oq and os overlap nothing that is read. */
 int q27x_swiglu_nvfp4_rows(const q27x_nvfp4_t* gate, const q27x_nvfp4_t* up, const int8_t* xq, int xstride,
                            const float* xs, int8_t* oq, float* os, float in_scale, int nr, q27x_stream_t s);
 
