@@ -17,7 +17,7 @@
 //     (logit, index) in steps of 8 bits, and these are counted like that.
 //   k_sample_one: all of that by one block, for rows of up to 4096 logits (7.8 us for 300, 8 to 11 for 4000, by the settings).
 //
-// Bound by latency: 62080 logits, 1 row, 17.0 us, of which k_sample_max has 2.4, k_sample_bins 6.4, k_sample_draw 8 (2.9 to read, 2.2 to
+// Bound by latency: 62080 logits, 1 row, 16.7 us, of which k_sample_max has 2.4, k_sample_bins 6, k_sample_draw 8 (2.9 to read, 2.2 to
 // sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 36 to 38 us: 4.9, 13.4 (the exponentials and the
 // atomics 2.6 each), 20 for the slowest row, whose cuts and draw are searches of about 5 us each, three trips to memory and some
 // ten barriers. All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000. A search down to 128
@@ -792,7 +792,9 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     const dim3 grid((unsigned)a.ns, (unsigned)nr);
     hipLaunchKernelGGL(k_sample_max, dim3((unsigned)a.parts, (unsigned)nr), dim3(256), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
-    if (a.slice == kLeastSlice) {
+    if (a.slice == kLeastSlice && (long long)a.ns * nr <= 256) {          // (a compute unit for each block: 1 row 16.7 us, else 17.2; 64 rows 29.4, else 28.7)
+        hipLaunchKernelGGL((k_sample_bins<1024, 4, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
+    } else if (a.slice == kLeastSlice) {
         hipLaunchKernelGGL((k_sample_bins<512, 8, false>), grid, dim3(512), 2 * a.slice, (hipStream_t)s, a);
     } else if (a.slice == 8192) {
         hipLaunchKernelGGL((k_sample_bins<1024, 8, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);

@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from ref64 import bf16_rne, bf2f
-from test_gpu_sample import HOW, answers, check, logits
+from test_gpu_sample import HOW, answers, check, logits, sample
 
 pytestmark = pytest.mark.gpu
 
@@ -42,3 +42,19 @@ def test_any_element(gpu, n, bf16, odd):
     f = np.float32
     for r in range(3):
         assert got[r] in answers(v[r], float(f(0.9)), 60, float(f(0.95)), float(f(0.01)), float(u[r]))
+
+
+@pytest.mark.parametrize("n", [4097, 20000, 62080])
+def test_few_and_many_blocks(gpu, n):
+    """Rows on both sides of one block for each compute unit have the same tokens and probabilities."""
+    X, rng = gpu, np.random.default_rng(n)
+    x = np.repeat(logits(rng, 5, n), 30, 0)
+    u = np.tile(rng.random(30).astype(np.float32), 5)
+    for how in ("all", "p high"):
+        t, k, p, m = HOW[how]
+        full = lambda v, dt: np.full(150, v, dt)
+        many = sample(X, x, full(t, np.float32), full(k, np.int32), full(p, np.float32), full(m, np.float32), u)
+        few = [sample(X, x[i:i + 5], full(t, np.float32)[:5], full(k, np.int32)[:5], full(p, np.float32)[:5], full(m, np.float32)[:5], u[i:i + 5])
+               for i in range(0, 150, 5)]
+        for j in range(2):
+            assert np.array_equal(np.concatenate([f[j] for f in few]), many[j])
