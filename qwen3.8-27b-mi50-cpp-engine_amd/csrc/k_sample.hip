@@ -13,15 +13,17 @@
 //   k_sample_bins: bins of z (a 16th of a binary order up to 16 of them, a quarter up to 48): a slice's tokens by bin, and each
 //     bin's weight; up to 16 slices a row.
 //   k_sample_draw: a row's bins summed and searched. Where all that can be drawn is 256 tokens or fewer, each of them counts and
-//     sums those before it, and the cuts and the draw are comparisons; else the bin that a search ends in is narrowed to 256 by
-//     (logit, index) in steps of 8 bits, and these are counted like that.
+//     sums those before it, and the cuts and the draw are comparisons; else the bin that a search ends in is narrowed to 64 tokens, by a
+//     256th of its z and then by (logit, index) in steps of 8 bits, and these are counted like that.
 //   k_sample_one: all of that by one block, for rows of up to 4096 logits (7.8 us for 300, 8 to 11 for 4000, by the settings).
 //
-// Bound by latency: 62080 logits, 1 row, 16.7 us, of which k_sample_max has 2.4, k_sample_bins 6, k_sample_draw 8 (2.9 to read, 2.2 to
-// sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 36 to 38 us: 4.9, 13.4 (the exponentials and the
-// atomics 2.6 each), 20 for the slowest row, whose cuts and draw are searches of about 5 us each, three trips to memory and some
-// ten barriers. All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000. A search down to 128
-// or 256 tokens in place of 64: 25.9 and 28.3 us. One copy of the bins: atomics of a wave wait for one another.
+// Bound by latency: 62080 logits, 1 row, 16.4 us, of which k_sample_max has 2.5, k_sample_bins 6, k_sample_draw 8 (2.9 to read, 2.2 to
+// sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 35 to 40 us: 4.8, 13.7 (the exponentials and the
+// atomics 2.6 each), the rest for the slowest row, whose cuts and draw are three searches (k = 1000 alone 24.5 us), or one in a bin
+// of thousands of tokens, which are read twice (p = 0.99, nothing before it: 29; by the ranks' range from the start, three times: 35).
+// All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000; ranks alone held, 4096 of them, and
+// weights computed anew: 26.5. A search down to 128 or 256 tokens in place of 64: 25.9 and 28.3 us. One copy of the bins: atomics of
+// a wave wait for one another.
 #include "q27x_paged.h"
 
 namespace q27x {
@@ -92,6 +94,11 @@ __device__ __forceinline__ u64 rank_of(float l, int i) {
     const uint32_t b = __float_as_uint(l + 0.0f);                // (-0 is 0)
     const uint32_t up = b & 0x80000000u ? ~b : b | 0x80000000u;
     return (u64)~up << 32 | (uint32_t)i;
+}
+
+__device__ __forceinline__ float logit_of(u64 rank) {
+    const uint32_t up = ~(uint32_t)(rank >> 32);
+    return __uint_as_float(up & 0x80000000u ? up & 0x7FFFFFFFu : ~up);
 }
 
 // four logits from i on, those behind the row as NaN
@@ -306,16 +313,18 @@ struct Lists {
     const uint16_t* list;
     const float* x;
     double l0, c;
-    // f(rank, weight) for each of bins b0 .. b1, the block's threads side by side
+    __device__ __forceinline__ double z_of(u64 rank) const { return order_of(logit_of(rank), l0, c); }
+    // f(rank, weight, z) for each of bins b0 .. b1, the block's threads side by side
     template <typename SH, typename F>
     __device__ __forceinline__ void each(const SH& sh, int b0, int b1, F f) const {
         if constexpr (ONE) {
             for (int i = sh.off[0][b0] + (int)threadIdx.x; i < sh.off[0][b1 + 1]; i += kDrawThreads) {
                 const int id = list[i];
-                f(rank_of(x[id], id), weight(order_of(x[id], l0, c)));
+                const double z = order_of(x[id], l0, c);
+                f(rank_of(x[id], id), weight(z), z);
             }
         } else {
-            // a wave's slices, 64 tokens of each requested at once (those behind a list's end are read as some token, and left out)
+            // a wave's slices, 64 tokens of each requested at once (what lies behind a list's end is left out)
             constexpr int kOf = kMostSlices * 64 / kDrawThreads;
             const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
             for (int i0 = 0;; i0 += 64) {
@@ -331,10 +340,13 @@ struct Lists {
                 }
                 if (!__ballot(any)) break;
 #pragma unroll
-                for (int j = 0; j < kOf; ++j) l[j] = logit_at(a, row, min(id[j], a.n - 1));
+                for (int j = 0; j < kOf; ++j) l[j] = logit_at(a, row, is[j] ? id[j] : 0);          // (idle lanes at one place)
 #pragma unroll
                 for (int j = 0; j < kOf; ++j)
-                    if (is[j]) f(rank_of(l[j], id[j]), weight(order_of(l[j], l0, c)));
+                    if (is[j]) {
+                        const double z = order_of(l[j], l0, c);
+                        f(rank_of(l[j], id[j]), weight(z), z);
+                    }
             }
         }
     }
@@ -374,56 +386,25 @@ __device__ __forceinline__ Counted count_held(const SH& sh, uint32_t n) {
 }
 
 // The token of bin b at which the running count (by_count) or weight, from the bin's beginning on, reaches `target` (at least 1, at
-// most the bin's): its rank, its weight and the running weight up to it, in sh.
+// most the bin's): its rank, its weight and the running weight up to it, in sh. Of many tokens first those of a 256th of the bin's z are
+// left, then of these those of a 256th of their ranks' range, until there are few.
 template <typename SH, typename LISTS>
 __device__ __forceinline__ void search(SH& sh, const LISTS& lists, bool by_count, int b, u64 target) {
     const int t = threadIdx.x;
     uint32_t n = sh.bn[b + 1] - sh.bn[b];
     u64 before = 0;                               // weight before what is left
     bool held = n <= kHeld;
-    __syncthreads();
-    if (held) {
-        if (t == 0) sh.held = 0;
-        __syncthreads();
-        lists.each(sh, b, b, [&](u64 q, u64 w) { sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w); });
-        __syncthreads();
-    }
-    u64 lo = 0, hi = ~0ull;
-    auto each = [&](auto f) {
-        if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.qw[i].x, sh.qw[i].y);
-        else lists.each(sh, b, b, f);
+    const bool split = n > kLeft;
+    int part = 0;
+    auto part_of = [&](double z) __attribute__((always_inline)) {          // (as bin_of: z and the tokens have one order)
+        const double y = b < 256 ? z * 16.0 - (double)b : (z - 16.0) * 4.0 - (double)(b - 256);
+        return min(max((int)(y * 256.0), 0), 255);
     };
-    while (n > kLeft) {
-        // the range of what is left, in 256 parts
-        u64 least = ~0ull, most = 0;
-        each([&](u64 q, u64) {
-            if (q >= lo && q <= hi) {
-                least = q < least ? q : least;
-                most = q > most ? q : most;
-            }
-        });
-#pragma unroll
-        for (int o = 1; o < 64; o *= 2) {
-            const u64 x = shfl_xor64(least, o), y = shfl_xor64(most, o);
-            least = x < least ? x : least;
-            most = y > most ? y : most;
-        }
+    auto clear = [&]() __attribute__((always_inline)) { sh.hw[t] = 0; sh.hn[t] = 0; };
+    // the part that `target` is in, by a wave, four parts a lane
+    auto choose = [&]() __attribute__((always_inline)) {
         __syncthreads();
-        if ((t & 63) == 0) { sh.lo[t >> 6] = least; sh.hi[t >> 6] = most; }
-        sh.hw[t] = 0;
-        sh.hn[t] = 0;
-        __syncthreads();
-        lo = min(min(sh.lo[0], sh.lo[1]), min(sh.lo[2], sh.lo[3]));
-        hi = max(max(sh.hi[0], sh.hi[1]), max(sh.hi[2], sh.hi[3]));
-        const int shift = max(0, 64 - __builtin_clzll((hi - lo) | 1) - 8);
-        each([&](u64 q, u64 w) {
-            if (q >= lo && q <= hi) {
-                atomicAdd(&sh.hw[(q - lo) >> shift], w);
-                atomicAdd(&sh.hn[(q - lo) >> shift], 1u);
-            }
-        });
-        __syncthreads();
-        if (t < 64) {                             // four parts a lane
+        if (t < 64) {
             Sum x = {0, 0};
 #pragma unroll
             for (int k = 0; k < 4; ++k) { x.n += sh.hn[4 * t + k]; x.w += sh.hw[4 * t + k]; }
@@ -444,33 +425,90 @@ __device__ __forceinline__ void search(SH& sh, const LISTS& lists, bool by_count
             if (t == 0) sh.held = 0;
         }
         __syncthreads();
-        lo += (u64)sh.digit << shift;
-        hi = min(hi, lo + ((1ull << shift) - 1));
         before += sh.digit_w;
         target -= by_count ? sh.digit_n : sh.digit_w;
+    };
+    auto each = [&](auto f) {                     // of what is left in the part
+        if (held) for (uint32_t i = t; i < n; i += kDrawThreads) f(sh.qw[i].x, sh.qw[i].y);
+        else lists.each(sh, b, b, [&](u64 q, u64 w, double z) { if (part_of(z) == part) f(q, w); });
+    };
+    // those that stay to the front, or into LDS once they fit
+    auto keep = [&](auto stays) {
         const uint32_t left = sh.left;
-        if (held || left <= kHeld) {              // these alone, at the front
-            if (held) {
-                ulonglong2 x[kHeld / kDrawThreads];
+        if (held) {
+            ulonglong2 x[kHeld / kDrawThreads];
 #pragma unroll
-                for (int k = 0; k < kHeld / kDrawThreads; ++k) {
-                    const uint32_t i = t + k * kDrawThreads;
-                    x[k] = sh.qw[i];
-                    if (i >= n || x[k].x < lo || x[k].x > hi) x[k].x = ~0ull;
-                }
-                __syncthreads();
-#pragma unroll
-                for (int k = 0; k < kHeld / kDrawThreads; ++k)
-                    if (x[k].x != ~0ull) sh.qw[atomicAdd(&sh.held, 1u)] = x[k];
-            } else {
-                lists.each(sh, b, b, [&](u64 q, u64 w) {
-                    if (q >= lo && q <= hi) sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w);
-                });
-                held = true;
+            for (int k = 0; k < kHeld / kDrawThreads; ++k) {
+                const uint32_t i = t + k * kDrawThreads;
+                x[k] = sh.qw[i];
+                if (i >= n || !stays(x[k].x)) x[k].x = ~0ull;
             }
             __syncthreads();
-            n = left;
+#pragma unroll
+            for (int k = 0; k < kHeld / kDrawThreads; ++k)
+                if (x[k].x != ~0ull) sh.qw[atomicAdd(&sh.held, 1u)] = x[k];
+        } else if (left <= kHeld) {
+            each([&](u64 q, u64 w) { if (stays(q)) sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w); });
+        } else {
+            return;
         }
+        held = true;
+        n = left;
+        __syncthreads();
+    };
+    __syncthreads();
+    clear();
+    if (t == 0) sh.held = 0;
+    __syncthreads();
+    if (held || split)
+        lists.each(sh, b, b, [&](u64 q, u64 w, double z) {
+            if (held) sh.qw[atomicAdd(&sh.held, 1u)] = make_ulonglong2(q, w);
+            if (split) {
+                const int k = part_of(z);
+                atomicAdd(&sh.hw[k], w);
+                atomicAdd(&sh.hn[k], 1u);
+            }
+        });
+    if (split) {
+        choose();
+        part = sh.digit;
+        keep([&](u64 q) { return part_of(lists.z_of(q)) == part; });
+    } else {
+        __syncthreads();
+    }
+    u64 lo = 0, hi = ~0ull;
+    while (n > kLeft) {
+        // the range of what is left, in 256 parts
+        u64 least = ~0ull, most = 0;
+        each([&](u64 q, u64) {
+            if (q >= lo && q <= hi) {
+                least = q < least ? q : least;
+                most = q > most ? q : most;
+            }
+        });
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const u64 x = shfl_xor64(least, o), y = shfl_xor64(most, o);
+            least = x < least ? x : least;
+            most = y > most ? y : most;
+        }
+        __syncthreads();
+        if ((t & 63) == 0) { sh.lo[t >> 6] = least; sh.hi[t >> 6] = most; }
+        clear();
+        __syncthreads();
+        lo = min(min(sh.lo[0], sh.lo[1]), min(sh.lo[2], sh.lo[3]));
+        hi = max(max(sh.hi[0], sh.hi[1]), max(sh.hi[2], sh.hi[3]));
+        const int shift = max(0, 64 - __builtin_clzll((hi - lo) | 1) - 8);
+        each([&](u64 q, u64 w) {
+            if (q >= lo && q <= hi) {
+                atomicAdd(&sh.hw[(q - lo) >> shift], w);
+                atomicAdd(&sh.hn[(q - lo) >> shift], 1u);
+            }
+        });
+        choose();
+        lo += (u64)sh.digit << shift;
+        hi = min(hi, lo + ((1ull << shift) - 1));
+        keep([&](u64 q) { return q >= lo && q <= hi; });
     }
     if (t < 4 * kBatch) sh.qw[n + t].x = ~0ull;
     __syncthreads();
@@ -599,7 +637,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, c
                 if (!by_p) continue;
             } else if (by_m) {
                 u64 sum = 0;
-                lists.each(sh, cuts.bm0, cuts.bm1, [&](u64, u64 w) { sum += w >= cuts.least ? w : 0; });
+                lists.each(sh, cuts.bm0, cuts.bm1, [&](u64, u64 w, double) { sum += w >= cuts.least ? w : 0; });
                 __syncthreads();
                 if (t == 0) sh.found_w = 0;
                 __syncthreads();
@@ -740,7 +778,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_one(SampleArgs a) {
     }
     const Lists<true> lists = {a, row, sh.list, sh.x, (double)top, cuts.c};
     draw_row(a, sh.draw, row, lists, cuts, n0, n1, w0, w1, [&](int upto) {
-        lists.each(sh.draw, 0, upto, [&](u64 q, u64 w) { sh.draw.qw[atomicAdd(&sh.draw.held, 1u)] = make_ulonglong2(q, w); });
+        lists.each(sh.draw, 0, upto, [&](u64 q, u64 w, double) { sh.draw.qw[atomicAdd(&sh.draw.held, 1u)] = make_ulonglong2(q, w); });
     });
 }
 
