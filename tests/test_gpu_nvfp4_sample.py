@@ -157,3 +157,46 @@ def test_streams_and_graphs(gpu):
             same(u.all(), seen[(i + j) % steps], f"two streams, step {i}")
     for _, s in pair:
         X.call("q27x_stream_destroy", s)
+
+
+@pytest.mark.parametrize("rows,K,nr", [(5121, 272, 8), (5120, 272, 2), (100, 528, 5), (5121, 17424, 6), (300, 20496, 3)])
+def test_residual_in_place(gpu, rows, K, nr):
+    """y over res, bf16, in every kernel: the bits of the call that writes elsewhere."""
+    X, rng = gpu, np.random.default_rng(rows + nr)
+    m = Matrix(X, rng, rows, K, alpha=0.01)
+    xq, xs = nvfp4.rows_of(rng, nr, K)
+    res = bf16_rne(rng.standard_normal((nr, rows + 3)).astype(np.float32))
+    apart = nvfp4.project(X, m, xq, xs, True, res, 1.0, pad=3)
+    y, dq, ds = X.DevBuf(array=res), X.DevBuf(array=xq), X.DevBuf(array=xs)
+    X.call("q27x_proj_nvfp4_rows", ctypes.byref(m.handle), dq.ptr, K, ds.ptr, y.ptr, rows + 3, 1, y.ptr, 1, rows + 3, 1.0, nr, None)
+    X.call("q27x_device_sync")
+    got = y.download(np.uint16, res.shape)
+    assert np.array_equal(got[:, :rows], apart) and np.array_equal(got[:, rows:], res[:, rows:])
+
+
+def test_one_row_needs_no_strides(gpu):
+    X, rng = gpu, np.random.default_rng(1)
+    m = Matrix(X, rng, 99, 400)
+    xq, xs = nvfp4.rows_of(rng, 1, 400)
+    want = nvfp4.project(X, m, xq, xs)
+    dq, ds, y = X.DevBuf(array=xq), X.DevBuf(array=xs), X.DevBuf(4 * 99)
+    X.call("q27x_proj_nvfp4_rows", ctypes.byref(m.handle), dq.ptr, 0, ds.ptr, y.ptr, -1, 0, None, 0, 0, 0.0, 1, None)
+    X.call("q27x_device_sync")
+    assert np.array_equal(y.download(np.float32, (1, 99)), want)
+
+
+def test_one_workspace_for_calls_in_turn(gpu):
+    """Calls of many sizes one behind another on a stream, with the largest one's workspace and no wait between."""
+    X, rng = gpu, np.random.default_rng(2)
+    sizes = [(62080, 3), (300, 40), (62080, 20), (5000, 7), (140000, 2), (4096, 1), (62080, 1), (20000, 30)]
+    work = X.DevBuf(max(X.lib().q27x_sample_work_bytes(n, nr) for n, nr in sizes))
+    calls = []
+    for n, nr in sizes:
+        x, u = sampling.logits(rng, nr, n), rng.random(nr).astype(np.float32)
+        calls.append((x, u, X.DevBuf(array=x), X.DevBuf(array=u), X.DevBuf(4 * nr), X.DevBuf(4 * nr)))
+    for (n, nr), (_, _, x, u, idx, prob) in zip(sizes, calls):
+        X.call("q27x_sample_rows", x.ptr, 0, n, n, nr, None, None, None, None, u.ptr, work.ptr, idx.ptr, prob.ptr, None)
+    X.call("q27x_device_sync")
+    for (n, nr), (x, u, _, _, idx, prob) in zip(sizes, calls):
+        want = sampling.sample(X, x, u=u)
+        assert np.array_equal(idx.download(np.int32, (nr,)), want[0]) and np.array_equal(prob.download(np.float32, (nr,)), want[1])
