@@ -276,7 +276,8 @@ __global__ __launch_bounds__((RESIDENT ? 64 : 32) * kNvWaves) void k_nvfp4(Nvfp4
     extern __shared__ __attribute__((aligned(16))) char lds[];
     const int t = threadIdx.x, l = t & 63, c = l & 15, g = l >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
-    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
+    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0);
+    const int turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
     const int wide = SWIGLU ? groups >> 1 : groups, each = SWIGLU ? 16 : tile_rows;
     constexpr int kIn = RESIDENT || PAIRS == 1 ? PAIRS : 2, kPasses = (PAIRS + kIn - 1) / kIn;        // pairs of a pass over the weights, and passes
     constexpr int kItems = !RESIDENT ? 5 : PAIRS <= 2 ? 4 : 3;       // (3 rows of 17408 at once: 18.6 us, by 3 items 19.5)
@@ -479,7 +480,8 @@ struct Nvfp4WideWeights {
     __device__ __forceinline__ void operands(int j, u32x4 (&q)[4]) const {
 #pragma unroll
         for (int d = 0; d < 4; ++d) {
-            const auto x = __builtin_amdgcn_permlane16_swap(w[j][0][d], w[j][2][d], false, false), y = __builtin_amdgcn_permlane16_swap(w[j][1][d], w[j][3][d], false, false);
+            const auto x = __builtin_amdgcn_permlane16_swap(w[j][0][d], w[j][2][d], false, false);
+            const auto y = __builtin_amdgcn_permlane16_swap(w[j][1][d], w[j][3][d], false, false);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 q[2 * h][d] = (uint32_t)__builtin_amdgcn_update_dpp((int)x[h], (int)y[h], 0x118, 0xF, 0xC, false);
@@ -497,7 +499,8 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     using Tile = Nvfp4Tile<kRows>;
     const int t = threadIdx.x, l = t & 63, c = l & 31, g = l >> 5;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6), grp = __builtin_amdgcn_readfirstlane((t >> 6) / waves), wv = wave - grp * waves;
-    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0), turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
+    const int full = a.K / kNvStep, rest = (a.K % kNvStep) >> 4, steps = full + (rest != 0);
+    const int turn = waves * per, held = RESIDENT ? steps : turn, count = 16 * held;
     const int each = SWIGLU ? kRows : tile_rows;
     const Nvfp4WideLds L(kIn, held, per, groups, waves, slots, rest != 0);
     char* tail = lds + L.tail + 4608 * grp;
@@ -534,7 +537,8 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     for (int first = (int)blockIdx.x * each; first < a.rows; first += turn_rows, parity ^= 1) {
         if (rest) {
 #pragma unroll
-            for (int m = 0; m < kMats; ++m) Tile::bring(a.w[m], a.s[m], a.K, row, min(row + each, a.rows), tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
+            for (int m = 0; m < kMats; ++m)
+                Tile::bring(a.w[m], a.s[m], a.K, row, min(row + each, a.rows), tail + m * kRows * 144, rest, t - 64 * grp * waves, 64 * waves);
             __syncthreads();
         }
         float* sums = (float*)(lds + L.sums) + parity * groups * slots * 32 * kIn;
@@ -629,8 +633,8 @@ template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
     const int tiles = (a.rows + p.tile_rows - 1) / p.tile_rows, units = (tiles + p.groups - 1) / p.groups, grid = units < 256 ? units : 256;
     Q27X_HIP((allow_lds<k_nvfp4_wide<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
-    hipLaunchKernelGGL((k_nvfp4_wide<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows, p.groups, p.waves,
-                       p.per, p.slots);
+    hipLaunchKernelGGL((k_nvfp4_wide<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows,
+                       p.groups, p.waves, p.per, p.slots);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
 }
@@ -643,7 +647,8 @@ static int launch_nvfp4_form(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t
     fit = fit < 1 ? 1 : fit;
     const int grid = 256 * fit < units ? 256 * fit : units;
     Q27X_HIP((allow_lds<k_nvfp4<PAIRS, SWIGLU, RESIDENT>>(kNvLds)));
-    hipLaunchKernelGGL((k_nvfp4<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows, p.groups, p.waves, p.per, p.slots);
+    hipLaunchKernelGGL((k_nvfp4<PAIRS, SWIGLU, RESIDENT>), dim3((unsigned)grid), dim3(64 * p.groups * p.waves), p.bytes, s, a, p.tile_rows, p.groups,
+                       p.waves, p.per, p.slots);
     Q27X_HIP(hipGetLastError());
     return Q27X_OK;
 }
@@ -728,7 +733,10 @@ static int nvfp4_args(const q27x_nvfp4_t* w, const char* who, const int8_t* xq, 
         set_error("%s: xstride=%d: at least K=%d, a multiple of 16", who, xstride, w->K);
         return Q27X_E_ARG;
     }
-    if ((long long)(nr - 1) * (nr > 1 ? xstride : 0) + w->K > 0x7fffffffLL) { set_error("%s: rows of activations over more than 2^31 - 1 bytes", who); return Q27X_E_RANGE; }
+    if ((long long)(nr - 1) * (nr > 1 ? xstride : 0) + w->K > 0x7fffffffLL) {
+        set_error("%s: rows of activations over more than 2^31 - 1 bytes", who);
+        return Q27X_E_RANGE;
+    }
     return Q27X_OK;
 }
 

@@ -565,7 +565,8 @@ struct Cuts {
 // The row's token, from its bins: this thread's are 2 t and 2 t + 1, of n0, n1 tokens and weights w0, w1. push(upto): the tokens of
 // bins 0 .. upto into sh.qw.
 template <typename SH, typename LISTS, typename PUSH>
-__device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, const LISTS& lists, const Cuts& cuts, uint32_t n0, uint32_t n1, u64 w0, u64 w1, PUSH push) {
+__device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, const LISTS& lists, const Cuts& cuts, uint32_t n0, uint32_t n1, u64 w0, u64 w1,
+                                         PUSH push) {
     const int t = threadIdx.x;
     Sum run = {0, 0};
     if (t < kBins / 2) {
@@ -819,7 +820,8 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     a.logits = logits; a.bf16 = logits_bf16 ? 1 : 0; a.n = n; a.ld = nr > 1 ? ld : 0; a.nr = nr;
     a.ns = wl.ns; a.slice = wl.slice; a.parts = wl.parts;
     a.temperature = temperature; a.top_k = top_k; a.top_p = top_p; a.min_p = min_p; a.u = u;
-    a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off); a.ahead = (float*)(p + wl.ahead); a.smax = (float*)(p + wl.smax);
+    a.bw = (u64*)(p + wl.bw); a.list = (uint16_t*)(p + wl.list); a.off = (uint16_t*)(p + wl.off);
+    a.ahead = (float*)(p + wl.ahead); a.smax = (float*)(p + wl.smax);
     a.idx = idx; a.prob = prob;
     if (a.ns == 1) {
         Q27X_HIP(allow_lds<k_sample_one>((int)sizeof(OneShared)));
