@@ -154,6 +154,18 @@ __device__ __forceinline__ u64 scan_wave(u64 x) {
     return x;
 }
 
+// The bins of T threads: of each, the waves that have some, and the threads that store their wave's count (a wave without bins has
+// none, as blocks of 512 and 1024 have: there is no place for it).
+template <int T>
+struct BinThreads {
+    static constexpr int kEach = (kBins + T - 1) / T, kWaves = (kBins + 64 * kEach - 1) / (64 * kEach);
+    static __host__ __device__ constexpr bool has_sum(int t) { return (t & 63) == 63 && t >> 6 < kWaves; }
+    static constexpr bool sums_within(int places) {
+        for (int t = 0; t < T; ++t)
+            if (has_sum(t) && t >> 6 >= places) return false;
+        return true;
+    }
+};
 struct BinShared {
     u64 w[kBins * kCopies];
     uint32_t n[kBins * kCopies], part[(kBins + 63) / 64];
@@ -200,7 +212,8 @@ __device__ __forceinline__ uint32_t bins_of(const SampleArgs& a, BinShared& sh, 
         }
     __syncthreads();
     // where each bin begins
-    constexpr int kEach = (kBins + T - 1) / T;    // bins of a thread
+    constexpr int kEach = BinThreads<T>::kEach, kWaves = BinThreads<T>::kWaves;
+    static_assert(BinThreads<T>::sums_within(sizeof(sh.part) / sizeof(sh.part[0])), "a place for each sum that is stored");
     uint32_t n[kEach][kCopies], run = 0;
     if (t * kEach < kBins) {
 #pragma unroll
@@ -214,10 +227,9 @@ __device__ __forceinline__ uint32_t bins_of(const SampleArgs& a, BinShared& sh, 
     }
     const uint32_t mine = run;
     run = scan_wave(run);
-    if ((t & 63) == 63 && t * kEach < kBins + 64 * kEach) sh.part[t >> 6] = run;
+    if (BinThreads<T>::has_sum(t)) sh.part[t >> 6] = run;
     run -= mine;
     __syncthreads();
-    constexpr int kWaves = (kBins + 64 * kEach - 1) / (64 * kEach);
     uint32_t total = 0;
 #pragma unroll
     for (int k = 0; k < kWaves; ++k) {
