@@ -364,8 +364,8 @@ int q27x_argmax_rows(const float* logits, int n, int ld, int nr, int32_t* idx, f
  * sampler, src/q27_main.cpp:2975-3007, with given random numbers, for every row of a batch, on the device). In order of falling
  * logits, equal ones by index, without those that are not finite, and with w = e^((l - l0) / temperature), l0 the largest:
  *   top_k >= 1 keeps the first top_k; top_p < 1 of these the fewest first ones whose w reach top_p of their sum (one at least);
- *   min_p > 0 of these those with w >= min_p (one at least); idx = the first token whose running sum of w passes u times the sum of
- *   what is kept, prob (nullable) = its w over that sum.
+ *   min_p > 0 of these those with w >= min_p (one at least: above 1 the first alone);
+ *   idx = the first token whose running sum of w passes u times the sum of what is kept, prob (nullable) = its w over that sum.
  * temperature, top_k, top_p, min_p, u: device [nr], read by the kernels (a captured graph follows them); each but u may be NULL
  * (temperature 1, no cut). temperature not above 0: the largest logit, as q27x_argmax_rows (top_p, min_p then cut nothing). u in
  * [0, 1); outside: the nearest token of the kept ones. No finite logit: idx 0, prob 0. Weights are whole multiples of 2^-44 (below

@@ -557,7 +557,7 @@ struct Cuts {
     int k;
     float p, m, u;
     double c;
-    u64 least;                                    // the weight that min_p asks for
+    u64 least;                                    // the weight that min_p asks for: above 1 one that no token has
     int bm0, bm1;                                 // bins around those that tokens of this weight are in (the logarithm is rounded)
     __device__ __forceinline__ Cuts(const SampleArgs& a, int row) {
         bool greedy;
@@ -566,7 +566,7 @@ struct Cuts {
         p = a.top_p ? a.top_p[row] : 1.0f;
         m = a.min_p ? a.min_p[row] : 0.0f;
         u = a.u[row];
-        least = m < 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit;
+        least = m <= 1.0f ? (u64)__builtin_ceil((double)m * (double)kUnit) : kUnit + 1;
         const double z = m < 1.0f ? -(double)__builtin_amdgcn_logf(m) : 0.0;
         const int bm = z < 48.0 ? bin_of(z) : kBins - 1;
         bm0 = bm > 0 ? bm - 1 : 0;
@@ -623,7 +623,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, c
         if (by_k) kept = sh.end_k;
         const u64 want = share_of<false>(cuts.p, kept);
         if (by_p && x.is && x.before.w < want && want <= end) sh.end_p = end;
-        if (by_m && x.is && x.before.n + 1 == sh.heavy) sh.end_m = end;
+        if (by_m && x.is && x.before.n + 1 == max(sh.heavy, 1u)) sh.end_m = end;       // (one at least)
         __syncthreads();
         u64 cut = kept;
         if (by_p) cut = min(cut, sh.end_p);
@@ -656,7 +656,7 @@ __device__ __forceinline__ void draw_row(const SampleArgs& a, SH& sh, int row, c
                 __syncthreads();
                 if (sum) atomicAdd(&sh.found_w, sum);
                 __syncthreads();
-                cut = min(cut, sh.bw[cuts.bm0] + sh.found_w);
+                cut = min(cut, max(sh.bw[cuts.bm0] + sh.found_w, kUnit));       // (one at least: the largest, of weight 1)
                 __syncthreads();
             }
             target = stage == 1 ? share_of<false>(cuts.p, kept) : share_of<true>(cuts.u, cut);
