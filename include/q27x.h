@@ -115,8 +115,8 @@ int q27x_proj_rows(const q27x_i8g_t* w, const int8_t* xq, int xstride, const flo
 
 /* NVFP4 weight handle (the reference's q27_nvfp4_t, include/q27.h:148-178, as its checkpoint holds the MLP and lm_head): w
  * [rows][K/2], two E2M1 codes a byte, the even column's in the low nibble (0, .5, 1, 1.5, 2, 3, 4, 6; bit 3 the sign); s
- * [rows][K/16] E4M3 scales (a scale that is not a number makes its row's outputs none); alpha the per-tensor multiplier
- * (weight_scale_2 x input_scale). Any alignment. */
+ * [rows][K/16] E4M3 scales (a scale that is not a number makes its row's outputs none, and behind SwiGLU the scale of their 16); alpha
+ * the per-tensor multiplier (weight_scale_2 x input_scale). Any alignment. */
 typedef struct q27x_nvfp4 {
     const uint8_t* w;
     const uint8_t* s;
@@ -136,6 +136,7 @@ int q27x_proj_nvfp4_rows(const q27x_nvfp4_t* w, const int8_t* xq, int xstride, c
 /* Gate and up of an MLP on NVFP4 weights, and q27x_swiglu_quant_rows of them, in one launch (the reference's fused
  * q27_proj_nvfp4_gu_nr, include/q27_nr.h:14-19): gate and up [rows][K] as q27x_proj_nvfp4_rows computes them, fp32, then
  *   v = (g/(1+e^-g)) * u * (1/in_scale); per 16: s = mx/127; q = clamp(rint(v/s)) -> oq [nr][rows], os [nr][rows/16].
+ * A v that is not a number makes its 16's s none and their q 0 (q27x_swiglu_quant_rows passes over it), so what reads them is none.
  * rows % 16 == 0, K as there; in_scale is that of the projection that reads oq; oq and os overlap nothing that is read. */
 int q27x_swiglu_nvfp4_rows(const q27x_nvfp4_t* gate, const q27x_nvfp4_t* up, const int8_t* xq, int xstride,
                            const float* xs, int8_t* oq, float* os, float in_scale, int nr, q27x_stream_t s);

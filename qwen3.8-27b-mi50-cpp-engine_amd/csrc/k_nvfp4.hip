@@ -246,11 +246,13 @@ __device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* su
         if constexpr (SWIGLU) {
             const float gate = a.alpha[0] * (kHalves ? total(k) : total(2 * k)), up = a.alpha[1] * (kHalves ? total(k, ROWS) : total(2 * k + 1));
             const float z = gate / (1.0f + qexp(-gate)) * up * a.g;
-            const float sc = max_xor(fabsf(z), 16) * (1.0f / 127.0f);
+            // (a maximum passes over what is not a number: a group that has such a value has it as its scale, and codes of 0)
+            const bool none = (__ballot(z != z) >> (threadIdx.x & 48)) & 0xFFFF;
+            const float mx = max_xor(fabsf(z), 16), sc = none ? __builtin_nanf("") : mx * (1.0f / 127.0f);
             const float inv = sc > 0.0f ? 1.0f / sc : 0.0f;
             if (is) {
                 const size_t at = (size_t)n * a.rows + row;
-                a.oq[at] = qcode(z, inv);
+                a.oq[at] = qcode(none ? 0.0f : z, inv);
                 if ((r & 15) == 0) a.os[at >> 4] = sc;
             }
         } else if (is) {
