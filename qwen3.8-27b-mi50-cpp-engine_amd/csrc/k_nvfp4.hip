@@ -262,7 +262,7 @@ __device__ __forceinline__ void nvfp4_finish(const Nvfp4Args& a, const float* su
                 y = __builtin_fmaf(a.rs, a.res_bf16 ? bf2f(((const uint16_t*)a.res)[at]) : ((const float*)a.res)[at], y);
             }
             const size_t at = (size_t)n * a.ystride + row;
-            if (a.out_bf16) ((uint16_t*)a.y)[at] = f2bf(y);
+            if (a.out_bf16) ((uint16_t*)a.y)[at] = y == y ? f2bf(y) : (uint16_t)0x7FC0;       // (rounded, one with all its bits set would be a 0)
             else ((float*)a.y)[at] = y;
         }
     }
