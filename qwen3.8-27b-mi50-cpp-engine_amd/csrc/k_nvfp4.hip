@@ -630,6 +630,23 @@ __global__ __launch_bounds__(64 * kNvWideWaves) void k_nvfp4_wide(Nvfp4Args a, i
     }
 }
 
+// Tiles side by side in a block, that share its activations: up to 1, 2, 4 or 4 for 1 to 4 pairs of rows, while there are as many for every
+// compute unit. Three tiles a unit are one block's: in blocks of two a unit has two or four (3 rows of 10240 x 5120 12.3 us, so 11.3; 5
+// rows of 9001 x 5136 17.0 and 14.8; 3 rows of 9216 x 16384 27.1 and 22.7).
+static constexpr int nvfp4_groups(int pairs, int least, int tiles) {
+    int groups = pairs == 1 ? 1 : pairs == 2 ? 2 : 4;
+    if (groups < least) groups = least;
+    while (groups > least && tiles * least < 256 * groups) groups >>= 1;
+    return least == 1 && groups == 2 && tiles > 512 && tiles <= 768 ? 3 : groups;
+}
+// (up to four tiles a unit: every unit's are whole blocks; from five on its blocks' rounds run into one another)
+static constexpr bool nvfp4_shares_are_even() {
+    for (int pairs = 1; pairs <= kMaxRows / 2; ++pairs)
+        for (int tiles = 1; tiles <= 4 * 256; ++tiles)
+            if ((tiles + 255) / 256 % nvfp4_groups(pairs, 1, tiles)) return false;
+    return true;
+}
+static_assert(nvfp4_shares_are_even(), "a compute unit's tiles are whole blocks");
 struct Nvfp4Plan { int per, slots, groups, waves, bytes, tile_rows, tiles; };
 template <int PAIRS, bool SWIGLU, bool RESIDENT>
 static int launch_nvfp4_wide(const Nvfp4Args& a, const Nvfp4Plan& p, hipStream_t s) {
@@ -677,16 +694,15 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
         p.tile_rows = SWIGLU ? 16 : 32;
         if (tiles32 >= (PAIRS == 4 ? 160 : 512) && fits_wide(kNvWideWaves / p.groups, true)) return launch_nvfp4_wide<PAIRS, SWIGLU, true>(a, p, s);
     }
-    // tiles of fewer rows where that gives every compute unit as many (5120 x 17408, 1 row: 10 of 16 rows 14.2 us, all 16 16.1; 5120 x
-    // 5120, 3 rows 8.4 and 9.7; where a compute unit has one at most it is no gain: 1024 x 768 4.2 and 3.9)
+    // tiles of fewer rows, as many for every compute unit (cold weights, 5120 x 17408, 1 row: 10 of 16 rows 14.4 us, all 16 16.7; 5120 x
+    // 5120, 3 rows 8.3 and 8.9; 17408 x 5120, five tiles a unit, 15.6 and 16.0; 34816 x 5120, nine, the same; where a unit has one at most it
+    // is no gain: 1024 x 768 4.2 and 3.9)
     const int n = SWIGLU || tiles <= 256 ? 0 : (tiles + 255) / 256;
     p.tile_rows = n ? (a.rows - 1) / (256 * n) + 1 : 16;
     p.tiles = (a.rows + p.tile_rows - 1) / p.tile_rows;
     // all activations in LDS, tiles side by side that share them
-    p.groups = PAIRS == 1 ? 1 : PAIRS == 2 ? 2 : 4;
-    if (p.groups < least) p.groups = least;
-    while (p.groups > least && p.tiles * least < 256 * p.groups) p.groups >>= 1;         // (tiles for every compute unit)
-    for (;; p.groups >>= 1) {
+    p.groups = nvfp4_groups(PAIRS, least, p.tiles);
+    for (;; p.groups = p.groups == 3 ? 2 : p.groups >> 1) {
         const int most = kNvWaves / p.groups, turns = (p.slots + most - 1) / most;
         p.waves = (p.slots + turns - 1) / turns;
         p.bytes = Nvfp4Lds(a.nr, steps, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
