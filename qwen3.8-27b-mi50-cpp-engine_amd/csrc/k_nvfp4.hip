@@ -679,6 +679,20 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
     Nvfp4Plan p;
     p.per = steps <= 4 ? 1 : steps <= 8 ? 2 : kNvSteps;
     p.slots = (steps + p.per - 1) / p.per;
+    // tiles of fewer rows, as many for every compute unit (cold weights, 5120 x 17408, 1 row: 10 of 16 rows 14.4 us, all 16 16.7; 5120 x
+    // 5120, 3 rows 8.3 and 8.9; 17408 x 5120, five tiles a unit, 15.6 and 16.0; 34816 x 5120, nine, the same; where a unit has one at most it
+    // is no gain: 1024 x 768 4.2 and 3.9)
+    const int n = SWIGLU || tiles <= 256 ? 0 : (tiles + 255) / 256;
+    p.tile_rows = n ? (a.rows - 1) / (256 * n) + 1 : 16;
+    p.tiles = (a.rows + p.tile_rows - 1) / p.tile_rows;
+    const int side = nvfp4_groups(PAIRS, least, p.tiles);
+    auto fits = [&](int groups) {                    // all activations in LDS, tiles side by side that share them
+        const int most = kNvWaves / groups, turns = (p.slots + most - 1) / most;
+        p.groups = groups;
+        p.waves = (p.slots + turns - 1) / turns;
+        p.bytes = Nvfp4Lds(a.nr, steps, p.per, groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
+        return p.bytes <= kNvLds;
+    };
     const int tiles32 = SWIGLU ? tiles : (tiles + 1) / 2;
     auto fits_wide = [&](int most, bool resident) {
         const int turns = (p.slots + most - 1) / most;
@@ -688,26 +702,20 @@ static int launch_nvfp4_pairs(const Nvfp4Args& a, hipStream_t s) {
     };
     // 5 rows and more: tiles of 32 weight rows, where there are enough of them. Against those of 16: 62080 x 5120, 8 rows 37 us (45), 5
     // rows 36 (39); gate | up 17408 x 5120 29.6 (36.8), 29 (32); 5120 x 5120 11.9 (15.3), 11.6 (11.5); with fewer tiles than here
-    // 1024 x 768 5.6 (4.8), and 9001 x 5136, 5 rows 19.8 (18.0); 3 rows 33.4 (33.2) and 26.8 (24.8).
+    // 1024 x 768 5.6 (4.8), and 9001 x 5136, 5 rows 19.8 (14.8); 3 rows 33.4 (33.2) and 26.8 (24.8). Not where three tiles of 16 are a
+    // unit's: cold weights, 9001 x 5136, 8 rows 20.8 (16.6), 10240 x 1024 8.5 (7.4), 12288 x 5120 16.4 (16.2).
     if constexpr (PAIRS >= kWidePairs) {
-        p.groups = tiles32 < 512 ? 1 : 2;            // (tiles for every compute unit)
-        p.tile_rows = SWIGLU ? 16 : 32;
-        if (tiles32 >= (PAIRS == 4 ? 160 : 512) && fits_wide(kNvWideWaves / p.groups, true)) return launch_nvfp4_wide<PAIRS, SWIGLU, true>(a, p, s);
+        if (tiles32 >= (PAIRS == 4 ? 160 : 512) && !(side == 3 && fits(3))) {
+            const Nvfp4Plan narrow = p;
+            p.groups = tiles32 < 512 ? 1 : 2;        // (tiles for every compute unit)
+            p.tile_rows = SWIGLU ? 16 : 32;
+            if (fits_wide(kNvWideWaves / p.groups, true)) return launch_nvfp4_wide<PAIRS, SWIGLU, true>(a, p, s);
+            p = narrow;
+        }
     }
-    // tiles of fewer rows, as many for every compute unit (cold weights, 5120 x 17408, 1 row: 10 of 16 rows 14.4 us, all 16 16.7; 5120 x
-    // 5120, 3 rows 8.3 and 8.9; 17408 x 5120, five tiles a unit, 15.6 and 16.0; 34816 x 5120, nine, the same; where a unit has one at most it
-    // is no gain: 1024 x 768 4.2 and 3.9)
-    const int n = SWIGLU || tiles <= 256 ? 0 : (tiles + 255) / 256;
-    p.tile_rows = n ? (a.rows - 1) / (256 * n) + 1 : 16;
-    p.tiles = (a.rows + p.tile_rows - 1) / p.tile_rows;
-    // all activations in LDS, tiles side by side that share them
-    p.groups = nvfp4_groups(PAIRS, least, p.tiles);
-    for (;; p.groups = p.groups == 3 ? 2 : p.groups >> 1) {
-        const int most = kNvWaves / p.groups, turns = (p.slots + most - 1) / most;
-        p.waves = (p.slots + turns - 1) / turns;
-        p.bytes = Nvfp4Lds(a.nr, steps, p.per, p.groups, p.waves, p.slots, 32 * PAIRS, ends_inside).total;
-        if (p.bytes <= kNvLds) return launch_nvfp4_form<PAIRS, SWIGLU, true>(a, p, s);
-        if (p.groups == least) break;
+    for (int groups = side;; groups = groups == 3 ? 2 : groups >> 1) {
+        if (fits(groups)) return launch_nvfp4_form<PAIRS, SWIGLU, true>(a, p, s);
+        if (groups == least) break;
     }
     // activations in turns: 32 weight rows where that is a tile for each compute unit at most, or 5 or 6 rows, or gate | up; and 4 waves have
     // room beside the sums. Against 16: 5120 x 17408, 5 rows 24.9 us (34.3), 8 rows 34.7 (37.6), 9001 x 17408 42 (49), 63 (54), gate |
