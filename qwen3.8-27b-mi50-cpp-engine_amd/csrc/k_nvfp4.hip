@@ -22,7 +22,8 @@
 // eighths: row 4 n + i of the operand holds slab i of row n, so one instruction serves 8 rows. It takes 40 cycles, the 16 x 16 x 128
 // with E4M3, two rows, 42: 8 rows 37 us, where those tiles take 45 to 48. Left are the scales' products and sums (2 operations a slab, row
 // and weight row) and the masks of the operands: without the sums 33.8 us; without preparing the activations 36.9.
-#include "q27x_paged.h"
+#include "q27x_dev.h"
+#include "q27x_int.h"
 
 namespace q27x {
 

@@ -24,7 +24,8 @@
 // All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000; ranks alone held, 4096 of them, and
 // weights computed anew: 26.5. A search down to 128 or 256 tokens in place of 64: 25.9 and 28.3 us. One copy of the bins: atomics of
 // a wave wait for one another.
-#include "q27x_paged.h"
+#include "q27x_dev.h"
+#include "q27x_int.h"
 
 namespace q27x {
 

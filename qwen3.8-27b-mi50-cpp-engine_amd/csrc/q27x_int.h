@@ -4,6 +4,8 @@
 #include <stddef.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/q27x.h"
 
 namespace q27x {
@@ -16,6 +18,19 @@ int hip_fail(hipError_t e, const char* what);
         hipError_t e_ = (call);                                          \
         if (e_ != hipSuccess) return ::q27x::hip_fail(e_, #call);        \
     } while (0)
+
+// Lets kernel K have `bytes` of dynamic LDS on the current device: once per device.
+template <auto K>
+inline hipError_t allow_lds(int bytes) {
+    static std::atomic<uint64_t> known{0};
+    int dev = 0;
+    if (hipError_t e = hipGetDevice(&dev)) return e;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if (known.load(std::memory_order_relaxed) & bit) return hipSuccess;
+    if (hipError_t e = hipFuncSetAttribute((const void*)K, hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+    known.fetch_or(bit, std::memory_order_relaxed);
+    return hipSuccess;
+}
 
 constexpr int kMaxRows = 8;      // verify rows (K <= 7) and prefill chunk
 constexpr int kSplit = 64;       // attention keys per split (fixed: results independent of NR)
