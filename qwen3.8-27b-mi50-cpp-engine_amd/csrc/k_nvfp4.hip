@@ -12,15 +12,16 @@
 // 16 x 16 result has the dots of 8 slabs of a pair of rows with 16 weight rows. An eighth of the operand holds something; the
 // matrix cores have the time.
 //
-// Up to 4 rows the bound is memory: 62080 x 5120, 1 row, 179 MB in 30.6 us (5.85 TB/s; a kernel that only reads them so, 26.0). What it
-// takes: whole 128-byte lines of 8 rows a load, exchanged in registers (16 rows by 64 bytes, which are operands at once, read
-// at 5.0 TB/s and no more); scales of several steps in one load (one a step: +9 us of 39); blocks that stay and keep the
-// activations, prepared, in LDS (a block a tile: 49.5 us, a third of it spent on them); the next tile on its way while one is worked on.
+// Up to 4 rows the bound is memory: 62080 x 5120, 1 row, 179 MB in 30.8 us where no cache holds them (5.8 TB/s), 28.9 over and over (a
+// kernel that only reads them so, 26.0). What it takes: whole 128-byte lines of 8 rows a load, exchanged in registers (16 rows by 64
+// bytes, which are operands at once, read at 5.0 TB/s and no more); scales of several steps in one load (one a step: +9 us of 39); blocks
+// that stay and keep the activations, prepared, in LDS (a block a tile: 49.5 us, a third of it spent on them); the next tile on its way
+// while one is worked on.
 // Chunks of K shorter than 5 steps: 33 us (3), 39 (2), 58 (1).
 //
 // From 5 rows on tiles of 32 weight rows, and v_mfma_scale_f32_32x32x64_f8f6f4 with the nibbles in E2M3, whose codes 0 .. 15 are as many
 // eighths: row 4 n + i of the operand holds slab i of row n, so one instruction serves 8 rows. It takes 40 cycles, the 16 x 16 x 128
-// with E4M3, two rows, 42: 8 rows 37 us, where those tiles take 45 to 48. Left are the scales' products and sums (2 operations a slab, row
+// with E4M3, two rows, 42: 8 rows 36 to 37 us, where those tiles take 45 to 48. Left are the scales' products and sums (2 operations a slab, row
 // and weight row) and the masks of the operands: without the sums 33.8 us; without preparing the activations 36.9.
 #include "q27x_dev.h"
 #include "q27x_int.h"

@@ -17,10 +17,11 @@
 //     256th of its z and then by (logit, index) in steps of 8 bits, and these are counted like that.
 //   k_sample_one: all of that by one block, for rows of up to 4096 logits (7.8 us for 300, 8 to 11 for 4000, by the settings).
 //
-// Bound by latency: 62080 logits, 1 row, 16.4 us, of which k_sample_max has 2.5, k_sample_bins 6, k_sample_draw 8 (2.9 to read, 2.2 to
-// sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 35 to 40 us: 4.8, 13.7 (the exponentials and the
-// atomics 2.6 each), the rest for the slowest row, whose cuts and draw are three searches (k = 1000 alone 24.5 us), or one in a bin
-// of thousands of tokens, which are read twice (p = 0.99, nothing before it: 29; by the ranks' range from the start, three times: 35).
+// Bound by latency: 62080 logits, 1 row, 16.4 to 18.1 us, of which k_sample_max has 2.5, k_sample_bins 6, k_sample_draw 8 (2.9 to read, 2.2
+// to sum the bins, 2 to count 117 tokens); their bytes take 0.05. 64 rows of every kind 33 to 39 us: 4.8, 15.1 (the exponentials and the
+// atomics 2.6 each; what the rest of these waits for was not measured), and for the slowest row, whose cuts and draw are three searches (k
+// = 1000 alone 24.5 us), or one in a bin of thousands of tokens, which are read twice (p = 0.99, nothing before it: 29; by the ranks'
+// range from the start, three times: 35).
 // All that can be drawn held in LDS and searched there: 32 us against 25 for a row of k = 1000; ranks alone held, 4096 of them, and
 // weights computed anew: 26.5. A search down to 128 or 256 tokens in place of 64: 25.9 and 28.3 us. One copy of the bins: atomics of
 // a wave wait for one another.
@@ -845,7 +846,7 @@ extern "C" int q27x_sample_rows(const void* logits, int logits_bf16, int n, int 
     const dim3 grid((unsigned)a.ns, (unsigned)nr);
     hipLaunchKernelGGL(k_sample_max, dim3((unsigned)a.parts, (unsigned)nr), dim3(256), 0, (hipStream_t)s, a);
     Q27X_HIP(hipGetLastError());
-    if (a.slice == kLeastSlice && (long long)a.ns * nr <= 256) {          // (a compute unit for each block: 1 row 16.7 us, else 17.2; 64 rows 29.4, else 28.7)
+    if (a.slice == kLeastSlice && (long long)a.ns * nr <= 256) {          // (a compute unit for each block: 1 row 16.2 us, by 512 threads 16.8; 64 rows of every kind 35.2 and 34.3)
         hipLaunchKernelGGL((k_sample_bins<1024, 4, false>), grid, dim3(1024), 2 * a.slice, (hipStream_t)s, a);
     } else if (a.slice == kLeastSlice) {
         hipLaunchKernelGGL((k_sample_bins<512, 8, false>), grid, dim3(512), 2 * a.slice, (hipStream_t)s, a);
