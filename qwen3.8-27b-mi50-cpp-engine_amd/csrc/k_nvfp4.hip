@@ -641,7 +641,7 @@ static constexpr int nvfp4_groups(int pairs, int least, int tiles) {
     while (groups > least && tiles * least < 256 * groups) groups >>= 1;
     return least == 1 && groups == 2 && tiles > 512 && tiles <= 768 ? 3 : groups;
 }
-// (up to four tiles a unit: every unit's are whole blocks; from five on its blocks' rounds run into one another)
+// (up to four tiles a unit, where LDS has room for a block's: every unit's are whole blocks; from five on rounds run into one another)
 static constexpr bool nvfp4_shares_are_even() {
     for (int pairs = 1; pairs <= kMaxRows / 2; ++pairs)
         for (int tiles = 1; tiles <= 4 * 256; ++tiles)
